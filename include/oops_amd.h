@@ -445,10 +445,97 @@ int oops_trimul_output_grad_products(const oops_trimul_geometry* geo, const void
                                      int64_t w_row, const void* y, int64_t y_row, void* d, int64_t d_row,
                                      float* g_parts, float* s_parts, void* stream);
 
+/* ---- root-mean-square norm of rows, with a residual and an 8-bit output ----
+ *
+ * h = x + residual, rounded to dtype and written to `sum` (residual NULL: h = x, sum not written);
+ * y = h * (mean(h^2) + eps)^-1/2 * weight over `width`, statistics in float32.  y, sum, values and the gradients
+ * are [rows][width]; weight is float32 (weight_f32) or of dtype, NULL for ones.
+ * 8-bit rows: values = rint(y * 127 / max|y|) and scales[row] = max|y| / 127 (y is not rounded before); a row of
+ * zeros has scale 0; a row that holds an infinity or a NaN has zero values and the scale NaN.
+ * No counterpart in the reference (its LayerNorm is oops/normalization/layer_norm). */
+typedef struct oops_rms_norm_geometry {
+  int32_t dtype;      /* OOPS_F32 / OOPS_BF16 / OOPS_F16 */
+  int32_t weight_f32; /* 1: float32 weight, 0: weight of dtype */
+  int32_t width;      /* 1..16384 */
+  float eps;
+  int64_t rows;
+  int64_t x_row; /* row strides of x (h in the backward) and of the residual, in elements */
+  int64_t r_row;
+} oops_rms_norm_geometry;
+
+/* rstd [rows] (float32) may be NULL where no backward follows. */
+int oops_rms_norm_forward(const oops_rms_norm_geometry* geo, const void* x, const void* residual, const void* weight,
+                          void* y, void* sum, float* rstd, void* stream);
+int oops_rms_norm_int8(const oops_rms_norm_geometry* geo, const void* x, const void* residual, const void* weight,
+                       void* values, float* scales, void* sum, void* stream);
+/* The 8-bit rows of x itself (no norm; eps, r_row and weight_f32 are not read). */
+int oops_quantize_int8(const oops_rms_norm_geometry* geo, const void* x, void* values, float* scales, void* stream);
+/* grad_x (also the residual's gradient) from grad_y and, unless NULL, the gradient of `sum`; grad_weight (NULL: not
+ * wanted) of weight's type, summed in a fixed order over float32 partials in the workspace of
+ * oops_rms_norm_backward_workspace_bytes bytes (256-byte aligned). */
+size_t oops_rms_norm_backward_workspace_bytes(const oops_rms_norm_geometry* geo);
+int oops_rms_norm_backward(const oops_rms_norm_geometry* geo, const void* h, const float* rstd, const void* weight,
+                           const void* grad_y, const void* grad_sum, void* grad_x, void* grad_weight, void* workspace,
+                           size_t ws_bytes, void* stream);
+
+/* ---- linear layer on 8-bit integers ----
+ *
+ * out[r][j] = x_scale[r] * w_scale[j] * sum_k x[r][k] * w[j][k] + bias[j], sums in 32-bit integers (exact: k at most
+ * 131071), out [rows][n] rounded once.  Any k, n, alignment; rows x_row and w_row bytes apart. */
+typedef struct oops_int8_geometry {
+  int64_t rows;
+  int64_t n;
+  int64_t k;
+  int64_t x_row;
+  int64_t w_row;
+  int32_t out_dtype;
+  int32_t bias_dtype; /* of a bias that is not NULL: OOPS_F32 or out_dtype */
+} oops_int8_geometry;
+size_t oops_int8_linear_workspace_bytes(const oops_int8_geometry* geo);
+int oops_int8_linear(const oops_int8_geometry* geo, const void* x, const float* x_scale, const void* w,
+                     const float* w_scale, const void* bias, void* out, void* workspace, size_t ws_bytes,
+                     void* stream);
+
+/* ---- linear attention with a decay for each head ----
+ *
+ * S_t = exp(log_decay[h]) S_(t-1) + k_t^T v_t, o_t = scale q_t S_t for each (batch, head), S_(-1) = initial (NULL:
+ * zeros).  lengths (NULL: all `length`) gives each batch element's tokens: rows behind them are not read, their
+ * outputs and gradients are zero, and `final` is the state behind the last token.  Element (b, h, t, i) of an
+ * operand is at b * stride[0] + h * stride[1] + t * stride[2] + i; strides of 0 broadcast operands that are read.
+ * States are float32 [batch][heads][key_size][value_size]; log_decay is float32 [heads]. */
+enum oops_linear_attn_operand {
+  OOPS_LA_Q, OOPS_LA_K, OOPS_LA_V, OOPS_LA_O, OOPS_LA_DO, OOPS_LA_DQ, OOPS_LA_DK, OOPS_LA_DV, OOPS_LA_OPERANDS
+};
+typedef struct oops_linear_attn_geometry {
+  int32_t dtype; /* of q, k, v, o and their gradients */
+  int32_t heads;
+  int32_t key_size;   /* 1..128 */
+  int32_t value_size; /* 1..128 */
+  int64_t batch;
+  int64_t length;
+  int64_t stride[OOPS_LA_OPERANDS][3];
+  float scale;
+  int32_t lengths_i64; /* lengths are int64 (1) or int32 (0) */
+} oops_linear_attn_geometry;
+size_t oops_linear_attn_forward_workspace_bytes(const oops_linear_attn_geometry* geo);
+int oops_linear_attn_forward(const oops_linear_attn_geometry* geo, const void* q, const void* k, const void* v,
+                             const float* log_decay, const void* lengths, const float* initial, void* out,
+                             float* final_state, void* workspace, size_t ws_bytes, void* stream);
+/* grad_final may be NULL (zeros); every gradient may be NULL (not wanted). */
+size_t oops_linear_attn_backward_workspace_bytes(const oops_linear_attn_geometry* geo);
+int oops_linear_attn_backward(const oops_linear_attn_geometry* geo, const void* q, const void* k, const void* v,
+                              const float* log_decay, const void* lengths, const float* initial, const void* grad_out,
+                              const float* grad_final, void* grad_q, void* grad_k, void* grad_v, float* grad_initial,
+                              void* workspace, size_t ws_bytes, void* stream);
+/* One token of every (batch, head): state is updated in place, then o = scale q state (length 1; token strides are
+ * not read). */
+int oops_linear_attn_step(const oops_linear_attn_geometry* geo, const void* q, const void* k, const void* v,
+                          const float* log_decay, float* state, void* out, void* stream);
+
 /* Thread-local description of the last failure (empty string if none). */
 const char* oops_last_error(void);
 
-/* Library ABI version; bumped on any change to the table or geometry layout. */
+/* Library ABI version; bumped on any change to the table or geometry layouts or to the set of functions. */
 int oops_abi_version(void);
 
 #ifdef __cplusplus

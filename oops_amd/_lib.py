@@ -20,7 +20,7 @@ BIAS_NONE, BIAS_FULL, BIAS_SHARED = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 32 << 20
 PHASE_DELTA, PHASE_DQ, PHASE_DKV, PHASE_DBIAS = 1, 2, 4, 8
 TABLE_WIDTH = 40
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 # geometry table columns (enum oops_table_column)
 (
@@ -77,6 +77,18 @@ EXPORTED_SYMBOLS = (
     "oops_trimul_output_grad_products",
     "oops_sum_partials_workspace_bytes",
     "oops_sum_partials",
+    "oops_rms_norm_forward",
+    "oops_rms_norm_int8",
+    "oops_quantize_int8",
+    "oops_rms_norm_backward_workspace_bytes",
+    "oops_rms_norm_backward",
+    "oops_int8_linear_workspace_bytes",
+    "oops_int8_linear",
+    "oops_linear_attn_forward_workspace_bytes",
+    "oops_linear_attn_forward",
+    "oops_linear_attn_backward_workspace_bytes",
+    "oops_linear_attn_backward",
+    "oops_linear_attn_step",
     "oops_last_error",
     "oops_abi_version",
 )
@@ -156,6 +168,48 @@ class SumSegment(ctypes.Structure):
         ("part_stride", ctypes.c_int64),
         ("out_dtype", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
+    ]
+
+
+class RmsNormGeometry(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("weight_f32", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("rows", ctypes.c_int64),
+        ("x_row", ctypes.c_int64),
+        ("r_row", ctypes.c_int64),
+    ]
+
+
+class Int8Geometry(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("x_row", ctypes.c_int64),
+        ("w_row", ctypes.c_int64),
+        ("out_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+    ]
+
+
+# operands of LinearAttnGeometry.stride (enum oops_linear_attn_operand)
+LA_Q, LA_K, LA_V, LA_O, LA_DO, LA_DQ, LA_DK, LA_DV, LA_OPERANDS = range(9)
+
+
+class LinearAttnGeometry(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("key_size", ctypes.c_int32),
+        ("value_size", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("length", ctypes.c_int64),
+        ("stride", (ctypes.c_int64 * 3) * LA_OPERANDS),
+        ("scale", ctypes.c_float),
+        ("lengths_i64", ctypes.c_int32),
     ]
 
 
@@ -264,6 +318,30 @@ def load() -> ctypes.CDLL:
         lib.oops_sum_partials_workspace_bytes.restype = sz
         lib.oops_sum_partials.argtypes = [ctypes.POINTER(SumSegment), ctypes.c_int32, vp, sz, vp]
         lib.oops_sum_partials.restype = i32
+        ng = ctypes.POINTER(RmsNormGeometry)
+        lib.oops_rms_norm_forward.argtypes = [ng, vp, vp, vp, vp, vp, vp, vp]
+        lib.oops_rms_norm_forward.restype = i32
+        lib.oops_rms_norm_int8.argtypes = [ng, vp, vp, vp, vp, vp, vp, vp]
+        lib.oops_rms_norm_int8.restype = i32
+        lib.oops_quantize_int8.argtypes = [ng, vp, vp, vp, vp]
+        lib.oops_quantize_int8.restype = i32
+        lib.oops_rms_norm_backward_workspace_bytes.argtypes = [ng]
+        lib.oops_rms_norm_backward_workspace_bytes.restype = sz
+        lib.oops_rms_norm_backward.argtypes = [ng, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.oops_rms_norm_backward.restype = i32
+        ig = ctypes.POINTER(Int8Geometry)
+        lib.oops_int8_linear_workspace_bytes.argtypes = [ig]
+        lib.oops_int8_linear_workspace_bytes.restype = sz
+        lib.oops_int8_linear.argtypes = [ig, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.oops_int8_linear.restype = i32
+        lg = ctypes.POINTER(LinearAttnGeometry)
+        for name, count in (("forward", 8), ("backward", 12)):
+            size = getattr(lib, f"oops_linear_attn_{name}_workspace_bytes")
+            size.argtypes, size.restype = [lg], sz
+            call = getattr(lib, f"oops_linear_attn_{name}")
+            call.argtypes, call.restype = [lg] + [vp] * count + [vp, sz, vp], i32
+        lib.oops_linear_attn_step.argtypes = [lg, vp, vp, vp, vp, vp, vp, vp]
+        lib.oops_linear_attn_step.restype = i32
         lib.oops_last_error.argtypes = []
         lib.oops_last_error.restype = ctypes.c_char_p
         lib.oops_abi_version.argtypes = []

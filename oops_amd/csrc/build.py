@@ -39,7 +39,11 @@ SOURCES = (
     "trimul_f32.hip",
     "trimul_grad.hip",
     "reduce.hip",
+    "rms_norm.hip",
+    "int8_linear.hip",
+    "linear_attn.hip",
     "capi.cpp",
+    "capi_layer.cpp",
 )
 FAST_MATH_SOURCES = ("attn_fwd_fast.hip", "attn_bwd_fast.hip", "attn_bwd_fused.hip")
 ARCH = "gfx950"

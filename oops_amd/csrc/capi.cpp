@@ -11,6 +11,7 @@
 
 #include "attn_kernels.h"
 #include "gate_kernels.h"
+#include "layer_kernels.h"
 #include "reduce_kernels.h"
 #include "trimul_kernels.h"
 
@@ -382,6 +383,20 @@ int gate_launch_result(hipError_t err, const char* what) {
   return OOPS_ELAUNCH;
 }
 
+}  // namespace
+
+// The same reports for the entry points of capi_layer.cpp.
+namespace oops {
+int report(int code, const char* fmt, long long a, long long b) { return fail(code, fmt, a, b); }
+void clear_report() { g_last_error.clear(); }
+int report_launch(hipError_t err, const char* what) { return gate_launch_result(err, what); }
+int report_workspace(const void* workspace, size_t given, size_t need) {
+  return check_workspace(const_cast<void*>(workspace), given, need);
+}
+}  // namespace oops
+
+namespace {
+
 // Device scratch of oops_attn_forward_noalloc: the fragment-major bias copy
 // that oops_attn_forward puts in its caller's workspace.  Every GPU the
 // library runs on holds its own copy of this array until the process ends.
@@ -440,7 +455,7 @@ int run_forward(const oops_attn_geometry* geo, const oops::Plan& plan, const voi
 
 extern "C" {
 
-int oops_abi_version(void) { return 7; }
+int oops_abi_version(void) { return 8; }
 
 const char* oops_last_error(void) { return g_last_error.c_str(); }
 
