@@ -13,7 +13,10 @@
 // token by token through chunks staged in LDS.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "attn_common.h"
+#include "attn_fast_common.h"
 #include "layer_kernels.h"
 
 namespace oops {
@@ -30,6 +33,13 @@ __device__ __forceinline__ int64_t walk_length(const LinearWalk& w, int64_t b) {
   const int64_t n = w.lengths_i64 ? static_cast<const int64_t*>(w.lengths)[b]
                                   : (int64_t) static_cast<const int32_t*>(w.lengths)[b];
   return n < 0 ? 0 : n > w.length ? w.length : n;
+}
+
+// x, of which the compiler no longer knows where it comes from: what is computed from it is computed here, and not
+// kept in registers over a loop because an expression before or in the loop looks the same
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 constexpr int kTok = 16;  // tokens of a chunk
@@ -103,6 +113,379 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(LinearWalk w) {
       const int d = g * DG + i;
       const int64_t at = state0 + (w.state_by_cols ? (int64_t)e * w.rows + d : (int64_t)d * w.cols + e);
       if (d < w.rows && e < w.cols) w.final_state[at] = s[i] * l;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- bfloat16, in chunks
+//
+// With the state kept one decay ahead in walks from the end (first = 1, else
+// 0), a chunk of m <= 64 tokens that starts from state S is
+//   out_i = scale sum_(j <= i) l^(i-j) (a_i . b_j) c_j + so l^(i+1-first) a_i S
+//   S    := l^m S + sum_j u l^(m-1-j+first) b_j^T c_j
+// (so, u) = (scale, 1), or (1, scale) from the end: four products on the
+// matrix units for 2 C D + 4 D^2 operations a token instead of the
+// recurrence's vector work.  A workgroup walks a segment of a (batch, head)
+// with the state in float32 accumulators, 32 columns a wave; the next chunk's
+// rows are loaded to registers meanwhile.  Few heads are split into segments:
+// walk_chunks_kernel<.., false> makes each segment's state from zero,
+// walk_scan_kernel joins them, then every segment starts from its own state.
+//
+// Operand layouts: accumulators hold [row of the state or value][lane], lane =
+// value column (state) or token (weights, outputs), so weights and state are
+// turned into the next product's operand in registers; the state's rows are
+// taken in the order that makes that operand's k run 8 half + 0..7, as a
+// 16-byte read of a row gives it (bits 2 and 3 of the row index swapped).
+//
+// Roundings to bfloat16: the weights scale l^(i-j) (a_i . b_j) and the state
+// where they are read by the second products, once each (different terms of
+// the output, 2^-8 of each at most, as in softmax attention).  The update's
+// operand u l^n c is split into three bfloat16 terms, which hold its float32
+// value: the state that is returned is a float32 one.
+constexpr int kChunk = 64;
+
+struct ChunkArgs {
+  LinearWalk w;
+  float* starts;       // [batch * heads][segs][state]: segments' own states, then the states they start from
+  int32_t segs;
+  int32_t seg_tokens;  // a multiple of kChunk
+};
+
+__device__ __forceinline__ int64_t state_at(const LinearWalk& w, int row, int col) {
+  return w.state_by_cols ? (int64_t)col * w.rows + row : (int64_t)row * w.cols + col;
+}
+__device__ __forceinline__ int64_t token_of(const LinearWalk& w, int64_t p, int64_t n) {
+  return w.from_end && p < n ? n - 1 - p : p;
+}
+
+// 16-byte slot of a tile row, XORed into the chunk index: rows of 256, 128 or
+// 64 bytes put the 16 rows of a read phase into distinct slots
+template <int D>
+__device__ __forceinline__ int row_swizzle(int row) {
+  return D == 128 ? row & 15 : D == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
+
+__device__ __forceinline__ bool has_non_finite(uint4 u) {
+  auto bad = [](uint32_t d) { return (d & 0x7F80u) == 0x7F80u || (d & 0x7F800000u) == 0x7F800000u; };
+  return bad(u.x) || bad(u.y) || bad(u.z) || bad(u.w);
+}
+
+#ifndef OOPS_SPLIT
+#define OOPS_SPLIT 3
+#endif
+constexpr int kSplit = OOPS_SPLIT;
+template <int D, bool VEC, bool MAIN>
+__global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(ChunkArgs ca) {
+  using T = __bf16;
+  using Frag = bf16x8;
+  constexpr int NT = 2 * D, NW = D / 32;      // threads, waves: 32 columns each
+  constexpr int RB = 2 * D, CPR = D / 8;      // bytes and 16-byte chunks of a tile row
+  constexpr int NL = kChunk * CPR / NT;       // 16-byte loads a thread and tile
+  __shared__ __align__(16) char tb[kChunk * RB], tc[kChunk * RB], ta[MAIN ? kChunk * RB : 16];
+  __shared__ __align__(16) char tp[MAIN ? kChunk * kChunk * 2 : 16];  // weights [token i][token j]
+  __shared__ __align__(16) float tw[kChunk];                          // decays of the update
+  __shared__ int bad[2];                                              // c holds an infinity or NaN
+  const LinearWalk& w = ca.w;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 31, g = lane >> 5;
+  const int64_t bh = (int64_t)blockIdx.x / ca.segs;
+  const int seg = (int)((int64_t)blockIdx.x % ca.segs);
+  if (!MAIN && seg == ca.segs - 1) return;  // (no segment starts from its state)
+  const int64_t b = bh / w.heads;
+  const int h = (int)(bh % w.heads);
+  const int64_t n = walk_length(w, b);
+  const int64_t s0 = (int64_t)seg * ca.seg_tokens;
+  const int64_t s1 = s0 + ca.seg_tokens < n ? s0 + ca.seg_tokens : n;  // (s1 <= s0: nothing to walk)
+  const int first = w.from_end ? 1 : 0;
+  const float l2 = log2_decay(w.log_decay[h]);
+  const float up = first ? w.scale : 1.f, so = first ? 1.f : w.scale;
+  const T* a = static_cast<const T*>(w.a) + b * w.a_stride[0] + h * w.a_stride[1];
+  const T* bp = static_cast<const T*>(w.b) + b * w.b_stride[0] + h * w.b_stride[1];
+  const T* c = static_cast<const T*>(w.c) + b * w.c_stride[0] + h * w.c_stride[1];
+
+  // the state: tile rt, register r is row 32 rt + 16 (r / 8) + 8 g + r % 8, column 32 wave + l
+  f32x16 S[NW];
+  const int col = 32 * wave + l;
+  const int64_t state_size = (int64_t)w.rows * w.cols;
+  {
+    const float* from = nullptr;
+    if (MAIN) from = ca.segs > 1 ? ca.starts + (bh * ca.segs + seg) * state_size
+                                 : w.initial ? w.initial + bh * state_size : nullptr;
+#pragma unroll
+    for (int rt = 0; rt < NW; ++rt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = 32 * rt + 16 * (r >> 3) + 8 * g + (r & 7);
+        S[rt][r] = from && row < w.rows && col < w.cols ? from[state_at(w, row, col)] : 0.f;
+      }
+  }
+
+  // lane addresses: rows as they are (16 bytes of row l), and transposed (4 x 4 blocks, see lds_read_tr4)
+  const int nat = l * RB + ((g ^ row_swizzle<D>(l)) << 4);
+  int tr_c, tr_b;
+  {
+    const int j = lane & 15, grp = lane >> 4;
+    const int row = ((grp >> 1) << 2) + (j >> 2);
+    auto at = [&](int cc) { return row * RB + (((cc >> 3) ^ row_swizzle<D>(row)) << 4) + (cc & 7) * 2; };
+    tr_c = at(((grp & 1) << 4) + ((j & 3) << 2));
+    tr_b = at(((grp & 1) << 4) + ((j & 1) << 3) + ((j & 2) << 1));
+  }
+  auto rows_frag = [&](const char* t, int tile, int kb) {
+    return __builtin_bit_cast(Frag, *reinterpret_cast<const uint4*>(t + tile * 32 * RB + (nat ^ (kb << 5))));
+  };
+  auto tr_frag = [&](const char* t, int lane_at, int kb, int ct) {
+    const int lo = (lane_at ^ (ct << 6)) + kb * 16 * RB, hi = (lane_at ^ (ct << 6) ^ (RB / 2)) + (kb * 16 + 8) * RB;
+    const s16x4 x = lds_read_tr4(t + lo), y = lds_read_tr4(t + hi);
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x8 v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    return __builtin_bit_cast(Frag, v);
+  };
+  const int pl = l * 128 + ((g ^ ((l >> 1) & 7)) << 4);
+
+  // scale l^(i-j) of this wave's weight tiles (it, jt): waves take tiles (0,0), (1,0), (1,1) in turn
+  constexpr int kPf = NW == 1 ? 2 : 1;
+  float pf[kPf][16], fo[2];
+  if (MAIN) {
+#pragma unroll
+    for (int q = 0; q < kPf; ++q) {
+      const int off = (NW == 1 ? q == 1 : wave == 1) ? 32 : 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int lag = off + l - kappa(g, r);
+        pf[q][r] = lag >= 0 ? w.scale * decay_power(l2, (float)lag) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int it = 0; it < 2; ++it) fo[it] = so * decay_power(l2, (float)(32 * it + l + 1 - first));
+  }
+
+  // this lane's 16 bytes of row row0 (then NT / CPR rows on) of the next chunk
+  constexpr int kRows = NT / CPR;
+  const int row0 = tid / CPR, cc0 = tid % CPR * 8;
+  const int64_t way = first ? -1 : 1, t0 = token_of(w, s0, n) + way * row0;
+  const T* pa = a + t0 * w.a_stride[2] + cc0;
+  const T* pb = bp + t0 * w.b_stride[2] + cc0;
+  const T* pc = c + t0 * w.c_stride[2] + cc0;
+  const int64_t da = way * w.a_stride[2], db = way * w.b_stride[2], dc = way * w.c_stride[2];
+  uint4 ra[NL], rb[NL], rc[NL];
+  auto fetch = [&](uint4(&reg)[NL], const T* p, int64_t d, int width, int left) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      reg[i] = make_uint4(0, 0, 0, 0);
+      if (row0 + i * kRows < left) {
+        const T* q = p + i * kRows * d;
+        if constexpr (VEC) {
+          if (cc0 < width) reg[i] = *reinterpret_cast<const uint4*>(q);
+        } else {
+          reg[i] = load16(q - cc0, cc0, width, false);
+        }
+      }
+    }
+  };
+  auto fetch_all = [&](int64_t left64) {
+    const int left = left64 < kChunk ? (int)left64 : kChunk;
+    if (MAIN) fetch(ra, pa, da, w.rows, left);
+    fetch(rb, pb, db, w.rows, left);
+    fetch(rc, pc, dc, w.cols, left);
+    pa += kChunk * da;
+    pb += kChunk * db;
+    pc += kChunk * dc;
+  };
+  if (s0 < s1) fetch_all(s1 - s0);
+  if (tid < 2) bad[tid] = 0;
+
+  int turn = 0;
+  for (int64_t p0 = s0; p0 < s1; p0 += kChunk, turn ^= 1) {
+    const int m = (int)(s1 - p0 < kChunk ? s1 - p0 : kChunk);
+    lds_barrier();  // the tiles have been read
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int idx = tid + i * NT, row = idx / CPR;
+      const int at = row * RB + ((idx % CPR ^ row_swizzle<D>(row)) << 4);
+      if (MAIN) *reinterpret_cast<uint4*>(ta + at) = ra[i];
+      *reinterpret_cast<uint4*>(tb + at) = rb[i];
+      *reinterpret_cast<uint4*>(tc + at) = rc[i];
+      if (MAIN) odd = odd || has_non_finite(rc[i]);
+    }
+    if (MAIN && odd) bad[turn] = 1;
+    if (MAIN && tid == 0) bad[turn ^ 1] = 0;
+    if (tid < kChunk) tw[tid] = tid < m ? up * decay_power(l2, (float)(m - 1 - tid + first)) : 0.f;
+    lds_barrier();
+    if (p0 + kChunk < s1) fetch_all(s1 - p0 - kChunk);
+
+    Frag cf[4];
+    if constexpr (MAIN) {
+      // weights: [j][i] accumulators, lane i
+      constexpr int kTiles = (3 + NW - 1) / NW;
+#pragma unroll
+      for (int q = 0; q < kTiles; ++q) {
+        const int tile = wave + q * NW;
+        if (tile < 3) {
+          const int it = tile > 0, jt = tile > 1;
+          f32x16 acc = {};
+#pragma unroll
+          for (int kb = 0; kb < D / 16; ++kb)
+            acc = Elem<T>::mma(rows_frag(tb, jt, kb), rows_frag(ta, it, kb), acc);
+          // (a later token's product may be infinite: masked by selection)
+          const int last = opaque(tile == 1 ? 32 : l);
+          float x[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            x[r] = kappa(g, r) <= last ? acc[r] * pf[NW == 1 && q == 1 ? 1 : 0][r] : 0.f;
+          }
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+            *reinterpret_cast<Frag*>(tp + it * 32 * 128 + (pl ^ ((jt * 4 + kb * 2) << 4))) = pack8<T>(x + 8 * kb);
+        }
+      }
+      // from the state: [value][token] accumulators, lane = token
+      f32x16 o[2] = {};
+#pragma unroll
+      for (int rt = 0; rt < NW; ++rt)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = S[rt][8 * kb + j];
+          const Frag sf = pack8<T>(x);
+#pragma unroll
+          for (int it = 0; it < 2; ++it) o[it] = Elem<T>::mma(sf, rows_frag(ta, it, 2 * rt + kb), o[it]);
+        }
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[it][r] *= fo[it];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) cf[kb] = tr_frag(tc, tr_c, kb, wave);
+      lds_barrier();
+      if (!bad[turn]) {
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll
+          for (int kb = 0; kb < 2 + 2 * it; ++kb) {
+            const Frag pfr = __builtin_bit_cast(
+                Frag, *reinterpret_cast<const uint4*>(tp + it * 32 * 128 + (pl ^ ((kb * 2) << 4))));
+            o[it] = Elem<T>::mma(cf[kb], pfr, o[it]);
+          }
+      } else {
+        // an infinity or NaN among the values: the products that the mask leaves out (0 times it is NaN) must not
+        // be made, so that no token sees a later one's
+        const int l_ = opaque(l), g_ = opaque(g);
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll 1
+          for (int j = 0; j <= 32 * it + l_; ++j) {
+            const int jj = j & 31, r = ((jj >> 3) << 2) | (jj & 3);
+            const int chunk = (j >> 5) * 4 + (r >> 3) * 2 + ((jj >> 2) & 1);
+            const int row = 32 * it + l_;
+            const float p = (float)*reinterpret_cast<const T*>(tp + row * 128 + ((chunk ^ ((l_ >> 1) & 7)) << 4) + (r & 7) * 2);
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+              const int cc = 32 * wave + kappa(g_, q);
+              const float v = (float)*reinterpret_cast<const T*>(tc + j * RB + (((cc >> 3) ^ row_swizzle<D>(j)) << 4) + (cc & 7) * 2);
+              o[it][q] = __builtin_fmaf(p, v, o[it][q]);
+            }
+          }
+      }
+      if (w.out) {
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const bool live = 32 * it + l < m;
+          T* row = static_cast<T*>(w.out) + b * w.out_stride[0] + h * w.out_stride[1] +
+                   token_of(w, live ? p0 + 32 * it + l : p0, n) * w.out_stride[2];
+          if constexpr (VEC) {
+            fast::store_tile<T>(row, 32 * wave, live ? w.cols : 0, g, o[it], 1.f);
+          } else if (live) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int cc = 32 * wave + kappa(g, r);
+              if (cc < w.cols) row[cc] = (T)o[it][r];
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) cf[kb] = tr_frag(tc, tr_c, kb, wave);
+    }
+    // the state's update
+    const float lm = decay_power(l2, (float)m);
+#pragma unroll
+    for (int rt = 0; rt < NW; ++rt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[rt][r] *= lm;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      // tokens 16 kb + kappa(g, 0..7) of this lane's column, decayed, in SPLIT terms
+      const f32x4 w0 = *reinterpret_cast<const f32x4*>(tw + 16 * kb + 4 * g);
+      const f32x4 w1 = *reinterpret_cast<const f32x4*>(tw + 16 * kb + 8 + 4 * g);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = (float)cf[kb][j] * (j < 4 ? w0[j & 3] : w1[j & 3]);
+      Frag part[kSplit];
+#pragma unroll
+      for (int q = 0; q < kSplit; ++q) {
+        part[q] = pack8<T>(x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] -= (float)part[q][j];
+      }
+#pragma unroll
+      for (int rt = 0; rt < NW; ++rt) {
+        const Frag bf = tr_frag(tb, tr_b, kb, rt);
+#pragma unroll
+        for (int q = 0; q < kSplit; ++q) S[rt] = Elem<T>::mma(bf, part[q], S[rt]);
+      }
+    }
+  }
+
+  // rows behind the sequence are zero
+  if (MAIN && w.out) {
+    int64_t e1 = s0 + ca.seg_tokens;
+    if (e1 > w.length || seg == ca.segs - 1) e1 = w.length;
+    T* out = static_cast<T*>(w.out) + b * w.out_stride[0] + h * w.out_stride[1];
+    const int64_t z0 = s0 > n ? s0 : n;
+    for (int64_t i = tid; i < (e1 - z0) * w.cols; i += NT) out[(z0 + i / w.cols) * w.out_stride[2] + i % w.cols] = (T)0.f;
+  }
+  // the state behind the segment, or behind the sequence
+  float* to = nullptr;
+  if (!MAIN) to = ca.starts + (bh * ca.segs + seg) * state_size;
+  else if (w.final_state && (n > 0 ? s0 < n && n <= s0 + ca.seg_tokens : seg == 0)) to = w.final_state + bh * state_size;
+  if (to) {
+    const int g_ = opaque(g), col_ = opaque(col);
+#pragma unroll
+    for (int rt = 0; rt < NW; ++rt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = 32 * rt + 16 * (r >> 3) + 8 * g_ + (r & 7);
+        if (row < w.rows && col_ < w.cols) to[state_at(w, row, col_)] = S[rt][r];
+      }
+  }
+}
+
+// Segments' own states to the states they start from, in place and in order:
+// start_0 = initial, start_(s+1) = l^(tokens of s) start_s + own_s.
+__global__ __launch_bounds__(kThreads) void walk_scan_kernel(ChunkArgs ca) {
+  const LinearWalk& w = ca.w;
+  const int64_t size = (int64_t)w.rows * w.cols;
+  const int64_t bh = blockIdx.y, at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (at >= size) return;
+  const int64_t n = walk_length(w, bh / w.heads);
+  const float l2 = log2_decay(w.log_decay[bh % w.heads]);
+  float* own = ca.starts + bh * ca.segs * size + at;
+  float cur = w.initial ? w.initial[bh * size + at] : 0.f;
+  const float whole = decay_power(l2, (float)ca.seg_tokens);
+  constexpr int U = 8;
+  for (int s0 = 0; s0 < ca.segs; s0 += U) {
+    float x[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) x[i] = s0 + i < ca.segs - 1 ? own[(s0 + i) * size] : 0.f;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (s0 + i >= ca.segs) break;
+      own[(s0 + i) * size] = cur;
+      const int64_t left = n - (int64_t)(s0 + i) * ca.seg_tokens;
+      const float lm = left >= ca.seg_tokens ? whole : left > 0 ? decay_power(l2, (float)left) : 1.f;
+      cur = __builtin_fmaf(cur, lm, x[i]);
     }
   }
 }
@@ -197,9 +580,67 @@ hipError_t by_type(int dtype, F&& f) {
 
 }  // namespace
 
-size_t linear_walk_workspace_bytes(int, const LinearWalk&) { return 0; }
+namespace {
 
-hipError_t launch_linear_walk(int dtype, const LinearWalk& w, void*, hipStream_t stream) {
+// Segments of a walk: enough workgroups for two on each CU, segments of at
+// least kMinSegChunks chunks (a segment's state costs its traffic once more).
+constexpr int64_t kTargetWalks = 512;
+constexpr int64_t kMinSegChunks = 4;
+void plan_segments(const LinearWalk& w, ChunkArgs& ca) {
+  const int64_t chunks = std::max<int64_t>(1, (w.length + kChunk - 1) / kChunk), bh = w.batch * w.heads;
+  int64_t segs = std::min((kTargetWalks + bh - 1) / bh, (chunks + kMinSegChunks - 1) / kMinSegChunks);
+  const int64_t per = (chunks + segs - 1) / segs;
+  ca.segs = (int32_t)((chunks + per - 1) / per);
+  ca.seg_tokens = (int32_t)(per * kChunk);
+}
+
+// 16-byte rows: 8 elements of 16 bits
+bool rows16(const void* p, const int64_t (&stride)[3], int width) {
+  return width % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride[0] % 8 == 0 && stride[1] % 8 == 0 &&
+         stride[2] % 8 == 0;
+}
+
+template <int D, bool VEC>
+hipError_t run_chunks(const ChunkArgs& ca, hipStream_t stream) {
+  const LinearWalk& w = ca.w;
+  const unsigned bh = (unsigned)(w.batch * w.heads);
+  const dim3 grid(bh * (unsigned)ca.segs);
+  if (ca.segs > 1) {
+    hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, false>), grid, dim3(2 * D), 0, stream, ca);
+    hipLaunchKernelGGL(walk_scan_kernel, dim3((unsigned)((w.rows * w.cols + kThreads - 1) / kThreads), bh),
+                       dim3(kThreads), 0, stream, ca);
+  }
+  hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, true>), grid, dim3(2 * D), 0, stream, ca);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t linear_walk_workspace_bytes(int dtype, const LinearWalk& w) {
+  if (dtype != OOPS_BF16 || w.batch == 0) return 0;
+  ChunkArgs ca{};
+  plan_segments(w, ca);
+  if (ca.segs == 1) return 0;
+  return (size_t)(w.batch * w.heads * ca.segs) * (size_t)w.rows * (size_t)w.cols * sizeof(float);
+}
+
+hipError_t launch_linear_walk(int dtype, const LinearWalk& w, void* workspace, hipStream_t stream) {
+  if (dtype == OOPS_BF16) {
+    ChunkArgs ca{};
+    ca.w = w;
+    plan_segments(w, ca);
+    ca.starts = static_cast<float*>(workspace);
+    const bool vec = rows16(w.a, w.a_stride, w.rows) && rows16(w.b, w.b_stride, w.rows) &&
+                     rows16(w.c, w.c_stride, w.cols) && rows16(w.out, w.out_stride, w.cols);
+    const int d = std::max(w.rows, w.cols);
+    auto run = [&](auto size) {
+      constexpr int D = decltype(size)::value;
+      return vec ? run_chunks<D, true>(ca, stream) : run_chunks<D, false>(ca, stream);
+    };
+    if (d <= 32) return run(std::integral_constant<int, 32>{});
+    if (d <= 64) return run(std::integral_constant<int, 64>{});
+    return run(std::integral_constant<int, 128>{});
+  }
   const dim3 grid((unsigned)(w.batch * w.heads), (unsigned)((w.cols + 63) / 64));
   return by_type(dtype, [&](auto tag) {
     using T = decltype(tag);
