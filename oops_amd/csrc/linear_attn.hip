@@ -151,8 +151,10 @@ struct ChunkArgs {
   int32_t seg_tokens;  // a multiple of kChunk
 };
 
-__device__ __forceinline__ int64_t state_at(const LinearWalk& w, int row, int col) {
-  return w.state_by_cols ? (int64_t)col * w.rows + row : (int64_t)row * w.cols + col;
+// byte of a state's element, or an offset past every resource (reads as 0, is not written)
+__device__ __forceinline__ uint32_t state_byte(const LinearWalk& w, int row, int col) {
+  const int rs = w.state_by_cols ? 1 : w.cols, cs = w.state_by_cols ? w.rows : 1;
+  return ((row < w.rows) & (col < w.cols)) ? (uint32_t)(row * rs + col * cs) * 4 : fast::kOut;
 }
 __device__ __forceinline__ int64_t token_of(const LinearWalk& w, int64_t p, int64_t n) {
   return w.from_end && p < n ? n - 1 - p : p;
@@ -165,15 +167,21 @@ __device__ __forceinline__ int row_swizzle(int row) {
   return D == 128 ? row & 15 : D == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
 }
 
-__device__ __forceinline__ bool has_non_finite(uint4 u) {
-  auto bad = [](uint32_t d) { return (d & 0x7F80u) == 0x7F80u || (d & 0x7F800000u) == 0x7F800000u; };
-  return bad(u.x) || bad(u.y) || bad(u.z) || bad(u.w);
+// Bits 15 and 31 of the result are set where a 16-bit half of u has its exponent all ones (an infinity or NaN): the
+// exponent's bits alone, plus its lowest one, carry out of it.
+__device__ __forceinline__ uint32_t non_finite(uint4 u) {
+  constexpr uint32_t kExp = 0x7F807F80u, kOne = 0x00800080u;
+  return ((u.x & kExp) + kOne) | ((u.y & kExp) + kOne) | ((u.z & kExp) + kOne) | ((u.w & kExp) + kOne);
 }
 
-#ifndef OOPS_SPLIT
-#define OOPS_SPLIT 3
-#endif
-constexpr int kSplit = OOPS_SPLIT;
+// eight floats in pairs (one conversion instruction each)
+__device__ __forceinline__ bf16x8 to_bf16x8(const float (&x)[8]) {
+  return __builtin_bit_cast(bf16x8, make_uint4(fast::pack2<__bf16>(x[0], x[1]), fast::pack2<__bf16>(x[2], x[3]),
+                                               fast::pack2<__bf16>(x[4], x[5]), fast::pack2<__bf16>(x[6], x[7])));
+}
+
+constexpr int kSplit = 3;
+
 template <int D, bool VEC, bool MAIN>
 __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(ChunkArgs ca) {
   using T = __bf16;
@@ -184,9 +192,11 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
   __shared__ __align__(16) char tb[kChunk * RB], tc[kChunk * RB], ta[MAIN ? kChunk * RB : 16];
   __shared__ __align__(16) char tp[MAIN ? kChunk * kChunk * 2 : 16];  // weights [token i][token j]
   __shared__ __align__(16) float tw[kChunk];                          // decays of the update
+  __shared__ float td[MAIN ? 2 * kChunk : 1];                         // scale l^(n - 64), 0 before 64
   __shared__ int bad[2];                                              // c holds an infinity or NaN
   const LinearWalk& w = ca.w;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 31, g = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t bh = (int64_t)blockIdx.x / ca.segs;
   const int seg = (int)((int64_t)blockIdx.x % ca.segs);
   if (!MAIN && seg == ca.segs - 1) return;  // (no segment starts from its state)
@@ -210,13 +220,14 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
     const float* from = nullptr;
     if (MAIN) from = ca.segs > 1 ? ca.starts + (bh * ca.segs + seg) * state_size
                                  : w.initial ? w.initial + bh * state_size : nullptr;
+    const auto rsrc = make_rsrc(from, from ? (uint32_t)state_size * 4 : 0u);
 #pragma unroll
     for (int rt = 0; rt < NW; ++rt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = 32 * rt + 16 * (r >> 3) + 8 * g + (r & 7);
-        S[rt][r] = from && row < w.rows && col < w.cols ? from[state_at(w, row, col)] : 0.f;
-      }
+      for (int r = 0; r < 16; ++r)
+        S[rt][r] = __builtin_bit_cast(
+            float, __builtin_amdgcn_raw_buffer_load_b32(
+                       rsrc, state_byte(w, 32 * rt + 16 * (r >> 3) + 8 * g + (r & 7), col), 0, 0));
   }
 
   // lane addresses: rows as they are (16 bytes of row l), and transposed (4 x 4 blocks, see lds_read_tr4)
@@ -241,63 +252,51 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
   };
   const int pl = l * 128 + ((g ^ ((l >> 1) & 7)) << 4);
 
-  // scale l^(i-j) of this wave's weight tiles (it, jt): waves take tiles (0,0), (1,0), (1,1) in turn
-  constexpr int kPf = NW == 1 ? 2 : 1;
-  float pf[kPf][16], fo[2];
+  float fo[2];
   if (MAIN) {
-#pragma unroll
-    for (int q = 0; q < kPf; ++q) {
-      const int off = (NW == 1 ? q == 1 : wave == 1) ? 32 : 0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int lag = off + l - kappa(g, r);
-        pf[q][r] = lag >= 0 ? w.scale * decay_power(l2, (float)lag) : 0.f;
-      }
-    }
+    for (int i = tid; i < 2 * kChunk; i += NT) td[i] = i < kChunk ? 0.f : w.scale * decay_power(l2, (float)(i - kChunk));
 #pragma unroll
     for (int it = 0; it < 2; ++it) fo[it] = so * decay_power(l2, (float)(32 * it + l + 1 - first));
   }
 
-  // this lane's 16 bytes of row row0 (then NT / CPR rows on) of the next chunk
+  // rows row0, row0 + kRows, ..: 16 bytes a lane, zeros behind the segment.  A chunk's resource starts at its lowest
+  // row, whichever way the walk goes.
   constexpr int kRows = NT / CPR;
   const int row0 = tid / CPR, cc0 = tid % CPR * 8;
-  const int64_t way = first ? -1 : 1, t0 = token_of(w, s0, n) + way * row0;
-  const T* pa = a + t0 * w.a_stride[2] + cc0;
-  const T* pb = bp + t0 * w.b_stride[2] + cc0;
-  const T* pc = c + t0 * w.c_stride[2] + cc0;
-  const int64_t da = way * w.a_stride[2], db = way * w.b_stride[2], dc = way * w.c_stride[2];
   uint4 ra[NL], rb[NL], rc[NL];
-  auto fetch = [&](uint4(&reg)[NL], const T* p, int64_t d, int width, int left) {
+  auto fetch = [&](uint4(&reg)[NL], const T* base, int64_t stride, int width, int64_t p0, int left) {
+    if constexpr (VEC) {
+      const T* lowest = base + (first ? n - kChunk - p0 : p0) * stride;
+      const auto rsrc = make_rsrc(lowest, 0x7FFFFFFFu);
+      const int bytes = (int)stride * 2;
+      // (row r of a walk from the end is kChunk - 1 - r rows up: kRows - 1 - row0, and whole steps of kRows)
+      const uint32_t off = cc0 < width ? (uint32_t)((first ? kRows - 1 - row0 : row0) * bytes + cc0 * 2) : fast::kOut;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      reg[i] = make_uint4(0, 0, 0, 0);
-      if (row0 + i * kRows < left) {
-        const T* q = p + i * kRows * d;
-        if constexpr (VEC) {
-          if (cc0 < width) reg[i] = *reinterpret_cast<const uint4*>(q);
-        } else {
-          reg[i] = load16(q - cc0, cc0, width, false);
-        }
+      for (int i = 0; i < NL; ++i)
+        reg[i] = fast::buffer_load16_s(rsrc, row0 + i * kRows < left ? off : fast::kOut,
+                                       (uint32_t)((first ? NL - 1 - i : i) * kRows * bytes));
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int row = row0 + i * kRows;
+        reg[i] = row < left ? load16(base + token_of(w, p0 + row, n) * stride, cc0, width, false) : make_uint4(0, 0, 0, 0);
       }
     }
   };
-  auto fetch_all = [&](int64_t left64) {
-    const int left = left64 < kChunk ? (int)left64 : kChunk;
-    if (MAIN) fetch(ra, pa, da, w.rows, left);
-    fetch(rb, pb, db, w.rows, left);
-    fetch(rc, pc, dc, w.cols, left);
-    pa += kChunk * da;
-    pb += kChunk * db;
-    pc += kChunk * dc;
+  auto fetch_all = [&](int64_t p0) {
+    const int left = s1 - p0 < kChunk ? (int)(s1 - p0) : kChunk;
+    if (MAIN) fetch(ra, a, w.a_stride[2], w.rows, p0, left);
+    fetch(rb, bp, w.b_stride[2], w.rows, p0, left);
+    fetch(rc, c, w.c_stride[2], w.cols, p0, left);
   };
-  if (s0 < s1) fetch_all(s1 - s0);
+  if (s0 < s1) fetch_all(s0);
   if (tid < 2) bad[tid] = 0;
 
   int turn = 0;
   for (int64_t p0 = s0; p0 < s1; p0 += kChunk, turn ^= 1) {
     const int m = (int)(s1 - p0 < kChunk ? s1 - p0 : kChunk);
     lds_barrier();  // the tiles have been read
-    bool odd = false;
+    uint32_t odd = 0;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int idx = tid + i * NT, row = idx / CPR;
@@ -305,17 +304,17 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
       if (MAIN) *reinterpret_cast<uint4*>(ta + at) = ra[i];
       *reinterpret_cast<uint4*>(tb + at) = rb[i];
       *reinterpret_cast<uint4*>(tc + at) = rc[i];
-      if (MAIN) odd = odd || has_non_finite(rc[i]);
+      if (MAIN) odd |= non_finite(rc[i]);
     }
-    if (MAIN && odd) bad[turn] = 1;
+    if (MAIN && (odd & 0x80008000u)) bad[turn] = 1;
     if (MAIN && tid == 0) bad[turn ^ 1] = 0;
     if (tid < kChunk) tw[tid] = tid < m ? up * decay_power(l2, (float)(m - 1 - tid + first)) : 0.f;
     lds_barrier();
-    if (p0 + kChunk < s1) fetch_all(s1 - p0 - kChunk);
+    if (p0 + kChunk < s1) fetch_all(p0 + kChunk);
 
     Frag cf[4];
     if constexpr (MAIN) {
-      // weights: [j][i] accumulators, lane i
+      // weights: [j][i] accumulators, lane i; waves take the tiles (0,0), (1,0), (1,1) in turn
       constexpr int kTiles = (3 + NW - 1) / NW;
 #pragma unroll
       for (int q = 0; q < kTiles; ++q) {
@@ -326,18 +325,21 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
 #pragma unroll
           for (int kb = 0; kb < D / 16; ++kb)
             acc = Elem<T>::mma(rows_frag(tb, jt, kb), rows_frag(ta, it, kb), acc);
-          // (a later token's product may be infinite: masked by selection)
-          const int last = opaque(tile == 1 ? 32 : l);
-          float x[16];
+          // (a later token's product may be infinite: masked by its bits)
+          const int last = opaque(32 * (it - jt) + l);
+          const float* f = td + (kChunk + last) - 4 * g;
+          float x[2][8];
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            x[r] = kappa(g, r) <= last ? acc[r] * pf[NW == 1 && q == 1 ? 1 : 0][r] : 0.f;
+            const int later = (last - 4 * g - kappa(0, r)) >> 31;  // all ones where j > i
+            x[r / 8][r % 8] = __builtin_bit_cast(float, __builtin_bit_cast(int, acc[r] * f[-kappa(0, r)]) & ~later);
           }
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
-            *reinterpret_cast<Frag*>(tp + it * 32 * 128 + (pl ^ ((jt * 4 + kb * 2) << 4))) = pack8<T>(x + 8 * kb);
+            *reinterpret_cast<Frag*>(tp + it * 32 * 128 + (pl ^ ((jt * 4 + kb * 2) << 4))) = to_bf16x8(x[kb]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);  // (the products' operands are not all held at once)
       // from the state: [value][token] accumulators, lane = token
       f32x16 o[2] = {};
 #pragma unroll
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
           float x[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = S[rt][8 * kb + j];
-          const Frag sf = pack8<T>(x);
+          const Frag sf = to_bf16x8(x);
 #pragma unroll
           for (int it = 0; it < 2; ++it) o[it] = Elem<T>::mma(sf, rows_frag(ta, it, 2 * rt + kb), o[it]);
         }
@@ -388,18 +390,30 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
           }
       }
       if (w.out) {
+        T* base = static_cast<T*>(w.out) + b * w.out_stride[0] + h * w.out_stride[1];
+        if constexpr (VEC) {
+          const auto rsrc = make_rsrc(base + (first ? n - kChunk - p0 : p0) * w.out_stride[2], 0x7FFFFFFFu);
 #pragma unroll
-        for (int it = 0; it < 2; ++it) {
-          const bool live = 32 * it + l < m;
-          T* row = static_cast<T*>(w.out) + b * w.out_stride[0] + h * w.out_stride[1] +
-                   token_of(w, live ? p0 + 32 * it + l : p0, n) * w.out_stride[2];
-          if constexpr (VEC) {
-            fast::store_tile<T>(row, 32 * wave, live ? w.cols : 0, g, o[it], 1.f);
-          } else if (live) {
+          for (int it = 0; it < 2; ++it) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) pk[q] = fast::pack2<T>(o[it][2 * q], o[it][2 * q + 1]);
+            uint4 lo, hi;
+            fast::trade16(pk, lo, hi);  // this lane: its token's columns cc .. cc+7 and cc+8 .. cc+15
+            const int i = 32 * it + l, cc = 32 * wave + 16 * g;
+            const uint32_t at = (uint32_t)((first ? kChunk - 1 - i : i) * (int)w.out_stride[2] + cc) * 2;
+            buffer_store16(rsrc, i < m && cc < w.cols ? at : fast::kOut, lo);
+            buffer_store16(rsrc, i < m && cc + 8 < w.cols ? at + 16 : fast::kOut, hi);
+          }
+        } else {
+#pragma unroll
+          for (int it = 0; it < 2; ++it) {
+            const int i = 32 * it + l;
+            T* row = base + token_of(w, i < m ? p0 + i : p0, n) * w.out_stride[2];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int cc = 32 * wave + kappa(g, r);
-              if (cc < w.cols) row[cc] = (T)o[it][r];
+              if (i < m && cc < w.cols) row[cc] = (T)o[it][r];
             }
           }
         }
@@ -408,6 +422,7 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) cf[kb] = tr_frag(tc, tr_c, kb, wave);
     }
+    __builtin_amdgcn_sched_barrier(0);
     // the state's update
     const float lm = decay_power(l2, (float)m);
 #pragma unroll
@@ -425,7 +440,7 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
       Frag part[kSplit];
 #pragma unroll
       for (int q = 0; q < kSplit; ++q) {
-        part[q] = pack8<T>(x);
+        part[q] = to_bf16x8(x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] -= (float)part[q][j];
       }
@@ -452,13 +467,12 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
   else if (w.final_state && (n > 0 ? s0 < n && n <= s0 + ca.seg_tokens : seg == 0)) to = w.final_state + bh * state_size;
   if (to) {
     const int g_ = opaque(g), col_ = opaque(col);
+    const auto rsrc = make_rsrc(to, (uint32_t)state_size * 4);
 #pragma unroll
     for (int rt = 0; rt < NW; ++rt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = 32 * rt + 16 * (r >> 3) + 8 * g_ + (r & 7);
-        if (row < w.rows && col_ < w.cols) to[state_at(w, row, col_)] = S[rt][r];
-      }
+      for (int r = 0; r < 16; ++r)
+        buffer_store4(rsrc, state_byte(w, 32 * rt + 16 * (r >> 3) + 8 * g_ + (r & 7), col_), S[rt][r]);
   }
 }
 
@@ -594,9 +608,9 @@ void plan_segments(const LinearWalk& w, ChunkArgs& ca) {
   ca.seg_tokens = (int32_t)(per * kChunk);
 }
 
-// 16-byte rows: 8 elements of 16 bits
+// 16-byte rows (8 elements of 16 bits) whose chunks span less than 2 GiB
 bool rows16(const void* p, const int64_t (&stride)[3], int width) {
-  return width % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride[0] % 8 == 0 && stride[1] % 8 == 0 &&
+  return width % 8 == 0 && stride[2] < (int64_t(1) << 31) / (2 * kChunk) - 128 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride[0] % 8 == 0 && stride[1] % 8 == 0 &&
          stride[2] % 8 == 0;
 }
 
