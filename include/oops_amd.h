@@ -521,12 +521,14 @@ size_t oops_linear_attn_forward_workspace_bytes(const oops_linear_attn_geometry*
 int oops_linear_attn_forward(const oops_linear_attn_geometry* geo, const void* q, const void* k, const void* v,
                              const float* log_decay, const void* lengths, const float* initial, void* out,
                              float* final_state, void* workspace, size_t ws_bytes, void* stream);
-/* grad_final may be NULL (zeros); every gradient may be NULL (not wanted). */
+/* forward_workspace: the workspace as the forward of the same operands left it, or NULL (what it holds is made
+ * again).  grad_final may be NULL (zeros); every gradient may be NULL (not wanted). */
 size_t oops_linear_attn_backward_workspace_bytes(const oops_linear_attn_geometry* geo);
 int oops_linear_attn_backward(const oops_linear_attn_geometry* geo, const void* q, const void* k, const void* v,
-                              const float* log_decay, const void* lengths, const float* initial, const void* grad_out,
-                              const float* grad_final, void* grad_q, void* grad_k, void* grad_v, float* grad_initial,
-                              void* workspace, size_t ws_bytes, void* stream);
+                              const float* log_decay, const void* lengths, const float* initial,
+                              const void* forward_workspace, const void* grad_out, const float* grad_final,
+                              void* grad_q, void* grad_k, void* grad_v, float* grad_initial, void* workspace,
+                              size_t ws_bytes, void* stream);
 /* One token of every (batch, head): state is updated in place, then o = scale q state (length 1; token strides are
  * not read). */
 int oops_linear_attn_step(const oops_linear_attn_geometry* geo, const void* q, const void* k, const void* v,

@@ -335,7 +335,7 @@ def load() -> ctypes.CDLL:
         lib.oops_int8_linear.argtypes = [ig, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         lib.oops_int8_linear.restype = i32
         lg = ctypes.POINTER(LinearAttnGeometry)
-        for name, count in (("forward", 8), ("backward", 12)):
+        for name, count in (("forward", 8), ("backward", 13)):
             size = getattr(lib, f"oops_linear_attn_{name}_workspace_bytes")
             size.argtypes, size.restype = [lg], sz
             call = getattr(lib, f"oops_linear_attn_{name}")

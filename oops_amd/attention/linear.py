@@ -231,6 +231,12 @@ def _is_i64(lengths: Optional[Tensor]) -> bool:
 
 def _forward_impl(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, lengths: Optional[Tensor],
                   initial: Optional[Tensor], scale: float, return_state: bool) -> Tuple[Tensor, Tensor]:  # fmt: skip
+    return _forward_with_workspace(q, k, v, log_decay, lengths, initial, scale, return_state)[:2]
+
+
+def _forward_with_workspace(q, k, v, log_decay, lengths, initial, scale, return_state):
+    """(out, state or empty, the workspace: the states that the sequence's segments start from, or None)."""
+
     lib = _lib.load()
     b, h, _, d = q.shape
     e = v.shape[-1]
@@ -244,12 +250,12 @@ def _forward_impl(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, lengths: O
             _ptr(state), _ptr(ws), ws_bytes, _stream(q.device),
         )
     _lib.check(rc, "linear attention forward")
-    return out, state
+    return out, state, ws
 
 
 def _backward_impl(dout: Tensor, dstate: Optional[Tensor], q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor,
-                   lengths: Optional[Tensor], initial: Optional[Tensor], scale: float,
-                   needs: List[bool]) -> Tuple[Tensor, Tensor, Tensor, Tensor]:  # fmt: skip
+                   lengths: Optional[Tensor], initial: Optional[Tensor], scale: float, needs: List[bool],
+                   forward_ws: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor, Tensor]:  # fmt: skip
     """(dq, dk, dv, dinitial), empty where not wanted."""
 
     lib = _lib.load()
@@ -265,8 +271,8 @@ def _backward_impl(dout: Tensor, dstate: Optional[Tensor], q: Tensor, k: Tensor,
     ws = _workspace(ws_bytes, q.device)
     with _on_device(q.device):
         rc = lib.oops_linear_attn_backward(
-            ctypes.byref(geo), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(lengths), _ptr(initial), _ptr(dout),
-            _ptr(dstate), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ds), _ptr(ws), ws_bytes, _stream(q.device),
+            ctypes.byref(geo), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(lengths), _ptr(initial),
+            _ptr(forward_ws), _ptr(dout), _ptr(dstate), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ds), _ptr(ws), ws_bytes, _stream(q.device),
         )
     _lib.check(rc, "linear attention backward")
     return dq, dk, dv, ds
@@ -330,8 +336,8 @@ def _(q, k, v, log_decay, state, scale):
 # ----------------------------------------------------------------- autograd
 
 
-def _save(ctx, q, k, v, log_decay, lengths, initial, scale, state):
-    ctx.save_for_backward(q, k, v, log_decay, lengths, initial)
+def _save(ctx, q, k, v, log_decay, lengths, initial, scale, state, ws=None):
+    ctx.save_for_backward(q, k, v, log_decay, lengths, initial, ws)
     ctx.scale = scale
     ctx.set_materialize_grads(False)
     if not state.numel():
@@ -341,12 +347,13 @@ def _save(ctx, q, k, v, log_decay, lengths, initial, scale, state):
 def _grads(ctx, dout, dstate, backward):
     """Gradients of (q, k, v, log_decay, lengths, initial, scale, return_state)."""
 
-    q, k, v, log_decay, lengths, initial = ctx.saved_tensors
+    q, k, v, log_decay, lengths, initial, ws = ctx.saved_tensors
     needs = [bool(n) for n in (*ctx.needs_input_grad[:3], ctx.needs_input_grad[5])]
     if dout is None:  # only the state was used
         dout = v.new_zeros(1).expand(*q.shape[:3], v.shape[-1])
         dout = dout.contiguous() if v.shape[-1] > 1 else dout
-    dq, dk, dv, ds = backward(dout, dstate, q, k, v, log_decay, lengths, initial, ctx.scale, needs)
+    args = (dout, dstate, q, k, v, log_decay, lengths, initial, ctx.scale, needs)
+    dq, dk, dv, ds = backward(*args) if ws is None else backward(*args, ws)
     keep = lambda g, need: g if need else None  # noqa: E731
     return (keep(dq, needs[0]), keep(dk, needs[1]), keep(dv, needs[2]), None, None,
             keep(ds, needs[3] and initial is not None), None, None)  # fmt: skip
@@ -372,8 +379,8 @@ class _EagerLinearAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, lengths, initial, scale, return_state):
-        out, state = _forward_impl(q, k, v, log_decay, lengths, initial, scale, return_state)
-        _save(ctx, q, k, v, log_decay, lengths, initial, scale, state)
+        out, state, ws = _forward_with_workspace(q, k, v, log_decay, lengths, initial, scale, return_state)
+        _save(ctx, q, k, v, log_decay, lengths, initial, scale, state, ws)
         return out, state
 
     @staticmethod

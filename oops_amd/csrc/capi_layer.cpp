@@ -228,28 +228,23 @@ int oops_linear_attn_forward(const oops_linear_attn_geometry* geo, const void* q
   if (!log_decay || (geo->length > 0 && (!q || !k || !v || !out)))
     return report(OOPS_EINVAL, "q, k, v, log_decay and out must be non-NULL");
   if (int rc = oops::report_workspace(workspace, ws_bytes, oops_linear_attn_forward_workspace_bytes(geo))) return rc;
-  return report_launch(
-      oops::launch_linear_walk(geo->dtype, walk_out(*geo, q, k, v, out, log_decay, lengths, initial, final_state),
-                               workspace, static_cast<hipStream_t>(stream)),
-      "linear attention forward");
+  const oops::LinearWalk w = walk_out(*geo, q, k, v, out, log_decay, lengths, initial, final_state);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e = oops::launch_linear_walk_starts(geo->dtype, w, workspace, st);
+  if (e == hipSuccess) e = oops::launch_linear_walk(geo->dtype, w, workspace, st);
+  return report_launch(e, "linear attention forward");
 }
 
 size_t oops_linear_attn_backward_workspace_bytes(const oops_linear_attn_geometry* geo) {
-  oops::clear_report();
-  if (check_linear(geo)) return 0;
-  float state;
-  const GradWalks w = grad_walks(*geo, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr,
-                                 nullptr, nullptr, &state);
-  // (the walks run one after the other and share the workspace)
-  return std::max({oops::linear_walk_workspace_bytes(geo->dtype, w.dq),
-                   oops::linear_walk_workspace_bytes(geo->dtype, w.dk),
-                   oops::linear_walk_workspace_bytes(geo->dtype, w.dv)});
+  // (the walks from the start, then those from the end, keep their segments' states there)
+  return oops_linear_attn_forward_workspace_bytes(geo);
 }
 
 int oops_linear_attn_backward(const oops_linear_attn_geometry* geo, const void* q, const void* k, const void* v,
-                              const float* log_decay, const void* lengths, const float* initial, const void* grad_out,
-                              const float* grad_final, void* grad_q, void* grad_k, void* grad_v, float* grad_initial,
-                              void* workspace, size_t ws_bytes, void* stream) {
+                              const float* log_decay, const void* lengths, const float* initial,
+                              const void* forward_workspace, const void* grad_out, const float* grad_final,
+                              void* grad_q, void* grad_k, void* grad_v, float* grad_initial, void* workspace,
+                              size_t ws_bytes, void* stream) {
   oops::clear_report();
   if (int rc = check_linear(geo)) return rc;
   if (geo->batch == 0) return OOPS_OK;
@@ -260,9 +255,17 @@ int oops_linear_attn_backward(const oops_linear_attn_geometry* geo, const void* 
                                  grad_v, grad_initial);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e = hipSuccess;
-  if (grad_q) e = oops::launch_linear_walk(geo->dtype, w.dq, workspace, st);
+  if (grad_q) {
+    if (!forward_workspace)
+      e = oops::launch_linear_walk_starts(
+          geo->dtype, walk_out(*geo, q, k, v, nullptr, log_decay, lengths, initial, nullptr), workspace, st);
+    if (e == hipSuccess)
+      e = oops::launch_linear_walk(geo->dtype, w.dq, forward_workspace ? forward_workspace : workspace, st);
+  }
+  const bool dv = grad_v || grad_initial;
+  if (e == hipSuccess && (grad_k || dv)) e = oops::launch_linear_walk_starts(geo->dtype, w.dv, workspace, st);
   if (e == hipSuccess && grad_k) e = oops::launch_linear_walk(geo->dtype, w.dk, workspace, st);
-  if (e == hipSuccess && (grad_v || grad_initial)) e = oops::launch_linear_walk(geo->dtype, w.dv, workspace, st);
+  if (e == hipSuccess && dv) e = oops::launch_linear_walk(geo->dtype, w.dv, workspace, st);
   return report_launch(e, "linear attention backward");
 }
 

@@ -141,7 +141,8 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(LinearWalk w) {
 // where they are read by the second products, once each (different terms of
 // the output, 2^-8 of each at most, as in softmax attention).  The update's
 // operand u l^n c is split into three bfloat16 terms, which hold its float32
-// value: the state that is returned is a float32 one.
+// value: the state that is returned is a float32 one.  Segments whose state
+// goes no further than their own outputs take two terms (2^-16).
 constexpr int kChunk = 64;
 
 struct ChunkArgs {
@@ -179,8 +180,6 @@ __device__ __forceinline__ bf16x8 to_bf16x8(const float (&x)[8]) {
   return __builtin_bit_cast(bf16x8, make_uint4(fast::pack2<__bf16>(x[0], x[1]), fast::pack2<__bf16>(x[2], x[3]),
                                                fast::pack2<__bf16>(x[4], x[5]), fast::pack2<__bf16>(x[6], x[7])));
 }
-
-constexpr int kSplit = 3;
 
 template <int D, bool VEC, bool MAIN>
 __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(ChunkArgs ca) {
@@ -229,6 +228,8 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
             float, __builtin_amdgcn_raw_buffer_load_b32(
                        rsrc, state_byte(w, 32 * rt + 16 * (r >> 3) + 8 * g + (r & 7), col), 0, 0));
   }
+
+  const bool kept = !MAIN || (s0 < n && n <= s0 + ca.seg_tokens);  // the state behind this segment is read again
 
   // lane addresses: rows as they are (16 bytes of row l), and transposed (4 x 4 blocks, see lds_read_tr4)
   const int nat = l * RB + ((g ^ row_swizzle<D>(l)) << 4);
@@ -437,10 +438,12 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = (float)cf[kb][j] * (j < 4 ? w0[j & 3] : w1[j & 3]);
-      Frag part[kSplit];
+      Frag part[3];
 #pragma unroll
-      for (int q = 0; q < kSplit; ++q) {
+      for (int q = 0; q < 3; ++q) {
+        if (q == 2 && !kept) break;
         part[q] = to_bf16x8(x);
+        if (q == 2) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] -= (float)part[q][j];
       }
@@ -448,7 +451,8 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
       for (int rt = 0; rt < NW; ++rt) {
         const Frag bf = tr_frag(tb, tr_b, kb, rt);
 #pragma unroll
-        for (int q = 0; q < kSplit; ++q) S[rt] = Elem<T>::mma(bf, part[q], S[rt]);
+        for (int q = 0; q < 2; ++q) S[rt] = Elem<T>::mma(bf, part[q], S[rt]);
+        if (kept) S[rt] = Elem<T>::mma(bf, part[2], S[rt]);
       }
     }
   }
@@ -615,46 +619,40 @@ bool rows16(const void* p, const int64_t (&stride)[3], int width) {
 }
 
 template <int D, bool VEC>
-hipError_t run_chunks(const ChunkArgs& ca, hipStream_t stream) {
+hipError_t run_chunks(const ChunkArgs& ca, bool starts, hipStream_t stream) {
   const LinearWalk& w = ca.w;
   const unsigned bh = (unsigned)(w.batch * w.heads);
   const dim3 grid(bh * (unsigned)ca.segs);
-  if (ca.segs > 1) {
+  if (starts) {
     hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, false>), grid, dim3(2 * D), 0, stream, ca);
     hipLaunchKernelGGL(walk_scan_kernel, dim3((unsigned)((w.rows * w.cols + kThreads - 1) / kThreads), bh),
                        dim3(kThreads), 0, stream, ca);
+  } else {
+    hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, true>), grid, dim3(2 * D), 0, stream, ca);
   }
-  hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, true>), grid, dim3(2 * D), 0, stream, ca);
   return hipGetLastError();
 }
 
-}  // namespace
-
-size_t linear_walk_workspace_bytes(int dtype, const LinearWalk& w) {
-  if (dtype != OOPS_BF16 || w.batch == 0) return 0;
-  ChunkArgs ca{};
-  plan_segments(w, ca);
-  if (ca.segs == 1) return 0;
-  return (size_t)(w.batch * w.heads * ca.segs) * (size_t)w.rows * (size_t)w.cols * sizeof(float);
-}
-
-hipError_t launch_linear_walk(int dtype, const LinearWalk& w, void* workspace, hipStream_t stream) {
+// The walk itself (with the states its segments start from in the workspace), or those states.
+hipError_t run_walk(int dtype, const LinearWalk& w, void* workspace, bool starts, hipStream_t stream) {
   if (dtype == OOPS_BF16) {
     ChunkArgs ca{};
     ca.w = w;
     plan_segments(w, ca);
     ca.starts = static_cast<float*>(workspace);
-    const bool vec = rows16(w.a, w.a_stride, w.rows) && rows16(w.b, w.b_stride, w.rows) &&
-                     rows16(w.c, w.c_stride, w.cols) && rows16(w.out, w.out_stride, w.cols);
+    if (starts && ca.segs == 1) return hipSuccess;
+    const bool vec = (starts || (rows16(w.a, w.a_stride, w.rows) && rows16(w.out, w.out_stride, w.cols))) &&
+                     rows16(w.b, w.b_stride, w.rows) && rows16(w.c, w.c_stride, w.cols);
     const int d = std::max(w.rows, w.cols);
     auto run = [&](auto size) {
       constexpr int D = decltype(size)::value;
-      return vec ? run_chunks<D, true>(ca, stream) : run_chunks<D, false>(ca, stream);
+      return vec ? run_chunks<D, true>(ca, starts, stream) : run_chunks<D, false>(ca, starts, stream);
     };
     if (d <= 32) return run(std::integral_constant<int, 32>{});
     if (d <= 64) return run(std::integral_constant<int, 64>{});
     return run(std::integral_constant<int, 128>{});
   }
+  if (starts) return hipSuccess;
   const dim3 grid((unsigned)(w.batch * w.heads), (unsigned)((w.cols + 63) / 64));
   return by_type(dtype, [&](auto tag) {
     using T = decltype(tag);
@@ -666,6 +664,22 @@ hipError_t launch_linear_walk(int dtype, const LinearWalk& w, void* workspace, h
       hipLaunchKernelGGL((walk_kernel<T, 128>), grid, dim3(kThreads), 0, stream, w);
     return hipGetLastError();
   });
+}
+
+}  // namespace
+
+size_t linear_walk_workspace_bytes(int dtype, const LinearWalk& w) {
+  if (dtype != OOPS_BF16 || w.batch == 0) return 0;
+  ChunkArgs ca{};
+  plan_segments(w, ca);
+  if (ca.segs == 1) return 0;
+  return (size_t)(w.batch * w.heads * ca.segs) * (size_t)w.rows * (size_t)w.cols * sizeof(float);
+}
+hipError_t launch_linear_walk_starts(int dtype, const LinearWalk& w, void* workspace, hipStream_t stream) {
+  return run_walk(dtype, w, workspace, true, stream);
+}
+hipError_t launch_linear_walk(int dtype, const LinearWalk& w, const void* workspace, hipStream_t stream) {
+  return run_walk(dtype, w, const_cast<void*>(workspace), false, stream);
 }
 
 hipError_t launch_linear_attn_step(const oops_linear_attn_geometry& g, const void* q, const void* k, const void* v,

@@ -129,6 +129,6 @@ def test_linear_attention_entry_points(lib):
     _refused(lib, forward(geo(), ld=None), 1, "non-NULL")
     assert forward(geo(batch=0)) == 0
     g = ctypes.byref(geo())
-    _refused(lib, lib.oops_linear_attn_backward(g, FAKE, FAKE, FAKE, FAKE, None, None, None, None, FAKE, None, None, None,
-                                                None, 0, None), 1, "grad_out")  # fmt: skip
+    _refused(lib, lib.oops_linear_attn_backward(g, FAKE, FAKE, FAKE, FAKE, None, None, None, None, None, FAKE, None, None,
+                                                None, None, 0, None), 1, "grad_out")  # fmt: skip
     _refused(lib, lib.oops_linear_attn_step(g, FAKE, FAKE, FAKE, FAKE, None, FAKE, None), 1, "non-NULL")
