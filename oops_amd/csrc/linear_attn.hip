@@ -7,10 +7,6 @@
 //   o  = walk(q, k, v)       dq = walk(do, v, k) on the transposed state
 //   dk = walk(v, do, q) and dv = walk(k, q, do) from the end, where the state
 //   R_t = l R_(t+1) + scale q_t^T do_t is the gradient of S_t.
-//
-// walk_kernel is the recurrence itself: a workgroup holds a (batch, head)'s
-// state for 64 columns in registers, a quarter of the rows each wave, and goes
-// token by token through chunks staged in LDS.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -42,81 +38,6 @@ __device__ __forceinline__ int opaque(int x) {
   return x;
 }
 
-constexpr int kTok = 16;  // tokens of a chunk
-
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void walk_kernel(LinearWalk w) {
-  constexpr int DG = DP / 4;  // state rows of a wave
-  __shared__ float sa[kTok][DP], sb[kTok][DP], sc[kTok][64], red[4][kTok][64];
-  const int64_t bh = blockIdx.x;
-  const int64_t b = bh / w.heads;
-  const int h = (int)(bh % w.heads);
-  const int col = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const int e = blockIdx.y * 64 + col;
-  const int64_t n = walk_length(w, b);
-  const float decay = decay_power(log2_decay(w.log_decay[h]), 1.f);
-  const T* a = static_cast<const T*>(w.a) + b * w.a_stride[0] + h * w.a_stride[1];
-  const T* bb = static_cast<const T*>(w.b) + b * w.b_stride[0] + h * w.b_stride[1];
-  const T* c = static_cast<const T*>(w.c) + b * w.c_stride[0] + h * w.c_stride[1];
-  T* out = static_cast<T*>(w.out);
-  if (out) out += b * w.out_stride[0] + h * w.out_stride[1];
-  const int64_t state0 = bh * w.rows * w.cols;
-  float s[DG];
-#pragma unroll
-  for (int i = 0; i < DG; ++i) {
-    const int d = g * DG + i;
-    const int64_t at = state0 + (w.state_by_cols ? (int64_t)e * w.rows + d : (int64_t)d * w.cols + e);
-    s[i] = w.initial && d < w.rows && e < w.cols ? w.initial[at] : 0.f;
-  }
-  const float up = w.from_end ? w.scale : 1.f, os = w.from_end ? 1.f : w.scale;
-  for (int64_t p0 = 0; p0 < n; p0 += kTok) {
-    const int m = (int)(n - p0 < kTok ? n - p0 : kTok);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTok * DP; i += kThreads) {
-      const int t = i / DP, d = i % DP;
-      const int64_t tok = w.from_end ? n - 1 - p0 - t : p0 + t;
-      const bool in = t < m && d < w.rows;
-      sa[t][d] = in ? (float)a[tok * w.a_stride[2] + d] : 0.f;
-      sb[t][d] = in ? (float)bb[tok * w.b_stride[2] + d] : 0.f;
-    }
-    for (int i = threadIdx.x; i < kTok * 64; i += kThreads) {
-      const int t = i / 64, d = blockIdx.y * 64 + i % 64;
-      const int64_t tok = w.from_end ? n - 1 - p0 - t : p0 + t;
-      sc[t][i % 64] = t < m && d < w.cols ? (float)c[tok * w.c_stride[2] + d] * up : 0.f;
-    }
-    __syncthreads();
-    for (int t = 0; t < m; ++t) {
-      const float l = w.from_end && p0 + t == 0 ? 1.f : decay;
-      const float cv = sc[t][col];
-      float o = 0.f;
-#pragma unroll
-      for (int i = 0; i < DG; ++i) {
-        s[i] = __builtin_fmaf(sb[t][g * DG + i], cv, s[i] * l);
-        o = __builtin_fmaf(sa[t][g * DG + i], s[i], o);
-      }
-      red[g][t][col] = o;
-    }
-    __syncthreads();
-    if (out)
-      for (int t = g; t < m; t += 4) {
-        const int64_t tok = w.from_end ? n - 1 - p0 - t : p0 + t;
-        const float o = (red[0][t][col] + red[1][t][col]) + (red[2][t][col] + red[3][t][col]);
-        if (e < w.cols) out[tok * w.out_stride[2] + e] = (T)(o * os);
-      }
-  }
-  if (out && e < w.cols)
-    for (int64_t t = n + g; t < w.length; t += 4) out[t * w.out_stride[2] + e] = (T)0.f;
-  if (w.final_state) {
-    const float l = w.from_end && n > 0 ? decay : 1.f;
-#pragma unroll
-    for (int i = 0; i < DG; ++i) {
-      const int d = g * DG + i;
-      const int64_t at = state0 + (w.state_by_cols ? (int64_t)e * w.rows + d : (int64_t)d * w.cols + e);
-      if (d < w.rows && e < w.cols) w.final_state[at] = s[i] * l;
-    }
-  }
-}
-
 // ---------------------------------------------------------------- bfloat16, in chunks
 //
 // With the state kept one decay ahead in walks from the end (first = 1, else
@@ -141,8 +62,7 @@ __global__ __launch_bounds__(kThreads) void walk_kernel(LinearWalk w) {
 // where they are read by the second products, once each (different terms of
 // the output, 2^-8 of each at most, as in softmax attention).  The update's
 // operand u l^n c is split into three bfloat16 terms, which hold its float32
-// value: the state that is returned is a float32 one.  Segments whose state
-// goes no further than their own outputs take two terms (2^-16).
+// value: the state that is returned is a float32 one.
 constexpr int kChunk = 64;
 
 struct ChunkArgs {
@@ -180,6 +100,8 @@ __device__ __forceinline__ bf16x8 to_bf16x8(const float (&x)[8]) {
   return __builtin_bit_cast(bf16x8, make_uint4(fast::pack2<__bf16>(x[0], x[1]), fast::pack2<__bf16>(x[2], x[3]),
                                                fast::pack2<__bf16>(x[4], x[5]), fast::pack2<__bf16>(x[6], x[7])));
 }
+
+constexpr int kTerms = 3;
 
 template <int D, bool VEC, bool MAIN>
 __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(ChunkArgs ca) {
@@ -228,8 +150,6 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
             float, __builtin_amdgcn_raw_buffer_load_b32(
                        rsrc, state_byte(w, 32 * rt + 16 * (r >> 3) + 8 * g + (r & 7), col), 0, 0));
   }
-
-  const bool kept = !MAIN || (s0 < n && n <= s0 + ca.seg_tokens);  // the state behind this segment is read again
 
   // lane addresses: rows as they are (16 bytes of row l), and transposed (4 x 4 blocks, see lds_read_tr4)
   const int nat = l * RB + ((g ^ row_swizzle<D>(l)) << 4);
@@ -432,18 +352,16 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
       for (int r = 0; r < 16; ++r) S[rt][r] *= lm;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
-      // tokens 16 kb + kappa(g, 0..7) of this lane's column, decayed, in SPLIT terms
+      // tokens 16 kb + kappa(g, 0..7) of this lane's column, decayed, in kTerms terms
       const f32x4 w0 = *reinterpret_cast<const f32x4*>(tw + 16 * kb + 4 * g);
       const f32x4 w1 = *reinterpret_cast<const f32x4*>(tw + 16 * kb + 8 + 4 * g);
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = (float)cf[kb][j] * (j < 4 ? w0[j & 3] : w1[j & 3]);
-      Frag part[3];
+      Frag part[kTerms];
 #pragma unroll
-      for (int q = 0; q < 3; ++q) {
-        if (q == 2 && !kept) break;
+      for (int q = 0; q < kTerms; ++q) {
         part[q] = to_bf16x8(x);
-        if (q == 2) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] -= (float)part[q][j];
       }
@@ -451,8 +369,7 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
       for (int rt = 0; rt < NW; ++rt) {
         const Frag bf = tr_frag(tb, tr_b, kb, rt);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) S[rt] = Elem<T>::mma(bf, part[q], S[rt]);
-        if (kept) S[rt] = Elem<T>::mma(bf, part[2], S[rt]);
+        for (int q = 0; q < kTerms; ++q) S[rt] = Elem<T>::mma(bf, part[q], S[rt]);
       }
     }
   }
@@ -477,6 +394,208 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         buffer_store4(rsrc, state_byte(w, 32 * rt + 16 * (r >> 3) + 8 * g_ + (r & 7), col_), S[rt][r]);
+  }
+}
+
+// ---------------------------------------------------------------- float32 and float16, in chunks
+//
+// The same chunks on the float32 matrix units (32x32x2 MFMA, products and
+// sums in float32), float16 operands widened on their way into LDS: the
+// unnormalised weights and states of linear attention pass float16's range
+// where its outputs do not.  Chunks of 32 tokens: a wave makes the whole
+// 32 x 32 weight tile for its 32 columns itself and keeps it in registers (an
+// accumulator register is the next MFMA's k-operand as it is), so there is no
+// exchange between waves: 13% more products than sharing 64-token tiles, no
+// barrier between them.  Bound by the float32 MFMA rate (a sixteenth of
+// bfloat16's).
+constexpr int kExactChunk = 32;
+
+template <typename T, int D, bool VEC, bool MAIN>
+__global__ __launch_bounds__(2 * D, 2) void walk_exact_kernel(ChunkArgs ca) {
+  constexpr int NT = 2 * D, NW = D / 32;
+  constexpr int VE = 16 / sizeof(T), CPR = D / VE;           // elements of a load, loads of a row
+  constexpr int NL = kExactChunk * CPR / NT, kRows = NT / CPR;  // loads a thread and tile, rows of one pass
+  constexpr int C4 = D / 4;                                  // float4 slots of a tile row
+  __shared__ f32x4 tb[kExactChunk * C4], tc[kExactChunk * C4], ta[MAIN ? kExactChunk * C4 : 1];
+  __shared__ float tw[kExactChunk], td[MAIN ? 2 * kExactChunk : 1];  // decays of the update; scale l^(n - 32), 0 before 32
+  const LinearWalk& w = ca.w;
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t bh = (int64_t)blockIdx.x / ca.segs;
+  const int seg = (int)((int64_t)blockIdx.x % ca.segs);
+  if (!MAIN && seg == ca.segs - 1) return;  // (no segment starts from its state)
+  const int64_t b = bh / w.heads;
+  const int h = (int)(bh % w.heads);
+  const int64_t n = walk_length(w, b);
+  const int64_t s0 = (int64_t)seg * ca.seg_tokens;
+  const int64_t s1 = s0 + ca.seg_tokens < n ? s0 + ca.seg_tokens : n;
+  const int first = w.from_end ? 1 : 0;
+  const float l2 = log2_decay(w.log_decay[h]);
+  const float up = first ? w.scale : 1.f, so = first ? 1.f : w.scale;
+  const T* a = static_cast<const T*>(w.a) + b * w.a_stride[0] + h * w.a_stride[1];
+  const T* bp = static_cast<const T*>(w.b) + b * w.b_stride[0] + h * w.b_stride[1];
+  const T* c = static_cast<const T*>(w.c) + b * w.c_stride[0] + h * w.c_stride[1];
+
+  // the state: tile rt, register r is row 32 rt + kappa(g, r), column 32 wave + l
+  f32x16 S[NW];
+  const int col = 32 * wave + l;
+  const int64_t state_size = (int64_t)w.rows * w.cols;
+  {
+    const float* from = nullptr;
+    if (MAIN) from = ca.segs > 1 ? ca.starts + (bh * ca.segs + seg) * state_size
+                                 : w.initial ? w.initial + bh * state_size : nullptr;
+    const auto rsrc = make_rsrc(from, from ? (uint32_t)state_size * 4 : 0u);
+#pragma unroll
+    for (int rt = 0; rt < NW; ++rt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        S[rt][r] = __builtin_bit_cast(
+            float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, state_byte(w, 32 * rt + kappa(g, r), col), 0, 0));
+  }
+
+  // float4 slot of a row: slots are XORed with the row, so that a read phase's rows use distinct banks
+  auto slot = [](int row, int c4) { return row * C4 + (c4 ^ (row & (C4 < 16 ? C4 - 1 : 15))); };
+  auto value = [&](const f32x4* t, int row, int cc) {
+    return reinterpret_cast<const float*>(t)[slot(row, cc >> 2) * 4 + (cc & 3)];
+  };
+
+  const int row0 = tid / CPR, cc0 = tid % CPR * VE;
+  uint4 ra[NL], rb[NL], rc[NL];
+  auto fetch = [&](uint4(&reg)[NL], const T* base, int64_t stride, int width, int64_t p0, int left) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = row0 + i * kRows;
+      reg[i] = make_uint4(0, 0, 0, 0);
+      if (row < left) {
+        const T* q = base + token_of(w, p0 + row, n) * stride;
+        if constexpr (VEC) {
+          if (cc0 < width) reg[i] = *reinterpret_cast<const uint4*>(q + cc0);
+        } else {
+          reg[i] = load16(q, cc0, width, false);
+        }
+      }
+    }
+  };
+  auto fetch_all = [&](int64_t p0) {
+    const int left = s1 - p0 < kExactChunk ? (int)(s1 - p0) : kExactChunk;
+    if (MAIN) fetch(ra, a, w.a_stride[2], w.rows, p0, left);
+    fetch(rb, bp, w.b_stride[2], w.rows, p0, left);
+    fetch(rc, c, w.c_stride[2], w.cols, p0, left);
+  };
+  auto put = [&](f32x4* t, const uint4(&reg)[NL]) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const T* e = reinterpret_cast<const T*>(&reg[i]);
+#pragma unroll
+      for (int q = 0; q < VE / 4; ++q)
+        t[slot(row0 + i * kRows, cc0 / 4 + q)] =
+            f32x4{(float)e[4 * q], (float)e[4 * q + 1], (float)e[4 * q + 2], (float)e[4 * q + 3]};
+    }
+  };
+  if (s0 < s1) fetch_all(s0);
+  if (MAIN && tid < 2 * kExactChunk)
+    td[tid] = tid < kExactChunk ? 0.f : w.scale * decay_power(l2, (float)(tid - kExactChunk));
+  const float fo = so * decay_power(l2, (float)(l + 1 - first));
+
+  for (int64_t p0 = s0; p0 < s1; p0 += kExactChunk) {
+    const int m = (int)(s1 - p0 < kExactChunk ? s1 - p0 : kExactChunk);
+    lds_barrier();  // the tiles have been read
+    if (MAIN) put(ta, ra);
+    put(tb, rb);
+    put(tc, rc);
+    if (tid < kExactChunk) tw[tid] = tid < m ? up * decay_power(l2, (float)(m - 1 - tid + first)) : 0.f;
+    lds_barrier();
+    if (p0 + kExactChunk < s1) fetch_all(p0 + kExactChunk);
+
+    float cv[16];  // this lane's column of tokens kappa(g, r)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) cv[r] = value(tc, kappa(g, r), col);
+    if constexpr (MAIN) {
+      // weights [j][i] and outputs from the state [value][i], lane i = l; k-slot g of MFMA (q, t) is column 8 q + 4 g + t
+      f32x16 p = {}, o = {};
+#pragma unroll
+      for (int q = 0; q < D / 8; ++q) {
+        const f32x4 av = ta[slot(l, 2 * q + g)], bv = tb[slot(l, 2 * q + g)];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          p = Elem<float>::mma(bv[t], av[t], p);
+          o = Elem<float>::mma(S[q / 4][4 * (q % 4) + t], av[t], o);
+        }
+      }
+      const float* f = td + (kExactChunk + l) - 4 * g;
+      bool odd = false;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        // (a later token's product may be infinite: masked by its bits)
+        const int later = (l - 4 * g - kappa(0, r)) >> 31;
+        p[r] = __builtin_bit_cast(float, __builtin_bit_cast(int, p[r] * f[-kappa(0, r)]) & ~later);
+        o[r] *= fo;
+        odd |= (__builtin_bit_cast(uint32_t, cv[r]) & 0x7F800000u) == 0x7F800000u;
+      }
+      if (!__any(odd)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o = Elem<float>::mma(cv[r], p[r], o);
+      } else {
+        // an infinity or NaN among the values: the products that the mask leaves out (0 times it is NaN) must not be
+        // made, so that no token sees a later one's
+        const int l_ = opaque(l), g_ = opaque(g);
+#pragma unroll 1
+        for (int j = 0; j <= l_; ++j) {
+          float x = 0.f;
+#pragma unroll 1
+          for (int d = 0; d < w.rows; ++d) x = __builtin_fmaf(value(ta, l_, d), value(tb, j, d), x);
+          x *= td[kExactChunk + l_ - j];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[r] = __builtin_fmaf(x, value(tc, j, 32 * wave + kappa(g_, r)), o[r]);
+        }
+      }
+      if (w.out && l < m) {
+        T* row = static_cast<T*>(w.out) + b * w.out_stride[0] + h * w.out_stride[1] +
+                 token_of(w, p0 + l, n) * w.out_stride[2];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int cc = 32 * wave + 8 * q + 4 * g;
+          if constexpr (VEC) {
+            if (cc < w.cols) fast::store4(row, cc, o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              if (cc + t < w.cols) row[cc + t] = (T)o[4 * q + t];
+          }
+        }
+      }
+    }
+    // the state's update: k-slot g of MFMA r is token kappa(g, r)
+    const float lm = decay_power(l2, (float)m);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) cv[r] *= tw[kappa(g, r)];
+#pragma unroll
+    for (int rt = 0; rt < NW; ++rt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[rt][r] *= lm;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[rt] = Elem<float>::mma(value(tb, kappa(g, r), 32 * rt + l), cv[r], S[rt]);
+    }
+  }
+
+  // rows behind the sequence are zero
+  if (MAIN && w.out) {
+    int64_t e1 = s0 + ca.seg_tokens;
+    if (e1 > w.length || seg == ca.segs - 1) e1 = w.length;
+    T* out = static_cast<T*>(w.out) + b * w.out_stride[0] + h * w.out_stride[1];
+    const int64_t z0 = s0 > n ? s0 : n;
+    for (int64_t i = tid; i < (e1 - z0) * w.cols; i += NT) out[(z0 + i / w.cols) * w.out_stride[2] + i % w.cols] = (T)0.f;
+  }
+  float* to = nullptr;
+  if (!MAIN) to = ca.starts + (bh * ca.segs + seg) * state_size;
+  else if (w.final_state && (n > 0 ? s0 < n && n <= s0 + ca.seg_tokens : seg == 0)) to = w.final_state + bh * state_size;
+  if (to) {
+    const int g_ = opaque(g), col_ = opaque(col);
+    const auto rsrc = make_rsrc(to, (uint32_t)state_size * 4);
+#pragma unroll
+    for (int rt = 0; rt < NW; ++rt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) buffer_store4(rsrc, state_byte(w, 32 * rt + kappa(g_, r), col_), S[rt][r]);
   }
 }
 
@@ -612,64 +731,63 @@ void plan_segments(const LinearWalk& w, ChunkArgs& ca) {
   ca.seg_tokens = (int32_t)(per * kChunk);
 }
 
-// 16-byte rows (8 elements of 16 bits) whose chunks span less than 2 GiB
-bool rows16(const void* p, const int64_t (&stride)[3], int width) {
-  return width % 8 == 0 && stride[2] < (int64_t(1) << 31) / (2 * kChunk) - 128 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride[0] % 8 == 0 && stride[1] % 8 == 0 &&
-         stride[2] % 8 == 0;
+// rows read and written 16 bytes at a time, whose chunks span less than 2 GiB
+bool rows16(const void* p, const int64_t (&stride)[3], int width, int element) {
+  const int v = 16 / element;
+  return width % v == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride[0] % v == 0 && stride[1] % v == 0 &&
+         stride[2] % v == 0 && stride[2] < (int64_t(1) << 31) / (4 * kChunk) - 128;
 }
 
-template <int D, bool VEC>
+template <typename T, int D, bool VEC, bool MAIN>
+void launch_chunks(const ChunkArgs& ca, dim3 grid, hipStream_t stream) {
+  if constexpr (std::is_same_v<T, __bf16>)
+    hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, MAIN>), grid, dim3(2 * D), 0, stream, ca);
+  else
+    hipLaunchKernelGGL((walk_exact_kernel<T, D, VEC, MAIN>), grid, dim3(2 * D), 0, stream, ca);
+}
+
+template <typename T, int D, bool VEC>
 hipError_t run_chunks(const ChunkArgs& ca, bool starts, hipStream_t stream) {
   const LinearWalk& w = ca.w;
   const unsigned bh = (unsigned)(w.batch * w.heads);
   const dim3 grid(bh * (unsigned)ca.segs);
   if (starts) {
-    hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, false>), grid, dim3(2 * D), 0, stream, ca);
+    launch_chunks<T, D, VEC, false>(ca, grid, stream);
     hipLaunchKernelGGL(walk_scan_kernel, dim3((unsigned)((w.rows * w.cols + kThreads - 1) / kThreads), bh),
                        dim3(kThreads), 0, stream, ca);
   } else {
-    hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, true>), grid, dim3(2 * D), 0, stream, ca);
+    launch_chunks<T, D, VEC, true>(ca, grid, stream);
   }
   return hipGetLastError();
 }
 
 // The walk itself (with the states its segments start from in the workspace), or those states.
 hipError_t run_walk(int dtype, const LinearWalk& w, void* workspace, bool starts, hipStream_t stream) {
-  if (dtype == OOPS_BF16) {
-    ChunkArgs ca{};
-    ca.w = w;
-    plan_segments(w, ca);
-    ca.starts = static_cast<float*>(workspace);
-    if (starts && ca.segs == 1) return hipSuccess;
-    const bool vec = (starts || (rows16(w.a, w.a_stride, w.rows) && rows16(w.out, w.out_stride, w.cols))) &&
-                     rows16(w.b, w.b_stride, w.rows) && rows16(w.c, w.c_stride, w.cols);
-    const int d = std::max(w.rows, w.cols);
+  ChunkArgs ca{};
+  ca.w = w;
+  plan_segments(w, ca);
+  ca.starts = static_cast<float*>(workspace);
+  if (starts && ca.segs == 1) return hipSuccess;
+  const int el = dtype == OOPS_F32 ? 4 : 2;
+  const bool vec = (starts || (rows16(w.a, w.a_stride, w.rows, el) && rows16(w.out, w.out_stride, w.cols, el))) &&
+                   rows16(w.b, w.b_stride, w.rows, el) && rows16(w.c, w.c_stride, w.cols, el);
+  const int d = std::max(w.rows, w.cols);
+  return by_type(dtype, [&](auto tag) {
+    using T = decltype(tag);
     auto run = [&](auto size) {
       constexpr int D = decltype(size)::value;
-      return vec ? run_chunks<D, true>(ca, starts, stream) : run_chunks<D, false>(ca, starts, stream);
+      return vec ? run_chunks<T, D, true>(ca, starts, stream) : run_chunks<T, D, false>(ca, starts, stream);
     };
     if (d <= 32) return run(std::integral_constant<int, 32>{});
     if (d <= 64) return run(std::integral_constant<int, 64>{});
     return run(std::integral_constant<int, 128>{});
-  }
-  if (starts) return hipSuccess;
-  const dim3 grid((unsigned)(w.batch * w.heads), (unsigned)((w.cols + 63) / 64));
-  return by_type(dtype, [&](auto tag) {
-    using T = decltype(tag);
-    if (w.rows <= 32)
-      hipLaunchKernelGGL((walk_kernel<T, 32>), grid, dim3(kThreads), 0, stream, w);
-    else if (w.rows <= 64)
-      hipLaunchKernelGGL((walk_kernel<T, 64>), grid, dim3(kThreads), 0, stream, w);
-    else
-      hipLaunchKernelGGL((walk_kernel<T, 128>), grid, dim3(kThreads), 0, stream, w);
-    return hipGetLastError();
   });
 }
 
 }  // namespace
 
-size_t linear_walk_workspace_bytes(int dtype, const LinearWalk& w) {
-  if (dtype != OOPS_BF16 || w.batch == 0) return 0;
+size_t linear_walk_workspace_bytes(const LinearWalk& w) {
+  if (w.batch == 0) return 0;
   ChunkArgs ca{};
   plan_segments(w, ca);
   if (ca.segs == 1) return 0;
