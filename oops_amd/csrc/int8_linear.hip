@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include "attn_common.h"
+#include "attn_fast_common.h"
 #include "layer_kernels.h"
 
 namespace oops {
@@ -103,11 +104,171 @@ __global__ __launch_bounds__(kThreads) void int8_any_kernel(Int8Args a) {
   }
 }
 
+// ---------------------------------------------------------------- whole tiles
+//
+// BM x BN outputs a workgroup of four waves (2 x 2, each BM/2 x BN/2 in 32 x
+// 32 accumulator tiles), operands whose rows are whole 16-byte pieces at
+// aligned places.  Steps of 64 bytes of k: four LDS buffers filled by direct
+// global-to-LDS loads three steps ahead, so that a step's own work (two k
+// slices of BM BN / 4096 MFMAs a wave) covers a third of a load's latency.  One
+// barrier a step, where all of a step's fragments are in registers and the
+// next step's bytes have landed: the last slice's MFMAs run behind it while
+// the next step's first fragments are read.
+constexpr int kBuffers = 4;
+constexpr int kTileStep = 64;
+
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(Int8Args a, int tiles_r, int tiles_j,
+                                                                               int grid_pad) {
+  constexpr int TR = BM / 64, TJ = BN / 64;                  // accumulator tiles of a wave
+  constexpr int kRowBytes = kTileStep, kStage = (BM + BN) * kRowBytes;
+  constexpr int LR = BM / 64, LJ = BN / 64;                  // loads a wave and step: 16 rows each
+  __shared__ __align__(16) char lds[kBuffers * kStage];
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Workgroups of one XCD take a contiguous run of tiles, eight rows of tiles
+  // deep: the 32 that run at once read 8 + 4 tiles' bytes through its L2.
+  const int t = (int)xcd_tile(blockIdx.x, grid_pad, 0);
+  if (t >= tiles_r * tiles_j) return;
+  const int group = t / (8 * tiles_j), deep = tiles_r - group * 8 < 8 ? tiles_r - group * 8 : 8;
+  const int in = t - group * 8 * tiles_j;
+  const int64_t r0 = (int64_t)(group * 8 + in % deep) * BM, j0 = (int64_t)(in / deep) * BN;
+
+  const int64_t left_r = a.rows - r0 < BM ? a.rows - r0 : BM, left_j = a.n - j0 < BN ? a.n - j0 : BN;
+  // (rows behind the last one lie outside the resource: zeros)
+  const fast::u32x4 rx = fast::rsrc_words(a.x + r0 * a.x_row, (uint32_t)((left_r - 1) * a.x_row + a.k));
+  const fast::u32x4 rw = fast::rsrc_words(a.w + j0 * a.w_row, (uint32_t)((left_j - 1) * a.w_row + a.k));
+  // a load fills 16 rows of four 16-byte slots; slot c of row r holds bytes 16 (c ^ (r / 4 % 4)) of the step, so that
+  // the 16 rows of a read phase use distinct banks
+  const int lc = (lane & 3) ^ ((lane >> 4) & 3);
+  uint32_t vx[LR], vw[LJ];
+#pragma unroll
+  for (int i = 0; i < LR; ++i) vx[i] = (uint32_t)(((i * 4 + wave) * 16 + (lane >> 2)) * (int)a.x_row + lc * 16);
+#pragma unroll
+  for (int i = 0; i < LJ; ++i) vw[i] = (uint32_t)(((i * 4 + wave) * 16 + (lane >> 2)) * (int)a.w_row + lc * 16);
+  auto load = [&](int step) {
+    const int k0 = step * kTileStep;
+    char* to = lds + (step % kBuffers) * kStage;
+    const bool in_k = k0 + lc * 16 < a.k;
+    const uint32_t at = k0 < a.k ? k0 : 0;  // (a scalar offset never past the resource)
+#pragma unroll
+    for (int i = 0; i < LR; ++i) fast::dma16_asm(rx, to + (i * 4 + wave) * 1024, in_k ? vx[i] : fast::kOut, at);
+#pragma unroll
+    for (int i = 0; i < LJ; ++i)
+      fast::dma16_asm(rw, to + BM * kRowBytes + (i * 4 + wave) * 1024, in_k ? vw[i] : fast::kOut, at);
+  };
+  const int steps = (a.k + kTileStep - 1) / kTileStep;
+#pragma unroll
+  for (int s = 0; s < kBuffers - 1; ++s) load(s);  // (steps behind k load zeros)
+
+  const int wr = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
+  const int lx = (wr + l) * kRowBytes + ((half ^ ((l >> 2) & 3)) << 4);
+  const int lw = BM * kRowBytes + (wj + l) * kRowBytes + ((half ^ ((l >> 2) & 3)) << 4);
+  i32x16 acc[TJ][TR];
+#pragma unroll
+  for (int q = 0; q < TJ; ++q)
+#pragma unroll
+    for (int p = 0; p < TR; ++p) acc[q][p] = i32x16{};
+  i32x4 fx[2][TR], fw[2][TJ];
+  auto read = [&](int step, int slice, i32x4(&x)[TR], i32x4(&w)[TJ]) {
+    const char* from = lds + (step % kBuffers) * kStage;
+#pragma unroll
+    for (int q = 0; q < TJ; ++q) w[q] = *reinterpret_cast<const i32x4*>(from + (lw ^ (slice << 5)) + q * 32 * kRowBytes);
+#pragma unroll
+    for (int p = 0; p < TR; ++p) x[p] = *reinterpret_cast<const i32x4*>(from + (lx ^ (slice << 5)) + p * 32 * kRowBytes);
+  };
+  auto multiply = [&](const i32x4(&x)[TR], const i32x4(&w)[TJ]) {
+#pragma unroll
+    for (int q = 0; q < TJ; ++q)
+#pragma unroll
+      for (int p = 0; p < TR; ++p) acc[q][p] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[q], x[p], acc[q][p], 0, 0, 0);
+  };
+  fast::vmem_wait<(kBuffers - 2) * (LR + LJ)>();
+  lds_barrier();
+  read(0, 0, fx[0], fw[0]);
+  for (int s = 0; s < steps; ++s) {
+    read(s, 1, fx[1], fw[1]);
+    multiply(fx[0], fw[0]);
+    load(s + kBuffers - 1);
+    fast::vmem_wait<(kBuffers - 2) * (LR + LJ)>();  // step s + 1 has landed (this wave's part)
+    lds_barrier();                                  // everywhere, and step s is in registers everywhere
+    read(s + 1, 0, fx[0], fw[0]);                   // (behind the last step: zeros, not used)
+    multiply(fx[1], fw[1]);
+  }
+
+  fast::vmem_wait<0>();  // (no load may land in LDS that is another workgroup's by then)
+
+  // out[r0 + wr + 32 p + l][j0 + wj + 32 q + kappa(half, i)]
+  float scale_x[TR];
+#pragma unroll
+  for (int p = 0; p < TR; ++p) {
+    const int64_t r = r0 + wr + 32 * p + l;
+    scale_x[p] = r < a.rows ? a.x_scale[r] : 0.f;
+  }
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = a.n % V == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+#pragma unroll
+  for (int q = 0; q < TJ; ++q) {
+    float scale_w[16], add[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int64_t j = j0 + wj + 32 * q + kappa(half, i);
+      scale_w[i] = j < a.n ? a.w_scale[j] : 0.f;
+      add[i] = j < a.n ? bias_at<T>(a, j) : 0.f;
+    }
+#pragma unroll
+    for (int p = 0; p < TR; ++p) {
+      const int64_t r = r0 + wr + 32 * p + l, jq = j0 + wj + 32 * q;
+      T* row = static_cast<T*>(a.out) + (r < a.rows ? r : 0) * a.n;
+      float y[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = __builtin_fmaf((float)acc[q][p][i] * scale_x[p], scale_w[i], add[i]);
+      if (!vec) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (r < a.rows && jq + kappa(half, i) < a.n) row[jq + kappa(half, i)] = (T)y[i];
+      } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          if (r < a.rows && jq + kappa(half, i) < a.n)
+            *reinterpret_cast<f32x4*>(row + jq + kappa(half, i)) = f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
+      } else {
+        uint32_t pk[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pk[i] = fast::pack2<T>(y[2 * i], y[2 * i + 1]);
+        uint4 lo, hi;
+        fast::trade16(pk, lo, hi);
+        const int64_t j = jq + 16 * half;
+        if (r < a.rows && j < a.n) *reinterpret_cast<uint4*>(row + j) = lo;
+        if (r < a.rows && j + 8 < a.n) *reinterpret_cast<uint4*>(row + j + 8) = hi;
+      }
+    }
+  }
+}
+
 template <typename F>
 hipError_t by_type(int dtype, F&& f) {
   if (dtype == OOPS_F32) return f(float{});
   if (dtype == OOPS_BF16) return f((__bf16)0.f);
   return f((_Float16)0.f);
+}
+
+// rows at multiples of 16 bytes, a tile of which spans less than 2 GiB
+bool aligned_rows(const void* p, int64_t rows, int64_t stride) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || (stride % 16 == 0 && stride < (int64_t(1) << 22)));
+}
+
+template <int B>
+hipError_t run_tiles(const oops_int8_geometry& g, Int8Args a, hipStream_t stream) {
+  if (g.rows == 1) a.x_row = g.k;
+  if (g.n == 1) a.w_row = g.k;
+  const int tr = (int)((g.rows + B - 1) / B), tj = (int)((g.n + B - 1) / B);
+  const int grid = (int)xcd_grid((int64_t)tr * tj, 0);
+  return by_type(g.out_dtype, [&](auto tag) {
+    using T = decltype(tag);
+    hipLaunchKernelGGL((int8_tile_kernel<T, B, B>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a, tr, tj, grid);
+    return hipGetLastError();
+  });
 }
 
 }  // namespace
@@ -118,6 +279,14 @@ hipError_t launch_int8_linear(const oops_int8_geometry& g, const void* x, const 
                               const float* w_scale, const void* bias, void* out, void*, hipStream_t stream) {
   const Int8Args a{static_cast<const int8_t*>(x), static_cast<const int8_t*>(w), x_scale, w_scale, bias, out, g.rows,
                    g.n, g.x_row, g.w_row, (int32_t)g.k, g.bias_dtype == OOPS_F32};
+  const bool whole = g.k % 16 == 0 && aligned_rows(x, g.rows, g.x_row) && aligned_rows(w, g.n, g.w_row);
+  if (whole && g.k > 0) {
+    // the largest tile that gives every CU one
+    auto tiles = [&](int64_t m) { return ((g.n + m - 1) / m) * ((g.rows + m - 1) / m); };
+    if (tiles(256) >= 192 && tiles(256) < kMaxTiles) return run_tiles<256>(g, a, stream);
+    if (tiles(128) < kMaxTiles && tiles(128) >= 128) return run_tiles<128>(g, a, stream);
+    if (tiles(64) < kMaxTiles) return run_tiles<64>(g, a, stream);
+  }
   const int64_t tiles = ((g.n + 63) / 64) * ((g.rows + 63) / 64);
   if (tiles > kMaxTiles) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)tiles);
