@@ -108,22 +108,31 @@ __global__ __launch_bounds__(kThreads) void int8_any_kernel(Int8Args a) {
 //
 // BM x BN outputs a workgroup of four waves (2 x 2, each BM/2 x BN/2 in 32 x
 // 32 accumulator tiles), operands whose rows are whole 16-byte pieces at
-// aligned places.  Steps of 64 bytes of k: four LDS buffers filled by direct
-// global-to-LDS loads three steps ahead, so that a step's own work (two k
-// slices of BM BN / 4096 MFMAs a wave) covers a third of a load's latency.  One
-// barrier a step, where all of a step's fragments are in registers and the
-// next step's bytes have landed: the last slice's MFMAs run behind it while
-// the next step's first fragments are read.
-constexpr int kBuffers = 4;
-constexpr int kTileStep = 64;
+// aligned places.  Steps of 128 bytes of k, whole cache lines: two LDS buffers
+// filled by direct global-to-LDS loads a step ahead.  One barrier a step, where
+// all of a step's fragments are in registers and the next step's bytes have
+// landed: the last slice's MFMAs run behind it while the next step's first
+// fragments are read.
+constexpr int kTileStep = 128;
+
+// fast::dma16_asm with the LDS address as a number (the conversion of a pointer checks it for NULL in five scalar
+// instructions, too many to hide behind an MFMA)
+__device__ __forceinline__ void load_lds(const fast::u32x4& r, uint32_t to, uint32_t voff, uint32_t soff) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to),
+      "v"(voff), "s"(r), "s"(soff)
+      : "memory", "m0");
+}
 
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(Int8Args a, int tiles_r, int tiles_j,
                                                                                int grid_pad) {
   constexpr int TR = BM / 64, TJ = BN / 64;                  // accumulator tiles of a wave
   constexpr int kRowBytes = kTileStep, kStage = (BM + BN) * kRowBytes;
-  constexpr int LR = BM / 64, LJ = BN / 64;                  // loads a wave and step: 16 rows each
-  __shared__ __align__(16) char lds[kBuffers * kStage];
+  constexpr int LR = BM / 32, LJ = BN / 32;                  // loads a wave and step: 8 rows each
+  __shared__ __align__(16) char lds[2 * kStage];
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Workgroups of one XCD take a contiguous run of tiles, eight rows of tiles
@@ -138,32 +147,29 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(
   // (rows behind the last one lie outside the resource: zeros)
   const fast::u32x4 rx = fast::rsrc_words(a.x + r0 * a.x_row, (uint32_t)((left_r - 1) * a.x_row + a.k));
   const fast::u32x4 rw = fast::rsrc_words(a.w + j0 * a.w_row, (uint32_t)((left_j - 1) * a.w_row + a.k));
-  // a load fills 16 rows of four 16-byte slots; slot c of row r holds bytes 16 (c ^ (r / 4 % 4)) of the step, so that
-  // the 16 rows of a read phase use distinct banks
-  const int lc = (lane & 3) ^ ((lane >> 4) & 3);
+  // a load fills 8 rows of eight 16-byte slots; slot c of row r holds bytes 16 (c ^ (r / 2 % 8)) of the step, so that
+  // the 16 rows of a read phase use distinct banks (rows r and r + 8 hold it alike: loads i and i + 1 differ by 32 rows)
   uint32_t vx[LR], vw[LJ];
+  const int lrow = wave * 8 + (lane >> 3), lc = (lane & 7) ^ ((lrow >> 1) & 7);
 #pragma unroll
-  for (int i = 0; i < LR; ++i) vx[i] = (uint32_t)(((i * 4 + wave) * 16 + (lane >> 2)) * (int)a.x_row + lc * 16);
+  for (int i = 0; i < LR; ++i) vx[i] = (uint32_t)((i * 32 + lrow) * (int)a.x_row + lc * 16);
 #pragma unroll
-  for (int i = 0; i < LJ; ++i) vw[i] = (uint32_t)(((i * 4 + wave) * 16 + (lane >> 2)) * (int)a.w_row + lc * 16);
-  auto load = [&](int step) {
+  for (int i = 0; i < LJ; ++i) vw[i] = (uint32_t)((i * 32 + lrow) * (int)a.w_row + lc * 16);
+  // load i of a step (x's rows, then w's); a scalar offset is never past the resource
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds + wave * 1024;
+  auto load = [&](int step, int i) {
     const int k0 = step * kTileStep;
-    char* to = lds + (step % kBuffers) * kStage;
-    const bool in_k = k0 + lc * 16 < a.k;
-    const uint32_t at = k0 < a.k ? k0 : 0;  // (a scalar offset never past the resource)
-#pragma unroll
-    for (int i = 0; i < LR; ++i) fast::dma16_asm(rx, to + (i * 4 + wave) * 1024, in_k ? vx[i] : fast::kOut, at);
-#pragma unroll
-    for (int i = 0; i < LJ; ++i)
-      fast::dma16_asm(rw, to + BM * kRowBytes + (i * 4 + wave) * 1024, in_k ? vw[i] : fast::kOut, at);
+    const uint32_t to = lds0 + (step & 1) * kStage + (i < LR ? i * 4096 : BM * kRowBytes + (i - LR) * 4096);
+    const uint32_t at = k0 < a.k ? k0 : 0, v = i < LR ? vx[i < LR ? i : 0] : vw[i < LR ? 0 : i - LR];
+    load_lds(i < LR ? rx : rw, __builtin_amdgcn_readfirstlane(to), k0 + lc * 16 < a.k ? v : fast::kOut, at);
   };
   const int steps = (a.k + kTileStep - 1) / kTileStep;
 #pragma unroll
-  for (int s = 0; s < kBuffers - 1; ++s) load(s);  // (steps behind k load zeros)
+  for (int i = 0; i < LR + LJ; ++i) load(0, i);
 
   const int wr = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
-  const int lx = (wr + l) * kRowBytes + ((half ^ ((l >> 2) & 3)) << 4);
-  const int lw = BM * kRowBytes + (wj + l) * kRowBytes + ((half ^ ((l >> 2) & 3)) << 4);
+  const int lx = (wr + l) * kRowBytes + ((half ^ ((l >> 1) & 7)) << 4);
+  const int lw = BM * kRowBytes + (wj + l) * kRowBytes + ((half ^ ((l >> 1) & 7)) << 4);
   i32x16 acc[TJ][TR];
 #pragma unroll
   for (int q = 0; q < TJ; ++q)
@@ -171,31 +177,48 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(
     for (int p = 0; p < TR; ++p) acc[q][p] = i32x16{};
   i32x4 fx[2][TR], fw[2][TJ];
   auto read = [&](int step, int slice, i32x4(&x)[TR], i32x4(&w)[TJ]) {
-    const char* from = lds + (step % kBuffers) * kStage;
+    const char* from = lds + (step & 1) * kStage;
 #pragma unroll
     for (int q = 0; q < TJ; ++q) w[q] = *reinterpret_cast<const i32x4*>(from + (lw ^ (slice << 5)) + q * 32 * kRowBytes);
 #pragma unroll
     for (int p = 0; p < TR; ++p) x[p] = *reinterpret_cast<const i32x4*>(from + (lx ^ (slice << 5)) + p * 32 * kRowBytes);
   };
-  auto multiply = [&](const i32x4(&x)[TR], const i32x4(&w)[TJ]) {
+  // the products of a slice; between them, PER loads of the next step behind each
+  auto multiply = [&](const i32x4(&x)[TR], const i32x4(&w)[TJ], int step) {
 #pragma unroll
-    for (int q = 0; q < TJ; ++q)
+    for (int i = 0; i < TJ * TR; ++i) {
+      acc[i / TR][i % TR] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[i / TR], x[i % TR], acc[i / TR][i % TR], 0, 0, 0);
+      constexpr int kPer = (LR + LJ + TJ * TR - 1) / (TJ * TR);
+      if (step >= 0) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int p = 0; p < TR; ++p) acc[q][p] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[q], x[p], acc[q][p], 0, 0, 0);
+        for (int q = i * kPer; q < (i + 1) * kPer && q < LR + LJ; ++q) load(step, q);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   };
-  fast::vmem_wait<(kBuffers - 2) * (LR + LJ)>();
+  fast::vmem_wait<0>();
   lds_barrier();
   read(0, 0, fx[0], fw[0]);
   for (int s = 0; s < steps; ++s) {
     read(s, 1, fx[1], fw[1]);
-    multiply(fx[0], fw[0]);
-    load(s + kBuffers - 1);
-    fast::vmem_wait<(kBuffers - 2) * (LR + LJ)>();  // step s + 1 has landed (this wave's part)
-    lds_barrier();                                  // everywhere, and step s is in registers everywhere
-    read(s + 1, 0, fx[0], fw[0]);                   // (behind the last step: zeros, not used)
-    multiply(fx[1], fw[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(fx[0], fw[0], s + 1);  // (behind the last step: zeros)
+    read(s, 2, fx[0], fw[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(fx[1], fw[1], -1);
+    __builtin_amdgcn_sched_barrier(0);
+    read(s, 3, fx[1], fw[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(fx[0], fw[0], -1);
+    __builtin_amdgcn_sched_barrier(0);
+    fast::vmem_wait<0>();          // step s + 1 has landed (this wave's part)
+    lds_barrier();                 // everywhere, and step s is in registers everywhere
+    read(s + 1, 0, fx[0], fw[0]);  // (behind the last step: not used)
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(fx[1], fw[1], -1);
+    __builtin_amdgcn_sched_barrier(0);
   }
-
   fast::vmem_wait<0>();  // (no load may land in LDS that is another workgroup's by then)
 
   // out[r0 + wr + 32 p + l][j0 + wj + 32 q + kappa(half, i)]
