@@ -11,6 +11,8 @@
 // one output row and four consecutive columns at a time.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "attn_common.h"
 #include "attn_fast_common.h"
 #include "layer_kernels.h"
@@ -32,6 +34,8 @@ struct Int8Args {
   void* out;
   int64_t rows, n, x_row, w_row;
   int32_t k, bias_f32;
+  int32_t* sums;  // parts > 1: [parts][rows][n] sums over part_k bytes of k each
+  int32_t parts, part_k;
 };
 
 // bytes col .. col+15 of a row of k bytes, zeros behind it, at any alignment
@@ -108,11 +112,11 @@ __global__ __launch_bounds__(kThreads) void int8_any_kernel(Int8Args a) {
 //
 // BM x BN outputs a workgroup of four waves (2 x 2, each BM/2 x BN/2 in 32 x
 // 32 accumulator tiles), operands whose rows are whole 16-byte pieces at
-// aligned places.  Steps of 128 bytes of k, whole cache lines: two LDS buffers
-// filled by direct global-to-LDS loads a step ahead.  One barrier a step, where
-// all of a step's fragments are in registers and the next step's bytes have
-// landed: the last slice's MFMAs run behind it while the next step's first
-// fragments are read.
+// aligned places.  Steps of 128 bytes of k, whole cache lines: NB LDS buffers
+// filled by direct global-to-LDS loads NB - 1 steps ahead.  One barrier a step,
+// where all of a step's fragments are in registers and the next step's bytes
+// have landed: the last slice's MFMAs run behind it while the next step's
+// first fragments are read.
 constexpr int kTileStep = 128;
 
 // fast::dma16_asm with the LDS address as a number (the conversion of a pointer checks it for NULL in five scalar
@@ -126,19 +130,21 @@ __device__ __forceinline__ void load_lds(const fast::u32x4& r, uint32_t to, uint
       : "memory", "m0");
 }
 
-template <typename T, int BM, int BN>
-__global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(Int8Args a, int tiles_r, int tiles_j,
+template <typename T, int BM, int BN, int NB>
+__global__ __launch_bounds__(kThreads, 1) void int8_tile_kernel(Int8Args a, int tiles_r, int tiles_j,
                                                                                int grid_pad) {
   constexpr int TR = BM / 64, TJ = BN / 64;                  // accumulator tiles of a wave
   constexpr int kRowBytes = kTileStep, kStage = (BM + BN) * kRowBytes;
   constexpr int LR = BM / 32, LJ = BN / 32;                  // loads a wave and step: 8 rows each
-  __shared__ __align__(16) char lds[2 * kStage];
+  __shared__ __align__(16) char lds[NB * kStage];
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Workgroups of one XCD take a contiguous run of tiles, eight rows of tiles
   // deep: the 32 that run at once read 8 + 4 tiles' bytes through its L2.
-  const int t = (int)xcd_tile(blockIdx.x, grid_pad, 0);
-  if (t >= tiles_r * tiles_j) return;
+  const int t_all = (int)xcd_tile(blockIdx.x, grid_pad, 0);
+  if (t_all >= tiles_r * tiles_j * a.parts) return;
+  const int part = __builtin_amdgcn_readfirstlane(t_all / (tiles_r * tiles_j)), t = t_all - part * tiles_r * tiles_j;
+  const int k_begin = part * a.part_k, k_end = a.k - k_begin < a.part_k ? a.k : k_begin + a.part_k;
   const int group = t / (8 * tiles_j), deep = tiles_r - group * 8 < 8 ? tiles_r - group * 8 : 8;
   const int in = t - group * 8 * tiles_j;
   const int64_t r0 = (int64_t)(group * 8 + in % deep) * BM, j0 = (int64_t)(in / deep) * BN;
@@ -158,14 +164,16 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(
   // load i of a step (x's rows, then w's); a scalar offset is never past the resource
   const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds + wave * 1024;
   auto load = [&](int step, int i) {
-    const int k0 = step * kTileStep;
-    const uint32_t to = lds0 + (step & 1) * kStage + (i < LR ? i * 4096 : BM * kRowBytes + (i - LR) * 4096);
-    const uint32_t at = k0 < a.k ? k0 : 0, v = i < LR ? vx[i < LR ? i : 0] : vw[i < LR ? 0 : i - LR];
-    load_lds(i < LR ? rx : rw, __builtin_amdgcn_readfirstlane(to), k0 + lc * 16 < a.k ? v : fast::kOut, at);
+    const int k0 = k_begin + step * kTileStep;
+    const uint32_t to = lds0 + (step % NB) * kStage + (i < LR ? i * 4096 : BM * kRowBytes + (i - LR) * 4096);
+    const uint32_t at = k0 < k_end ? k0 : 0, v = i < LR ? vx[i < LR ? i : 0] : vw[i < LR ? 0 : i - LR];
+    load_lds(i < LR ? rx : rw, __builtin_amdgcn_readfirstlane(to), k0 + lc * 16 < k_end ? v : fast::kOut, at);
   };
-  const int steps = (a.k + kTileStep - 1) / kTileStep;
+  const int steps = (k_end - k_begin + kTileStep - 1) / kTileStep;
 #pragma unroll
-  for (int i = 0; i < LR + LJ; ++i) load(0, i);
+  for (int s = 0; s < NB - 1; ++s)  // (steps behind k load zeros)
+#pragma unroll
+    for (int i = 0; i < LR + LJ; ++i) load(s, i);
 
   const int wr = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
   const int lx = (wr + l) * kRowBytes + ((half ^ ((l >> 1) & 7)) << 4);
@@ -177,13 +185,13 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(
     for (int p = 0; p < TR; ++p) acc[q][p] = i32x16{};
   i32x4 fx[2][TR], fw[2][TJ];
   auto read = [&](int step, int slice, i32x4(&x)[TR], i32x4(&w)[TJ]) {
-    const char* from = lds + (step & 1) * kStage;
+    const char* from = lds + (step % NB) * kStage;
 #pragma unroll
     for (int q = 0; q < TJ; ++q) w[q] = *reinterpret_cast<const i32x4*>(from + (lw ^ (slice << 5)) + q * 32 * kRowBytes);
 #pragma unroll
     for (int p = 0; p < TR; ++p) x[p] = *reinterpret_cast<const i32x4*>(from + (lx ^ (slice << 5)) + p * 32 * kRowBytes);
   };
-  // the products of a slice; between them, PER loads of the next step behind each
+  // the products of a slice; between them, the loads of a later step
   auto multiply = [&](const i32x4(&x)[TR], const i32x4(&w)[TJ], int step) {
 #pragma unroll
     for (int i = 0; i < TJ * TR; ++i) {
@@ -197,13 +205,14 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(
       }
     }
   };
-  fast::vmem_wait<0>();
+  constexpr int kLater = (NB - 2) * (LR + LJ);  // loads behind the next step's
+  fast::vmem_wait<kLater>();
   lds_barrier();
   read(0, 0, fx[0], fw[0]);
   for (int s = 0; s < steps; ++s) {
     read(s, 1, fx[1], fw[1]);
     __builtin_amdgcn_sched_barrier(0);
-    multiply(fx[0], fw[0], s + 1);  // (behind the last step: zeros)
+    multiply(fx[0], fw[0], s + NB - 1);
     read(s, 2, fx[0], fw[0]);
     __builtin_amdgcn_sched_barrier(0);
     multiply(fx[1], fw[1], -1);
@@ -212,7 +221,7 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(
     __builtin_amdgcn_sched_barrier(0);
     multiply(fx[0], fw[0], -1);
     __builtin_amdgcn_sched_barrier(0);
-    fast::vmem_wait<0>();          // step s + 1 has landed (this wave's part)
+    fast::vmem_wait<kLater>();     // step s + 1 has landed (this wave's part)
     lds_barrier();                 // everywhere, and step s is in registers everywhere
     read(s + 1, 0, fx[0], fw[0]);  // (behind the last step: not used)
     __builtin_amdgcn_sched_barrier(0);
@@ -222,6 +231,20 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(
   fast::vmem_wait<0>();  // (no load may land in LDS that is another workgroup's by then)
 
   // out[r0 + wr + 32 p + l][j0 + wj + 32 q + kappa(half, i)]
+  if (BM * BN == 64 * 64 && a.parts > 1) {
+    int32_t* sums = a.sums + (int64_t)part * a.rows * a.n;
+#pragma unroll
+    for (int q = 0; q < TJ; ++q)
+#pragma unroll
+      for (int p = 0; p < TR; ++p) {
+        const int64_t r = r0 + wr + 32 * p + l, jq = j0 + wj + 32 * q;
+        if (r < a.rows)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (jq + kappa(half, i) < a.n) sums[r * a.n + jq + kappa(half, i)] = acc[q][p][i];
+      }
+    return;
+  }
   float scale_x[TR];
 #pragma unroll
   for (int p = 0; p < TR; ++p) {
@@ -269,6 +292,69 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void int8_tile_kernel(
   }
 }
 
+// ---------------------------------------------------------------- few rows
+//
+// Up to 16 rows of x: bound by the weight's bytes, each read once.  A
+// workgroup takes 16 weight rows; its W waves take whole lines of k in turn, U
+// lines in flight each, the operands loaded straight into the 16x16x64 MFMA's
+// layout (a quarter wave reads 64 bytes of a row), and join their sums in LDS.
+// W U lines are k where it can be had: all loads of a wave then fly at once
+// (4 x 4096 x 16384: W, U = 8, 4 16.0 us or 4.2 TB/s; 4, 8 18.4; 16, 4 20.2;
+// 8 x 1024 x 50000: 8, 2 15.7; 8, 4 22.6;  4 x 16384 x 4096: 16, 4 16.1; 8, 4 22.3).
+template <typename T, int W, int U>
+__global__ __launch_bounds__(64 * W) void int8_few_kernel(Int8Args a) {
+  __shared__ i32x4 red[W][64];
+  const int tid = threadIdx.x, lane = tid & 63, row = lane & 15, part = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t j0 = (int64_t)blockIdx.x * 16;
+  const int64_t left = a.n - j0 < 16 ? a.n - j0 : 16;
+  // (weight rows behind the last one lie outside the resource: zeros)
+  const auto rw = make_rsrc(a.w + j0 * a.w_row, (uint32_t)((left - 1) * a.w_row + a.k));
+  const auto rx = make_rsrc(a.x, (uint32_t)((a.rows - 1) * a.x_row + a.k));
+  const uint32_t vw = row * (uint32_t)a.w_row + part * 16, vx = row * (uint32_t)a.x_row + part * 16;
+  const int64_t j = j0 + 4 * part;
+  i32x4 acc = {};
+  for (int k0 = wave * 128; k0 < a.k; k0 += W * U * 128) {
+    i32x4 fw[2 * U], fx[2 * U];
+#pragma unroll
+    for (int u = 0; u < 2 * U; ++u) {
+      const int k = k0 + (u / 2) * W * 128 + (u % 2) * 64;
+      const bool in = k + part * 16 < a.k;
+      fw[u] = __builtin_bit_cast(i32x4, buffer_load16(rw, in ? vw + k : fast::kOut));
+      fx[u] = __builtin_bit_cast(i32x4, buffer_load16(rx, in && row < a.rows ? vx + k : fast::kOut));
+    }
+#pragma unroll
+    for (int u = 0; u < 2 * U; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], fx[u], acc, 0, 0, 0);
+  }
+  red[wave][lane] = acc;
+  __syncthreads();
+  if (wave > 0 || row >= a.rows) return;
+  i32x4 sum = red[0][lane];
+#pragma unroll
+  for (int q = 1; q < W; ++q) sum += red[q][lane];
+  // out[row][j0 + 4 part + i]
+  const float sx = a.x_scale[row];
+  T* out = static_cast<T*>(a.out) + row * a.n + j;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (j + i < a.n) out[i] = (T)__builtin_fmaf((float)sum[i] * sx, a.w_scale[j + i], bias_at<T>(a, j + i));
+}
+
+// ---------------------------------------------------------------- joined parts
+//
+// Few tiles and a long k: the tiles' parts of k write their sums, and this
+// kernel adds them (whole numbers: in any order) and scales the result.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void int8_join_kernel(Int8Args a) {
+  const int64_t size = a.rows * a.n;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < size; i += (int64_t)gridDim.x * kThreads) {
+    int sum = 0;
+    for (int p = 0; p < a.parts; ++p) sum += a.sums[p * size + i];
+    const int64_t r = i / a.n, j = i - r * a.n;
+    static_cast<T*>(a.out)[i] = (T)__builtin_fmaf((float)sum * a.x_scale[r], a.w_scale[j], bias_at<T>(a, j));
+  }
+}
+
 template <typename F>
 hipError_t by_type(int dtype, F&& f) {
   if (dtype == OOPS_F32) return f(float{});
@@ -281,41 +367,102 @@ bool aligned_rows(const void* p, int64_t rows, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || (stride % 16 == 0 && stride < (int64_t(1) << 22)));
 }
 
-template <int B>
+hipError_t run_few(const oops_int8_geometry& g, Int8Args a, hipStream_t stream) {
+  if (g.rows == 1) a.x_row = g.k;
+  if (g.n == 1) a.w_row = g.k;
+  const dim3 grid((unsigned)((g.n + 15) / 16));
+  return by_type(g.out_dtype, [&](auto tag) {
+    using T = decltype(tag);
+    if (g.k <= 2048)
+      hipLaunchKernelGGL((int8_few_kernel<T, 8, 2>), grid, dim3(512), 0, stream, a);
+    else if (g.k <= 4096)
+      hipLaunchKernelGGL((int8_few_kernel<T, 8, 4>), grid, dim3(512), 0, stream, a);
+    else
+      hipLaunchKernelGGL((int8_few_kernel<T, 16, 4>), grid, dim3(1024), 0, stream, a);
+    return hipGetLastError();
+  });
+}
+
+// Rows that go to int8_few_kernel: up to 8, or 16 where the weight has few rows (16 x 4096 x 4096: 7.5 us, tiles 10.2;
+// 16 x 4096 x 16384: 20.8, tiles 17.6).
+bool few_rows(const oops_int8_geometry& g) {
+  return g.rows <= (g.n <= 8192 ? 16 : 8) && g.n < kMaxTiles * 8;
+}
+
+int64_t tiles_of(const oops_int8_geometry& g, int64_t m, int64_t n) {
+  return ((g.n + n - 1) / n) * ((g.rows + m - 1) / m);
+}
+
+// Parts of k: where the smallest tiles are too few for the CUs, as many as fill them with at least kMinPart bytes each;
+// fewer than four do not pay for the join (48 x 16384 x 4096: 36 us, eight parts 18 + 5; 32 x 4096 x 4096: 10.1, four
+// parts 7.2 + 3.4).
+constexpr int64_t kMinPart = 2048;
+struct KParts {
+  int parts, part_k;
+};
+KParts k_parts(const oops_int8_geometry& g) {
+  const int64_t tiles = tiles_of(g, 64, 64);
+  int64_t parts = 1;
+  if (g.k % 16 == 0 && !few_rows(g) && tiles > 0 && tiles <= 128) parts = std::min(256 / tiles, g.k / kMinPart);
+  if (parts < 4) return {1, (int)g.k};
+  const int64_t per = ((g.k + parts - 1) / parts + kTileStep - 1) / kTileStep * kTileStep;
+  return {(int)((g.k + per - 1) / per), (int)per};
+}
+
+template <int BM, int BN, int NB>
 hipError_t run_tiles(const oops_int8_geometry& g, Int8Args a, hipStream_t stream) {
   if (g.rows == 1) a.x_row = g.k;
   if (g.n == 1) a.w_row = g.k;
-  const int tr = (int)((g.rows + B - 1) / B), tj = (int)((g.n + B - 1) / B);
-  const int grid = (int)xcd_grid((int64_t)tr * tj, 0);
+  const int tr = (int)((g.rows + BM - 1) / BM), tj = (int)((g.n + BN - 1) / BN);
+  const int grid = (int)xcd_grid((int64_t)tr * tj * a.parts, 0);
   return by_type(g.out_dtype, [&](auto tag) {
     using T = decltype(tag);
-    hipLaunchKernelGGL((int8_tile_kernel<T, B, B>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a, tr, tj, grid);
+    hipLaunchKernelGGL((int8_tile_kernel<T, BM, BN, NB>), dim3((unsigned)grid), dim3(kThreads), 0, stream, a, tr, tj, grid);
     return hipGetLastError();
   });
 }
 
 }  // namespace
 
-size_t int8_linear_workspace_bytes(const oops_int8_geometry&) { return 0; }
+size_t int8_linear_workspace_bytes(const oops_int8_geometry& g) {
+  const int parts = k_parts(g).parts;
+  return parts > 1 ? (size_t)parts * (size_t)g.rows * (size_t)g.n * sizeof(int32_t) : 0;
+}
 
 hipError_t launch_int8_linear(const oops_int8_geometry& g, const void* x, const float* x_scale, const void* w,
-                              const float* w_scale, const void* bias, void* out, void*, hipStream_t stream) {
-  const Int8Args a{static_cast<const int8_t*>(x), static_cast<const int8_t*>(w), x_scale, w_scale, bias, out, g.rows,
-                   g.n, g.x_row, g.w_row, (int32_t)g.k, g.bias_dtype == OOPS_F32};
-  const bool whole = g.k % 16 == 0 && aligned_rows(x, g.rows, g.x_row) && aligned_rows(w, g.n, g.w_row);
-  if (whole && g.k > 0) {
-    // the largest tile that gives every CU one
-    auto tiles = [&](int64_t m) { return ((g.n + m - 1) / m) * ((g.rows + m - 1) / m); };
-    if (tiles(256) >= 192 && tiles(256) < kMaxTiles) return run_tiles<256>(g, a, stream);
-    if (tiles(128) < kMaxTiles && tiles(128) >= 128) return run_tiles<128>(g, a, stream);
-    if (tiles(64) < kMaxTiles) return run_tiles<64>(g, a, stream);
+                              const float* w_scale, const void* bias, void* out, void* workspace, hipStream_t stream) {
+  Int8Args a{static_cast<const int8_t*>(x), static_cast<const int8_t*>(w), x_scale, w_scale, bias, out, g.rows, g.n,
+             g.x_row, g.w_row, (int32_t)g.k, g.bias_dtype == OOPS_F32, nullptr, 1, (int32_t)g.k};
+  const bool whole = g.k > 0 && g.k % 16 == 0 && aligned_rows(x, g.rows, g.x_row) && aligned_rows(w, g.n, g.w_row) &&
+                     tiles_of(g, 64, 64) < kMaxTiles;
+  if (whole) {
+    if (few_rows(g)) return run_few(g, a, stream);
+    // the largest tile that gives (nearly) every CU one, measured in us at rows x n x k:
+    //   4096 x 4096 x 4096: 256^2 69, 128^2 83 (two a CU);   2048 x 4096 x 4096: 256^2 56, 128^2 40
+    //   1024 x 4096 x 4096: 128^2 24 (four buffers; two: 31), 64 x 128 29;   512 x 4096 x 4096: 128^2 21, 64 x 128 17
+    const int64_t t128 = tiles_of(g, 128, 128);
+    if (tiles_of(g, 256, 256) >= 192) return run_tiles<256, 256, 2>(g, a, stream);
+    if (t128 > 256) return run_tiles<128, 128, 2>(g, a, stream);
+    if (t128 >= 192) return run_tiles<128, 128, 4>(g, a, stream);
+    if (tiles_of(g, 64, 128) >= 192) return run_tiles<64, 128, 4>(g, a, stream);
+    const KParts kp = k_parts(g);
+    a.sums = static_cast<int32_t*>(workspace);
+    a.parts = kp.parts;
+    a.part_k = kp.part_k;
+    const hipError_t e = run_tiles<64, 64, 4>(g, a, stream);
+    if (e != hipSuccess || a.parts == 1) return e;
+    return by_type(g.out_dtype, [&](auto tag) {
+      using T = decltype(tag);
+      const int64_t blocks = std::min<int64_t>((g.rows * g.n + kThreads - 1) / kThreads, 2048);
+      hipLaunchKernelGGL((int8_join_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+      return hipGetLastError();
+    });
   }
-  const int64_t tiles = ((g.n + 63) / 64) * ((g.rows + 63) / 64);
+  const int64_t tiles = tiles_of(g, 64, 64);
   if (tiles > kMaxTiles) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)tiles);
   return by_type(g.out_dtype, [&](auto tag) {
     using T = decltype(tag);
-    hipLaunchKernelGGL((int8_any_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((int8_any_kernel<T>), dim3((unsigned)tiles), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
   });
 }

@@ -49,6 +49,15 @@ def test_sizes(rows, k, n, dtype):
         _check(int8_linear(*args, b, dtype=dtype), *args, b, dtype)
 
 
+@pytest.mark.parametrize("rows,k,n", [(20, 8192, 100), (70, 16400, 72), (128, 9008, 256), (17, 65536, 16)])
+def test_long_sums_of_few_outputs(rows, k, n):
+    """k in parts that are joined: whole and partial last ones; and a longer call right behind a shorter one."""
+
+    args, bias = _operands(rows, k, n, seed=k)
+    _check(int8_linear(*args, bias, dtype=torch.float32), *args, bias, torch.float32)
+    _check(int8_linear(*args), *args, None, torch.bfloat16)
+
+
 @pytest.mark.parametrize("rows", [1, 7, 40, 300])
 @pytest.mark.parametrize("value", [-128, 127])
 def test_largest_sums(rows, value):
