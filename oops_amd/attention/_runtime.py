@@ -50,6 +50,34 @@ def require_same_device(operator: str, *tensors) -> None:
         raise ValueError(f"{operator} operands must share one device, got {sorted(map(str, devices))}")
 
 
+def on_one_device(device: torch.device, *tensors) -> bool:
+    """Whether every tensor that is not None is on ``device``."""
+
+    for t in tensors:
+        if t is not None and t.device != device:
+            return False
+    return True
+
+
+def wants_gradient(*tensors) -> bool:
+    """Whether a call of these operands (None ones aside) has to be recorded by autograd."""
+
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def call_on(device_index: int, entry, *args) -> int:
+    """A C entry point on a device's current stream (its last argument); the device becomes current for the call."""
+
+    if torch._C._cuda_getDevice() == device_index:
+        return entry(*args, torch._C._cuda_getCurrentRawStream(device_index))
+    with torch.cuda.device(device_index):
+        return entry(*args, torch._C._cuda_getCurrentRawStream(device_index))
+
+
 def needs_custom_op(tensor) -> bool:
     """True where an operator must go through its ``torch.library`` custom op (fake kernel, traced
     graph): under ``torch.compile``, for fake or subclass tensors and under a Python dispatch mode.

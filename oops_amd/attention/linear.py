@@ -22,12 +22,15 @@ from torch import Tensor
 
 from .. import _lib
 from .._errors import unsupported
-from ._core import SUPPORTED_DTYPES, _DTYPE_CODE, _on_device, _ptr, _stream
+from ._core import SUPPORTED_DTYPES, _DTYPE_CODE, _ptr
 from ._runtime import (
+    call_on,
     is_nested,
     needs_custom_op,
+    on_one_device,
     require_no_forward_mode,
     require_same_device,
+    wants_gradient,
     without_second_derivative,
 )
 
@@ -81,7 +84,7 @@ def linear_attention(
         s0 = initial_state.resolve_neg().reshape(q.shape[0], heads, d, e).contiguous()
     scale = d**-0.5 if scale is None else float(scale)
     ld = log_decay.resolve_neg().contiguous()
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (query, key, value, initial_state))
+    grad = wants_gradient(query, key, value, initial_state)
     args = (q, k, v, ld, lengths, s0, scale, bool(return_state))
     if needs_custom_op(q):
         out, state = linear_attention_forward(*args)
@@ -111,7 +114,7 @@ def linear_attention_step(
 
     operator = "linear_attention_step"
     _check(operator, query, key, value, log_decay, state, False)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, value, state)):
+    if wants_gradient(query, key, value, state):
         raise unsupported(operator, "has no gradient", hint="call it under torch.no_grad() or on detached tensors")
     if not state.is_contiguous():
         raise unsupported(operator, "updates the state in place: it must be contiguous", stride=state.stride())
@@ -126,11 +129,11 @@ def linear_attention_step(
 
 
 def _check(operator: str, query, key, value, log_decay, state, whole: bool) -> None:
-    tensors = (query, key, value, log_decay, state)
-    if any(is_nested(t) for t in tensors):
+    if is_nested(query) or is_nested(key) or is_nested(value):
         raise unsupported(operator, "takes dense tensors", hint="pad the batch and pass lengths")
-    require_no_forward_mode(operator, *tensors)
-    require_same_device(operator, *tensors)
+    require_no_forward_mode(operator, query, key, value, log_decay, state)
+    if not on_one_device(query.device, key, value, log_decay, state):
+        require_same_device(operator, query, key, value, log_decay, state)
     least = 3 if whole else 2
     names = "(*prefix, H, L, D)" if whole else "(*prefix, H, D)"
     if query.dim() < least or key.shape != query.shape or value.dim() != query.dim() or value.shape[:-1] != query.shape[:-1]:
@@ -213,8 +216,15 @@ def _geometry(lib, dtype, shape: tuple, e: int, scale: float, i64: bool, strides
     g.batch, g.length, g.scale, g.lengths_i64 = b, n, scale, int(i64)
     for i, s in enumerate(strides):
         g.stride[i][:] = s
-    ref = ctypes.byref(g)
-    return g, lib.oops_linear_attn_forward_workspace_bytes(ref), lib.oops_linear_attn_backward_workspace_bytes(ref)
+    ref = ctypes.pointer(g)
+    return ref, lib.oops_linear_attn_forward_workspace_bytes(ref), lib.oops_linear_attn_backward_workspace_bytes(ref)
+
+
+@functools.lru_cache(maxsize=512)
+def _step_geometry(lib, dtype, shape: tuple, e: int, scale: float, q: tuple, k: tuple, v: tuple):
+    b, h, d = shape
+    strides = ((*q[:2], 0), (*k[:2], 0), (*v[:2], 0), (h * e, e, 0))
+    return _geometry(lib, dtype, (b, h, 1, d), e, scale, False, strides)[0]
 
 
 def _strides(*tensors: Optional[Tensor]) -> tuple:
@@ -244,11 +254,8 @@ def _forward_with_workspace(q, k, v, log_decay, lengths, initial, scale, return_
     state = torch.empty((b, h, d, e) if return_state else 0, dtype=torch.float32, device=q.device)
     geo, ws_bytes, _ = _geometry(lib, q.dtype, tuple(q.shape), e, scale, _is_i64(lengths), _strides(q, k, v, out))
     ws = _workspace(ws_bytes, q.device)
-    with _on_device(q.device):
-        rc = lib.oops_linear_attn_forward(
-            ctypes.byref(geo), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(lengths), _ptr(initial), _ptr(out),
-            _ptr(state), _ptr(ws), ws_bytes, _stream(q.device),
-        )
+    rc = call_on(q.device.index, lib.oops_linear_attn_forward, geo, _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay),
+                 _ptr(lengths), _ptr(initial), _ptr(out), _ptr(state), _ptr(ws), ws_bytes)  # fmt: skip
     _lib.check(rc, "linear attention forward")
     return out, state, ws
 
@@ -269,11 +276,9 @@ def _backward_impl(dout: Tensor, dstate: Optional[Tensor], q: Tensor, k: Tensor,
     geo, _, ws_bytes = _geometry(lib, q.dtype, tuple(q.shape), e, scale, _is_i64(lengths),
                                  _strides(q, k, v, None, dout, dq, dk, dv))  # fmt: skip
     ws = _workspace(ws_bytes, q.device)
-    with _on_device(q.device):
-        rc = lib.oops_linear_attn_backward(
-            ctypes.byref(geo), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(lengths), _ptr(initial),
-            _ptr(forward_ws), _ptr(dout), _ptr(dstate), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ds), _ptr(ws), ws_bytes, _stream(q.device),
-        )
+    rc = call_on(q.device.index, lib.oops_linear_attn_backward, geo, _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay),
+                 _ptr(lengths), _ptr(initial), _ptr(forward_ws), _ptr(dout), _ptr(dstate), _ptr(dq), _ptr(dk), _ptr(dv),
+                 _ptr(ds), _ptr(ws), ws_bytes)  # fmt: skip
     _lib.check(rc, "linear attention backward")
     return dq, dk, dv, ds
 
@@ -282,14 +287,12 @@ def _step_impl(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor
     if state.is_neg():
         raise unsupported("linear_attention_step", "updates the state in place: it must not be a lazily negated view")
     lib = _lib.load()
-    b, h, d = q.shape
+    device = q.device
     e = v.shape[-1]
-    out = torch.empty(b, h, e, dtype=q.dtype, device=q.device)
-    strides = tuple((*t.stride()[:2], 0) for t in (q, k, v, out))
-    geo = _geometry(lib, q.dtype, (b, h, 1, d), e, scale, False, strides)[0]
-    with _on_device(q.device):
-        rc = lib.oops_linear_attn_step(ctypes.byref(geo), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state),
-                                       _ptr(out), _stream(q.device))  # fmt: skip
+    out = torch.empty((*q.shape[:2], e), dtype=q.dtype, device=device)
+    geo = _step_geometry(lib, q.dtype, q.shape, e, scale, q.stride(), k.stride(), v.stride())
+    rc = call_on(device.index, lib.oops_linear_attn_step, geo, _ptr(q), _ptr(k), _ptr(v), log_decay.data_ptr(),
+                 _ptr(state), _ptr(out))  # fmt: skip
     _lib.check(rc, "linear attention step")
     return out
 

@@ -19,8 +19,14 @@ from torch import Tensor
 
 from .. import _lib
 from .._errors import unsupported
-from ..attention._core import _on_device, _ptr, _stream
-from ..attention._runtime import needs_custom_op, require_no_forward_mode, require_same_device
+from ..attention._runtime import (
+    call_on,
+    needs_custom_op,
+    on_one_device,
+    require_no_forward_mode,
+    require_same_device,
+    wants_gradient,
+)
 
 _OPERATOR = "int8_linear"
 _DTYPE_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
@@ -50,9 +56,9 @@ def int8_linear(
     pointers that are multiples of 16 bytes are the fast case.
     """
 
-    tensors = (input, input_scale, weight, weight_scale, bias)
-    require_no_forward_mode(_OPERATOR, *tensors)
-    require_same_device(_OPERATOR, *tensors)
+    require_no_forward_mode(_OPERATOR, input, input_scale, weight, weight_scale, bias)
+    if not on_one_device(input.device, input_scale, weight, weight_scale, bias):
+        require_same_device(_OPERATOR, input, input_scale, weight, weight_scale, bias)
     if input.dim() < 1 or weight.dim() != 2 or input.shape[-1] != weight.shape[1]:
         raise ValueError(f"{_OPERATOR} takes input (..., K) and weight (N, K), got {tuple(input.shape)} and "
                          f"{tuple(weight.shape)}")  # fmt: skip
@@ -85,7 +91,7 @@ def int8_linear(
             bias_dtype=None if bias is None else bias.dtype,
             features=k,
         )
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input_scale, weight_scale, bias)):
+    if wants_gradient(input_scale, weight_scale, bias):
         raise unsupported(_OPERATOR, "has no gradient", hint="call it under torch.no_grad() or on detached tensors")
     rows = input_scale.numel()
     x = _rows(input if input.dim() == 2 else input.reshape(rows, k))
@@ -109,8 +115,8 @@ def _flat(t: Tensor) -> Tensor:
 def _geometry(lib, rows: int, n: int, k: int, x_row: int, w_row: int, out_dtype, bias_dtype) -> tuple:
     """The launch geometry and its workspace (cached: the library only reads it)."""
 
-    geo = _lib.Int8Geometry(rows, n, k, x_row, w_row, _DTYPE_CODE[out_dtype], _DTYPE_CODE[bias_dtype])
-    return geo, lib.oops_int8_linear_workspace_bytes(ctypes.byref(geo))
+    geo = ctypes.pointer(_lib.Int8Geometry(rows, n, k, x_row, w_row, _DTYPE_CODE[out_dtype], _DTYPE_CODE[bias_dtype]))
+    return geo, lib.oops_int8_linear_workspace_bytes(geo)
 
 
 def _forward_impl(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor],
@@ -120,11 +126,12 @@ def _forward_impl(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tens
     n = weight.shape[0]
     geo, ws_bytes = _geometry(lib, rows, n, k, x.stride(0) if rows > 1 else k, weight.stride(0) if n > 1 else k, dtype,
                               dtype if bias is None else bias.dtype)  # fmt: skip
-    out = torch.empty(rows, n, dtype=dtype, device=x.device)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-    with _on_device(x.device):
-        rc = lib.oops_int8_linear(ctypes.byref(geo), _ptr(x), _ptr(x_scale), _ptr(weight), _ptr(weight_scale),
-                                  _ptr(bias), _ptr(out), _ptr(ws), ws_bytes, _stream(x.device))  # fmt: skip
+    device = x.device
+    out = torch.empty((rows, n), dtype=dtype, device=device)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+    rc = call_on(device.index, lib.oops_int8_linear, geo, x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(),
+                 weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
+                 None if ws is None else ws.data_ptr(), ws_bytes)
     _lib.check(rc, _OPERATOR)
     return out
 

@@ -22,13 +22,16 @@ from torch import Tensor
 from .. import _lib
 from .._errors import unsupported
 from ..attention._runtime import (
+    call_on,
     is_nested,
     needs_custom_op,
+    on_one_device,
     require_no_forward_mode,
     require_same_device,
+    wants_gradient,
     without_second_derivative,
 )
-from .layer_norm import _on_device, _ptr, _stream
+from .layer_norm import _ptr
 
 _DTYPE_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 MAX_WIDTH = 16384
@@ -61,7 +64,7 @@ def rms_norm(
     _check("rms_norm", input, normalized_shape, weight, residual)
     x, r = _rows(input), _rows(residual)
     w = None if weight is None else weight.resolve_neg().contiguous()
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, residual))
+    grad = wants_gradient(input, weight, residual)
     if needs_custom_op(x):
         y, summed, _ = rms_norm_forward(x, w, r, float(eps), grad)
     elif grad:
@@ -97,8 +100,10 @@ def rms_norm_int8(
     w = None if weight is None else weight.resolve_neg().contiguous()
     call = rms_norm_int8_forward if needs_custom_op(x) else _int8_impl
     values, scales, summed = call(x, w, r, float(eps))
-    values, scales = values.view(input.shape), scales.view(input.shape[:-1])
-    return (values, scales) if residual is None else (values, scales, summed.view(input.shape))
+    if input.dim() != 2:
+        values, scales = values.view(input.shape), scales.view(input.shape[:-1])
+        summed = summed.view(input.shape) if residual is not None else summed
+    return (values, scales) if residual is None else (values, scales, summed)
 
 
 def quantize_int8(input: Tensor) -> Tuple[Tensor, Tensor]:
@@ -115,7 +120,7 @@ def quantize_int8(input: Tensor) -> Tuple[Tensor, Tensor]:
     x = _rows(input)
     call = quantize_int8_forward if needs_custom_op(x) else _quantize_impl
     values, scales = call(x)
-    return values.view(input.shape), scales.view(input.shape[:-1])
+    return (values, scales) if input.dim() == 2 else (values.view(input.shape), scales.view(input.shape[:-1]))
 
 
 # ----------------------------------------------------------------- checks
@@ -123,7 +128,8 @@ def quantize_int8(input: Tensor) -> Tuple[Tensor, Tensor]:
 
 def _check(operator: str, input: Tensor, normalized_shape, weight: Optional[Tensor], residual: Optional[Tensor]) -> None:
     require_no_forward_mode(operator, input, weight, residual)
-    require_same_device(operator, input, weight, residual)
+    if not on_one_device(input.device, weight, residual):
+        require_same_device(operator, input, weight, residual)
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     if len(shape) != 1:
         raise unsupported(operator, "normalizes over the final dimension only", normalized_shape=shape)
@@ -154,7 +160,7 @@ def _check(operator: str, input: Tensor, normalized_shape, weight: Optional[Tens
 
 
 def _require_inference(operator: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if wants_gradient(*tensors):
         raise unsupported(operator, "has no gradient", hint="call it under torch.no_grad() or on detached tensors")
 
 
@@ -193,13 +199,13 @@ def _rows(t: Optional[Tensor]) -> Optional[Tensor]:
 
 
 @functools.lru_cache(maxsize=256)
-def _geometry(dtype, weight_f32: bool, rows: int, width: int, x_row: int, r_row: int, eps: float) -> _lib.RmsNormGeometry:
+def _geometry(dtype, weight_f32: bool, rows: int, width: int, x_row: int, r_row: int, eps: float) -> "ctypes._Pointer":
     """The launch geometry (cached: the library only reads it)."""
 
-    return _lib.RmsNormGeometry(_DTYPE_CODE[dtype], int(weight_f32), width, eps, rows, x_row, r_row)
+    return ctypes.pointer(_lib.RmsNormGeometry(_DTYPE_CODE[dtype], int(weight_f32), width, eps, rows, x_row, r_row))
 
 
-def _geometry_of(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float) -> _lib.RmsNormGeometry:
+def _geometry_of(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], eps: float) -> "ctypes._Pointer":
     rows, width = x.shape
     x_row = x.stride(0) if rows > 1 else width
     r_row = residual.stride(0) if residual is not None and rows > 1 else width
@@ -208,8 +214,7 @@ def _geometry_of(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor]
 
 @functools.lru_cache(maxsize=64)
 def _workspace_bytes(lib, dtype, weight_f32: bool, rows: int, width: int) -> int:
-    geo = _geometry(dtype, weight_f32, rows, width, width, width, 0.0)
-    return lib.oops_rms_norm_backward_workspace_bytes(ctypes.byref(geo))
+    return lib.oops_rms_norm_backward_workspace_bytes(_geometry(dtype, weight_f32, rows, width, width, width, 0.0))
 
 
 def _empty_rows(x: Tensor, dtype=None) -> Tensor:
@@ -223,9 +228,8 @@ def _forward_impl(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor
     summed = _empty_rows(x) if residual is not None else x.new_empty(0)
     rstd = torch.empty(x.shape[0] if save else 0, dtype=torch.float32, device=x.device)
     geo = _geometry_of(x, weight, residual, eps)
-    with _on_device(x.device):
-        rc = lib.oops_rms_norm_forward(ctypes.byref(geo), _ptr(x), _ptr(residual), _ptr(weight), _ptr(y),
-                                       _ptr(summed), _ptr(rstd), _stream(x.device))  # fmt: skip
+    rc = call_on(x.device.index, lib.oops_rms_norm_forward, geo, _ptr(x), _ptr(residual), _ptr(weight), _ptr(y),
+                 _ptr(summed), _ptr(rstd))  # fmt: skip
     _lib.check(rc, "rms_norm forward")
     return y, summed, rstd
 
@@ -236,9 +240,8 @@ def _int8_impl(x: Tensor, weight: Optional[Tensor], residual: Optional[Tensor], 
     summed = _empty_rows(x) if residual is not None else x.new_empty(0)
     scales = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
     geo = _geometry_of(x, weight, residual, eps)
-    with _on_device(x.device):
-        rc = lib.oops_rms_norm_int8(ctypes.byref(geo), _ptr(x), _ptr(residual), _ptr(weight), _ptr(values),
-                                    _ptr(scales), _ptr(summed), _stream(x.device))  # fmt: skip
+    rc = call_on(x.device.index, lib.oops_rms_norm_int8, geo, _ptr(x), _ptr(residual), _ptr(weight), _ptr(values),
+                 _ptr(scales), _ptr(summed))  # fmt: skip
     _lib.check(rc, "rms_norm_int8")
     return values, scales, summed
 
@@ -248,8 +251,7 @@ def _quantize_impl(x: Tensor) -> Tuple[Tensor, Tensor]:
     values = _empty_rows(x, torch.int8)
     scales = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
     geo = _geometry_of(x, None, None, 0.0)
-    with _on_device(x.device):
-        rc = lib.oops_quantize_int8(ctypes.byref(geo), _ptr(x), _ptr(values), _ptr(scales), _stream(x.device))
+    rc = call_on(x.device.index, lib.oops_quantize_int8, geo, _ptr(x), _ptr(values), _ptr(scales))
     _lib.check(rc, "quantize_int8")
     return values, scales
 
@@ -270,9 +272,8 @@ def _backward_impl(dy: Tensor, dsum: Optional[Tensor], h: Tensor, weight: Option
     ws_bytes = _workspace_bytes(lib, h.dtype, f32, rows, width) if need_weight else 0
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=h.device) if ws_bytes else None
     geo = _geometry_of(h, weight, None, 0.0)
-    with _on_device(h.device):
-        rc = lib.oops_rms_norm_backward(ctypes.byref(geo), _ptr(h), _ptr(rstd), _ptr(weight), _ptr(dy), _ptr(dsum),
-                                        _ptr(dx), _ptr(dw), _ptr(ws), ws_bytes, _stream(h.device))  # fmt: skip
+    rc = call_on(h.device.index, lib.oops_rms_norm_backward, geo, _ptr(h), _ptr(rstd), _ptr(weight), _ptr(dy), _ptr(dsum),
+                 _ptr(dx), _ptr(dw), _ptr(ws), ws_bytes)  # fmt: skip
     _lib.check(rc, "rms_norm backward")
     return dx, dw
 
