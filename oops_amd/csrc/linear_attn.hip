@@ -62,7 +62,9 @@ __device__ __forceinline__ int opaque(int x) {
 // where they are read by the second products, once each (different terms of
 // the output, 2^-8 of each at most, as in softmax attention).  The update's
 // operand u l^n c is split into three bfloat16 terms, which hold its float32
-// value: the state that is returned is a float32 one.
+// value, where the state is kept (the last state is a float32 result), and into
+// two (2^-16) where it only goes into the segment's own outputs: walks in
+// several segments have their last state from walk_scan_kernel.
 constexpr int kChunk = 64;
 
 struct ChunkArgs {
@@ -101,9 +103,7 @@ __device__ __forceinline__ bf16x8 to_bf16x8(const float (&x)[8]) {
                                                fast::pack2<__bf16>(x[4], x[5]), fast::pack2<__bf16>(x[6], x[7])));
 }
 
-constexpr int kTerms = 3;
-
-template <int D, bool VEC, bool MAIN>
+template <int D, bool VEC, bool MAIN, int kTerms>
 __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(ChunkArgs ca) {
   using T = __bf16;
   using Frag = bf16x8;
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t bh = (int64_t)blockIdx.x / ca.segs;
   const int seg = (int)((int64_t)blockIdx.x % ca.segs);
-  if (!MAIN && seg == ca.segs - 1) return;  // (no segment starts from its state)
+  if (!MAIN && seg == ca.segs - 1 && !w.final_state) return;  // (no segment starts from its state)
   const int64_t b = bh / w.heads;
   const int h = (int)(bh % w.heads);
   const int64_t n = walk_length(w, b);
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(Ch
   // the state behind the segment, or behind the sequence
   float* to = nullptr;
   if (!MAIN) to = ca.starts + (bh * ca.segs + seg) * state_size;
-  else if (w.final_state && (n > 0 ? s0 < n && n <= s0 + ca.seg_tokens : seg == 0)) to = w.final_state + bh * state_size;
+  else if (kTerms == 3 && w.final_state) to = w.final_state + bh * state_size;
   if (to) {
     const int g_ = opaque(g), col_ = opaque(col);
     const auto rsrc = make_rsrc(to, (uint32_t)state_size * 4);
@@ -600,8 +600,9 @@ __global__ __launch_bounds__(2 * D, 2) void walk_exact_kernel(ChunkArgs ca) {
 }
 
 // Segments' own states to the states they start from, in place and in order:
-// start_0 = initial, start_(s+1) = l^(tokens of s) start_s + own_s.
-__global__ __launch_bounds__(kThreads) void walk_scan_kernel(ChunkArgs ca) {
+// start_0 = initial, start_(s+1) = l^(tokens of s) start_s + own_s; the last
+// state, where it is wanted here.
+__global__ __launch_bounds__(kThreads) void walk_scan_kernel(ChunkArgs ca, float* last) {
   const LinearWalk& w = ca.w;
   const int64_t size = (int64_t)w.rows * w.cols;
   const int64_t bh = blockIdx.y, at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -615,7 +616,7 @@ __global__ __launch_bounds__(kThreads) void walk_scan_kernel(ChunkArgs ca) {
   for (int s0 = 0; s0 < ca.segs; s0 += U) {
     float x[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) x[i] = s0 + i < ca.segs - 1 ? own[(s0 + i) * size] : 0.f;
+    for (int i = 0; i < U; ++i) x[i] = s0 + i < ca.segs - (last ? 0 : 1) ? own[(s0 + i) * size] : 0.f;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       if (s0 + i >= ca.segs) break;
@@ -625,6 +626,7 @@ __global__ __launch_bounds__(kThreads) void walk_scan_kernel(ChunkArgs ca) {
       cur = __builtin_fmaf(cur, lm, x[i]);
     }
   }
+  if (last) last[bh * size + at] = cur;
 }
 
 // ---------------------------------------------------------------- one token
@@ -740,10 +742,12 @@ bool rows16(const void* p, const int64_t (&stride)[3], int width, int element) {
 
 template <typename T, int D, bool VEC, bool MAIN>
 void launch_chunks(const ChunkArgs& ca, dim3 grid, hipStream_t stream) {
-  if constexpr (std::is_same_v<T, __bf16>)
-    hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, MAIN>), grid, dim3(2 * D), 0, stream, ca);
-  else
+  if constexpr (!std::is_same_v<T, __bf16>)
     hipLaunchKernelGGL((walk_exact_kernel<T, D, VEC, MAIN>), grid, dim3(2 * D), 0, stream, ca);
+  else if (MAIN && ca.segs > 1)
+    hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, MAIN, MAIN ? 2 : 3>), grid, dim3(2 * D), 0, stream, ca);
+  else
+    hipLaunchKernelGGL((walk_chunks_kernel<D, VEC, MAIN, 3>), grid, dim3(2 * D), 0, stream, ca);
 }
 
 template <typename T, int D, bool VEC>
@@ -754,8 +758,8 @@ hipError_t run_chunks(const ChunkArgs& ca, bool starts, hipStream_t stream) {
   if (starts) {
     launch_chunks<T, D, VEC, false>(ca, grid, stream);
     hipLaunchKernelGGL(walk_scan_kernel, dim3((unsigned)((w.rows * w.cols + kThreads - 1) / kThreads), bh),
-                       dim3(kThreads), 0, stream, ca);
-  } else {
+                       dim3(kThreads), 0, stream, ca, std::is_same_v<T, __bf16> ? w.final_state : nullptr);
+  } else if (w.out || ca.segs == 1 || !std::is_same_v<T, __bf16>) {
     launch_chunks<T, D, VEC, true>(ca, grid, stream);
   }
   return hipGetLastError();
