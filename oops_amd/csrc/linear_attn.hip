@@ -104,7 +104,7 @@ __device__ __forceinline__ bf16x8 to_bf16x8(const float (&x)[8]) {
 }
 
 template <int D, bool VEC, bool MAIN, int kTerms>
-__global__ __launch_bounds__(2 * D, D == 128 ? 2 : 4) void walk_chunks_kernel(ChunkArgs ca) {
+__global__ __launch_bounds__(2 * D, MAIN || D == 128 ? 2 : 4) void walk_chunks_kernel(ChunkArgs ca) {
   using T = __bf16;
   using Frag = bf16x8;
   constexpr int NT = 2 * D, NW = D / 32;      // threads, waves: 32 columns each
@@ -721,13 +721,20 @@ hipError_t by_type(int dtype, F&& f) {
 
 namespace {
 
-// Segments of a walk: enough workgroups for two on each CU, segments of at
-// least kMinSegChunks chunks (a segment's state costs its traffic once more).
-constexpr int64_t kTargetWalks = 512;
-constexpr int64_t kMinSegChunks = 4;
+// Segments of a walk.  They cost its state's traffic and half its products once
+// more, so walks that give most CUs a workgroup go in one (256 heads x 512
+// tokens x 128: 42 us, in two segments 91).  Others get segments of at least
+// four chunks until there are eight waves a CU, or of two while there are not
+// four (16 x 1024 x 128: 34 us, with four chunks 42; 8 x 8192 x 128: 57, 51).
 void plan_segments(const LinearWalk& w, ChunkArgs& ca) {
   const int64_t chunks = std::max<int64_t>(1, (w.length + kChunk - 1) / kChunk), bh = w.batch * w.heads;
-  int64_t segs = std::min((kTargetWalks + bh - 1) / bh, (chunks + kMinSegChunks - 1) / kMinSegChunks);
+  const int widest = std::max(w.rows, w.cols);
+  const int64_t wide = widest <= 32 ? 4 : widest <= 64 ? 2 : 1;  // workgroups of four waves' worth
+  int64_t segs = 1;
+  if (bh < 192 * wide) {
+    segs = std::min((512 * wide + bh - 1) / bh, (chunks + 3) / 4);
+    segs = std::max(segs, std::min((256 * wide + bh - 1) / bh, (chunks + 1) / 2));
+  }
   const int64_t per = (chunks + segs - 1) / segs;
   ca.segs = (int32_t)((chunks + per - 1) / per);
   ca.seg_tokens = (int32_t)(per * kChunk);

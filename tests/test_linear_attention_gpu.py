@@ -142,6 +142,19 @@ def test_ragged_batches(dtype, kind):
     assert torch.equal(linear_attention(*clean_qkv(clean), x["ld"], x["s0"], over), ref)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,e", [(128, 128), (64, 40), (24, 32)])
+def test_ragged_batches_in_segments(dtype, d, e):
+    """Sequences that end in the first, a middle and the last of a walk's segments, at their borders and before them."""
+
+    n = 900
+    lengths = torch.tensor([n, 0, 1, 128, 129, 500, 512, 700], dtype=torch.int32, device=DEV)
+    x = _case(13, 8, 1, n, d, e, dtype)
+    _run(x, lengths)
+    x = {k: t for k, t in x.items() if k not in ("s0", "ds")}
+    _run(x, lengths)
+
+
 def clean_qkv(x):
     return x["q"], x["k"], x["v"]
 
