@@ -228,7 +228,8 @@ __global__ __launch_bounds__(kThreads, 1) void int8_tile_kernel(Int8Args a, int 
     multiply(fx[1], fw[1], -1);
     __builtin_amdgcn_sched_barrier(0);
   }
-  fast::vmem_wait<0>();  // (no load may land in LDS that is another workgroup's by then)
+  fast::vmem_wait<0>();  // (no load may land in LDS that is used otherwise by then, or another workgroup's)
+  lds_barrier();
 
   // out[r0 + wr + 32 p + l][j0 + wj + 32 q + kappa(half, i)]
   if (BM * BN == 64 * 64 && a.parts > 1) {
@@ -251,8 +252,12 @@ __global__ __launch_bounds__(kThreads, 1) void int8_tile_kernel(Int8Args a, int 
     const int64_t r = r0 + wr + 32 * p + l;
     scale_x[p] = r < a.rows ? a.x_scale[r] : 0.f;
   }
-  constexpr int V = 16 / sizeof(T);
+  // Whole lines to memory: a wave's rows of 128 bytes (64 outputs of 16 bits, 32 of float32) pass through 16 KB of LDS
+  // of its own, from lanes that hold a row each to eight lanes a row; slots are XORed with the row.
+  constexpr int V = 16 / sizeof(T), kTilesLine = sizeof(T) == 4 || TJ == 1 ? 1 : 2;  // column tiles of a line
+  constexpr int kLanes = kTilesLine * 32 / V;                                        // lanes of a line (64 bytes: TJ 1)
   const bool vec = a.n % V == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+  char* line = lds + wave * (BM / 2 * 128);
 #pragma unroll
   for (int q = 0; q < TJ; ++q) {
     float scale_w[16], add[16];
@@ -265,28 +270,40 @@ __global__ __launch_bounds__(kThreads, 1) void int8_tile_kernel(Int8Args a, int 
 #pragma unroll
     for (int p = 0; p < TR; ++p) {
       const int64_t r = r0 + wr + 32 * p + l, jq = j0 + wj + 32 * q;
-      T* row = static_cast<T*>(a.out) + (r < a.rows ? r : 0) * a.n;
       float y[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) y[i] = __builtin_fmaf((float)acc[q][p][i] * scale_x[p], scale_w[i], add[i]);
       if (!vec) {
+        T* row = static_cast<T*>(a.out) + (r < a.rows ? r : 0) * a.n;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (r < a.rows && jq + kappa(half, i) < a.n) row[jq + kappa(half, i)] = (T)y[i];
-      } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          if (r < a.rows && jq + kappa(half, i) < a.n)
-            *reinterpret_cast<f32x4*>(row + jq + kappa(half, i)) = f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
       } else {
-        uint32_t pk[8];
+        char* to = line + (32 * p + l) * 128;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pk[i] = fast::pack2<T>(y[2 * i], y[2 * i + 1]);
-        uint4 lo, hi;
-        fast::trade16(pk, lo, hi);
-        const int64_t j = jq + 16 * half;
-        if (r < a.rows && j < a.n) *reinterpret_cast<uint4*>(row + j) = lo;
-        if (r < a.rows && j + 8 < a.n) *reinterpret_cast<uint4*>(row + j + 8) = hi;
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<f32x4*>(to + (((i / 2 + half) ^ (l & 7)) << 4)) = f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
+        } else {
+          uint32_t pk[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pk[i] = fast::pack2<T>(y[2 * i], y[2 * i + 1]);
+          uint4 lo, hi;
+          fast::trade16(pk, lo, hi);  // this lane: columns 16 half .. and 16 half + 8 .. of its row
+          const int c = q % kTilesLine * 4 + 2 * half;
+          *reinterpret_cast<uint4*>(to + ((c ^ (l & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(to + (((c + 1) ^ (l & 7)) << 4)) = hi;
+        }
+      }
+    }
+    if (vec && q % kTilesLine == kTilesLine - 1) {
+      const int64_t j = j0 + wj + 32 * (q - kTilesLine + 1) + lane % kLanes * V;
+#pragma unroll
+      for (int i = 0; i < BM / 2 * kLanes / 64; ++i) {
+        const int row = (i * 64 + lane) / kLanes;
+        const uint4 u = *reinterpret_cast<const uint4*>(line + row * 128 + ((lane % kLanes ^ (row & 7)) << 4));
+        const int64_t r = r0 + wr + row;
+        if (r < a.rows && j < a.n) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + r * a.n + j) = u;
       }
     }
   }
@@ -301,7 +318,8 @@ __global__ __launch_bounds__(kThreads, 1) void int8_tile_kernel(Int8Args a, int 
 // W U lines are k where it can be had: all loads of a wave then fly at once
 // (4 x 4096 x 16384: W, U = 8, 4 16.0 us or 4.2 TB/s; 4, 8 18.4; 16, 4 20.2;
 // 8 x 1024 x 50000: 8, 2 15.7; 8, 4 22.6;  4 x 16384 x 4096: 16, 4 16.1; 8, 4 22.3).
-template <typename T, int W, int U>
+// WHOLE: rows of whole 16-byte pieces at aligned places; else any.
+template <typename T, int W, int U, bool WHOLE>
 __global__ __launch_bounds__(64 * W) void int8_few_kernel(Int8Args a) {
   __shared__ i32x4 red[W][64];
   const int tid = threadIdx.x, lane = tid & 63, row = lane & 15, part = lane >> 4;
@@ -319,9 +337,14 @@ __global__ __launch_bounds__(64 * W) void int8_few_kernel(Int8Args a) {
 #pragma unroll
     for (int u = 0; u < 2 * U; ++u) {
       const int k = k0 + (u / 2) * W * 128 + (u % 2) * 64;
-      const bool in = k + part * 16 < a.k;
-      fw[u] = __builtin_bit_cast(i32x4, buffer_load16(rw, in ? vw + k : fast::kOut));
-      fx[u] = __builtin_bit_cast(i32x4, buffer_load16(rx, in && row < a.rows ? vx + k : fast::kOut));
+      if constexpr (WHOLE) {
+        const bool in = k + part * 16 < a.k;
+        fw[u] = __builtin_bit_cast(i32x4, buffer_load16(rw, in ? vw + k : fast::kOut));
+        fx[u] = __builtin_bit_cast(i32x4, buffer_load16(rx, in && row < a.rows ? vx + k : fast::kOut));
+      } else {
+        fw[u] = load_bytes(a.w + (j0 + (row < left ? row : 0)) * a.w_row, k + part * 16, a.k, row < left);
+        fx[u] = load_bytes(a.x + (row < a.rows ? row : 0) * a.x_row, k + part * 16, a.k, row < a.rows);
+      }
     }
 #pragma unroll
     for (int u = 0; u < 2 * U; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], fx[u], acc, 0, 0, 0);
@@ -338,6 +361,27 @@ __global__ __launch_bounds__(64 * W) void int8_few_kernel(Int8Args a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (j + i < a.n) out[i] = (T)__builtin_fmaf((float)sum[i] * sx, a.w_scale[j + i], bias_at<T>(a, j + i));
+}
+
+// ---------------------------------------------------------------- padded operands
+//
+// Rows that are no whole pieces at aligned places, copied to ones that are
+// (zeros behind k): two passes over the bytes, where the products are many
+// enough that whole tiles earn them back.
+struct PadArgs {
+  const int8_t* from[2];
+  int8_t* to[2];
+  int64_t rows[2], stride[2];
+  int32_t k, pieces;  // 16-byte pieces of a padded row
+};
+__global__ __launch_bounds__(kThreads) void int8_pad_kernel(PadArgs a) {
+  const int64_t first = a.rows[0] * a.pieces, all = first + a.rows[1] * a.pieces;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kThreads) {
+    const int op = i >= first;
+    const int64_t at = op ? i - first : i, row = at / a.pieces;
+    const int piece = (int)(at - row * a.pieces);
+    reinterpret_cast<i32x4*>(a.to[op])[at] = load_bytes(a.from[op] + row * a.stride[op], piece * 16, a.k, true);
+  }
 }
 
 // ---------------------------------------------------------------- joined parts
@@ -367,6 +411,7 @@ bool aligned_rows(const void* p, int64_t rows, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || (stride % 16 == 0 && stride < (int64_t(1) << 22)));
 }
 
+template <bool WHOLE>
 hipError_t run_few(const oops_int8_geometry& g, Int8Args a, hipStream_t stream) {
   if (g.rows == 1) a.x_row = g.k;
   if (g.n == 1) a.w_row = g.k;
@@ -374,11 +419,11 @@ hipError_t run_few(const oops_int8_geometry& g, Int8Args a, hipStream_t stream) 
   return by_type(g.out_dtype, [&](auto tag) {
     using T = decltype(tag);
     if (g.k <= 2048)
-      hipLaunchKernelGGL((int8_few_kernel<T, 8, 2>), grid, dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((int8_few_kernel<T, 8, 2, WHOLE>), grid, dim3(512), 0, stream, a);
     else if (g.k <= 4096)
-      hipLaunchKernelGGL((int8_few_kernel<T, 8, 4>), grid, dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((int8_few_kernel<T, 8, 4, WHOLE>), grid, dim3(512), 0, stream, a);
     else
-      hipLaunchKernelGGL((int8_few_kernel<T, 16, 4>), grid, dim3(1024), 0, stream, a);
+      hipLaunchKernelGGL((int8_few_kernel<T, 16, 4, WHOLE>), grid, dim3(1024), 0, stream, a);
     return hipGetLastError();
   });
 }
@@ -409,6 +454,21 @@ KParts k_parts(const oops_int8_geometry& g) {
   return {(int)((g.k + per - 1) / per), (int)per};
 }
 
+// Operands to be copied to padded rows (a size's own: pointers off 16 bytes go to int8_any_kernel).
+struct Pads {
+  bool x, w;
+  int64_t row, x_bytes, w_bytes;
+};
+Pads pads(const oops_int8_geometry& g) {
+  Pads p{g.k % 16 != 0 || (g.rows > 1 && g.x_row % 16 != 0), g.k % 16 != 0 || (g.n > 1 && g.w_row % 16 != 0),
+         (g.k + 15) / 16 * 16, 0, 0};
+  // (1024 x 4097 x 4096: 40 us, int8_any_kernel 73; 512 x 2001 x 4096: 22.5, 24; 256 x 1001 x 1024: no gain)
+  if (few_rows(g) || (double)g.rows * (double)g.n * (double)g.k < 1e9) p.x = p.w = false;
+  if (p.x) p.x_bytes = (g.rows * p.row + 255) / 256 * 256;
+  if (p.w) p.w_bytes = (g.n * p.row + 255) / 256 * 256;
+  return p;
+}
+
 template <int BM, int BN, int NB>
 hipError_t run_tiles(const oops_int8_geometry& g, Int8Args a, hipStream_t stream) {
   if (g.rows == 1) a.x_row = g.k;
@@ -424,42 +484,78 @@ hipError_t run_tiles(const oops_int8_geometry& g, Int8Args a, hipStream_t stream
 
 }  // namespace
 
+namespace {
+
+// whole rows: the kernels by size, `sums` for the parts of k
+hipError_t run_whole(const oops_int8_geometry& g, Int8Args a, void* sums, hipStream_t stream) {
+  if (few_rows(g)) return run_few<true>(g, a, stream);
+  // the largest tile that gives (nearly) every CU one, measured in us at rows x n x k:
+  //   4096 x 4096 x 4096: 256^2 69, 128^2 83 (two a CU);   2048 x 4096 x 4096: 256^2 56, 128^2 40
+  //   1024 x 4096 x 4096: 128^2 24 (four buffers; two: 31), 64 x 128 29;   512 x 4096 x 4096: 128^2 21, 64 x 128 17
+  const int64_t t128 = tiles_of(g, 128, 128);
+  if (tiles_of(g, 256, 256) >= 192) return run_tiles<256, 256, 2>(g, a, stream);
+  if (t128 > 256) return run_tiles<128, 128, 2>(g, a, stream);
+  if (t128 >= 192) return run_tiles<128, 128, 4>(g, a, stream);
+  if (tiles_of(g, 64, 128) >= 192) return run_tiles<64, 128, 4>(g, a, stream);
+  const KParts kp = k_parts(g);
+  a.sums = static_cast<int32_t*>(sums);
+  a.parts = kp.parts;
+  a.part_k = kp.part_k;
+  const hipError_t e = run_tiles<64, 64, 4>(g, a, stream);
+  if (e != hipSuccess || a.parts == 1) return e;
+  return by_type(g.out_dtype, [&](auto tag) {
+    using T = decltype(tag);
+    const int64_t blocks = std::min<int64_t>((g.rows * g.n + kThreads - 1) / kThreads, 2048);
+    hipLaunchKernelGGL((int8_join_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+  });
+}
+
+// The geometry of the padded operands (of the given ones where nothing is padded).
+oops_int8_geometry padded(const oops_int8_geometry& g, const Pads& p) {
+  oops_int8_geometry t = g;
+  if (p.x || p.w) t.k = p.row;  // (a padded row's zeros meet zeros, or bytes of the other operand that is whole)
+  if (p.x) t.x_row = p.row;
+  if (p.w) t.w_row = p.row;
+  return t;
+}
+
+}  // namespace
+
 size_t int8_linear_workspace_bytes(const oops_int8_geometry& g) {
-  const int parts = k_parts(g).parts;
-  return parts > 1 ? (size_t)parts * (size_t)g.rows * (size_t)g.n * sizeof(int32_t) : 0;
+  const Pads p = pads(g);
+  const int parts = k_parts(padded(g, p)).parts;
+  return (size_t)(p.x_bytes + p.w_bytes) + (parts > 1 ? (size_t)parts * (size_t)g.rows * (size_t)g.n * sizeof(int32_t) : 0);
 }
 
 hipError_t launch_int8_linear(const oops_int8_geometry& g, const void* x, const float* x_scale, const void* w,
                               const float* w_scale, const void* bias, void* out, void* workspace, hipStream_t stream) {
   Int8Args a{static_cast<const int8_t*>(x), static_cast<const int8_t*>(w), x_scale, w_scale, bias, out, g.rows, g.n,
              g.x_row, g.w_row, (int32_t)g.k, g.bias_dtype == OOPS_F32, nullptr, 1, (int32_t)g.k};
-  const bool whole = g.k > 0 && g.k % 16 == 0 && aligned_rows(x, g.rows, g.x_row) && aligned_rows(w, g.n, g.w_row) &&
-                     tiles_of(g, 64, 64) < kMaxTiles;
-  if (whole) {
-    if (few_rows(g)) return run_few(g, a, stream);
-    // the largest tile that gives (nearly) every CU one, measured in us at rows x n x k:
-    //   4096 x 4096 x 4096: 256^2 69, 128^2 83 (two a CU);   2048 x 4096 x 4096: 256^2 56, 128^2 40
-    //   1024 x 4096 x 4096: 128^2 24 (four buffers; two: 31), 64 x 128 29;   512 x 4096 x 4096: 128^2 21, 64 x 128 17
-    const int64_t t128 = tiles_of(g, 128, 128);
-    if (tiles_of(g, 256, 256) >= 192) return run_tiles<256, 256, 2>(g, a, stream);
-    if (t128 > 256) return run_tiles<128, 128, 2>(g, a, stream);
-    if (t128 >= 192) return run_tiles<128, 128, 4>(g, a, stream);
-    if (tiles_of(g, 64, 128) >= 192) return run_tiles<64, 128, 4>(g, a, stream);
-    const KParts kp = k_parts(g);
-    a.sums = static_cast<int32_t*>(workspace);
-    a.parts = kp.parts;
-    a.part_k = kp.part_k;
-    const hipError_t e = run_tiles<64, 64, 4>(g, a, stream);
-    if (e != hipSuccess || a.parts == 1) return e;
-    return by_type(g.out_dtype, [&](auto tag) {
-      using T = decltype(tag);
-      const int64_t blocks = std::min<int64_t>((g.rows * g.n + kThreads - 1) / kThreads, 2048);
-      hipLaunchKernelGGL((int8_join_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
-      return hipGetLastError();
-    });
-  }
   const int64_t tiles = tiles_of(g, 64, 64);
-  if (tiles > kMaxTiles) return hipErrorInvalidConfiguration;
+  const Pads p = pads(g);
+  const oops_int8_geometry t = padded(g, p);
+  const bool whole = g.k > 0 && t.k % 16 == 0 && (p.x || aligned_rows(x, g.rows, g.x_row)) &&
+                     (p.w || aligned_rows(w, g.n, g.w_row)) && tiles < kMaxTiles;
+  if (whole) {
+    char* ws = static_cast<char*>(workspace);
+    if (p.x || p.w) {
+      PadArgs pa{{a.x, a.w}, {reinterpret_cast<int8_t*>(ws), reinterpret_cast<int8_t*>(ws + p.x_bytes)},
+                 {p.x ? g.rows : 0, p.w ? g.n : 0}, {g.x_row, g.w_row}, (int32_t)g.k, (int32_t)(p.row / 16)};
+      const int64_t pieces = (pa.rows[0] + pa.rows[1]) * pa.pieces;
+      const dim3 grid((unsigned)std::min<int64_t>((pieces + kThreads - 1) / kThreads, 8192));
+      hipLaunchKernelGGL(int8_pad_kernel, grid, dim3(kThreads), 0, stream, pa);
+      if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+      if (p.x) a.x = pa.to[0];
+      if (p.w) a.w = pa.to[1];
+      a.k = a.part_k = (int32_t)t.k;
+      a.x_row = t.x_row;
+      a.w_row = t.w_row;
+    }
+    return run_whole(t, a, ws + p.x_bytes + p.w_bytes, stream);
+  }
+  if (few_rows(g)) return run_few<false>(g, a, stream);
+  if (tiles >= kMaxTiles) return hipErrorInvalidConfiguration;
   return by_type(g.out_dtype, [&](auto tag) {
     using T = decltype(tag);
     hipLaunchKernelGGL((int8_any_kernel<T>), dim3((unsigned)tiles), dim3(kThreads), 0, stream, a);

@@ -411,7 +411,7 @@ __global__ __launch_bounds__(2 * D, MAIN || D == 128 ? 2 : 4) void walk_chunks_k
 constexpr int kExactChunk = 32;
 
 template <typename T, int D, bool VEC, bool MAIN>
-__global__ __launch_bounds__(2 * D, 2) void walk_exact_kernel(ChunkArgs ca) {
+__global__ __launch_bounds__(2 * D, D == 32 ? 2 : 1) void walk_exact_kernel(ChunkArgs ca) {
   constexpr int NT = 2 * D, NW = D / 32;
   constexpr int VE = 16 / sizeof(T), CPR = D / VE;           // elements of a load, loads of a row
   constexpr int NL = kExactChunk * CPR / NT, kRows = NT / CPR;  // loads a thread and tile, rows of one pass
