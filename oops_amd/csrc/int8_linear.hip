@@ -246,12 +246,14 @@ __global__ __launch_bounds__(kThreads, 1) void int8_tile_kernel(Int8Args a, int 
       }
     return;
   }
+  // scales and biases without branches: zeros behind the last row and column
+  const auto rs_x = make_rsrc(a.x_scale + r0, (uint32_t)left_r * 4), rs_w = make_rsrc(a.w_scale + j0, (uint32_t)left_j * 4);
+  const int bias_bytes = a.bias == nullptr ? 0 : a.bias_f32 ? 4 : (int)sizeof(T);
+  const auto rs_b = make_rsrc(static_cast<const char*>(a.bias) + j0 * bias_bytes, (uint32_t)(left_j * bias_bytes));
   float scale_x[TR];
 #pragma unroll
-  for (int p = 0; p < TR; ++p) {
-    const int64_t r = r0 + wr + 32 * p + l;
-    scale_x[p] = r < a.rows ? a.x_scale[r] : 0.f;
-  }
+  for (int p = 0; p < TR; ++p)
+    scale_x[p] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs_x, (wr + 32 * p + l) * 4, 0, 0));
   // Whole lines to memory: a wave's rows of 128 bytes (64 outputs of 16 bits, 32 of float32) pass through 16 KB of LDS
   // of its own, from lanes that hold a row each to eight lanes a row; slots are XORed with the row.
   constexpr int V = 16 / sizeof(T), kTilesLine = sizeof(T) == 4 || TJ == 1 ? 1 : 2;  // column tiles of a line
@@ -260,12 +262,29 @@ __global__ __launch_bounds__(kThreads, 1) void int8_tile_kernel(Int8Args a, int 
   char* line = lds + wave * (BM / 2 * 128);
 #pragma unroll
   for (int q = 0; q < TJ; ++q) {
-    float scale_w[16], add[16];
+    float scale_w[16], add[16] = {};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int64_t j = j0 + wj + 32 * q + kappa(half, i);
-      scale_w[i] = j < a.n ? a.w_scale[j] : 0.f;
-      add[i] = j < a.n ? bias_at<T>(a, j) : 0.f;
+    for (int i = 0; i < 16; i += 4) {
+      const uint32_t j = wj + 32 * q + kappa(half, i);
+      const f32x4 u = __builtin_bit_cast(f32x4, buffer_load16(rs_w, j * 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) scale_w[i + e] = u[e];
+    }
+    if (bias_bytes == 4) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 u = __builtin_bit_cast(f32x4, buffer_load16(rs_b, (wj + 32 * q + kappa(half, i)) * 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) add[i + e] = u[e];
+      }
+    } else if (bias_bytes == 2) {
+      if constexpr (sizeof(T) == 2) {
+        // (one by one: a pair that straddles the last column would be outside as a whole)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          add[i] = (float)__builtin_bit_cast(
+              T, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs_b, (wj + 32 * q + kappa(half, i)) * 2, 0, 0));
+      }
     }
 #pragma unroll
     for (int p = 0; p < TR; ++p) {
