@@ -20,8 +20,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// exp(log_decay n) for n >= 0: n = 0 gives 1 for every decay, -inf included
-__device__ __forceinline__ float log2_decay(float log_decay) { return fmaxf(log_decay * kLog2e, -1e30f); }
+// exp(log_decay n) for n >= 0: n = 0 gives 1 for every decay, -inf included (a NaN stays one)
+__device__ __forceinline__ float log2_decay(float log_decay) {
+  const float l2 = log_decay * kLog2e;
+  return l2 < -1e30f ? -1e30f : l2;
+}
 __device__ __forceinline__ float decay_power(float l2, float n) { return exp2f(l2 * n); }
 
 __device__ __forceinline__ int64_t walk_length(const LinearWalk& w, int64_t b) {
@@ -70,8 +73,8 @@ constexpr int kChunk = 64;
 struct ChunkArgs {
   LinearWalk w;
   float* starts;       // [batch * heads][segs][state]: segments' own states, then the states they start from
+  int64_t seg_tokens;  // a multiple of kChunk
   int32_t segs;
-  int32_t seg_tokens;  // a multiple of kChunk
 };
 
 // byte of a state's element, or an offset past every resource (reads as 0, is not written)
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(2 * D, MAIN || D == 128 ? 2 : 4) void walk_chunks_k
   const int64_t b = bh / w.heads;
   const int h = (int)(bh % w.heads);
   const int64_t n = walk_length(w, b);
-  const int64_t s0 = (int64_t)seg * ca.seg_tokens;
+  const int64_t s0 = seg * ca.seg_tokens;
   const int64_t s1 = s0 + ca.seg_tokens < n ? s0 + ca.seg_tokens : n;  // (s1 <= s0: nothing to walk)
   const int first = w.from_end ? 1 : 0;
   const float l2 = log2_decay(w.log_decay[h]);
@@ -427,7 +430,7 @@ __global__ __launch_bounds__(2 * D, D == 32 ? 2 : 1) void walk_exact_kernel(Chun
   const int64_t b = bh / w.heads;
   const int h = (int)(bh % w.heads);
   const int64_t n = walk_length(w, b);
-  const int64_t s0 = (int64_t)seg * ca.seg_tokens;
+  const int64_t s0 = seg * ca.seg_tokens;
   const int64_t s1 = s0 + ca.seg_tokens < n ? s0 + ca.seg_tokens : n;
   const int first = w.from_end ? 1 : 0;
   const float l2 = log2_decay(w.log_decay[h]);
@@ -621,7 +624,7 @@ __global__ __launch_bounds__(kThreads) void walk_scan_kernel(ChunkArgs ca, float
     for (int i = 0; i < U; ++i) {
       if (s0 + i >= ca.segs) break;
       own[(s0 + i) * size] = cur;
-      const int64_t left = n - (int64_t)(s0 + i) * ca.seg_tokens;
+      const int64_t left = n - (s0 + i) * ca.seg_tokens;
       const float lm = left >= ca.seg_tokens ? whole : left > 0 ? decay_power(l2, (float)left) : 1.f;
       cur = __builtin_fmaf(cur, lm, x[i]);
     }
@@ -737,7 +740,7 @@ void plan_segments(const LinearWalk& w, ChunkArgs& ca) {
   }
   const int64_t per = (chunks + segs - 1) / segs;
   ca.segs = (int32_t)((chunks + per - 1) / per);
-  ca.seg_tokens = (int32_t)(per * kChunk);
+  ca.seg_tokens = per * kChunk;
 }
 
 // rows read and written 16 bytes at a time, whose chunks span less than 2 GiB

@@ -58,6 +58,25 @@ def test_long_sums_of_few_outputs(rows, k, n):
     _check(int8_linear(*args), *args, None, torch.bfloat16)
 
 
+@pytest.mark.parametrize("rows,k,n,xpad,wpad", [(1025, 1001, 1100, 0, 0), (700, 2064, 900, 3, 0), (700, 2064, 900, 0, 5),
+                                                 (300, 8201, 600, 7, 9)])  # fmt: skip
+def test_many_products_of_odd_rows(rows, k, n, xpad, wpad):
+    """Rows that are no whole 16-byte pieces, copied to padded ones where there are many products."""
+
+    (x, xs, w, ws), bias = _operands(rows, k, n, seed=k + xpad)
+    wide = lambda t, pad: torch.full((t.shape[0], k + pad), 99, dtype=torch.int8, device=DEV)[:, :k]  # noqa: E731
+    xv, wv = wide(x, xpad).copy_(x), wide(w, wpad).copy_(w)
+    _check(int8_linear(xv, xs, wv, ws, bias), x, xs, w, ws, bias, torch.bfloat16)
+
+
+def test_more_than_32_bits_of_results():
+    rows, n, k = 40003, 54000, 32
+    (x, xs, w, ws), bias = _operands(rows, k, n, seed=7)
+    out = int8_linear(x, xs, w, ws, bias)
+    for r in (0, 20001, rows - 1):
+        assert torch.equal(out[r : r + 1], int8_linear(x[r : r + 1], xs[r : r + 1], w, ws, bias))
+
+
 @pytest.mark.parametrize("rows", [1, 7, 40, 300])
 @pytest.mark.parametrize("value", [-128, 127])
 def test_largest_sums(rows, value):

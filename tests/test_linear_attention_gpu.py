@@ -317,6 +317,43 @@ def test_non_finite_values_stay_with_their_tokens():
         assert fine[0, 0][:, other].all()
 
 
+def test_a_decay_that_is_nan():
+    x = _case(49, 1, 2, 70, 32, 32, torch.bfloat16, state=False)
+    x["ld"][1] = float("nan")
+    out, state = linear_attention(x["q"], x["k"], x["v"], x["ld"], return_state=True)
+    assert out[:, 1, 1:].isnan().all() and state[:, 1].isnan().all() and not out[:, 0].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_offsets_past_32_bits(dtype):
+    """Batch elements, heads and tokens further apart than 2^31 elements."""
+
+    far = 2**31 + 64
+    base = torch.empty(far + 3 * 64 * 200, dtype=dtype, device=DEV)
+    ld = torch.tensor([-0.1, -0.02], device=DEV)
+    g = torch.Generator().manual_seed(51)
+    tight = [_randn(g, 2, 2, 50, 64, dtype=dtype) for _ in range(3)]
+    for strides in ((far, 64 * 50, 64), (64 * 50, far, 64)):
+        views = [base[64 * 200 * i :].as_strided((2, 2, 50, 64), (*strides, 1)) for i in range(3)]
+        for v, t in zip(views, tight):
+            v.copy_(t)
+        got, want = (linear_attention(*ts, ld, return_state=True) for ts in (views, tight))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    del base, views
+    apart = 2**26 + 8  # 33 tokens span more than 2^31 elements, 32 less
+    base = torch.empty(34 * apart, dtype=dtype, device=DEV)
+    q = base.as_strided((1, 1, 34, 64), (0, 0, apart, 1))
+    small = _randn(g, 1, 1, 34, 64, dtype=dtype)
+    q.copy_(small)
+    assert torch.equal(linear_attention(q, q, q, ld[:1]), linear_attention(small, small, small, ld[:1]))
+    state = torch.empty(2**17 + 1, 1, 128, 128, device=DEV)  # more than 2^31 elements
+    state[-1], state[0] = 1.0, 2.0
+    qs = torch.ones(2**17 + 1, 1, 128, device=DEV, dtype=dtype)
+    out = linear_attention_step(qs, qs, qs, torch.zeros(1, device=DEV), state)
+    assert (state[-1] == 2).all() and (state[0] == 3).all()
+    assert torch.equal(out[-1].float(), torch.full((1, 128), 256 * 128**-0.5, device=DEV).to(dtype).float())
+
+
 def test_refusals():
     x = _case(53, 1, 2, 8, 16, 16, torch.float32)
     q, k, v, ld, s0 = (x[n] for n in ("q", "k", "v", "ld", "s0"))

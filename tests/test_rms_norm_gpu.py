@@ -90,6 +90,19 @@ def test_many_rows_and_repeated_calls():
     _check_backward(runs[0], x, dy, None, w, torch.bfloat16, 16)
 
 
+def test_more_than_32_bits_of_elements():
+    rows, width = 2**17 + 3, 16384
+    x = torch.empty(rows, width, dtype=torch.bfloat16, device=DEV)
+    x.fill_(1.0)
+    x[-1].normal_(), x[0].normal_()
+    y = rms_norm(x, width)
+    values, scales = quantize_int8(x)
+    for i in (0, rows - 1):
+        assert torch.equal(y[i], rms_norm(x[i], width))
+        assert torch.equal(values[i], quantize_int8(x[i])[0]) and torch.equal(scales[i], quantize_int8(x[i])[1])
+    assert (values[1:-1] == 127).all()
+
+
 def test_strides_and_prefixes():
     g = torch.Generator().manual_seed(5)
     base, rbase = (_randn(g, 3, 20, 80, dtype=torch.bfloat16) for _ in range(2))
