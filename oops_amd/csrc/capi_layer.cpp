@@ -5,7 +5,6 @@
 #include <algorithm>
 
 #include "layer_kernels.h"
-#include "reduce_kernels.h"
 
 namespace {
 
@@ -28,9 +27,6 @@ int check_rms(const oops_rms_norm_geometry* g, bool residual) {
 }
 size_t rms_parts_bytes(const oops_rms_norm_geometry& g) {
   return align256((size_t)oops::rms_norm_parts(g) * (size_t)g.width * sizeof(float));
-}
-oops_sum_segment rms_segment(const oops_rms_norm_geometry& g, float* parts, void* out) {
-  return oops_sum_segment{parts, out, oops::rms_norm_parts(g), g.width, g.width, g.weight_f32 ? OOPS_F32 : g.dtype, 0};
 }
 
 
@@ -166,8 +162,7 @@ int oops_quantize_int8(const oops_rms_norm_geometry* geo, const void* x, void* v
 size_t oops_rms_norm_backward_workspace_bytes(const oops_rms_norm_geometry* geo) {
   oops::clear_report();
   if (check_rms(geo, false)) return 0;
-  const oops_sum_segment seg = rms_segment(*geo, nullptr, nullptr);
-  return rms_parts_bytes(*geo) + oops::sum_partials_workspace_bytes(&seg, 1);
+  return rms_parts_bytes(*geo);
 }
 
 int oops_rms_norm_backward(const oops_rms_norm_geometry* geo, const void* h, const float* rstd, const void* weight,
@@ -184,10 +179,7 @@ int oops_rms_norm_backward(const oops_rms_norm_geometry* geo, const void* h, con
   oops_rms_norm_geometry g = *geo;
   g.r_row = g.width;
   hipError_t e = oops::launch_rms_norm_backward(g, h, rstd, weight, grad_y, grad_sum, grad_x, parts, st);
-  if (e == hipSuccess && grad_weight) {
-    const oops_sum_segment seg = rms_segment(g, parts, grad_weight);
-    e = oops::launch_sum_partials(&seg, 1, static_cast<char*>(workspace) + rms_parts_bytes(g), st);
-  }
+  if (e == hipSuccess && grad_weight) e = oops::launch_rms_weight_sum(g, parts, grad_weight, st);
   return report_launch(e, "rms_norm backward");
 }
 

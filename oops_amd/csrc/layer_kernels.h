@@ -24,6 +24,8 @@ int64_t rms_norm_parts(const oops_rms_norm_geometry& g);  // rows of weight-grad
 hipError_t launch_rms_norm_backward(const oops_rms_norm_geometry& g, const void* h, const float* rstd,
                                     const void* weight, const void* grad_y, const void* grad_sum, void* grad_x,
                                     float* weight_parts, hipStream_t stream);
+// the partials' sum, of the weight's type
+hipError_t launch_rms_weight_sum(const oops_rms_norm_geometry& g, const float* parts, void* out, hipStream_t stream);
 
 // ---- int8_linear.hip
 size_t int8_linear_workspace_bytes(const oops_int8_geometry& g);

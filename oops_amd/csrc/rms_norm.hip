@@ -345,6 +345,25 @@ __global__ __launch_bounds__(kThreads) void rms_backward_kernel(RmsGradArgs a) {
   }
 }
 
+// The partial rows' sum, in a fixed order and one launch: a workgroup takes 16
+// columns, its 64 slices every 64th row each, then the slices in a tree.
+template <typename W>
+__global__ __launch_bounds__(1024) void rms_weight_sum_kernel(const float* parts, W* out, int rows, int width) {
+  __shared__ float sum[64][17];
+  const int c = threadIdx.x & 15, slice = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
+  float s = 0.f;
+  if (col < width) {
+#pragma unroll 4
+    for (int r = slice; r < rows; r += 64) s += parts[(int64_t)r * width + col];
+  }
+  sum[slice][c] = s;
+  for (int d = 32; d > 0; d /= 2) {
+    __syncthreads();
+    if (slice < d) sum[slice][c] += sum[slice + d][c];
+  }
+  if (slice == 0 && col < width) out[col] = (W)sum[0][c];
+}
+
 // ------------------------------------------------------------------ launchers
 
 // Lanes and 16-byte chunks a lane of a row: as many lanes as chunks up to a
@@ -456,6 +475,16 @@ hipError_t launch_rms_norm_backward(const oops_rms_norm_geometry& g, const void*
         hipLaunchKernelGGL((rms_backward_kernel<T, S::TPR, S::CH, false>), grid, dim3(kThreads), 0, stream, a);
       return hipGetLastError();
     });
+  });
+}
+
+hipError_t launch_rms_weight_sum(const oops_rms_norm_geometry& g, const float* parts, void* out, hipStream_t stream) {
+  const int rows = (int)rms_norm_parts(g);
+  const dim3 grid((unsigned)(g.width + 15) / 16);
+  return by_type(g.weight_f32 ? OOPS_F32 : g.dtype, [&](auto tag) {
+    using W = decltype(tag);
+    hipLaunchKernelGGL((rms_weight_sum_kernel<W>), grid, dim3(1024), 0, stream, parts, static_cast<W*>(out), rows, g.width);
+    return hipGetLastError();
   });
 }
 
