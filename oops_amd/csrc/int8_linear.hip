@@ -5,10 +5,15 @@
 // sums exact in 32-bit integers on the int8 matrix units (32x32x32 MFMA, twice
 // the bf16 rate), one rounding at the end.
 //
-// int8_any_kernel serves every size and alignment: 64 x 64 outputs a
-// workgroup, 128 bytes of k a step through LDS, the next step's bytes loaded
-// to registers meanwhile.  The weight is MFMA's row operand: a lane then holds
-// one output row and four consecutive columns at a time.
+// The weight is MFMA's row operand: a lane then holds one output row and four
+// consecutive columns at a time.  By size and alignment:
+//   up to 16 rows                   int8_few_kernel     the weight read once
+//   whole 16-byte pieces a row      int8_tile_kernel    LDS tiles, 64^2 to 256^2
+//   else, 10^9 products and more    int8_pad_kernel     copies, then tiles
+//   else                            int8_any_kernel, or int8_small_kernel for few
+//
+// Measured: 8192 x 8192 x 8192 2.25 PFLOP/s (a library's product 2.12),
+// rows x n x k of 8192 x 16384 x 4096 1.95; 4 x 16384 x 4096 4.4 TB/s of weight.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -63,6 +68,9 @@ __device__ __forceinline__ float bias_at(const Int8Args& a, int64_t j) {
   return a.bias_f32 ? static_cast<const float*>(a.bias)[j] : (float)static_cast<const T*>(a.bias)[j];
 }
 
+// Every size and alignment: 64 x 64 outputs a workgroup, 128 bytes of k a step
+// through LDS, the next step's bytes loaded to registers meanwhile.  Bound by
+// the waits of its steps (1001 bytes of k: 15 us up to one tile a CU).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void int8_any_kernel(Int8Args a) {
   __shared__ i32x4 tw[64 * 8], tx[64 * 8];
@@ -382,6 +390,49 @@ __global__ __launch_bounds__(64 * W) void int8_few_kernel(Int8Args a) {
     if (j + i < a.n) out[i] = (T)__builtin_fmaf((float)sum[i] * sx, a.w_scale[j + i], bias_at<T>(a, j + i));
 }
 
+// ---------------------------------------------------------------- few products of odd rows
+//
+// 32 x 32 outputs a workgroup, whose W waves take lines of k in turn with the
+// operands loaded straight into the 32x32x32 MFMA's layout, at any alignment,
+// and join their sums in LDS: 64 x 64 tiles would leave most CUs idle and go
+// through k one wait after the other.
+template <typename T, int W>
+__global__ __launch_bounds__(64 * W) void int8_small_kernel(Int8Args a) {
+  __shared__ i32x4 red[W][4][64];
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t tiles = (a.n + 31) / 32;
+  const int64_t j0 = (int64_t)blockIdx.x % tiles * 32, r0 = (int64_t)blockIdx.x / tiles * 32;
+  const bool in_w = j0 + l < a.n, in_x = r0 + l < a.rows;
+  const int8_t* w = a.w + (in_w ? j0 + l : 0) * a.w_row;
+  const int8_t* x = a.x + (in_x ? r0 + l : 0) * a.x_row;
+  i32x16 acc = {};
+  for (int k0 = wave * 128; k0 < a.k; k0 += W * 128) {
+    i32x4 fw[4], fx[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      fw[c] = load_bytes(w, k0 + 32 * c + 16 * half, a.k, in_w);
+      fx[c] = load_bytes(x, k0 + 32 * c + 16 * half, a.k, in_x);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[c], fx[c], acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) red[wave][q][lane] = i32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  __syncthreads();
+  if (wave >= 4 || !in_x) return;
+  i32x4 sum = red[0][wave][lane];
+#pragma unroll
+  for (int q = 1; q < W; ++q) sum += red[q][wave][lane];
+  // out[r0 + l][j0 + 8 wave + 4 half + i]
+  const int64_t r = r0 + l, j = j0 + 8 * wave + 4 * half;
+  const float sx = a.x_scale[r];
+  T* out = static_cast<T*>(a.out) + r * a.n + j;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (j + i < a.n) out[i] = (T)__builtin_fmaf((float)sum[i] * sx, a.w_scale[j + i], bias_at<T>(a, j + i));
+}
+
 // ---------------------------------------------------------------- padded operands
 //
 // Rows that are no whole pieces at aligned places, copied to ones that are
@@ -577,6 +628,13 @@ hipError_t launch_int8_linear(const oops_int8_geometry& g, const void* x, const 
   if (tiles >= kMaxTiles) return hipErrorInvalidConfiguration;
   return by_type(g.out_dtype, [&](auto tag) {
     using T = decltype(tag);
+    // up to two 32 x 32 tiles a CU, or 64 x 64 ones (333 x 777 x 1001: 11 us, 15.4;
+    // 500 x 1000 x 1001: 12.8, 14.8; 576 x 1000 x 1001: 17.2, 14.8)
+    if (tiles <= 128) {
+      const dim3 grid((unsigned)tiles_of(g, 32, 32));
+      hipLaunchKernelGGL((int8_small_kernel<T, 8>), grid, dim3(512), 0, stream, a);
+      return hipGetLastError();
+    }
     hipLaunchKernelGGL((int8_any_kernel<T>), dim3((unsigned)tiles), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
   });

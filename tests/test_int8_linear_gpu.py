@@ -69,6 +69,15 @@ def test_many_products_of_odd_rows(rows, k, n, xpad, wpad):
     _check(int8_linear(xv, xs, wv, ws, bias), x, xs, w, ws, bias, torch.bfloat16)
 
 
+@pytest.mark.parametrize("rows,k,n", [(500, 1001, 1000), (570, 333, 1050), (31, 777, 95), (64, 5, 64), (200, 2049, 33)])
+def test_fewer_products_of_odd_rows(rows, k, n):
+    """Few tiles, and more of them."""
+
+    args, bias = _operands(rows, k, n, seed=k)
+    _check(int8_linear(*args, bias), *args, bias, torch.bfloat16)
+    _check(int8_linear(*args, dtype=torch.float32), *args, None, torch.float32)
+
+
 def test_more_than_32_bits_of_results():
     rows, n, k = 40003, 54000, 32
     (x, xs, w, ws), bias = _operands(rows, k, n, seed=7)
