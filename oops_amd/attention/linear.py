@@ -120,8 +120,13 @@ def linear_attention_step(
         raise unsupported(operator, "updates the state in place: it must be contiguous", stride=state.stride())
     q, k, v = (_batched(t, None) for t in (query, key, value))
     scale = query.shape[-1] ** -0.5 if scale is None else float(scale)
-    call = linear_attention_step_op if needs_custom_op(q) else _step_impl
-    out = call(q, k, v, log_decay.resolve_neg().contiguous(), state, scale)
+    args = (q, k, v, log_decay.resolve_neg().contiguous(), state, scale)
+    if needs_custom_op(q):
+        out = linear_attention_step_op(*args)
+    else:
+        out = _step_impl(*args)
+        # (autograd has to know: a graph that saved this state must not be differentiated with the new one)
+        torch.autograd.graph.increment_version(state)
     return out if query.dim() == 3 else out.view(*query.shape[:-1], value.shape[-1])
 
 

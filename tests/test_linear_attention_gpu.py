@@ -271,6 +271,23 @@ def test_step(dtype, b, h, d, e):
     assert_within(out, want, (140 + 8) * U * size + half(dtype) * abs(want) + smallest(dtype), "out")
 
 
+def test_step_counts_as_a_change_of_the_state():
+    """A state that a recorded call started from and a step then changed: the call's backward raises."""
+
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    q, k, v = (torch.randn(1, 2, 6, 16, device=DEV, generator=gen) for _ in range(3))
+    ld, state = torch.full((2,), -0.1, device=DEV), torch.randn(1, 2, 16, 16, device=DEV, generator=gen)
+    out = linear_attention(q.requires_grad_(True), k, v, ld, state)
+    with torch.no_grad():
+        linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], ld, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    with torch.inference_mode():
+        own = torch.zeros(1, 2, 16, 16, device=DEV)
+        linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], ld, own)
+    assert bool(own.any())
+
+
 def test_step_layouts():
     g = torch.Generator().manual_seed(41)
     qkv = _randn(g, 3, 1, 4, 3, 40, dtype=torch.bfloat16)
