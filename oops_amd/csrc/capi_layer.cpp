@@ -208,7 +208,7 @@ size_t oops_linear_attn_forward_workspace_bytes(const oops_linear_attn_geometry*
   if (check_linear(geo)) return 0;
   float state;
   return oops::linear_walk_workspace_bytes(
-      walk_out(*geo, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &state));
+      geo->dtype, walk_out(*geo, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &state));
 }
 
 int oops_linear_attn_forward(const oops_linear_attn_geometry* geo, const void* q, const void* k, const void* v,

@@ -53,7 +53,7 @@ struct LinearWalk {
 // A long walk of few heads runs in segments: launch_linear_walk_starts writes the states they start from to the
 // workspace (0 bytes: one segment), where launch_linear_walk reads them.  They depend on b, c and the decays alone
 // and are laid out like `initial`, so walks over the same state from the same end share them.
-size_t linear_walk_workspace_bytes(const LinearWalk& w);
+size_t linear_walk_workspace_bytes(int dtype, const LinearWalk& w);
 hipError_t launch_linear_walk_starts(int dtype, const LinearWalk& w, void* workspace, hipStream_t stream);
 hipError_t launch_linear_walk(int dtype, const LinearWalk& w, const void* workspace, hipStream_t stream);
 hipError_t launch_linear_attn_step(const oops_linear_attn_geometry& g, const void* q, const void* k, const void* v,

@@ -79,7 +79,7 @@ constexpr int kChunk = 64;
 struct ChunkArgs {
   LinearWalk w;
   float* starts;       // [batch * heads][segs][state]: segments' own states, then the states they start from
-  int64_t seg_tokens;  // a multiple of kChunk
+  int64_t seg_tokens;  // whole chunks
   int32_t segs;
 };
 
@@ -738,18 +738,30 @@ namespace {
 // tokens x 128: 42 us, in two segments 91).  Others get segments of at least
 // four chunks until there are eight waves a CU, or of two while there are not
 // four (16 x 1024 x 128: 34 us, with four chunks 42; 8 x 8192 x 128: 57, 51).
-void plan_segments(const LinearWalk& w, ChunkArgs& ca) {
-  const int64_t chunks = std::max<int64_t>(1, (w.length + kChunk - 1) / kChunk), bh = w.batch * w.heads;
+// Below that, single chunks: of 32 tokens in the float32 products, whose time is
+// the larger part (training 2 x 300 x 64 in float16 87 us, 192 with segments of
+// two 64-token chunks; 48 x 777 x 64 123, 147), of 64 in bfloat16 while there are
+// not two waves a CU (2 x 300 x 64 63, 80; 64 x 512 x 64 70, without them 66).
+// More than 256 segments are not worth their scan (32768 x 64: 154, 107).
+void plan_segments(int dtype, const LinearWalk& w, ChunkArgs& ca) {
+  const bool exact = dtype != OOPS_BF16;
+  const int64_t tokens = exact ? kExactChunk : kChunk, unit = kChunk / tokens;
+  const int64_t chunks = std::max<int64_t>(1, (w.length + tokens - 1) / tokens), bh = w.batch * w.heads;
   const int widest = std::max(w.rows, w.cols);
   const int64_t wide = widest <= 32 ? 4 : widest <= 64 ? 2 : 1;  // workgroups of four waves' worth
   int64_t segs = 1;
   if (bh < 192 * wide) {
-    segs = std::min((512 * wide + bh - 1) / bh, (chunks + 3) / 4);
-    segs = std::max(segs, std::min((256 * wide + bh - 1) / bh, (chunks + 1) / 2));
+    auto split = [&](int64_t target, int64_t least) {
+      segs = std::max(segs, std::min((target * wide + bh - 1) / bh, (chunks + least - 1) / least));
+    };
+    split(512, 4 * unit);
+    split(256, 2 * unit);
+    if (segs < 256 && (exact || chunks >= 4))
+      split(std::min<int64_t>(exact ? 256 : 128, 256 * bh / wide), 1);
   }
   const int64_t per = (chunks + segs - 1) / segs;
   ca.segs = (int32_t)((chunks + per - 1) / per);
-  ca.seg_tokens = per * kChunk;
+  ca.seg_tokens = per * tokens;
 }
 
 // rows read and written 16 bytes at a time, whose chunks span less than 2 GiB
@@ -788,7 +800,7 @@ hipError_t run_chunks(const ChunkArgs& ca, bool starts, hipStream_t stream) {
 hipError_t run_walk(int dtype, const LinearWalk& w, void* workspace, bool starts, hipStream_t stream) {
   ChunkArgs ca{};
   ca.w = w;
-  plan_segments(w, ca);
+  plan_segments(dtype, w, ca);
   ca.starts = static_cast<float*>(workspace);
   if (starts && ca.segs == 1) return hipSuccess;
   const int el = dtype == OOPS_F32 ? 4 : 2;
@@ -809,10 +821,10 @@ hipError_t run_walk(int dtype, const LinearWalk& w, void* workspace, bool starts
 
 }  // namespace
 
-size_t linear_walk_workspace_bytes(const LinearWalk& w) {
+size_t linear_walk_workspace_bytes(int dtype, const LinearWalk& w) {
   if (w.batch == 0) return 0;
   ChunkArgs ca{};
-  plan_segments(w, ca);
+  plan_segments(dtype, w, ca);
   if (ca.segs == 1) return 0;
   return (size_t)(w.batch * w.heads * ca.segs) * (size_t)w.rows * (size_t)w.cols * sizeof(float);
 }
