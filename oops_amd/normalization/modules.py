@@ -35,7 +35,8 @@ class RMSNorm(nn.RMSNorm):
     ``(y, input + residual)``."""
 
     def forward(self, input: Tensor, residual: Tensor | None = None):
-        eps = torch.finfo(input.dtype).eps if self.eps is None else self.eps
+        # (PyTorch's default is the eps of the type it computes in: float32's for every type that rms_norm takes)
+        eps = torch.finfo(torch.float32).eps if self.eps is None else self.eps
         try:
             return rms_norm(input, self.normalized_shape, self.weight, eps, residual)
         except OOpsUnsupportedError:

@@ -306,3 +306,27 @@ def test_other_stream():
         got = oops_amd.rms_norm(big, 512)
     torch.cuda.current_stream().wait_stream(side)
     _check_forward(got, x + 1, None, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [1e-4, 0.02, 1.0])
+def test_default_eps_of_the_module(dtype, scale):
+    """A module of default eps against PyTorch's, on rows small enough that the eps decides the result: each result is
+    rounded once, and a gradient of the type is off by one rounding and the arithmetic of its terms on either side."""
+
+    g = torch.Generator().manual_seed(21)
+    ours, theirs = (m(96, device=DEV, dtype=dtype) for m in (RMSNorm, torch.nn.RMSNorm))
+    x, dy = _randn(g, 40, 96, dtype=dtype, scale=scale), _randn(g, 40, 96, dtype=dtype)
+    eps = torch.finfo(torch.float32).eps
+    _check_forward(ours(x), x, None, dtype, eps)
+    want = f64(theirs(x))
+    assert_within(ours(x), want, (2 * half(dtype) + 2 * ARITH) * abs(want) + 2 * smallest(dtype), "y")
+    y, s = ours(x, x)
+    _check_forward(y, s, None, dtype, eps)
+    leaf = x.clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(ours(leaf), leaf, dy)
+    h, want_dx = f64(x), layers.rms_norm_backward(f64(x), f64(dy), None, eps)[0]
+    rstd = 1 / ((h**2).mean(-1, keepdims=True) + eps) ** 0.5
+    n, d = abs(h) * rstd, abs(f64(dy))
+    size = rstd * (d + n * (d * n).mean(-1, keepdims=True))
+    assert_within(dx, want_dx, half(dtype) * abs(want_dx) + 2 * ARITH * size + smallest(dtype), "dx")
