@@ -197,6 +197,12 @@ def _empty_like(t: Tensor, width: int) -> Tensor:
     return torch.empty_strided(*_dense(t.shape, t.stride(), width), dtype=t.dtype, device=t.device)
 
 
+def _fake_like(t: Tensor, width: int) -> Tensor:
+    """``_empty_like`` for traced code, whose sizes may be symbols: they cannot be a cache's key."""
+
+    return torch.empty_strided(*_dense.__wrapped__(t.shape, t.stride(), width), dtype=t.dtype, device=t.device)
+
+
 @functools.lru_cache(maxsize=256)
 def _dense(shape: tuple, stride: tuple, width: int) -> Tuple[tuple, tuple]:
     sizes = (*shape[:-1], width)
@@ -313,7 +319,7 @@ def linear_attention_forward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor,
 @linear_attention_forward.register_fake
 def _(q, k, v, log_decay, lengths, initial, scale, return_state):
     b, h, _, d = q.shape
-    return _empty_like(q, v.shape[-1]), log_decay.new_empty((b, h, d, v.shape[-1]) if return_state else (0,))
+    return _fake_like(q, v.shape[-1]), log_decay.new_empty((b, h, d, v.shape[-1]) if return_state else (0,))
 
 
 @torch.library.custom_op("oops_amd::linear_attention_backward", mutates_args=(), device_types="cuda")
@@ -325,7 +331,7 @@ def linear_attention_backward(dout: Tensor, dstate: Optional[Tensor], q: Tensor,
 
 @linear_attention_backward.register_fake
 def _(dout, dstate, q, k, v, log_decay, lengths, initial, scale, needs):
-    dq, dk, dv = (_empty_like(t, t.shape[-1]) if need else t.new_empty(0) for t, need in zip((q, k, v), needs))
+    dq, dk, dv = (_fake_like(t, t.shape[-1]) if need else t.new_empty(0) for t, need in zip((q, k, v), needs))
     return dq, dk, dv, torch.empty_like(initial) if needs[3] and initial is not None else log_decay.new_empty(0)
 
 

@@ -479,3 +479,21 @@ def test_into_the_gated_output_stage():
     assert out.transpose(1, 2).is_contiguous()
     got = gate_attention_output(out, single, wg, wo)
     assert torch.equal(got, gate_attention_output(out.contiguous(), single, wg, wo))
+
+
+def test_compile_with_sizes_that_change():
+    """One compiled function over several lengths and batches: the second one makes the sizes dynamic."""
+
+    def run(q, k, v, ld, s0):
+        return linear_attention(q, k, v, ld, s0, return_state=True)
+
+    compiled = torch.compile(run, fullgraph=True)
+    for b, n in ((2, 150), (2, 70), (3, 201), (2, 64)):
+        x = _case(63, b, 2, n, 64, 32, torch.bfloat16)
+        results = []
+        for fn in (run, compiled):
+            leaves = [x[name].detach().clone().requires_grad_(True) for name in ("q", "k", "v", "s0")]
+            outs = fn(*leaves[:3], x["ld"], leaves[3])
+            results.append((*outs, *torch.autograd.grad(outs, leaves, (x["do"], x["ds"]))))
+        for got, ref in zip(*results):
+            torch.testing.assert_close(got, ref, atol=0, rtol=0)
