@@ -78,12 +78,22 @@ def call_on(device_index: int, entry, *args) -> int:
         return entry(*args, torch._C._cuda_getCurrentRawStream(device_index))
 
 
-def needs_custom_op(tensor) -> bool:
+_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
+
+
+def needs_custom_op(tensor, *others) -> bool:
     """True where an operator must go through its ``torch.library`` custom op (fake kernel, traced
     graph): under ``torch.compile``, for fake or subclass tensors and under a Python dispatch mode.
-    Elsewhere eager calls may skip the dispatcher."""
+    Elsewhere eager calls may skip the dispatcher.  ``others`` are the operator's further operands, where
+    parameters are plain: a wrapper subclass has no memory of its own, and its NULL pointer would be taken
+    as an operand that is not given."""
 
-    return torch.compiler.is_compiling() or type(tensor) is not torch.Tensor or _get_current_dispatch_mode() is not None
+    if torch.compiler.is_compiling() or type(tensor) is not torch.Tensor or _get_current_dispatch_mode() is not None:
+        return True
+    for t in others:
+        if type(t) not in _PLAIN:
+            return True
+    return False
 
 
 def without_second_derivative(grads, ctx, grad_output, differentiable: bool = False):

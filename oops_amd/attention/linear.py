@@ -85,8 +85,9 @@ def linear_attention(
     scale = d**-0.5 if scale is None else float(scale)
     ld = log_decay.resolve_neg().contiguous()
     grad = wants_gradient(query, key, value, initial_state)
-    args = (q, k, v, ld, lengths, s0, scale, bool(return_state))
-    if needs_custom_op(q):
+    operands = (q, k, v, ld, lengths, s0)
+    args = (*operands, scale, bool(return_state))
+    if needs_custom_op(*operands):
         out, state = linear_attention_forward(*args)
     elif grad:
         out, state = _EagerLinearAttention.apply(*args)
@@ -120,11 +121,11 @@ def linear_attention_step(
         raise unsupported(operator, "updates the state in place: it must be contiguous", stride=state.stride())
     q, k, v = (_batched(t, None) for t in (query, key, value))
     scale = query.shape[-1] ** -0.5 if scale is None else float(scale)
-    args = (q, k, v, log_decay.resolve_neg().contiguous(), state, scale)
-    if needs_custom_op(q):
-        out = linear_attention_step_op(*args)
+    operands = (q, k, v, log_decay.resolve_neg().contiguous(), state)
+    if needs_custom_op(*operands):
+        out = linear_attention_step_op(*operands, scale)
     else:
-        out = _step_impl(*args)
+        out = _step_impl(*operands, scale)
         # (autograd has to know: a graph that saved this state must not be differentiated with the new one)
         torch.autograd.graph.increment_version(state)
     return out if query.dim() == 3 else out.view(*query.shape[:-1], value.shape[-1])
@@ -358,7 +359,7 @@ def _save(ctx, q, k, v, log_decay, lengths, initial, scale, state, ws=None):
         ctx.mark_non_differentiable(state)
 
 
-def _grads(ctx, dout, dstate, backward):
+def _grads(ctx, dout, dstate, traced):
     """Gradients of (q, k, v, log_decay, lengths, initial, scale, return_state)."""
 
     q, k, v, log_decay, lengths, initial, ws = ctx.saved_tensors
@@ -367,7 +368,7 @@ def _grads(ctx, dout, dstate, backward):
         dout = v.new_zeros(1).expand(*q.shape[:3], v.shape[-1])
         dout = dout.contiguous() if v.shape[-1] > 1 else dout
     args = (dout, dstate, q, k, v, log_decay, lengths, initial, ctx.scale, needs)
-    dq, dk, dv, ds = backward(*args) if ws is None else backward(*args, ws)
+    dq, dk, dv, ds = linear_attention_backward(*args) if traced else _backward_impl(*args, ws)
     keep = lambda g, need: g if need else None  # noqa: E731
     return (keep(dq, needs[0]), keep(dk, needs[1]), keep(dv, needs[2]), None, None,
             keep(ds, needs[3] and initial is not None), None, None)  # fmt: skip
@@ -381,7 +382,7 @@ def _setup_context(ctx, inputs, output):
 def _backward(ctx, dout, dstate):
     if dout is None and dstate is None:
         return (None,) * 8
-    return _grads(ctx, dout, dstate, linear_attention_backward)
+    return _grads(ctx, dout, dstate, True)
 
 
 linear_attention_forward.register_autograd(_backward, setup_context=_setup_context)
@@ -401,6 +402,6 @@ class _EagerLinearAttention(torch.autograd.Function):
     def backward(ctx, dout, dstate):
         if dout is None and dstate is None:
             return (None,) * 8
-        grads = _grads(ctx, dout, dstate, _backward_impl)
+        grads = _grads(ctx, dout, dstate, needs_custom_op(dstate if dout is None else dout, dstate))
         later = any(t is not None and t.requires_grad for t in (dout, dstate))
         return without_second_derivative(grads, ctx, dout, differentiable=later)

@@ -96,7 +96,7 @@ def int8_linear(
     rows = input_scale.numel()
     x = _rows(input if input.dim() == 2 else input.reshape(rows, k))
     args = (x, _flat(input_scale), _rows(weight), _flat(weight_scale), None if bias is None else _flat(bias), dtype)
-    out = int8_linear_forward(*args) if needs_custom_op(x) else _forward_impl(*args)
+    out = int8_linear_forward(*args) if needs_custom_op(*args[:-1]) else _forward_impl(*args)
     return out if input.dim() == 2 else out.view(*input.shape[:-1], n)
 
 

@@ -65,7 +65,7 @@ def rms_norm(
     x, r = _rows(input), _rows(residual)
     w = None if weight is None else weight.resolve_neg().contiguous()
     grad = wants_gradient(input, weight, residual)
-    if needs_custom_op(x):
+    if needs_custom_op(x, w, r):
         y, summed, _ = rms_norm_forward(x, w, r, float(eps), grad)
     elif grad:
         y, summed = _EagerRmsNorm.apply(x, w, r, float(eps))
@@ -98,7 +98,7 @@ def rms_norm_int8(
     _require_inference(operator, input, weight, residual)
     x, r = _rows(input), _rows(residual)
     w = None if weight is None else weight.resolve_neg().contiguous()
-    call = rms_norm_int8_forward if needs_custom_op(x) else _int8_impl
+    call = rms_norm_int8_forward if needs_custom_op(x, w, r) else _int8_impl
     values, scales, summed = call(x, w, r, float(eps))
     if input.dim() != 2:
         values, scales = values.view(input.shape), scales.view(input.shape[:-1])
@@ -378,6 +378,7 @@ class _EagerRmsNorm(torch.autograd.Function):
     def backward(ctx, dy, dsum):
         if dy is None and dsum is None:
             return None, None, None, None
-        grads = _grads(ctx, dy, dsum, _backward_impl)
+        traced = needs_custom_op(dsum if dy is None else dy, dsum)
+        grads = _grads(ctx, dy, dsum, rms_norm_backward if traced else _backward_impl)
         later = any(t is not None and t.requires_grad for t in (dy, dsum))
         return (*without_second_derivative(grads, ctx, dy, differentiable=later), None)

@@ -1,5 +1,7 @@
 """The layer operators' front-ends on the host: what they hand to the kernels.  No kernel is launched."""
 
+import importlib
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -9,8 +11,11 @@ import oops_amd
 from layer_tolerance import U, assert_within, f64, half
 from oops_amd import RMSNorm
 from oops_amd.attention import linear
+from oops_amd.linear import int8
 from oops_amd.normalization import modules
 from oracle import layers
+
+rms_norm = importlib.import_module("oops_amd.normalization.rms_norm")  # (the package's name is the function)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -58,3 +63,81 @@ def test_symbolic_sizes():
         assert [g.shape for g in grads] == [q.shape, q.shape, v.shape, s0.shape]
         assert all(g.transpose(1, 2).is_contiguous() for g in grads[:3])
         assert oops_amd.linear_attention_step(q[:, :, 0], q[:, :, 0], v[:, :, 0], ld, s0).shape == (b, 4, 16)
+
+
+class _Dispatched(Exception):
+    pass
+
+
+class _Wrapped(torch.Tensor):
+    """A wrapper without storage of its own, as quantised and distributed tensors are; an operator of the framework
+    that it is given to is reported."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        out = torch.Tensor._make_wrapper_subclass(cls, inner.shape, strides=inner.stride(), dtype=inner.dtype,
+                                                  device=inner.device)  # fmt: skip
+        out.inner = inner
+        return out
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        if func.namespace == "oops_amd":
+            raise _Dispatched(func._schema.name)
+        if func in (torch.ops.aten.view.default, torch.ops.aten.detach.default):
+            return cls(func(args[0].inner, *args[1:]))
+        unwrap = lambda t: t.inner if isinstance(t, cls) else t  # noqa: E731
+        return func(*torch.utils._pytree.tree_map(unwrap, args), **(kwargs or {}))
+
+
+@pytest.fixture
+def no_launches(monkeypatch):
+    """Checks see device tensors; a launch is an error."""
+
+    def launched(*args):
+        raise AssertionError("a launch with a wrapper's address")
+
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    for module, names in ((rms_norm, ("_forward_impl", "_int8_impl", "_quantize_impl", "_backward_impl")),
+                          (int8, ("_forward_impl",)),
+                          (linear, ("_forward_impl", "_forward_with_workspace", "_backward_impl", "_step_impl"))):  # fmt: skip
+        for name in names:
+            monkeypatch.setattr(module, name, launched)
+    return launched
+
+
+def _each_wrapped(call, operands):
+    """``call`` with each operand in turn as a wrapper has to reach the dispatcher."""
+
+    for i in range(len(operands)):
+        wrapped = [_Wrapped(t) if i == j else t for j, t in enumerate(operands)]
+        with torch.no_grad(), pytest.raises(_Dispatched):
+            call(*wrapped)
+
+
+def test_wrappers_in_the_place_of_any_operand_are_dispatched(no_launches):
+    x, r, w = torch.randn(3, 8), torch.randn(3, 8), torch.randn(8)
+    for norm in (oops_amd.rms_norm, oops_amd.rms_norm_int8):
+        _each_wrapped(lambda x, w, r, norm=norm: norm(x, 8, w, residual=r), [x, w, r])
+    _each_wrapped(oops_amd.quantize_int8, [x])
+    i8, w8 = torch.zeros(3, 8, dtype=torch.int8), torch.zeros(5, 8, dtype=torch.int8)
+    _each_wrapped(oops_amd.int8_linear, [i8, torch.ones(3), w8, torch.ones(5), torch.ones(5)])
+    q, v, ld, s0 = torch.randn(2, 3, 7, 8), torch.randn(2, 3, 7, 4), torch.zeros(3), torch.zeros(2, 3, 8, 4)
+    lengths = torch.tensor([7, 5], dtype=torch.int32)
+    _each_wrapped(oops_amd.linear_attention, [q, q.clone(), v, ld, s0, lengths])
+    _each_wrapped(oops_amd.linear_attention_step, [q[:, :, 0], q[:, :, 1], v[:, :, 0], ld, s0])
+    with pytest.raises(AssertionError, match="launch"):  # (a parameter is no wrapper)
+        oops_amd.rms_norm(x, 8, torch.nn.Parameter(w), residual=r)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_wrapped_gradients_are_dispatched(no_launches, monkeypatch, which):
+    monkeypatch.setattr(rms_norm, "_forward_impl", lambda x, w, r, eps, save: (x + 0, x + r, torch.ones(3)))
+    monkeypatch.setattr(linear, "_forward_with_workspace", lambda q, k, v, ld, n, s0, scale, state: (
+        q + 0, torch.zeros(2, 3, 8, 8), torch.zeros(4)))  # fmt: skip
+    x, w, q = (torch.randn(*shape, requires_grad=True) for shape in ((3, 8), (8,), (2, 3, 7, 8)))
+    for leaf, outs in ((x, oops_amd.rms_norm(x, 8, w, residual=x.detach())),
+                       (q, oops_amd.linear_attention(q, q, q, torch.zeros(3), return_state=True))):  # fmt: skip
+        grads = [_Wrapped(torch.randn(t.shape)) if i == which else torch.randn(t.shape) for i, t in enumerate(outs)]
+        with pytest.raises(_Dispatched):
+            torch.autograd.grad(outs, leaf, grads)
