@@ -77,7 +77,7 @@ def linear_attention(
             raise ValueError(f"{operator} lengths must have the prefix shape {tuple(prefix)}, got {tuple(lengths.shape)}")
         if lengths.dtype not in (torch.int32, torch.int64):
             raise unsupported(operator, "takes lengths in int32 or int64", dtype=lengths.dtype)
-        lengths = lengths.reshape(-1).contiguous()
+        lengths = lengths.resolve_neg().reshape(-1).contiguous()
     q, k, v = _batched(query, length), _batched(key, length), _batched(value, length)
     s0 = None
     if initial_state is not None:

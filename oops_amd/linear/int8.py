@@ -101,6 +101,7 @@ def int8_linear(
 
 
 def _rows(t: Tensor) -> Tensor:
+    t = t.resolve_neg()
     if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t

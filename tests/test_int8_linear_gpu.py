@@ -180,3 +180,12 @@ def test_two_streams():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+def test_lazily_negated_operands():
+    args, bias = _operands(5, 48, 20, low=-127)
+    want = int8_linear(*args, bias)
+    for i in range(5):
+        ops = [torch._neg_view(-t) if i == j else t for j, t in enumerate((*args, bias))]
+        assert ops[i].is_neg()
+        assert torch.equal(int8_linear(*ops), want)

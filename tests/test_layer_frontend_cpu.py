@@ -130,6 +130,29 @@ def test_wrappers_in_the_place_of_any_operand_are_dispatched(no_launches):
         oops_amd.rms_norm(x, 8, torch.nn.Parameter(w), residual=r)
 
 
+def test_lazily_negated_operands_are_resolved(no_launches, monkeypatch):
+    """Addresses cannot carry a lazy negation: the launch of each operator gets the negated values."""
+
+    def launched(*args):
+        raise _Dispatched(*args)
+
+    for module, name in ((rms_norm, "_int8_impl"), (int8, "_forward_impl"), (linear, "_forward_impl"), (linear, "_step_impl")):
+        monkeypatch.setattr(module, name, launched)
+    i8, w8 = torch.arange(24, dtype=torch.int8).view(3, 8), torch.arange(40, dtype=torch.int8).view(5, 8)
+    x, q, v, ld, s0 = torch.randn(3, 8), torch.randn(2, 3, 7, 8), torch.randn(2, 3, 7, 4), torch.rand(3), torch.randn(2, 3, 8, 4)
+    calls = [(lambda x, w, r: oops_amd.rms_norm_int8(x, 8, w, residual=r), [x, torch.randn(8), torch.randn(3, 8)]),
+             (oops_amd.int8_linear, [i8, torch.rand(3), w8, torch.rand(5), torch.rand(5)]),
+             (oops_amd.linear_attention, [q, q + 1, v, ld, s0, torch.tensor([-7, -5])]),
+             (lambda *t: oops_amd.linear_attention_step(*t, s0), [q[:, :, 0], q[:, :, 1], v[:, :, 0], ld])]  # fmt: skip
+    for call, operands in calls:
+        for i, negated in enumerate(operands):
+            with pytest.raises(_Dispatched) as launch:
+                call(*[torch._neg_view(t) if i == j else t for j, t in enumerate(operands)])
+            passed = [t for t in launch.value.args if isinstance(t, torch.Tensor)]
+            assert not any(t.is_neg() for t in passed)
+            assert any(t.shape == negated.shape and torch.equal(t, -negated) for t in passed)
+
+
 @pytest.mark.parametrize("which", [0, 1])
 def test_wrapped_gradients_are_dispatched(no_launches, monkeypatch, which):
     monkeypatch.setattr(rms_norm, "_forward_impl", lambda x, w, r, eps, save: (x + 0, x + r, torch.ones(3)))
