@@ -355,6 +355,15 @@ __global__ __launch_bounds__(2 * D, MAIN || D == 128 ? 2 : 4) void walk_chunks_k
     __builtin_amdgcn_sched_barrier(0);
     // the state's update
     const float lm = decay_power(l2, (float)m);
+    // An infinity is its own first term: its difference with that is NaN, so a lane that holds one (or a NaN) among
+    // its column's tokens has no further terms (4 x 16 heads x 4096 x 128 in training: 373 us, without this 368).
+    uint32_t keep = ~0u;
+    if (!MAIN || bad[turn]) {
+      uint32_t odd = 0;
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) odd |= non_finite(__builtin_bit_cast(uint4, cf[kb]));
+      keep = odd & 0x80008000u ? 0u : ~0u;
+    }
 #pragma unroll
     for (int rt = 0; rt < NW; ++rt)
 #pragma unroll
@@ -373,6 +382,11 @@ __global__ __launch_bounds__(2 * D, MAIN || D == 128 ? 2 : 4) void walk_chunks_k
         part[q] = to_bf16x8(x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] -= (float)part[q][j];
+        if (q > 0) {
+          uint4 u = __builtin_bit_cast(uint4, part[q]);
+          u.x &= keep, u.y &= keep, u.z &= keep, u.w &= keep;
+          part[q] = __builtin_bit_cast(Frag, u);
+        }
       }
 #pragma unroll
       for (int rt = 0; rt < NW; ++rt) {

@@ -497,3 +497,71 @@ def test_compile_with_sizes_that_change():
             results.append((*outs, *torch.autograd.grad(outs, leaves, (x["do"], x["ds"]))))
         for got, ref in zip(*results):
             torch.testing.assert_close(got, ref, atol=0, rtol=0)
+
+
+def _gradients_and_results(x):
+    """(name, the operator's, the recurrence's), of the first and last batch element's first and last head."""
+
+    names = ("q", "k", "v", "s0")
+    b, h = x["q"].shape[:2]
+    ends = lambda t: t[:: max(b - 1, 1), :: max(h - 1, 1)]  # noqa: E731
+    leaves = [x[name].detach().requires_grad_(True) for name in names]
+    outs = linear_attention(*leaves[:3], x["ld"], leaves[3], return_state=True)
+    got = [t.detach() for t in (*outs, *torch.autograd.grad(outs, leaves, (x["do"], x["ds"])))]
+    q, k, v, s0, do, ds = (f64(ends(x[name])) for name in (*names, "do", "ds"))
+    ld = f64(x["ld"])[:: max(h - 1, 1)]
+    with np.errstate(invalid="ignore"):
+        want = layers.linear_attention_forward(q, k, v, ld, s0)
+        want += layers.linear_attention_backward(q, k, v, ld, do, ds, s0)
+    return zip(("out", "state", "dq", "dk", "dv", "dinitial"), map(ends, got), want, strict=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,e,b,h", [(32, 32, 1, 2), (40, 24, 2, 1), (64, 64, 1, 2), (128, 128, 1, 2), (128, 64, 2, 1),
+                                     (64, 64, 32, 12), (128, 128, 16, 12)])  # fmt: skip
+def test_non_finite_operands(dtype, d, e, b, h):
+    """An infinity or a NaN in any operand or gradient: results are finite exactly where the recurrence's are, with
+    one, two and four waves a workgroup, in segments and in one."""
+
+    for i, (name, value) in enumerate([("v", "inf"), ("v", "nan"), ("k", "-inf"), ("q", "inf"), ("do", "inf"), ("s0", "nan"),
+                                       ("ds", "inf")]):  # fmt: skip
+        x = _case(67 + i, b, h, 150, d, e, dtype)
+        x["ld"] = torch.linspace(-0.3, -0.01, h, device=DEV)
+        row = 70 if name not in ("s0", "ds") else 3
+        x[name][0, -1, row, 5] = float(value)
+        for what, got, want in _gradients_and_results(x):
+            assert np.array_equal(np.isfinite(f64(got)), np.isfinite(want)), f"{what}: {value} in {name}"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("decay", [float("-inf"), -200.0])
+def test_non_finite_operands_and_no_memory(dtype, decay):
+    """A head without memory multiplies what it forgets by zero: after an infinity its column is NaN, as the
+    recurrence's is; the other heads stay finite."""
+
+    x = _case(75, 1, 2, 150, 32, 32, dtype)
+    x["ld"] = torch.tensor([decay, -0.01], device=DEV)
+    x["v"][0, 0, 70, 5] = float("inf")
+    out, state = linear_attention(x["q"], x["k"], x["v"], x["ld"], x["s0"], return_state=True)
+    with np.errstate(invalid="ignore"):
+        want, last = layers.linear_attention_forward(*(f64(x[n]) for n in ("q", "k", "v", "ld", "s0")))
+    assert np.array_equal(np.isfinite(f64(out)), np.isfinite(want))
+    assert np.array_equal(np.isfinite(f64(state)), np.isfinite(last))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,b,h", [(32, 1, 2), (64, 1, 2), (128, 1, 2), (128, 16, 12)])
+def test_an_infinite_value_leaves_an_infinity_in_the_state(dtype, d, b, h):
+    """Positive keys and queries: the state's column and the outputs are that infinity, not NaN; so is a gradient's."""
+
+    x = _case(77, b, h, 150, d, d, dtype)
+    x["ld"] = torch.linspace(-0.1, -0.01, h, device=DEV)
+    for name in ("q", "k"):
+        x[name] = x[name].abs() + 0.125
+    x["v"][0, -1, 70, 5] = float("-inf")
+    x["do"][0, 0, 30, 7] = float("inf")
+    for what, got, want in _gradients_and_results(x):
+        if what in ("out", "state", "dv", "dinitial"):
+            got = f64(got)
+            assert np.array_equal(np.isnan(got), np.isnan(want)), what
+            assert np.array_equal(np.where(np.isinf(got), got, 0), np.where(np.isinf(want), want, 0)), what
