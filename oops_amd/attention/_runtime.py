@@ -78,7 +78,13 @@ def call_on(device_index: int, entry, *args) -> int:
         return entry(*args, torch._C._cuda_getCurrentRawStream(device_index))
 
 
-_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
+
+
+def any_wrapped(*tensors) -> bool:
+    """Whether any operand (None ones aside) is of a tensor subclass, which need not have memory of its own."""
+
+    return not _PLAIN.issuperset(map(type, tensors))
 
 
 def needs_custom_op(tensor, *others) -> bool:
@@ -88,12 +94,12 @@ def needs_custom_op(tensor, *others) -> bool:
     parameters are plain: a wrapper subclass has no memory of its own, and its NULL pointer would be taken
     as an operand that is not given."""
 
-    if torch.compiler.is_compiling() or type(tensor) is not torch.Tensor or _get_current_dispatch_mode() is not None:
-        return True
-    for t in others:
-        if type(t) not in _PLAIN:
-            return True
-    return False
+    return (
+        torch.compiler.is_compiling()
+        or type(tensor) is not torch.Tensor
+        or _get_current_dispatch_mode() is not None
+        or any_wrapped(*others)
+    )
 
 
 def without_second_derivative(grads, ctx, grad_output, differentiable: bool = False):

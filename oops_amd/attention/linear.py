@@ -24,6 +24,7 @@ from .. import _lib
 from .._errors import unsupported
 from ._core import SUPPORTED_DTYPES, _DTYPE_CODE, _ptr
 from ._runtime import (
+    any_wrapped,
     call_on,
     is_nested,
     needs_custom_op,
@@ -402,6 +403,6 @@ class _EagerLinearAttention(torch.autograd.Function):
     def backward(ctx, dout, dstate):
         if dout is None and dstate is None:
             return (None,) * 8
-        grads = _grads(ctx, dout, dstate, needs_custom_op(dstate if dout is None else dout, dstate))
+        grads = _grads(ctx, dout, dstate, any_wrapped(dout, dstate))
         later = any(t is not None and t.requires_grad for t in (dout, dstate))
         return without_second_derivative(grads, ctx, dout, differentiable=later)

@@ -22,6 +22,7 @@ from torch import Tensor
 from .. import _lib
 from .._errors import unsupported
 from ..attention._runtime import (
+    any_wrapped,
     call_on,
     is_nested,
     needs_custom_op,
@@ -378,7 +379,6 @@ class _EagerRmsNorm(torch.autograd.Function):
     def backward(ctx, dy, dsum):
         if dy is None and dsum is None:
             return None, None, None, None
-        traced = needs_custom_op(dsum if dy is None else dy, dsum)
-        grads = _grads(ctx, dy, dsum, rms_norm_backward if traced else _backward_impl)
+        grads = _grads(ctx, dy, dsum, rms_norm_backward if any_wrapped(dy, dsum) else _backward_impl)
         later = any(t is not None and t.requires_grad for t in (dy, dsum))
         return (*without_second_derivative(grads, ctx, dy, differentiable=later), None)
