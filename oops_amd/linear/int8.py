@@ -21,6 +21,7 @@ from .. import _lib
 from .._errors import unsupported
 from ..attention._runtime import (
     call_on,
+    is_nested,
     needs_custom_op,
     on_one_device,
     require_no_forward_mode,
@@ -56,6 +57,8 @@ def int8_linear(
     pointers that are multiples of 16 bytes are the fast case.
     """
 
+    if is_nested(input):
+        raise unsupported(_OPERATOR, "takes dense tensors", hint="pass the packed values")
     require_no_forward_mode(_OPERATOR, input, input_scale, weight, weight_scale, bias)
     if not on_one_device(input.device, input_scale, weight, weight_scale, bias):
         require_same_device(_OPERATOR, input, input_scale, weight, weight_scale, bias)

@@ -116,7 +116,7 @@ def quantize_int8(input: Tensor) -> Tuple[Tensor, Tensor]:
     """
 
     operator = "quantize_int8"
-    _check(operator, input, input.shape[-1] if input.dim() else 0, None, None)
+    _check(operator, input, 0 if is_nested(input) or not input.dim() else input.shape[-1], None, None)
     _require_inference(operator, input)
     x = _rows(input)
     call = quantize_int8_forward if needs_custom_op(x) else _quantize_impl
@@ -128,6 +128,10 @@ def quantize_int8(input: Tensor) -> Tuple[Tensor, Tensor]:
 
 
 def _check(operator: str, input: Tensor, normalized_shape, weight: Optional[Tensor], residual: Optional[Tensor]) -> None:
+    if is_nested(input):  # (rms_norm has taken its packed values)
+        raise unsupported(operator, "takes dense tensors", hint="pass the packed values")
+    if is_nested(residual):
+        raise ValueError(f"{operator} residual must have the input's shape")
     require_no_forward_mode(operator, input, weight, residual)
     if not on_one_device(input.device, weight, residual):
         require_same_device(operator, input, weight, residual)
@@ -135,7 +139,7 @@ def _check(operator: str, input: Tensor, normalized_shape, weight: Optional[Tens
     if len(shape) != 1:
         raise unsupported(operator, "normalizes over the final dimension only", normalized_shape=shape)
     width = shape[0]
-    if residual is not None and (is_nested(residual) or residual.shape != input.shape):
+    if residual is not None and residual.shape != input.shape:
         raise ValueError(f"{operator} residual must have the input's shape")
     ok = (
         input.is_cuda

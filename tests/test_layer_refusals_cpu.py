@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import oops_amd
+from nested_standin import NestedTensor
 from oops_amd import OOpsUnsupportedError, _lib
 
 
@@ -132,3 +133,16 @@ def test_linear_attention_entry_points(lib):
     _refused(lib, lib.oops_linear_attn_backward(g, FAKE, FAKE, FAKE, FAKE, None, None, None, None, None, FAKE, None, None,
                                                 None, None, 0, None), 1, "grad_out")  # fmt: skip
     _refused(lib, lib.oops_linear_attn_step(g, FAKE, FAKE, FAKE, FAKE, None, FAKE, None), 1, "non-NULL")
+
+
+def test_nested_operands():
+    a = NestedTensor([torch.randn(n, 8) for n in (3, 5)], ragged_dims=(0,))
+    i8, s = torch.zeros(5, 8, dtype=torch.int8), torch.ones(5)
+    for call in (lambda: oops_amd.rms_norm_int8(a, 8), lambda: oops_amd.rms_norm_int8(a, 8, residual=a),
+                 lambda: oops_amd.quantize_int8(a), lambda: oops_amd.int8_linear(a, s, i8, s),
+                 lambda: oops_amd.linear_attention(a, a, a, s), lambda: oops_amd.linear_attention_step(a, a, a, s, s)):  # fmt: skip
+        with pytest.raises(OOpsUnsupportedError, match="dense"):
+            call()
+    for norm in (oops_amd.rms_norm, oops_amd.rms_norm_int8):
+        with pytest.raises(ValueError, match="residual"):
+            norm(a.concat, 8, residual=a)
