@@ -255,9 +255,9 @@ __global__ __launch_bounds__(kThreads) void rms_forward_kernel(RmsArgs a) {
       top = row_max<TPR>(top, red_max[turn]);
       const bool fine = top < 0x7F800000u;
       const float amax = __builtin_bit_cast(float, top);
-      // (rows of magnitudes below 2^-100 are scaled up first: 127 / amax would be infinite)
-      const float up = amax < 0x1p-100f ? 0x1p64f : 1.0f;
-      const float inv = fine && top ? 127.0f / (amax * up) : 0.f;
+      // (rows of magnitudes far from 1 are scaled first: 1 / amax, or 127 amax, would be infinite)
+      const float up = amax < 0x1p-100f ? 0x1p64f : amax > 0x1p100f ? 0x1p-64f : 1.0f;
+      const float most = amax * up, inv = fine && top ? 1.0f / most : 0.f;
       if (lane == 0) a.rstd[row] = fine ? amax / 127.0f : __builtin_nanf("");
       int8_t* q = static_cast<int8_t*>(a.y) + row * a.width;
 #pragma unroll
@@ -265,8 +265,12 @@ __global__ __launch_bounds__(kThreads) void rms_forward_kernel(RmsArgs a) {
         int qi[VE];
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-          const float v = fine ? (h[c][j] * up) * inv : 0.f;
-          qi[j] = (int)__builtin_rintf(fminf(fmaxf(v, -127.f), 127.f));
+          // The quotient corrected by its residual: 127 x / amax to float32, so that what lies exactly between two
+          // steps (half the largest: 63.5) goes to the even one.  (127 x is exact for 16-bit rows.)
+          const float x = h[c][j] * up, x127 = x * 127.f, near = x127 * inv;
+          float rest = __builtin_fmaf(-near, most, x127);
+          if constexpr (MODE != kInt8 || sizeof(T) == 4) rest += __builtin_fmaf(x, 127.f, -x127);
+          qi[j] = fine ? (int)__builtin_rintf(__builtin_fmaf(rest, inv, near)) : 0;
         }
         store_int8<T, TPR, VEC>(q, a.width, lane, c, qi);
       }

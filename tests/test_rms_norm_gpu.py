@@ -330,3 +330,29 @@ def test_default_eps_of_the_module(dtype, scale):
     n, d = abs(h) * rstd, abs(f64(dy))
     size = rstd * (d + n * (d * n).mean(-1, keepdims=True))
     assert_within(dx, want_dx, half(dtype) * abs(want_dx) + 2 * ARITH * size + smallest(dtype), "dx")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [24, 1000, 4096])
+def test_int8_values_are_the_exact_quotients(dtype, width):
+    """rint(x 127 / max|row|) with ties to even: half the largest lies exactly between 63 and 64.  16-bit rows have the
+    values of exact arithmetic everywhere: with significands of p bits, a quotient that is no tie n + 1/2 is at least
+    1 / (254 2^p) of itself away from one (254 x and (2 n + 1) max|row| are different whole multiples of one power of
+    two, the first below 254 2^p of them), 2^-19 in float16, where float32 arithmetic is off by a few 2^-24."""
+
+    g = torch.Generator().manual_seed(31)
+    x = _randn(g, 700, width, dtype=dtype)
+    x[:, 0] = x.abs().amax(-1) * 1.5
+    x[:, 1], x[:, 2] = x[:, 0] / 2, x[:, 0] / -2
+    x[350:] *= -1
+    for scale in (1.0, 2.0**-9, 2.0**7) if dtype == torch.float16 else (1.0, 2.0**-110, 2.0**120):
+        rows = x * scale
+        values, _ = quantize_int8(rows)
+        y = rows.double()
+        want = torch.round(y * 127 / y.abs().amax(-1, keepdim=True))
+        assert (values[:, 1:3].abs() == 64).all()
+        if dtype != torch.float32:
+            assert torch.equal(values.double(), want)
+        assert (values.double() - want).abs().max() <= 1
+    values, _ = rms_norm_int8(x, width)  # (a norm without weight keeps the half exactly)
+    assert (values[:, 1:3].abs() == 64).all()
