@@ -481,7 +481,8 @@ int oops_rms_norm_backward(const oops_rms_norm_geometry* geo, const void* h, con
 /* ---- linear layer on 8-bit integers ----
  *
  * out[r][j] = x_scale[r] * w_scale[j] * sum_k x[r][k] * w[j][k] + bias[j], sums in 32-bit integers (exact: k at most
- * 131071), out [rows][n] rounded once.  Any k, n, alignment; rows x_row and w_row bytes apart. */
+ * 131071), scales and bias applied in float32, out [rows][n].  Any k, n, alignment; rows x_row and w_row bytes
+ * apart. */
 typedef struct oops_int8_geometry {
   int64_t rows;
   int64_t n;

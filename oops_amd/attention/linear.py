@@ -66,6 +66,10 @@ def linear_attention(
 
     Returns the outputs ``(*prefix, H, L, E)`` in the query's dtype and dimension order, or ``(out, state)``.
     Gradients reach query, key, value and ``initial_state``; second derivatives raise.
+
+    Infinities and NaN act as in the recurrence: what they do not reach stays finite (nothing before their token or in
+    other heads, and of a value's only its own column), what they reach is infinite or NaN; a head whose decay is ``-inf``
+    multiplies what it forgets by zero, which is NaN for them.
     """
 
     operator = "linear_attention"

@@ -3,7 +3,9 @@
 //   out[r][j] = x_scale[r] w_scale[j] sum_k x[r][k] w[j][k] + bias[j]
 //
 // sums exact in 32-bit integers on the int8 matrix units (32x32x32 MFMA, twice
-// the bf16 rate), one rounding at the end.
+// the bf16 rate); scales and bias in float32 (three roundings: the conversion
+// of sums above 2^24, the product with x_scale, one fused product and
+// addition), then the result's type.
 //
 // The weight is MFMA's row operand: a lane then holds one output row and four
 // consecutive columns at a time.  By size and alignment:

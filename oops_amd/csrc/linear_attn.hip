@@ -55,11 +55,11 @@ __device__ __forceinline__ int opaque(int x) {
 // walk_chunks_kernel<.., false> makes each segment's state from zero,
 // walk_scan_kernel joins them, then every segment starts from its own state.
 //
-// Measured, 4 x 16 heads x 4096 x 128: 46 us the segments' states, 15 the scan,
-// 78 the outputs (the matrix units busy 19% and 14% of it): bound by the loads'
-// latency and the LDS exchanges between a chunk's four products.  Three
-// workgroups a CU on single direct-to-LDS buffers took 95, outputs written in
-// whole rows through LDS 87.
+// Measured, 4 x 16 heads x 4096 x 128: 47 us the segments' states, 15 the scan,
+// 71 to 85 the outputs and each gradient (the matrix units busy 20% and 17% of
+// it): bound by the loads' latency and the LDS exchanges between a chunk's four
+// products.  Three workgroups a CU on single direct-to-LDS buffers took 95,
+// outputs written in whole rows through LDS 87.
 //
 // Operand layouts: accumulators hold [row of the state or value][lane], lane =
 // value column (state) or token (weights, outputs), so weights and state are
@@ -429,9 +429,12 @@ __global__ __launch_bounds__(2 * D, MAIN || D == 128 ? 2 : 4) void walk_chunks_k
 // 32 x 32 weight tile for its 32 columns itself and keeps it in registers (an
 // accumulator register is the next MFMA's k-operand as it is), so there is no
 // exchange between waves: 13% more products than sharing 64-token tiles, no
-// barrier between them.  Bound by the float32 MFMA rate (a sixteenth of
-// bfloat16's).  64 heads x 2048 x 128 float32 229 us (two workgroups a CU 289,
-// with spills).
+// barrier between them.  64 heads x 2048 x 128 float32: 70 us the segments'
+// states, 14 the scan, 159 the outputs, the matrix units busy 32% and 60% of it
+// (their rate is a sixteenth of bfloat16's; the rest is one wave a SIMD waiting
+// for its own chain of products; two workgroups a CU spill: 289 us, not 229).
+// Small calls are bound by that latency alone: 48 x 777 x 64 in float16 gives
+// 864 waves for 1024 SIMDs, busy 5% and 13%.
 constexpr int kExactChunk = 32;
 
 template <typename T, int D, bool VEC, bool MAIN>
@@ -756,7 +759,8 @@ namespace {
 // the larger part (training 2 x 300 x 64 in float16 87 us, 192 with segments of
 // two 64-token chunks; 48 x 777 x 64 123, 147), of 64 in bfloat16 while there are
 // not two waves a CU (2 x 300 x 64 63, 80; 64 x 512 x 64 70, without them 66).
-// More than 256 segments are not worth their scan (32768 x 64: 154, 107).
+// (At most 256 segments a head are made so: more single chunks are not worth
+// their scan, 32768 x 64: 154, 107.  Segments of several chunks have no limit.)
 void plan_segments(int dtype, const LinearWalk& w, ChunkArgs& ca) {
   const bool exact = dtype != OOPS_BF16;
   const int64_t tokens = exact ? kExactChunk : kChunk, unit = kChunk / tokens;

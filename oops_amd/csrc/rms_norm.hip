@@ -9,14 +9,17 @@
 // About ten operations an element against 4 to 10 bytes: bound by HBM.  A row
 // is held in the registers of TPR lanes (16 bytes a lane and load, CH loads a
 // lane), so every tensor is read and written once; statistics, products and
-// the maximum are float32.  Rows of up to 16 * 64 bytes stay in one wave (no
-// barrier); longer ones take the four waves of a workgroup.  The backward
-// walks its rows with a bounded grid, dw in registers, one partial row a
-// workgroup, summed afterwards in a fixed order.
+// the maximum are float32.  Rows of up to 256 pieces of 16 bytes (4 KB) stay
+// in one wave, of up to 16 pieces in 16 lanes of it (no barrier); longer ones
+// take the four waves of a workgroup.  The backward walks its rows with a
+// bounded grid, dw in registers, one partial row a workgroup, summed afterwards
+// in a fixed order.
 //
 // Measured (a copy reaches 4.9 TB/s): 8192 x 4096 bfloat16 with the residual's
-// addition 50 us forward (5.3 TB/s), 57 backward (4.9), 6.5 the weight's sum;
-// 8-bit output of 8192 x 8192 102 (4.6); 65536 x 128 8.4, 10.5 and 3.9.
+// addition 50 us forward (5.3 TB/s), 57 backward (4.7), 6.7 the weight's sum;
+// 8-bit output of 8192 x 8192 102 (4.6); 65536 x 128 8.3, 10.0 and 3.9; 8-bit
+// rows of 8192 x 4096 21 (4.7), 30 where the launch before has left 268 MB of
+// output to be written back.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

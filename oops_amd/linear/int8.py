@@ -4,7 +4,9 @@
 
 The serving form of the projections around attention and its gated output stage: ``rms_norm_int8`` makes the
 activations behind a norm, ``quantize_int8`` elsewhere, and the weight once, when a model is loaded.  The sums
-are exact 32-bit integers on the int8 matrix units; the result is rounded once.  Kernels: csrc/int8_linear.hip.
+are exact 32-bit integers on the int8 matrix units; scales and bias are applied in float32 (the conversion of a sum
+above 2^24, the product with the token's scale and a fused product and addition round once each), then the result is
+rounded to its type.  Kernels: csrc/int8_linear.hip.
 The reference has no counterpart.
 """
 
@@ -54,7 +56,9 @@ def int8_linear(
         dtype: of the result, bfloat16 (default), float16 or float32.
 
     Returns ``(..., N)`` in ``dtype``.  Rows are read in place where the last dimension is contiguous; rows and
-    pointers that are multiples of 16 bytes are the fast case.
+    pointers that are multiples of 16 bytes are the fast case.  ``quantize_int8`` and ``rms_norm_int8`` make rows of up
+    to 16384 values; wider ones take the same formula in PyTorch, with x in float32: ``scale = x.abs().amax(-1) / 127``
+    and ``torch.round(x / scale.clamp_min(1e-30)[..., None]).to(torch.int8)``.
     """
 
     if is_nested(input):

@@ -111,8 +111,8 @@ def quantize_int8(input: Tensor) -> Tuple[Tensor, Tensor]:
     r"""Each row of the last dimension in 8 bits: ``values = rint(input * 127 / max|row|)``, ``scales = max|row| / 127``.
 
     ``input``: CUDA float16 / bfloat16 / float32 ``(..., C)``, ``C`` in 1..16384: activations, or the weight
-    ``(out_features, in_features)`` of an 8-bit linear layer.  Returns int8 values and float32 scales as
-    ``rms_norm_int8`` does; inference only.
+    ``(out_features, in_features)`` of an 8-bit linear layer (wider rows: see ``int8_linear``).  Returns int8 values and
+    float32 scales as ``rms_norm_int8`` does; inference only.
     """
 
     operator = "quantize_int8"
