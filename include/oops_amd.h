@@ -535,6 +535,122 @@ int oops_linear_attn_backward(const oops_linear_attn_geometry* geo, const void* 
 int oops_linear_attn_step(const oops_linear_attn_geometry* geo, const void* q, const void* k, const void* v,
                           const float* log_decay, float* state, void* out, void* stream);
 
+/* ---- norm of queries and keys for each head, and rotation by their position ----
+ *
+ * For every (batch, head, token) row x of `size` elements: n = x * (mean(x^2) + eps)^-1/2 * weight, then elements i and
+ * i + rotary / 2 (i < rotary / 2) are turned by the token's angle, elements from `rotary` on stay.  table is float32
+ * [table_rows][2][rotary / 2], cosines then sines; positions [batch][length] chooses a token's row (NULL: the token's
+ * index; values outside the table are taken as the nearer end).  Operands 0 are the queries', 1 the keys'; element
+ * (b, h, t, i) is at b * stride[0] + h * stride[1] + t * stride[2] + i.  weight [size] is float32 (weight_f32) or of
+ * dtype, NULL for ones. */
+enum oops_rotary_operand { OOPS_RO_X, OOPS_RO_Y, OOPS_RO_DY, OOPS_RO_DX, OOPS_RO_OPERANDS };
+typedef struct oops_rotary_geometry {
+  int32_t dtype;
+  int32_t size;   /* 1..256 */
+  int32_t rotary; /* even, 0..size */
+  int32_t positions_i64;
+  int32_t heads[2];
+  int32_t weight_f32[2];
+  int64_t batch;
+  int64_t length;
+  int64_t table_rows;
+  int64_t stride[OOPS_RO_OPERANDS][2][3];
+  float eps;
+} oops_rotary_geometry;
+int oops_rms_norm_rotary_forward(const oops_rotary_geometry* geo, const void* query, const void* key,
+                                 const void* query_weight, const void* key_weight, const float* table,
+                                 const void* positions, void* query_out, void* key_out, void* stream);
+/* Gradients from those of the outputs (either pair grad / input gradient may be NULL: not wanted); a weight's gradient
+ * (NULL: not wanted) is of its type, summed in a fixed order over float32 partials in the workspace. */
+size_t oops_rms_norm_rotary_backward_workspace_bytes(const oops_rotary_geometry* geo);
+int oops_rms_norm_rotary_backward(const oops_rotary_geometry* geo, const void* query, const void* key,
+                                  const void* query_weight, const void* key_weight, const float* table,
+                                  const void* positions, const void* grad_query_out, const void* grad_key_out,
+                                  void* grad_query, void* grad_key, void* grad_query_weight, void* grad_key_weight,
+                                  void* workspace, size_t ws_bytes, void* stream);
+
+/* ---- causal attention over whole prompts ----
+ *
+ * o_i = sum_j softmax_j(scale q_i . k_j) v_j over the tokens j <= i of i's sequence; query head h reads key head
+ * h / (heads / kv_heads).  offsets (NULL: each batch element is one sequence) has sequences + 1 non-decreasing bounds of
+ * sequences packed along the tokens, for every batch element; tokens outside them have zero outputs and gradients.
+ * Element (b, h, t, i) of an operand is at b * stride[0] + h * stride[1] + t * stride[2] + i; pointers, strides and sizes
+ * times the element's size are multiples of 16 bytes (stride[i][0] of a single batch element and stride[i][1] of a single
+ * head are not read).  lse is float32 [batch][heads][length] in log2 units, out_low (16-bit types) the rounding's
+ * remainder of out with out's strides; both are NULL where no backward follows. */
+enum oops_causal_operand {
+  OOPS_CA_Q, OOPS_CA_K, OOPS_CA_V, OOPS_CA_O, OOPS_CA_DO, OOPS_CA_DQ, OOPS_CA_DK, OOPS_CA_DV, OOPS_CA_OPERANDS
+};
+typedef struct oops_causal_geometry {
+  int32_t dtype;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t key_size;   /* 1..128 */
+  int32_t value_size; /* 1..128 */
+  int32_t sequences;  /* with offsets */
+  int32_t offsets_i64;
+  float scale;
+  int64_t batch;
+  int64_t length;
+  int64_t stride[OOPS_CA_OPERANDS][3];
+} oops_causal_geometry;
+int oops_causal_attn_forward(const oops_causal_geometry* geo, const void* q, const void* k, const void* v,
+                             const void* offsets, void* out, void* out_low, float* lse, void* stream);
+size_t oops_causal_attn_backward_workspace_bytes(const oops_causal_geometry* geo);
+int oops_causal_attn_backward(const oops_causal_geometry* geo, const void* q, const void* k, const void* v,
+                              const void* offsets, const void* out, const void* out_low, const float* lse,
+                              const void* grad_out, void* grad_q, void* grad_k, void* grad_v, void* workspace,
+                              size_t ws_bytes, void* stream);
+
+/* ---- paged key/value cache in 4 bits ----
+ *
+ * codes [pages][heads][2][page][size / 2] and scales [pages][heads][2][page][size / 32] (keys, then values; size a
+ * multiple of 32 up to 128, page a multiple of 16): each block of 32 channels has one exponent byte e and stands for
+ * code * 2^(e - 127), codes 0..7 for 0, 0.5, 1, 1.5, 2, 3, 4, 6 and 8..15 for their negatives; channel 2 i is the low
+ * half of byte i.  A written block has the smallest e (1..252) with max|block| <= 6 * 2^(e - 127) and values rounded to
+ * the nearest code, ties to even codes (saturated above 6 * 2^125); one with an infinity or a NaN has e = 255, which
+ * stands for NaN.  slots [batch][length]: token's page * page_size + place; others (negative ones, say) are not written
+ * and read as zeros; of tokens with the same slot the last is kept.  Element (b, h, t, i) of key and value is at
+ * b * stride[0] + h * stride[1] + t * stride[2] + i. */
+typedef struct oops_cache_geometry {
+  int32_t dtype;
+  int32_t heads;
+  int32_t size;
+  int32_t page;
+  int32_t slots_i64;
+  int64_t pages;
+  int64_t batch;
+  int64_t length;
+  int64_t stride[2][3]; /* key, value */
+} oops_cache_geometry;
+size_t oops_cache_write_workspace_bytes(const oops_cache_geometry* geo);
+int oops_cache_write(const oops_cache_geometry* geo, void* codes, void* scales, const void* key, const void* value,
+                     const void* slots, void* workspace, size_t ws_bytes, void* stream);
+int oops_cache_read(const oops_cache_geometry* geo, const void* codes, const void* scales, const void* slots, void* key,
+                    void* value, void* stream);
+
+/* One query token of each sequence over such a cache: out = softmax(scale q . k) v over the first lengths[b] tokens of
+ * sequence b, whose token t is in page table[b * max_pages + t / page] at place t % page.  Query head h reads key head
+ * h / (heads / kv_heads).  Tokens behind max_pages * page and those of pages outside 0..pages-1 do not take part; a
+ * sequence without tokens has zeros.  query is [batch][heads][size] with the given strides, out contiguous. */
+typedef struct oops_cache_attn_geometry {
+  int32_t dtype;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t size;
+  int32_t page;
+  int32_t lengths_i64;
+  int64_t pages;
+  int64_t batch;
+  int64_t max_pages;
+  int64_t stride[2]; /* of the query: batch, head */
+  float scale;
+} oops_cache_attn_geometry;
+size_t oops_cache_attn_workspace_bytes(const oops_cache_attn_geometry* geo);
+int oops_cache_attn(const oops_cache_attn_geometry* geo, const void* query, const void* codes, const void* scales,
+                    const int32_t* table, const void* lengths, void* out, void* workspace, size_t ws_bytes,
+                    void* stream);
+
 /* Thread-local description of the last failure (empty string if none). */
 const char* oops_last_error(void);
 

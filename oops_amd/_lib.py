@@ -20,7 +20,7 @@ BIAS_NONE, BIAS_FULL, BIAS_SHARED = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 32 << 20
 PHASE_DELTA, PHASE_DQ, PHASE_DKV, PHASE_DBIAS = 1, 2, 4, 8
 TABLE_WIDTH = 40
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 # geometry table columns (enum oops_table_column)
 (
@@ -89,6 +89,17 @@ EXPORTED_SYMBOLS = (
     "oops_linear_attn_backward_workspace_bytes",
     "oops_linear_attn_backward",
     "oops_linear_attn_step",
+    "oops_rms_norm_rotary_forward",
+    "oops_rms_norm_rotary_backward_workspace_bytes",
+    "oops_rms_norm_rotary_backward",
+    "oops_causal_attn_forward",
+    "oops_causal_attn_backward_workspace_bytes",
+    "oops_causal_attn_backward",
+    "oops_cache_write_workspace_bytes",
+    "oops_cache_write",
+    "oops_cache_read",
+    "oops_cache_attn_workspace_bytes",
+    "oops_cache_attn",
     "oops_last_error",
     "oops_abi_version",
 )
@@ -210,6 +221,76 @@ class LinearAttnGeometry(ctypes.Structure):
         ("stride", (ctypes.c_int64 * 3) * LA_OPERANDS),
         ("scale", ctypes.c_float),
         ("lengths_i64", ctypes.c_int32),
+    ]
+
+
+# operands of RotaryGeometry.stride (enum oops_rotary_operand), each for the queries and the keys
+RO_X, RO_Y, RO_DY, RO_DX, RO_OPERANDS = range(5)
+
+
+class RotaryGeometry(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("size", ctypes.c_int32),
+        ("rotary", ctypes.c_int32),
+        ("positions_i64", ctypes.c_int32),
+        ("heads", ctypes.c_int32 * 2),
+        ("weight_f32", ctypes.c_int32 * 2),
+        ("batch", ctypes.c_int64),
+        ("length", ctypes.c_int64),
+        ("table_rows", ctypes.c_int64),
+        ("stride", ((ctypes.c_int64 * 3) * 2) * RO_OPERANDS),
+        ("eps", ctypes.c_float),
+    ]
+
+
+# operands of CausalGeometry.stride (enum oops_causal_operand)
+CA_Q, CA_K, CA_V, CA_O, CA_DO, CA_DQ, CA_DK, CA_DV, CA_OPERANDS = range(9)
+
+
+class CausalGeometry(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("key_size", ctypes.c_int32),
+        ("value_size", ctypes.c_int32),
+        ("sequences", ctypes.c_int32),
+        ("offsets_i64", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("batch", ctypes.c_int64),
+        ("length", ctypes.c_int64),
+        ("stride", (ctypes.c_int64 * 3) * CA_OPERANDS),
+    ]
+
+
+class CacheGeometry(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("size", ctypes.c_int32),
+        ("page", ctypes.c_int32),
+        ("slots_i64", ctypes.c_int32),
+        ("pages", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+        ("length", ctypes.c_int64),
+        ("stride", (ctypes.c_int64 * 3) * 2),
+    ]
+
+
+class CacheAttnGeometry(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("size", ctypes.c_int32),
+        ("page", ctypes.c_int32),
+        ("lengths_i64", ctypes.c_int32),
+        ("pages", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+        ("max_pages", ctypes.c_int64),
+        ("stride", ctypes.c_int64 * 2),
+        ("scale", ctypes.c_float),
     ]
 
 
@@ -342,6 +423,22 @@ def load() -> ctypes.CDLL:
             call.argtypes, call.restype = [lg] + [vp] * count + [vp, sz, vp], i32
         lib.oops_linear_attn_step.argtypes = [lg, vp, vp, vp, vp, vp, vp, vp]
         lib.oops_linear_attn_step.restype = i32
+        og, cg = ctypes.POINTER(RotaryGeometry), ctypes.POINTER(CausalGeometry)
+        kg, dg = ctypes.POINTER(CacheGeometry), ctypes.POINTER(CacheAttnGeometry)
+        lib.oops_rms_norm_rotary_forward.argtypes = [og] + [vp] * 9
+        lib.oops_rms_norm_rotary_backward.argtypes = [og] + [vp] * 13 + [sz, vp]
+        lib.oops_causal_attn_forward.argtypes = [cg] + [vp] * 8
+        lib.oops_causal_attn_backward.argtypes = [cg] + [vp] * 12 + [sz, vp]
+        lib.oops_cache_write.argtypes = [kg] + [vp] * 6 + [sz, vp]
+        lib.oops_cache_read.argtypes = [kg] + [vp] * 6
+        lib.oops_cache_attn.argtypes = [dg] + [vp] * 7 + [sz, vp]
+        for call in (lib.oops_rms_norm_rotary_forward, lib.oops_rms_norm_rotary_backward, lib.oops_causal_attn_forward,
+                     lib.oops_causal_attn_backward, lib.oops_cache_write, lib.oops_cache_read, lib.oops_cache_attn):  # fmt: skip
+            call.restype = i32
+        for size, geometry in ((lib.oops_rms_norm_rotary_backward_workspace_bytes, og),
+                               (lib.oops_causal_attn_backward_workspace_bytes, cg),
+                               (lib.oops_cache_write_workspace_bytes, kg), (lib.oops_cache_attn_workspace_bytes, dg)):  # fmt: skip
+            size.argtypes, size.restype = [geometry], sz
         lib.oops_last_error.argtypes = []
         lib.oops_last_error.restype = ctypes.c_char_p
         lib.oops_abi_version.argtypes = []

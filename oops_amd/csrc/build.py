@@ -42,8 +42,13 @@ SOURCES = (
     "rms_norm.hip",
     "int8_linear.hip",
     "linear_attn.hip",
+    "rotary.hip",
+    "causal_attn.hip",
+    "causal_attn_bwd.hip",
+    "cache.hip",
     "capi.cpp",
     "capi_layer.cpp",
+    "capi_decoder.cpp",
 )
 FAST_MATH_SOURCES = ("attn_fwd_fast.hip", "attn_bwd_fast.hip", "attn_bwd_fused.hip")
 ARCH = "gfx950"

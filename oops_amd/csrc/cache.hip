@@ -1,0 +1,599 @@
+// The paged key/value cache in 4 bits: written, read back, and attended to by single tokens.
+//
+// A token of a head is size / 2 bytes of codes and one exponent byte a block of
+// 32 channels, for its key and its value: 144 bytes at 128 channels where
+// bfloat16 takes 512.
+//
+// Writing and reading move each byte once (HBM): a lane takes eight channels,
+// four lanes a block.  The codes are made by comparisons and exact products with
+// powers of two, so they are those of exact arithmetic.
+//
+// Attention: a workgroup takes one key head, up to 16 query heads that share it,
+// and a range of the sequence; each of its waves passes tiles of 32 tokens.  Codes
+// become bfloat16 (exact: a code has two significant bits) with the scaled
+// conversion, one instruction for two values.  S^T = K Q^T by 16 x 16 x 32 MFMAs:
+// a lane loads its token's codes as they lie in memory, and the channels' order is
+// the query's fragments'.  S^T leaves the probabilities as the second product's
+// operand; V^T comes from LDS by transposed reads (each wave has a region of its
+// own, so there is no barrier in the loop).  float16 and float32 queries and
+// probabilities are split into two and three bfloat16 terms, whose products are
+// exact and added in float32: a result has its own type's precision whatever the
+// cache's.  Few sequences are split over their length; a second launch joins the
+// parts by their maxima and sums.
+#include <algorithm>
+
+#include "attn_common.h"
+#include "decoder_kernels.h"
+
+namespace oops {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kScanTokens = 1024;  // up to here later tokens of the same slot are looked for by reading the slots
+
+template <typename F>
+hipError_t by_type(int dtype, F&& f) {
+  if (dtype == OOPS_F32) return f(float{});
+  if (dtype == OOPS_BF16) return f((__bf16)0.f);
+  return f((_Float16)0.f);
+}
+
+struct CacheArgs {
+  uint8_t *codes, *scales;
+  const void *key, *value;
+  void *key_out, *value_out;
+  const void* slots;
+  const int32_t* owner;
+  int64_t stride[2][3];
+  int64_t slots_count, tokens, length;
+  int32_t heads, size, page, slots_i64, whole;
+};
+__device__ __forceinline__ int64_t slot_of(const void* slots, int i64, int64_t t) {
+  return i64 ? static_cast<const int64_t*>(slots)[t] : static_cast<const int32_t*>(slots)[t];
+}
+// One lane's eight channels of a token's key or value.
+struct Place {
+  int64_t token, slot;
+  int which, head, piece;
+};
+__device__ __forceinline__ Place place_of(const CacheArgs& a, int64_t i) {
+  const int pieces = a.size / 8;
+  Place p;
+  p.piece = (int)(i % pieces);
+  i /= pieces;
+  p.head = (int)(i % a.heads);
+  i /= a.heads;
+  p.which = (int)(i & 1);
+  p.token = i >> 1;
+  p.slot = -1;
+  if (p.token < a.tokens) {
+    p.slot = slot_of(a.slots, a.slots_i64, p.token);
+    if (p.slot < 0 || p.slot >= a.slots_count) p.slot = -1;
+  }
+  return p;
+}
+// row of the codes and scales
+__device__ __forceinline__ int64_t cache_row(const CacheArgs& a, const Place& p) {
+  return ((p.slot / a.page * a.heads + p.head) * 2 + p.which) * a.page + p.slot % a.page;
+}
+__device__ __forceinline__ int64_t operand_at(const CacheArgs& a, const Place& p) {
+  const int64_t* s = a.stride[p.which];
+  return p.token / a.length * s[0] + p.head * s[1] + p.token % a.length * s[2] + p.piece * 8;
+}
+
+// ---- of tokens with the same slot the last is kept (long calls: owners are settled first)
+__global__ __launch_bounds__(kThreads) void slot_clear_kernel(const void* slots, int i64, int64_t tokens, int64_t count, int32_t* owner) {
+  const int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (t >= tokens) return;
+  const int64_t s = slot_of(slots, i64, t);
+  if (s >= 0 && s < count) owner[s] = -1;
+}
+__global__ __launch_bounds__(kThreads) void slot_owner_kernel(const void* slots, int i64, int64_t tokens, int64_t count, int32_t* owner) {
+  const int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (t >= tokens) return;
+  const int64_t s = slot_of(slots, i64, t);
+  // (the largest token: any order of the additions gives it)
+  if (s >= 0 && s < count) atomicMax(&owner[s], (int32_t)t);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void cache_write_kernel(CacheArgs a) {
+  const Place p = place_of(a, (int64_t)blockIdx.x * kThreads + threadIdx.x);
+  bool write = p.slot >= 0;
+  if (a.owner) {
+    write = write && a.owner[p.slot] == (int32_t)p.token;
+  } else {
+    // the wave's tokens one after the other, the later slots 64 at a time
+    const int lane = threadIdx.x & 63;
+    const int first = __builtin_amdgcn_readlane((int)p.token, 0), last = __builtin_amdgcn_readlane((int)p.token, 63);
+    for (int t = first; t <= last && t < a.tokens; ++t) {
+      const int64_t mine = slot_of(a.slots, a.slots_i64, t);
+      bool again = false;
+      for (int64_t u = t + 1 + lane; u < a.tokens; u += 64) again |= slot_of(a.slots, a.slots_i64, u) == mine;
+      if (__any(again) && p.token == t) write = false;
+    }
+  }
+  float v[8] = {};
+  if (write) {
+    const T* x = static_cast<const T*>(p.which ? a.value : a.key) + operand_at(a, p);
+    if (a.whole) {
+      uint4 u[sizeof(T) / 2];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(x)[i];
+      const T* e = reinterpret_cast<const T*>(u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)e[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+    }
+  }
+  // the block's largest magnitude as a bit pattern (a NaN's is above infinity's); its lanes are four neighbours
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = std::max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
+  top = std::max(top, (uint32_t)__shfl_xor((int)top, 1));
+  top = std::max(top, (uint32_t)__shfl_xor((int)top, 2));
+  if (!write) return;
+  // top = 1.f * 2^(exp - 127) <= 6 * 2^e = 1.5 * 2^(e + 2)
+  const int exp = (int)(top >> 23);
+  const bool lost = exp == 255;
+  int e = exp - ((top & 0x7FFFFFu) > 0x400000u ? 1 : 2);
+  e = lost ? 255 : e < 1 ? 1 : e > 252 ? 252 : e;
+  const float inv = __builtin_bit_cast(float, (uint32_t)(254 - e) << 23);  // 2^(127 - e)
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // 2^k units below 2, 2 .. 4 and 4 .. 6: the code is their count from zero
+    const float q = fminf(fabsf(v[i]) * inv, 6.0f);
+    const float c = q < 2.f ? __builtin_rintf(q * 2.f) : q < 4.f ? __builtin_rintf(q) + 2.f : __builtin_rintf(q * 0.5f) + 4.f;
+    const uint32_t sign = __builtin_bit_cast(uint32_t, v[i]) >> 31 << 3;
+    word |= ((uint32_t)c | sign) << (4 * i);
+  }
+  if (lost) word = 0;
+  const int64_t row = cache_row(a, p);
+  *reinterpret_cast<uint32_t*>(a.codes + row * (a.size / 2) + p.piece * 4) = word;
+  if (p.piece % 4 == 0) a.scales[row * (a.size / 32) + p.piece / 4] = (uint8_t)e;
+}
+
+__device__ __forceinline__ float scale_value(uint32_t e) {
+  return __builtin_bit_cast(float, e == 255 ? 0x7FC00000u : e == 0 ? 0x00400000u : e << 23);
+}
+__device__ __forceinline__ float code_value(uint32_t c, float scale) {
+  const uint32_t m = c & 7;
+  const float v = m < 2 ? 0.5f * (float)m : __builtin_bit_cast(float, (((m >> 1) + 126) << 23) | ((m & 1) << 22));
+  return (c & 8 ? -v : v) * scale;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void cache_read_kernel(CacheArgs a) {
+  const Place p = place_of(a, (int64_t)blockIdx.x * kThreads + threadIdx.x);
+  if (p.token >= a.tokens) return;
+  uint32_t word = 0, e = 1;
+  if (p.slot >= 0) {
+    const int64_t row = cache_row(a, p);
+    word = *reinterpret_cast<const uint32_t*>(a.codes + row * (a.size / 2) + p.piece * 4);
+    e = a.scales[row * (a.size / 32) + p.piece / 4];
+  }
+  const float scale = scale_value(e);
+  union {
+    uint4 u[sizeof(T) / 2];
+    T y[8];
+  } r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.y[i] = (T)code_value(word >> (4 * i) & 15, scale);
+  // (results are allocated in whole pieces)
+  uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.which ? a.value_out : a.key_out) + operand_at(a, p));
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) to[i] = r.u[i];
+}
+
+// ------------------------------------------------------------------ attention
+
+constexpr int kTile = 32;      // tokens of a wave's step
+constexpr int kHeadTile = 16;  // query heads of a workgroup
+
+struct DecodeArgs {
+  const void *query, *lengths;
+  const uint8_t *codes, *scales;
+  const int32_t* table;
+  void* out;
+  float* parts;  // (batch, heads, splits, size + 2): O, maximum, sum (-1: no token)
+  int64_t pages, batch, max_pages, q_batch, q_head;
+  int32_t heads, kv_heads, group, tiles, page, lengths_i64, splits;
+  float scale;
+};
+
+template <typename T> struct Terms { static constexpr int N = 2; };
+template <> struct Terms<__bf16> { static constexpr int N = 1; };
+template <> struct Terms<float> { static constexpr int N = 3; };
+
+// x as bfloat16 terms, whose sum is x for the types above (an infinity or a NaN is the first term's alone)
+template <int N>
+__device__ __forceinline__ void split(float x, __bf16 (&t)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    t[i] = (__bf16)x;
+    x -= (float)t[i];
+    if (!__builtin_isfinite(x)) x = 0.f;
+  }
+}
+
+typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+// a wave's tile as loaded: token lane % 16 of each half, 8 NS channels a lane
+template <int NS>
+struct Raw {
+  uint32_t k[2][NS], v[2][NS];
+  uint32_t ks[2][NS == 4 ? 1 : NS], vs[2][NS == 4 ? 1 : NS];
+};
+
+// eight codes to bfloat16, times the scale
+__device__ __forceinline__ bf16x8 values8(uint32_t word, float scale) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ float max_rows(float x) {  // over the four 16-lane rows, in every lane
+  const int i = __builtin_bit_cast(int, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+  const int y = __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1])));
+  const auto s = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return fmaxf(__builtin_bit_cast(float, (int)s[0]), __builtin_bit_cast(float, (int)s[1]));
+}
+__device__ __forceinline__ float sum_rows(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+template <typename T, int NS>
+__global__ __launch_bounds__(kThreads) void cache_attn_kernel(DecodeArgs a) {
+  constexpr int N = Terms<T>::N, D = 32 * NS, ND = D / 16;
+  // channels of step s of lane group g: with four steps a lane's sixteen bytes lie together
+  auto channel = [](int s, int g) { return NS == 4 ? 32 * g + 8 * s : 32 * s + 8 * g; };
+  constexpr int kPitch = 2 * D + 32;  // bytes: 8 rows' pieces of 32 bytes lie in different banks
+  constexpr int kRegion = std::max(kTile * kPitch, kHeadTile * (D + 2) * 4);
+  __shared__ __attribute__((aligned(16))) char lds[4][kRegion];
+
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  const int split_at = blockIdx.x % a.splits, job = blockIdx.x / a.splits;
+  const int tile_at = job % a.tiles, hk = job / a.tiles % a.kv_heads, b = job / a.tiles / a.kv_heads;
+  const int h = hk * a.group + tile_at * kHeadTile + c;  // this lane's query head
+  const bool head_live = tile_at * kHeadTile + c < a.group;
+
+  int64_t count = a.lengths_i64 ? static_cast<const int64_t*>(a.lengths)[b] : static_cast<const int32_t*>(a.lengths)[b];
+  count = std::min<int64_t>(std::max<int64_t>(count, 0), a.max_pages * a.page);
+  const int steps = (int)((count + kTile - 1) / kTile), per = (steps + a.splits - 1) / a.splits;
+  const int from = split_at * per, to = std::min(steps, from + per);
+
+  bf16x8 q[NS][N];
+  {
+    const T* x = static_cast<const T*>(a.query) + b * a.q_batch + h * a.q_head;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __bf16 t[N];
+        split<N>(head_live ? (float)x[channel(s, g) + i] : 0.f, t);
+#pragma unroll
+        for (int n = 0; n < N; ++n) q[s][n][i] = t[n];
+      }
+  }
+
+  // page of the 16 tokens from t0, or -1
+  auto page_at = [&](int t0) -> int64_t {
+    if (t0 >= count) return -1;
+    const int64_t id = a.table[b * a.max_pages + t0 / a.page];
+    return id >= 0 && id < a.pages ? id : -1;
+  };
+  auto load = [&](int step, Raw<NS>& r) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t0 = step * kTile + 16 * i;
+      const int64_t id = page_at(t0);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) r.k[i][s] = r.v[i][s] = 0;
+#pragma unroll
+      for (int s = 0; s < (NS == 4 ? 1 : NS); ++s) r.ks[i][s] = r.vs[i][s] = 127;
+      if (id < 0) continue;
+      // (places behind the last token lie in the page: what they hold is taken out below)
+      const int64_t row = ((id * a.kv_heads + hk) * 2) * a.page + t0 % a.page + c;
+      const uint8_t* kc = a.codes + row * (D / 2);
+      const uint8_t* vc = kc + (int64_t)a.page * (D / 2);
+      const uint8_t* ks = a.scales + row * NS;
+      const uint8_t* vs = ks + (int64_t)a.page * NS;
+      if constexpr (NS == 4) {
+        const u32x4v k = *reinterpret_cast<const u32x4v*>(kc + 16 * g), v = *reinterpret_cast<const u32x4v*>(vc + 16 * g);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) r.k[i][s] = k[s], r.v[i][s] = v[s];
+        r.ks[i][0] = ks[g];
+        r.vs[i][0] = vs[g];
+      } else {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          r.k[i][s] = *reinterpret_cast<const uint32_t*>(kc + 16 * s + 4 * g);
+          r.v[i][s] = *reinterpret_cast<const uint32_t*>(vc + 16 * s + 4 * g);
+          r.ks[i][s] = ks[s];
+          r.vs[i][s] = vs[s];
+        }
+      }
+    }
+  };
+
+  float m_run = kNegInf, neg_m = 0.f, l_run = 0.f;
+  bool seen = false;
+  f32x4 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) o[d] = f32x4{};
+  const float c1 = a.scale * kLog2e;
+  char* mine = lds[wave];
+
+  Raw<NS> raw;
+  if (from + wave < to) load(from + wave, raw);
+  for (int step = from + wave; step < to; step += 4) {
+    Raw<NS> now = raw;
+    if (step + 4 < to) load(step + 4, raw);
+    const bool have[2] = {page_at(step * kTile) >= 0, page_at(step * kTile + 16) >= 0};
+    if (!have[0] && !have[1]) continue;
+    seen = true;
+    const int left = (int)std::min<int64_t>(count - step * kTile, kTile);
+    // tokens of this lane that take part: key and value rows c + 16 i
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool live = have[i] && c + 16 * i < left;
+      if (!live) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) now.v[i][s] = 0;
+#pragma unroll
+        for (int s = 0; s < (NS == 4 ? 1 : NS); ++s) now.vs[i][s] = 127;
+      }
+    }
+    // V to LDS in bfloat16
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        *reinterpret_cast<bf16x8*>(mine + (c + 16 * i) * kPitch + channel(s, g) * 2) =
+            values8(now.v[i][s], scale_value(now.vs[i][NS == 4 ? 0 : s]));
+    // S^T: rows (registers) tokens 16 i + 4 g + r, columns (lanes) query heads
+    f32x4 st[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      st[i] = f32x4{};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const bf16x8 k = values8(now.k[i][s], scale_value(now.ks[i][NS == 4 ? 0 : s]));
+#pragma unroll
+        for (int n = 0; n < N; ++n) st[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[s][n], st[i], 0, 0, 0);
+      }
+    }
+    if (left < kTile || !have[0] || !have[1]) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[i][r] = have[i] && 16 * i + 4 * g + r < left ? st[i][r] * c1 : kNegInf;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) st[i] *= c1;
+    }
+    float mx = kNegInf;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[i][r]);
+    mx = max_rows(mx);
+    const bool grow = mx > m_run + 8.0f;  // (a difference of 2^8 is nothing to float32 sums)
+    if (__any(grow)) {
+      const float m_new = grow ? mx : m_run;
+      const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      m_run = m_new;
+      neg_m = m_run == kNegInf ? 0.f : -m_run;
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= alpha;
+    }
+    bf16x8 p[N];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = __builtin_amdgcn_exp2f(st[i][r] + neg_m);
+        l_run += x;
+        __bf16 t[N];
+        split<N>(x, t);
+#pragma unroll
+        for (int n = 0; n < N; ++n) p[n][4 * i + r] = t[n];
+      }
+    // O^T += V^T P^T; lane (c, g) gets V[4 g + k][16 d + c] for k = 0..3, then rows + 16
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const char* at = mine + (4 * g + (c >> 2)) * kPitch + (16 * d + 4 * (c & 3)) * 2;
+      const s16x4 lo = lds_read_tr4(at), hi = lds_read_tr4(at + 16 * kPitch);
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      const bf16x8 v = __builtin_bit_cast(bf16x8, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+#pragma unroll
+      for (int n = 0; n < N; ++n) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n], o[d], 0, 0, 0);
+    }
+    asm volatile("" ::: "memory");
+  }
+
+  // the waves' parts: maximum and sum of each query head, then O, joined in order
+  l_run = sum_rows(l_run);
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(mine);
+  if (g == 0) part[c] = m_run, part[16 + c] = seen ? l_run : -1.f;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) part[32 + c * D + 16 * d + 4 * g + r] = o[d][r];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kHeadTile * D; i += kThreads) {
+    const int col = i / D, d = i % D;
+    if (tile_at * kHeadTile + col >= a.group) continue;
+    float m = kNegInf, l = 0.f, x = 0.f;
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float* f = reinterpret_cast<const float*>(lds[w]);
+      if (f[16 + col] != -1.f) m = fmaxf(m, f[col]), any = true;
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float* f = reinterpret_cast<const float*>(lds[w]);
+      if (f[16 + col] == -1.f) continue;
+      const float by = f[col] == m && m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(f[col] - m);
+      l = __builtin_fmaf(f[16 + col], by, l);
+      x = __builtin_fmaf(f[32 + col * D + d], by, x);
+    }
+    const int64_t row = (int64_t)b * a.heads + hk * a.group + tile_at * kHeadTile + col;
+    if (a.splits == 1) {
+      // (no token: zeros; every logit -inf: 0 / 0)
+      static_cast<T*>(a.out)[row * D + d] = (T)(any ? x / l : 0.f);
+    } else {
+      float* to_part = a.parts + (row * a.splits + split_at) * (D + 2);
+      to_part[d] = x;
+      if (d == 0) to_part[D] = m, to_part[D + 1] = any ? l : -1.f;
+    }
+  }
+}
+
+// The splits of one row, joined in order.
+template <typename T>
+__global__ __launch_bounds__(128) void cache_join_kernel(const float* parts, void* out, int splits, int size) {
+  const int64_t row = blockIdx.x;
+  const float* p = parts + row * splits * (size + 2);
+  const int d = threadIdx.x;
+  float m = kNegInf, l = 0.f, x = 0.f;
+  bool any = false;
+  for (int s = 0; s < splits; ++s)
+    if (p[s * (size + 2) + size + 1] != -1.f) m = fmaxf(m, p[s * (size + 2) + size]), any = true;
+  if (d >= size) return;
+  for (int s = 0; s < splits; ++s) {
+    const float* f = p + s * (size + 2);
+    if (f[size + 1] == -1.f) continue;
+    const float by = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(f[size] - m);
+    l = __builtin_fmaf(f[size + 1], by, l);
+    x = __builtin_fmaf(f[d], by, x);
+  }
+  static_cast<T*>(out)[row * size + d] = (T)(any ? x / l : 0.f);
+}
+
+// Parts of the length: workgroups for eight on every CU, so that sequences of different lengths even out, but no part
+// shorter than one step of each wave.
+int decode_splits(const oops_cache_attn_geometry& g) {
+  const int64_t group = g.heads / g.kv_heads;
+  const int64_t jobs = g.batch * g.kv_heads * ((group + kHeadTile - 1) / kHeadTile);
+  if (jobs == 0) return 1;
+  const int64_t most = (g.max_pages * g.page + 4 * kTile - 1) / (4 * kTile);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + jobs - 1) / jobs, most, 256}));
+}
+
+}  // namespace
+
+size_t cache_write_workspace_bytes(const oops_cache_geometry& g) {
+  return g.batch * g.length > kScanTokens ? (size_t)(g.pages * g.page) * sizeof(int32_t) : 0;
+}
+
+namespace {
+CacheArgs cache_args(const oops_cache_geometry& g, const void* codes, const void* scales, const void* slots) {
+  CacheArgs a{};
+  a.codes = static_cast<uint8_t*>(const_cast<void*>(codes));
+  a.scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+  a.slots = slots;
+  for (int i = 0; i < 2; ++i) std::copy(g.stride[i], g.stride[i] + 3, a.stride[i]);
+  a.slots_count = g.pages * g.page;
+  a.tokens = g.batch * g.length;
+  a.length = g.length;
+  a.heads = g.heads;
+  a.size = g.size;
+  a.page = g.page;
+  a.slots_i64 = g.slots_i64;
+  return a;
+}
+unsigned cache_grid(const oops_cache_geometry& g) {
+  return (unsigned)((g.batch * g.length * 2 * g.heads * (g.size / 8) + kThreads - 1) / kThreads);
+}
+}  // namespace
+
+hipError_t launch_cache_write(const oops_cache_geometry& g, void* codes, void* scales, const void* key, const void* value,
+                              const void* slots, void* workspace, hipStream_t stream) {
+  CacheArgs a = cache_args(g, codes, scales, slots);
+  a.key = key;
+  a.value = value;
+  const int n = g.dtype == OOPS_F32 ? 4 : 8;
+  a.whole = reinterpret_cast<uintptr_t>(key) % 16 == 0 && reinterpret_cast<uintptr_t>(value) % 16 == 0;
+  for (int i = 0; i < 2; ++i)
+    for (int d = 0; d < 3; ++d) a.whole = a.whole && g.stride[i][d] % n == 0;
+  if (a.tokens > kScanTokens) {
+    int32_t* owner = static_cast<int32_t*>(workspace);
+    const dim3 grid((unsigned)((a.tokens + kThreads - 1) / kThreads));
+    hipLaunchKernelGGL(slot_clear_kernel, grid, dim3(kThreads), 0, stream, slots, g.slots_i64, a.tokens, a.slots_count, owner);
+    hipLaunchKernelGGL(slot_owner_kernel, grid, dim3(kThreads), 0, stream, slots, g.slots_i64, a.tokens, a.slots_count, owner);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    a.owner = owner;
+  }
+  return by_type(g.dtype, [&](auto tag) {
+    hipLaunchKernelGGL((cache_write_kernel<decltype(tag)>), dim3(cache_grid(g)), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+  });
+}
+
+hipError_t launch_cache_read(const oops_cache_geometry& g, const void* codes, const void* scales, const void* slots,
+                             void* key, void* value, hipStream_t stream) {
+  CacheArgs a = cache_args(g, codes, scales, slots);
+  a.key_out = key;
+  a.value_out = value;
+  return by_type(g.dtype, [&](auto tag) {
+    hipLaunchKernelGGL((cache_read_kernel<decltype(tag)>), dim3(cache_grid(g)), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+  });
+}
+
+size_t cache_attn_workspace_bytes(const oops_cache_attn_geometry& g) {
+  const int splits = decode_splits(g);
+  return splits > 1 ? (size_t)(g.batch * g.heads) * splits * (g.size + 2) * sizeof(float) : 0;
+}
+
+hipError_t launch_cache_attn(const oops_cache_attn_geometry& g, const void* query, const void* codes, const void* scales,
+                             const int32_t* pages, const void* lengths, void* out, void* workspace, hipStream_t stream) {
+  DecodeArgs a{};
+  a.query = query;
+  a.lengths = lengths;
+  a.codes = static_cast<const uint8_t*>(codes);
+  a.scales = static_cast<const uint8_t*>(scales);
+  a.table = pages;
+  a.out = out;
+  a.parts = static_cast<float*>(workspace);
+  a.pages = g.pages;
+  a.batch = g.batch;
+  a.max_pages = g.max_pages;
+  a.q_batch = g.stride[0];
+  a.q_head = g.stride[1];
+  a.heads = g.heads;
+  a.kv_heads = g.kv_heads;
+  a.group = g.heads / g.kv_heads;
+  a.tiles = (a.group + kHeadTile - 1) / kHeadTile;
+  a.page = g.page;
+  a.lengths_i64 = g.lengths_i64;
+  a.splits = decode_splits(g);
+  a.scale = g.scale;
+  const dim3 grid((unsigned)(g.batch * g.kv_heads * a.tiles * a.splits));
+  return by_type(g.dtype, [&](auto tag) {
+    using T = decltype(tag);
+    if (g.size == 32) hipLaunchKernelGGL((cache_attn_kernel<T, 1>), grid, dim3(kThreads), 0, stream, a);
+    else if (g.size == 64) hipLaunchKernelGGL((cache_attn_kernel<T, 2>), grid, dim3(kThreads), 0, stream, a);
+    else if (g.size == 96) hipLaunchKernelGGL((cache_attn_kernel<T, 3>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((cache_attn_kernel<T, 4>), grid, dim3(kThreads), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.splits == 1) return e;
+    hipLaunchKernelGGL((cache_join_kernel<T>), dim3((unsigned)(g.batch * g.heads)), dim3(128), 0, stream, a.parts, out, a.splits,
+                       g.size);
+    return hipGetLastError();
+  });
+}
+
+}  // namespace oops

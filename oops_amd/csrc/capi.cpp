@@ -455,7 +455,7 @@ int run_forward(const oops_attn_geometry* geo, const oops::Plan& plan, const voi
 
 extern "C" {
 
-int oops_abi_version(void) { return 8; }
+int oops_abi_version(void) { return 9; }
 
 const char* oops_last_error(void) { return g_last_error.c_str(); }
 

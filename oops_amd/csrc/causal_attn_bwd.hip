@@ -1,0 +1,346 @@
+// Causal attention over whole prompts, backward.
+//
+// With P_ij = exp(scale q_i.k_j - LSE_i) and delta_i = sum_d O_id dO_id:
+//   dS_ij = P_ij (dO_i.v_j - delta_i)
+//   dQ_i = scale sum_j dS_ij k_j,  dK_j = scale sum_i dS_ij q_i,  dV_j = sum_i P_ij dO_i
+// the sums of dK and dV also over the query heads that share key head j.
+//
+// Two kernels, both without atomics, so results do not depend on the order of
+// workgroups.  The first is laid out like the forward (128 queries a workgroup,
+// dQ^T in registers, K and V in LDS) and writes delta; the second holds 128 keys,
+// 32 a wave, with dK^T and dV^T in registers, while queries and dO pass through
+// LDS, over the query heads of its group in turn.  P and dS are made twice: seven
+// products where five are needed, against partial gradients in memory or atomics.
+// Where key blocks and heads are too few to fill the chip, the query heads of a
+// group are split and the parts' float32 gradients added in order by a third
+// kernel.
+#include <algorithm>
+
+#include "causal_common.h"
+
+namespace oops {
+namespace causal {
+namespace {
+
+constexpr int kBlock = 128;  // queries, or keys, of a workgroup
+template <typename T, int DP>
+constexpr int kOcc = sizeof(T) == 4 && DP == 128 ? 1 : 2;
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(CausalArgs a, uint32_t blocks) {
+  using TL = Tile<T, DP>;
+  using A = Att<T>;
+  constexpr int KT = TL::kRows, NS = DP / 16, NDT = DP / 32, SUB = KT / 32;
+  __shared__ __attribute__((aligned(1024))) char k_lds[2][TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds[2][TL::kBytes];
+
+  const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.heads), blocks);
+  const int b = w.head / a.heads, h = w.head % a.heads;
+  const int block = (int)blocks - 1 - w.block;
+  const int length = (int)a.length;
+
+  const int q0 = block * kBlock + wave * 32, row = q0 + lq;
+  const bool valid = row < length;
+  const Span span = span_of(a, valid ? row : length - 1);
+  const int start = span.start;
+  const bool empty = !valid || start > row;
+  const uint32_t reach = empty ? 0u : (uint32_t)(row - start);
+  const int last = q0 + 31 < length ? q0 + 31 : length - 1;
+  const bool idle = q0 >= length;
+  const int first_start = __builtin_amdgcn_readlane(start, 0), last_start = __builtin_amdgcn_readlane(start, idle ? 0 : last - q0);
+
+  const Rows qr = rows_of<T>(a.q, a.q_stride, b, h, a.key_size, length);
+  const Rows kr = rows_of<T>(a.k, a.k_stride, b, h / a.group, a.key_size, length);
+  const Rows vr = rows_of<T>(a.v, a.v_stride, b, h / a.group, a.value_size, length);
+  const Rows dor = rows_of<T>(a.dout, a.do_stride, b, h, a.value_size, length);
+  const Rows outr = rows_of<T>(a.out, a.o_stride, b, h, a.value_size, length);
+
+  Frag<T> dof[NS];
+  load_row<T, DP>(dof, dor, row, valid, g);
+  float delta = 0.f;
+  {
+    Frag<T> of[NS];
+    load_row<T, DP>(of, outr, row, valid, g);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)of[s][i], (float)dof[s][i], delta);
+    if (a.low) {
+      const Rows lowr = rows_of<T>(a.low, a.o_stride, b, h, a.value_size, length);
+      load_row<T, DP>(of, lowr, row, valid, g);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)of[s][i], (float)dof[s][i], delta);
+    }
+    delta = fast::sum_halves(delta);
+  }
+  const int64_t stat = ((int64_t)b * a.heads + h) * length + row;
+  if (valid && g == 0) a.delta[stat] = delta;
+  if (!a.dq) return;
+  const float neg_lse = valid ? -a.lse[stat] : 0.f;
+  Frag<T> qf[NS];
+  load_row<T, DP>(qf, qr, row, valid, g, a.flip);
+
+  Loader<T, DP> kl, vl;
+  kl.init(kr, wave, lane);
+  vl.init(vr, wave, lane);
+  const int block_start = span_of(a, block * kBlock).start;
+  const int block_last = std::min(block * kBlock + kBlock, length) - 1;
+  const int t0 = std::min(block_start, block * kBlock) / KT, t1 = block_last / KT;
+
+  f32x16 dq[NDT];
+#pragma unroll
+  for (int t = 0; t < NDT; ++t) dq[t] = f32x16{};
+  const float c1 = a.scale * kLog2e;
+
+  fast::vmem_wait<0>();  // (the rows, before loads that the compiler does not count)
+  kl.load(kr, (int64_t)t0 * KT, k_lds[0]);
+  vl.load(vr, (int64_t)t0 * KT, v_lds[0]);
+  for (int t = t0; t <= t1; ++t) {
+    const int buf = (t - t0) & 1, k0 = t * KT;
+    fast::vmem_wait<0>();
+    lds_barrier();
+    if (t < t1) {
+      kl.load(kr, (int64_t)(t + 1) * KT, k_lds[buf ^ 1]);
+      vl.load(vr, (int64_t)(t + 1) * KT, v_lds[buf ^ 1]);
+    }
+    if (idle || k0 > last || k0 + KT <= first_start) continue;
+    const bool whole = k0 >= last_start && k0 + KT - 1 <= q0;
+    const char* kt = k_lds[buf];
+    const char* vt = v_lds[buf];
+    auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int i = 0; i < NS; ++i) s = A::mma(TL::row(kt, 32 * u + lq, i, g), qf[i], s);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) dp = A::mma(TL::row(vt, 32 * u + lq, i, g), dof[i], dp);
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, neg_lse)) * (dp[j] - delta);
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = keep(32 * u + kappa(g, j)) ? s[j] : 0.f;
+      }
+      Frag<T> ds[2] = {pack<T>(s, 0), pack<T>(s, 1)};
+      if (whole) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int d = 0; d < NDT; ++d) dq[d] = A::mma(TL::transposed(kt, 32 * u + 16 * m, 32 * d, lane), ds[m], dq[d]);
+      } else {
+        masked_product<T, DP, false>(dq, kt, 32 * u, ds, lane, keep);
+      }
+    }
+  }
+  if (!valid) return;
+  const float scale = a.flip ? -a.scale : a.scale;
+  char* to = static_cast<char*>(a.dq) + (b * a.dq_stride[0] + h * a.dq_stride[1] + row * a.dq_stride[2]) * (int64_t)sizeof(T);
+#pragma unroll
+  for (int d = 0; d < NDT; ++d) store_columns<T>(to, 32 * d, a.key_size, g, dq[d], scale);
+}
+
+// 4 bytes a lane from a buffer to 64 consecutive words at lds; an offset out of range writes zeros
+__device__ __forceinline__ void dma4_asm(const fast::u32x4& r, const void* lds, uint32_t voff) {
+  const uint32_t m0 =
+      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)(lds));
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %1, %2, 0 offen lds" ::"s"(m0),
+      "v"(voff), "s"(r)
+      : "memory", "m0");
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kernel(CausalArgs a, uint32_t blocks) {
+  using TL = Tile<T, DP>;
+  using A = Att<T>;
+  constexpr int QT = TL::kRows, NS = DP / 16, NDT = DP / 32, SUB = QT / 32;
+  __shared__ __attribute__((aligned(1024))) char q_lds[2][TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) char do_lds[2][TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) float lse_lds[2][64], delta_lds[2][64];
+
+  const int tid = threadIdx.x, lane = tid & 63, lk = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.kv_heads * a.parts), blocks);
+  const int part = w.head % a.parts, hk = w.head / a.parts % a.kv_heads, b = w.head / a.parts / a.kv_heads;
+  const int block = w.block;
+  const int length = (int)a.length;
+
+  const int k0 = block * kBlock + wave * 32, key = k0 + lk;
+  const bool valid = key < length;
+  const Span span = span_of(a, valid ? key : length - 1);
+  // queries this lane's key is paired with: [key, key + width)
+  const uint32_t width = valid && span.end > key ? (uint32_t)(span.end - key) : 0u;
+  const int last = k0 + 31 < length ? k0 + 31 : length - 1;
+  const bool idle = k0 >= length;
+  const int first_end = __builtin_amdgcn_readlane(span.end, 0);
+  const int last_end = __builtin_amdgcn_readlane(span.end, idle ? 0 : last - k0);
+
+  Frag<T> kf[NS], vf[NS];
+  load_row<T, DP>(kf, rows_of<T>(a.k, a.k_stride, b, hk, a.key_size, length), key, valid, g, a.flip);
+  load_row<T, DP>(vf, rows_of<T>(a.v, a.v_stride, b, hk, a.value_size, length), key, valid, g);
+
+  const int block_last = std::min(block * kBlock + kBlock, length) - 1;
+  const int block_end = std::max(span_of(a, block_last).end, block_last + 1);
+  const int t0 = block * kBlock / QT, tiles = (block_end - 1) / QT - t0 + 1;
+  const int h0 = hk * a.group + part * a.group / a.parts, h1 = hk * a.group + (part + 1) * a.group / a.parts;
+  const int steps = (h1 - h0) * tiles;
+
+  f32x16 dk[NDT], dv[NDT];
+#pragma unroll
+  for (int t = 0; t < NDT; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
+  const float c1 = a.scale * kLog2e;
+
+  Loader<T, DP> ql, dl;
+  ql.init(rows_of<T>(a.q, a.q_stride, b, h0, a.key_size, length), wave, lane);
+  dl.init(rows_of<T>(a.dout, a.do_stride, b, h0, a.value_size, length), wave, lane);
+  auto load = [&](int step, int buf) {
+    const int h = h0 + step / tiles;
+    const int64_t row0 = (int64_t)(t0 + step % tiles) * QT;
+    ql.load(rows_of<T>(a.q, a.q_stride, b, h, a.key_size, length), row0, q_lds[buf]);
+    dl.load(rows_of<T>(a.dout, a.do_stride, b, h, a.value_size, length), row0, do_lds[buf]);
+    if (wave < 2) {
+      const int64_t left = length - row0;
+      const int n = left < QT ? (int)left : QT;
+      const float* p = (wave == 0 ? a.lse : a.delta) + ((int64_t)b * a.heads + h) * length + row0;
+      dma4_asm(fast::rsrc_words(p, (uint32_t)n * 4), wave == 0 ? lse_lds[buf] : delta_lds[buf], (uint32_t)lane * 4);
+    }
+  };
+
+  fast::vmem_wait<0>();  // (the rows, before loads that the compiler does not count)
+  load(0, 0);
+  for (int step = 0; step < steps; ++step) {
+    const int buf = step & 1, q0 = (t0 + step % tiles) * QT;
+    fast::vmem_wait<0>();
+    lds_barrier();
+    if (step + 1 < steps) load(step + 1, buf ^ 1);
+    if (idle || q0 + QT <= k0 || q0 >= last_end) continue;
+    const bool whole = q0 >= k0 + 31 && q0 + QT <= first_end;
+    const char* qt = q_lds[buf];
+    const char* dot = do_lds[buf];
+    auto keep = [&](int r) { return (uint32_t)(q0 + r - key) < width; };
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int i = 0; i < NS; ++i) s = A::mma(TL::row(qt, 32 * u + lk, i, g), kf[i], s);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) dp = A::mma(TL::row(dot, 32 * u + lk, i, g), vf[i], dp);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        // rows kappa(g, 4 q ..) are consecutive
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&lse_lds[buf][32 * u + 8 * q + 4 * g]);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_lds[buf][32 * u + 8 * q + 4 * g]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * q + i;
+          s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, -lse[i]));
+          dp[j] = s[j] * (dp[j] - delta[i]);
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const bool pair = keep(32 * u + kappa(g, j));
+          s[j] = pair ? s[j] : 0.f;
+          dp[j] = pair ? dp[j] : 0.f;
+        }
+      }
+      const Frag<T> p[2] = {pack<T>(s, 0), pack<T>(s, 1)}, ds[2] = {pack<T>(dp, 0), pack<T>(dp, 1)};
+      if (whole) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int d = 0; d < NDT; ++d) {
+            dv[d] = A::mma(TL::transposed(dot, 32 * u + 16 * m, 32 * d, lane), p[m], dv[d]);
+            dk[d] = A::mma(TL::transposed(qt, 32 * u + 16 * m, 32 * d, lane), ds[m], dk[d]);
+          }
+      } else {
+        masked_product<T, DP, true>(dv, dot, 32 * u, p, lane, keep);
+        masked_product<T, DP, false>(dk, qt, 32 * u, ds, lane, keep);
+      }
+    }
+  }
+  if (!valid) return;
+  const float scale = a.flip ? -a.scale : a.scale;
+  if (a.parts > 1) {
+    const int64_t at = (((int64_t)part * a.batch + b) * a.kv_heads + hk) * length + key;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) {
+      if (a.dk) store_columns<float>(reinterpret_cast<char*>(a.dk_parts + at * a.key_size), 32 * d, a.key_size, g, dk[d], scale);
+      if (a.dv) store_columns<float>(reinterpret_cast<char*>(a.dv_parts + at * a.value_size), 32 * d, a.value_size, g, dv[d], 1.f);
+    }
+    return;
+  }
+  char* to_k = static_cast<char*>(a.dk) + (b * a.dk_stride[0] + hk * a.dk_stride[1] + key * a.dk_stride[2]) * (int64_t)sizeof(T);
+  char* to_v = static_cast<char*>(a.dv) + (b * a.dv_stride[0] + hk * a.dv_stride[1] + key * a.dv_stride[2]) * (int64_t)sizeof(T);
+#pragma unroll
+  for (int d = 0; d < NDT; ++d) {
+    if (a.dk) store_columns<T>(to_k, 32 * d, a.key_size, g, dk[d], scale);
+    if (a.dv) store_columns<T>(to_v, 32 * d, a.value_size, g, dv[d], 1.f);
+  }
+}
+
+// The parts' gradients (part, batch, head, token, size), added in order; four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void causal_parts_kernel(const float* parts, void* out, int64_t s0, int64_t s1, int64_t s2,
+                                                           int64_t heads, int64_t length, int size, int count, int64_t cells) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= cells) return;
+  f32x4 s = *reinterpret_cast<const f32x4*>(parts + i);
+  for (int p = 1; p < count; ++p) s += *reinterpret_cast<const f32x4*>(parts + p * cells + i);
+  const int64_t rows = i / size, t = rows % length, h = rows / length % heads, b = rows / length / heads;
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  v4 y;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) y[k] = (T)s[k];
+  *reinterpret_cast<v4*>(static_cast<T*>(out) + b * s0 + h * s1 + t * s2 + i % size) = y;
+}
+
+}  // namespace
+}  // namespace causal
+
+// Parts of a group's query heads: workgroups for every CU's two places twice over, so that the heavy blocks (the first
+// keys, paired with every query) find light ones to even them out.
+int causal_grad_parts(const oops_causal_geometry& g) {
+  const int64_t blocks = (g.length + causal::kBlock - 1) / causal::kBlock * g.batch * g.kv_heads;
+  const int64_t want = blocks > 0 ? (1024 + blocks - 1) / blocks : 1;
+  return (int)std::min<int64_t>(want, g.heads / g.kv_heads);
+}
+
+hipError_t launch_causal_backward(int dtype, const CausalArgs& a, hipStream_t stream) {
+  if (a.length == 0 || a.batch == 0) return hipSuccess;
+  const uint32_t blocks = (uint32_t)((a.length + causal::kBlock - 1) / causal::kBlock);
+  const bool wide = a.key_size > 64 || a.value_size > 64;
+  const dim3 grid_q(blocks * (uint32_t)(a.batch * a.heads)), grid_kv(blocks * (uint32_t)(a.batch * a.kv_heads * a.parts));
+  auto go = [&](auto tag) {
+    using T = decltype(tag);
+    if (wide) hipLaunchKernelGGL((causal::causal_grad_query_kernel<T, 128>), grid_q, dim3(256), 0, stream, a, blocks);
+    else hipLaunchKernelGGL((causal::causal_grad_query_kernel<T, 64>), grid_q, dim3(256), 0, stream, a, blocks);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || (!a.dk && !a.dv)) return e;
+    if (wide) hipLaunchKernelGGL((causal::causal_grad_key_value_kernel<T, 128>), grid_kv, dim3(256), 0, stream, a, blocks);
+    else hipLaunchKernelGGL((causal::causal_grad_key_value_kernel<T, 64>), grid_kv, dim3(256), 0, stream, a, blocks);
+    e = hipGetLastError();
+    auto add = [&](const float* parts, void* out, const int64_t(&s)[3], int size) {
+      const int64_t cells = a.batch * a.kv_heads * a.length * size;
+      hipLaunchKernelGGL((causal::causal_parts_kernel<T>), dim3((uint32_t)((cells / 4 + 255) / 256)), dim3(256), 0, stream, parts,
+                         out, s[0], s[1], s[2], (int64_t)a.kv_heads, a.length, size, a.parts, cells);
+      return hipGetLastError();
+    };
+    if (e == hipSuccess && a.parts > 1 && a.dk) e = add(a.dk_parts, a.dk, a.dk_stride, a.key_size);
+    if (e == hipSuccess && a.parts > 1 && a.dv) e = add(a.dv_parts, a.dv, a.dv_stride, a.value_size);
+    return e;
+  };
+  if (dtype == OOPS_F32) return go(float{});
+  if (dtype == OOPS_BF16) return go((__bf16)0.f);
+  return go((_Float16)0.f);
+}
+
+}  // namespace oops

@@ -1,0 +1,330 @@
+// Device code shared by the causal attention kernels (forward and backward).
+//
+// Every product is a 32 x 32 x 16 step on fragments of eight elements a lane
+// (16-bit types: one MFMA; float32: eight exact float32 MFMAs).  Lane (c =
+// lane % 32, g = lane / 32) holds elements 16 s + 8 g .. + 7 of row c along
+// the contracted axis.  An accumulator's rows are kappa(g, j), so eight of its
+// registers are the other operand of the next product as they stand, if the
+// tile in LDS is read in the same order (tr_frag).
+//
+// Tiles of KT rows (64 of 16 bits, 32 of float32) go from memory straight to
+// LDS in 16-byte pieces.  Piece c of row r is kept in place c ^ swizzle(r): 16
+// lanes that read the same piece of 16 rows, and the 8 lanes groups of a
+// transposed read (32 bytes of each of 8 rows), meet 16 different bank groups.
+#pragma once
+#include "attn_fast_common.h"
+#include "decoder_kernels.h"
+
+namespace oops {
+namespace causal {
+
+using fast::kOut;
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Att {
+  using Frag = typename Elem<T>::Frag;
+  static constexpr int kRows = 64;  // rows of a tile in LDS
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return Elem<T>::mma(a, b, c); }
+};
+template <> struct Att<float> {
+  using Frag = f32x8;
+  static constexpr int kRows = 32;
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+template <typename T> using Frag = typename Att<T>::Frag;
+
+// ---- tiles in LDS: KT rows of DP elements
+template <typename T, int DP>
+struct Tile {
+  static constexpr int kRows = Att<T>::kRows;
+  static constexpr int kBytes = kRows * DP * (int)sizeof(T);
+  static constexpr int kPieces = DP * (int)sizeof(T) / 16;          // of a row
+  static constexpr int kLoads = kRows * kPieces / 256;              // of a wave, four waves a tile
+  static constexpr int kRowsPerLoad = 64 / kPieces;
+  static constexpr bool k16 = sizeof(T) == 2;
+
+  // (the lower bit of the place changes last: 32-byte pairs of 8 rows lie in 8 different pairs of bank groups;
+  // float32 fragments are such pairs)
+  static __device__ __forceinline__ int swizzle(int r) {
+    if constexpr (!k16) return (kPieces == 16 ? r & 7 : r & 15) << 1;
+    else if constexpr (kPieces == 16) return ((r & 7) << 1) | ((r >> 3) & 1);
+    else return (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+  }
+  static __device__ __forceinline__ int at(int r, int piece) { return r * (DP * (int)sizeof(T)) + ((piece ^ swizzle(r)) << 4); }
+
+  // elements 16 s + 8 g .. + 7 of row r
+  static __device__ __forceinline__ Frag<T> row(const char* tile, int r, int s, int g) {
+    if constexpr (k16) {
+      return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const uint4*>(tile + at(r, 2 * s + g)));
+    } else {
+      const int p = at(r, 4 * s + 2 * g);
+      f32x8 f;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + p), hi = *reinterpret_cast<const f32x4*>(tile + p + 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = lo[i], f[4 + i] = hi[i];
+      return f;
+    }
+  }
+  static __device__ __forceinline__ float element(const char* tile, int r, int c) {
+    constexpr int n = 16 / (int)sizeof(T);
+    return (float)*reinterpret_cast<const T*>(tile + at(r, c / n) + c % n * (int)sizeof(T));
+  }
+  // column c0 + lane % 32 of rows r0 + kappa(g, 0..7) (r0 a multiple of 16, c0 of 32)
+  static __device__ __forceinline__ Frag<T> transposed(const char* tile, int r0, int c0, int lane) {
+    if constexpr (k16) {
+      const int j = lane & 15, grp = lane >> 4;
+      const int r = ((grp >> 1) << 2) + (j >> 2), col = c0 + ((grp & 1) << 4) + ((j & 3) << 2);
+      const char* lo_at = tile + r0 * DP * 2 + at(r, col >> 3) + (col & 7) * 2;
+      const char* hi_at = tile + r0 * DP * 2 + at(r + 8, col >> 3) + (col & 7) * 2;
+      const s16x4 lo = lds_read_tr4(lo_at), hi = lds_read_tr4(hi_at);
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(Frag<T>, v);
+    } else {
+      const int col = c0 + (lane & 31), g = lane >> 5;
+      f32x8 f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        f[j] = *reinterpret_cast<const float*>(tile + r0 * DP * 4 + at(kappa(g, j), col >> 2) + (col & 3) * 4);
+      return f;
+    }
+  }
+};
+
+// Rows of an operand of one (batch, head): 64-bit base, row pitch in bytes, row length in bytes.
+struct Rows {
+  const char* base;
+  int64_t pitch;
+  int32_t bytes;
+  int64_t count;
+};
+template <typename T>
+__device__ __forceinline__ Rows rows_of(const void* p, const int64_t (&stride)[3], int64_t b, int64_t h, int size, int64_t count) {
+  return Rows{static_cast<const char*>(p) + (b * stride[0] + h * stride[1]) * (int64_t)sizeof(T),
+              stride[2] * (int64_t)sizeof(T), size * (int)sizeof(T), count};
+}
+// Rows row0 .. of `r` to the tile at `lds`; rows behind the last and columns behind the size are zeros.  The
+// resource starts at the tile's first row, so that offsets stay small however long the operand is (the host
+// refuses row pitches of 2^24 bytes and more).
+template <typename T, int DP>
+struct Loader {
+  using TL = Tile<T, DP>;
+  uint32_t off[TL::kLoads];
+  int wave;
+  __device__ __forceinline__ void init(const Rows& r, int wave_, int lane) {
+    wave = wave_;
+#pragma unroll
+    for (int i = 0; i < TL::kLoads; ++i) {
+      const int row = (wave * TL::kLoads + i) * TL::kRowsPerLoad + lane / TL::kPieces;
+      const int col = ((lane % TL::kPieces) ^ TL::swizzle(row)) * 16;
+      off[i] = col < r.bytes ? (uint32_t)(row * (int)r.pitch + col) : kOut;
+    }
+  }
+  __device__ __forceinline__ void load(const Rows& r, int64_t row0, const char* lds) const {
+    const int64_t left = r.count - row0;
+    const int n = left < TL::kRows ? (left > 0 ? (int)left : 0) : TL::kRows;
+    const fast::u32x4 rs = fast::rsrc_words(r.base + row0 * r.pitch, n > 0 ? (uint32_t)((n - 1) * (int)r.pitch + r.bytes) : 0u);
+#pragma unroll
+    for (int i = 0; i < TL::kLoads; ++i) fast::dma16_asm(rs, lds + (wave * TL::kLoads + i) * 1024, off[i], 0);
+  }
+};
+
+// A row's fragments from memory (zeros behind the size and for absent rows); `flip` changes the sign.
+template <typename T, int DP>
+__device__ __forceinline__ void load_row(Frag<T> (&f)[DP / 16], const Rows& r, int64_t row, bool valid, int g, bool flip = false) {
+  const char* p = r.base + row * r.pitch;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    constexpr int n = 8 * (int)sizeof(T) / 16;
+    const int col = (16 * s + 8 * g) * (int)sizeof(T);
+    uint4 u[n];
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      u[i] = make_uint4(0, 0, 0, 0);
+      if (valid && col + 16 * i < r.bytes) u[i] = *reinterpret_cast<const uint4*>(p + col + 16 * i);
+      if (flip) {
+        constexpr uint32_t m = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+        u[i].x ^= m, u[i].y ^= m, u[i].z ^= m, u[i].w ^= m;
+      }
+    }
+    __builtin_memcpy(&f[s], u, sizeof(f[s]));
+  }
+}
+
+// ---- packed sequences: bounds offsets[0 .. n] along the tokens
+__device__ __forceinline__ int64_t bound(const CausalArgs& a, int i, int64_t length) {
+  const int64_t v = a.offsets_i64 ? static_cast<const int64_t*>(a.offsets)[i] : static_cast<const int32_t*>(a.offsets)[i];
+  return v < 0 ? 0 : v > length ? length : v;
+}
+// The sequence that holds token i: [start, end); a token of none has start = i + 1 and end = i.
+struct Span {
+  int start, end;
+};
+__device__ __forceinline__ Span span_of(const CausalArgs& a, int i) {
+  const int length = (int)a.length;
+  if (!a.offsets) return Span{0, length};
+  // the first bound above i
+  int lo = 0, hi = a.sequences + 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (bound(a, mid, length) > i) hi = mid;
+    else lo = mid + 1;
+  }
+  if (lo == 0 || lo > a.sequences) return Span{i + 1, i};
+  // (bounds that do not increase: what is read stays inside the operands)
+  const int start = (int)bound(a, lo - 1, length), end = (int)bound(a, lo, length);
+  return Span{start < i ? start : i, end > i ? end : i + 1};
+}
+
+template <typename T>
+__device__ __forceinline__ Frag<T> pack(const f32x16& x, int m) {
+  Frag<T> f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (T)x[8 * m + i];
+  return f;
+}
+
+// ---- products over tiles where some pairs are masked
+//
+// A masked pair's weight is 0, but 0 times an infinity or a NaN in the tile
+// is NaN: such elements are taken out of the product, and what they add to the
+// pairs that are not masked is added afterwards, one by one.  Whether there are
+// any is looked at first, so ordinary tiles pay for one more read of the tile.
+
+// largest magnitudes so far, as bit patterns (two of 16 bits, or one of 32)
+template <typename T>
+__device__ __forceinline__ uint32_t raise_bits(uint32_t top, const Frag<T>& f) {
+  constexpr int n = (int)sizeof(Frag<T>) / 4;
+  uint32_t u[n];
+  __builtin_memcpy(u, &f, sizeof(f));
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                                   __builtin_bit_cast(u16x2, u[i] & 0x7FFF7FFFu)));
+    } else {
+      const uint32_t m = u[i] & 0x7FFFFFFFu;
+      top = m > top ? m : top;
+    }
+  }
+  return top;
+}
+template <typename T> struct Bits;
+template <> struct Bits<float> { static constexpr uint32_t kExp = 0x7F800000u; };
+template <> struct Bits<__bf16> { static constexpr uint32_t kExp = 0x7F80u; };
+template <> struct Bits<_Float16> { static constexpr uint32_t kExp = 0x7C00u; };
+template <typename T>
+__device__ __forceinline__ bool non_finite(uint32_t top) {
+  constexpr uint32_t e = Bits<T>::kExp;
+  return sizeof(T) == 2 ? (top & 0xFFFFu) >= e || (top >> 16) >= e : top >= e;
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> cleaned(const Frag<T>& f) {
+  constexpr int n = (int)sizeof(Frag<T>) / 4;
+  constexpr uint32_t e = Bits<T>::kExp;
+  uint32_t u[n];
+  __builtin_memcpy(u, &f, sizeof(f));
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      if ((u[i] & e) == e) u[i] &= 0xFFFF0000u;
+      if ((u[i] >> 16 & e) == e) u[i] &= 0xFFFFu;
+    } else if ((u[i] & e) == e) {
+      u[i] = 0;
+    }
+  }
+  Frag<T> c;
+  __builtin_memcpy(&c, u, sizeof(c));
+  return c;
+}
+// acc[t] += X^T W for the tile X (kRows x DP): W's fragments w[m] over the rows 16 m .. 16 m + 15, keep(row) says which
+// rows this lane's column is paired with.  SIGNED: the weights are positive, an infinity stays one; else what is not
+// finite makes NaN.
+template <typename T, int DP, bool SIGNED, int M, typename Keep>
+__device__ __forceinline__ void masked_product(f32x16 (&acc)[DP / 32], const char* tile, int r0, const Frag<T> (&w)[M],
+                                               int lane, Keep keep) {
+  using TL = Tile<T, DP>;
+  constexpr int NDT = DP / 32;
+  uint32_t top = 0;
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int t = 0; t < NDT; ++t) top = raise_bits<T>(top, TL::transposed(tile, r0 + 16 * m, 32 * t, lane));
+  if (!__any(non_finite<T>(top))) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int t = 0; t < NDT; ++t) acc[t] = Att<T>::mma(TL::transposed(tile, r0 + 16 * m, 32 * t, lane), w[m], acc[t]);
+    return;
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int t = 0; t < NDT; ++t)
+      acc[t] = Att<T>::mma(cleaned<T>(TL::transposed(tile, r0 + 16 * m, 32 * t, lane)), w[m], acc[t]);
+  const int g = lane >> 5;
+#pragma unroll 1
+  for (int r = 0; r < 16 * M; ++r) {
+    const bool pair = keep(r0 + r);
+#pragma unroll
+    for (int t = 0; t < NDT; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float x = TL::element(tile, r0 + r, 32 * t + kappa(g, j));
+        if (pair && !__builtin_isfinite(x)) acc[t][j] += SIGNED ? x : __builtin_nanf("");
+      }
+  }
+}
+
+// A 32 x 32 accumulator tile (rows: elements d0 ..+31, this lane's column: one row of the result) to row[d0 ..], times
+// s, where below `size`; `low` (16-bit types, optional) takes what the rounding left.
+template <typename T>
+__device__ __forceinline__ void store_columns(char* row, int d0, int size, int g, const f32x16& acc, float s, char* low = nullptr) {
+  if constexpr (sizeof(T) == 2) {
+    f32x16 y;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) y[j] = acc[j] * s;
+    fast::store_tile<T>(reinterpret_cast<T*>(row), d0, size, g, y, 1.0f);
+    if (low) {
+      // (an infinity or a NaN leaves no remainder)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float r = y[j] - (float)(T)y[j];
+        y[j] = __builtin_isfinite(r) ? r : 0.f;
+      }
+      fast::store_tile<T>(reinterpret_cast<T*>(low), d0, size, g, y, 1.0f);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = d0 + 8 * q + 4 * g;
+      f32x4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = acc[4 * q + i] * s;
+      if (d < size) *reinterpret_cast<f32x4*>(row + d * 4) = v;
+    }
+  }
+}
+
+// Workgroup `id` of `blocks` blocks of `heads` (batch, head) pairs: the longest blocks first, and, where the heads can
+// be dealt evenly, those of one XCD (workgroups id % 8) next to each other, so that heads that share keys meet in one
+// L2.
+struct Work {
+  int head, block;  // block counted from the heaviest
+};
+__device__ __forceinline__ Work work_of(uint32_t id, uint32_t heads, uint32_t /*blocks*/) {
+  if (heads % kNumXcds == 0) {
+    const uint32_t per = heads / kNumXcds, x = id % kNumXcds, r = id / kNumXcds;
+    return Work{(int)(x * per + r % per), (int)(r / per)};
+  }
+  return Work{(int)(id % heads), (int)(id / heads)};
+}
+
+}  // namespace causal
+}  // namespace oops

@@ -3,5 +3,6 @@
 from .layer_norm import layer_norm
 from .modules import LayerNorm, RMSNorm
 from .rms_norm import quantize_int8, rms_norm, rms_norm_int8
+from .rotary import rms_norm_rotary, rotary_table
 
-__all__ = ["LayerNorm", "RMSNorm", "layer_norm", "quantize_int8", "rms_norm", "rms_norm_int8"]
+__all__ = ["LayerNorm", "RMSNorm", "layer_norm", "quantize_int8", "rms_norm", "rms_norm_int8", "rms_norm_rotary", "rotary_table"]
