@@ -67,6 +67,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
   const int block_start = span_of(a, block * kBlock).start;
   const int block_last = std::min(block * kBlock + kBlock, length) - 1;
   const int t0 = std::min(block_start, block * kBlock) / KT, t1 = block_last / KT;
+  const int block_last_start = span_of(a, block_last).start;
 
   float m_run = kNegInf, neg_m = 0.f, l_run = 0.f;
   f32x16 o[NDT];
@@ -86,6 +87,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
       kl.load(kr, (int64_t)(t + 1) * KT, k_lds[buf ^ 1]);
       vl.load(vr, (int64_t)(t + 1) * KT, v_lds[buf ^ 1]);
     }
+    auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
+    if (k0 < block_last_start || k0 + KT - 1 > block * kBlock) {
+      // (masked pairs for some wave)
+      if (__syncthreads_or(tile_non_finite<TL, T>(v_lds[buf]))) {
+        add_non_finite<TL, true>(o, v_lds[buf], g, keep);
+        __syncthreads();
+        clean_tile<TL, T>(v_lds[buf]);
+        __syncthreads();
+      }
+    }
     if (idle || k0 > last || k0 + KT <= first_start) continue;
     const bool whole = k0 >= last_start && k0 + KT - 1 <= q0;
     const char* kt = k_lds[buf];
@@ -98,7 +109,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 #pragma unroll
       for (int i = 0; i < NS; ++i) s[u] = A::mma(TL::row(kt, 32 * u + lq, i, g), qf[i], s[u]);
     }
-    auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
     if (!whole) {
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
@@ -125,21 +135,17 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        s[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], c1, neg_m));
-        l_run += s[u][j];
+      for (int j = 0; j < 16; ++j) s[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], c1, neg_m));
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        p[2 * u + m] = pack<T>(s[u], m);
+        l_run = add_elements<T>(p[2 * u + m], l_run);
       }
-      p[2 * u] = pack<T>(s[u], 0);
-      p[2 * u + 1] = pack<T>(s[u], 1);
     }
-    if (whole) {
 #pragma unroll
-      for (int m = 0; m < KT / 16; ++m)
+    for (int m = 0; m < KT / 16; ++m)
 #pragma unroll
-        for (int d = 0; d < NDT; ++d) o[d] = A::mma(TL::transposed(vt, 16 * m, 32 * d, lane), p[m], o[d]);
-    } else {
-      masked_product<T, DP, true>(o, vt, 0, p, lane, keep);
-    }
+      for (int d = 0; d < NDT; ++d) o[d] = A::mma(TL::transposed(vt, 16 * m, 32 * d, lane), p[m], o[d]);
   }
 
   const float l = fast::sum_halves(l_run);

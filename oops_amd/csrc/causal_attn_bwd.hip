@@ -33,6 +33,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   constexpr int KT = TL::kRows, NS = DP / 16, NDT = DP / 32, SUB = KT / 32;
   __shared__ __attribute__((aligned(1024))) char k_lds[2][TL::kBytes];
   __shared__ __attribute__((aligned(1024))) char v_lds[2][TL::kBytes];
+  __shared__ uint32_t lost_lds[2];
 
   const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
@@ -90,6 +91,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   const int block_start = span_of(a, block * kBlock).start;
   const int block_last = std::min(block * kBlock + kBlock, length) - 1;
   const int t0 = std::min(block_start, block * kBlock) / KT, t1 = block_last / KT;
+  const int block_last_start = span_of(a, block_last).start;
 
   f32x16 dq[NDT];
 #pragma unroll
@@ -107,11 +109,22 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
       kl.load(kr, (int64_t)(t + 1) * KT, k_lds[buf ^ 1]);
       vl.load(vr, (int64_t)(t + 1) * KT, v_lds[buf ^ 1]);
     }
+    auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
+    uint64_t lost = 0;
+    if (k0 < block_last_start || k0 + KT - 1 > block * kBlock) {
+      // (masked pairs for some wave)
+      if (__syncthreads_or(tile_non_finite<TL, T>(k_lds[buf]))) {
+        lost = rows_non_finite<TL, T>(k_lds[buf], lost_lds);
+        add_non_finite<TL, false>(dq, k_lds[buf], g, keep);
+        __syncthreads();
+        clean_tile<TL, T>(k_lds[buf]);
+        __syncthreads();
+      }
+    }
     if (idle || k0 > last || k0 + KT <= first_start) continue;
     const bool whole = k0 >= last_start && k0 + KT - 1 <= q0;
     const char* kt = k_lds[buf];
     const char* vt = v_lds[buf];
-    auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       f32x16 s{}, dp{};
@@ -122,19 +135,21 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, neg_lse)) * (dp[j] - delta);
+      if (lost) {
+        // (a pair with a lost key: its weight was 0, or made the row's sum NaN)
+        const uint32_t rows = (uint32_t)(lost >> (32 * u)) >> (4 * g);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = rows & (1u << kappa(0, j)) ? 0.f * neg_lse : s[j];
+      }
       if (!whole) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[j] = keep(32 * u + kappa(g, j)) ? s[j] : 0.f;
       }
       Frag<T> ds[2] = {pack<T>(s, 0), pack<T>(s, 1)};
-      if (whole) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int d = 0; d < NDT; ++d) dq[d] = A::mma(TL::transposed(kt, 32 * u + 16 * m, 32 * d, lane), ds[m], dq[d]);
-      } else {
-        masked_product<T, DP, false>(dq, kt, 32 * u, ds, lane, keep);
-      }
+        for (int d = 0; d < NDT; ++d) dq[d] = A::mma(TL::transposed(kt, 32 * u + 16 * m, 32 * d, lane), ds[m], dq[d]);
     }
   }
   if (!valid) return;
@@ -158,11 +173,13 @@ __device__ __forceinline__ void dma4_asm(const fast::u32x4& r, const void* lds, 
 
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kernel(CausalArgs a, uint32_t blocks) {
-  using TL = Tile<T, DP>;
+  using TL = Tile<T, DP, 32>;
   using A = Att<T>;
-  constexpr int QT = TL::kRows, NS = DP / 16, NDT = DP / 32, SUB = QT / 32;
+  constexpr int QT = 32, NS = DP / 16, NDT = DP / 32;
+  constexpr bool kValuesInLds = DP == 128;
   __shared__ __attribute__((aligned(1024))) char q_lds[2][TL::kBytes];
   __shared__ __attribute__((aligned(1024))) char do_lds[2][TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds[kValuesInLds ? 4 : 1][kValuesInLds ? TL::kBytes : 16];
   __shared__ __attribute__((aligned(1024))) float lse_lds[2][64], delta_lds[2][64];
 
   const int tid = threadIdx.x, lane = tid & 63, lk = lane & 31, g = lane >> 5;
@@ -182,12 +199,14 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   const int first_end = __builtin_amdgcn_readlane(span.end, 0);
   const int last_end = __builtin_amdgcn_readlane(span.end, idle ? 0 : last - k0);
 
-  Frag<T> kf[NS], vf[NS];
+  Frag<T> kf[NS], vf[kValuesInLds ? 1 : NS];
   load_row<T, DP>(kf, rows_of<T>(a.k, a.k_stride, b, hk, a.key_size, length), key, valid, g, a.flip);
-  load_row<T, DP>(vf, rows_of<T>(a.v, a.v_stride, b, hk, a.value_size, length), key, valid, g);
+  const Rows vr = rows_of<T>(a.v, a.v_stride, b, hk, a.value_size, length);
+  if constexpr (!kValuesInLds) load_row<T, DP>(vf, vr, key, valid, g);
 
   const int block_last = std::min(block * kBlock + kBlock, length) - 1;
   const int block_end = std::max(span_of(a, block_last).end, block_last + 1);
+  const int block_first_end = span_of(a, block * kBlock).end;
   const int t0 = block * kBlock / QT, tiles = (block_end - 1) / QT - t0 + 1;
   const int h0 = hk * a.group + part * a.group / a.parts, h1 = hk * a.group + (part + 1) * a.group / a.parts;
   const int steps = (h1 - h0) * tiles;
@@ -197,7 +216,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   for (int t = 0; t < NDT; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
   const float c1 = a.scale * kLog2e;
 
-  Loader<T, DP> ql, dl;
+  Loader<T, DP, 32> ql, dl;
   ql.init(rows_of<T>(a.q, a.q_stride, b, h0, a.key_size, length), wave, lane);
   dl.init(rows_of<T>(a.dout, a.do_stride, b, h0, a.value_size, length), wave, lane);
   auto load = [&](int step, int buf) {
@@ -214,58 +233,69 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   };
 
   fast::vmem_wait<0>();  // (the rows, before loads that the compiler does not count)
+  if constexpr (kValuesInLds) {
+    Loader<T, DP, 32> vl;
+    vl.init(vr, wave, lane);
+    for (int i = 0; i < 4; ++i) vl.load(vr, block * kBlock + 32 * i, v_lds[i]);
+  }
   load(0, 0);
   for (int step = 0; step < steps; ++step) {
     const int buf = step & 1, q0 = (t0 + step % tiles) * QT;
     fast::vmem_wait<0>();
     lds_barrier();
     if (step + 1 < steps) load(step + 1, buf ^ 1);
+    auto keep = [&](int r) { return (uint32_t)(q0 + r - key) < width; };
+    if (q0 < block * kBlock + kBlock - 1 || q0 + QT > block_first_end) {
+      // (masked pairs for some wave; a query that is not finite has made its LSE, a dO its delta, NaN or infinite)
+      if (__syncthreads_or(tile_non_finite<TL, T>(q_lds[buf]) | tile_non_finite<TL, T>(do_lds[buf]))) {
+        add_non_finite<TL, false>(dk, q_lds[buf], g, keep);
+        add_non_finite<TL, true>(dv, do_lds[buf], g, keep);
+        __syncthreads();
+        clean_tile<TL, T>(q_lds[buf]);
+        clean_tile<TL, T>(do_lds[buf]);
+        __syncthreads();
+      }
+    }
     if (idle || q0 + QT <= k0 || q0 >= last_end) continue;
     const bool whole = q0 >= k0 + 31 && q0 + QT <= first_end;
     const char* qt = q_lds[buf];
     const char* dot = do_lds[buf];
-    auto keep = [&](int r) { return (uint32_t)(q0 + r - key) < width; };
+    f32x16 s{}, dp{};
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      f32x16 s{}, dp{};
+    for (int i = 0; i < NS; ++i) s = A::mma(TL::row(qt, lk, i, g), kf[i], s);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) s = A::mma(TL::row(qt, 32 * u + lk, i, g), kf[i], s);
+    for (int i = 0; i < NS; ++i) {
+      if constexpr (kValuesInLds) dp = A::mma(TL::row(dot, lk, i, g), TL::row(v_lds[wave], lk, i, g), dp);
+      else dp = A::mma(TL::row(dot, lk, i, g), vf[i], dp);
+    }
 #pragma unroll
-      for (int i = 0; i < NS; ++i) dp = A::mma(TL::row(dot, 32 * u + lk, i, g), vf[i], dp);
+    for (int q = 0; q < 4; ++q) {
+      // rows kappa(g, 4 q ..) are consecutive
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&lse_lds[buf][8 * q + 4 * g]);
+      const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_lds[buf][8 * q + 4 * g]);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        // rows kappa(g, 4 q ..) are consecutive
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(&lse_lds[buf][32 * u + 8 * q + 4 * g]);
-        const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_lds[buf][32 * u + 8 * q + 4 * g]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = 4 * q + i;
-          s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, -lse[i]));
-          dp[j] = s[j] * (dp[j] - delta[i]);
-        }
-      }
-      if (!whole) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const bool pair = keep(32 * u + kappa(g, j));
-          s[j] = pair ? s[j] : 0.f;
-          dp[j] = pair ? dp[j] : 0.f;
-        }
-      }
-      const Frag<T> p[2] = {pack<T>(s, 0), pack<T>(s, 1)}, ds[2] = {pack<T>(dp, 0), pack<T>(dp, 1)};
-      if (whole) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int d = 0; d < NDT; ++d) {
-            dv[d] = A::mma(TL::transposed(dot, 32 * u + 16 * m, 32 * d, lane), p[m], dv[d]);
-            dk[d] = A::mma(TL::transposed(qt, 32 * u + 16 * m, 32 * d, lane), ds[m], dk[d]);
-          }
-      } else {
-        masked_product<T, DP, true>(dv, dot, 32 * u, p, lane, keep);
-        masked_product<T, DP, false>(dk, qt, 32 * u, ds, lane, keep);
+      for (int i = 0; i < 4; ++i) {
+        const int j = 4 * q + i;
+        s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, -lse[i]));
+        dp[j] = s[j] * (dp[j] - delta[i]);
       }
     }
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const bool pair = keep(kappa(g, j));
+        s[j] = pair ? s[j] : 0.f;
+        dp[j] = pair ? dp[j] : 0.f;
+      }
+    }
+    const Frag<T> p[2] = {pack<T>(s, 0), pack<T>(s, 1)}, ds[2] = {pack<T>(dp, 0), pack<T>(dp, 1)};
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) {
+        dv[d] = A::mma(TL::transposed(dot, 16 * m, 32 * d, lane), p[m], dv[d]);
+        dk[d] = A::mma(TL::transposed(qt, 16 * m, 32 * d, lane), ds[m], dk[d]);
+      }
   }
   if (!valid) return;
   const float scale = a.flip ? -a.scale : a.scale;

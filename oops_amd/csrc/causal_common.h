@@ -38,10 +38,10 @@ template <> struct Att<float> {
 };
 template <typename T> using Frag = typename Att<T>::Frag;
 
-// ---- tiles in LDS: KT rows of DP elements
-template <typename T, int DP>
+// ---- tiles in LDS: ROWS rows of DP elements
+template <typename T, int DP, int ROWS = Att<T>::kRows>
 struct Tile {
-  static constexpr int kRows = Att<T>::kRows;
+  static constexpr int kRows = ROWS;
   static constexpr int kBytes = kRows * DP * (int)sizeof(T);
   static constexpr int kPieces = DP * (int)sizeof(T) / 16;          // of a row
   static constexpr int kLoads = kRows * kPieces / 256;              // of a wave, four waves a tile
@@ -111,9 +111,9 @@ __device__ __forceinline__ Rows rows_of(const void* p, const int64_t (&stride)[3
 // Rows row0 .. of `r` to the tile at `lds`; rows behind the last and columns behind the size are zeros.  The
 // resource starts at the tile's first row, so that offsets stay small however long the operand is (the host
 // refuses row pitches of 2^24 bytes and more).
-template <typename T, int DP>
+template <typename T, int DP, int ROWS = Att<T>::kRows>
 struct Loader {
-  using TL = Tile<T, DP>;
+  using TL = Tile<T, DP, ROWS>;
   uint32_t off[TL::kLoads];
   int wave;
   __device__ __forceinline__ void init(const Rows& r, int wave_, int lane) {
@@ -189,96 +189,91 @@ __device__ __forceinline__ Frag<T> pack(const f32x16& x, int m) {
   return f;
 }
 
-// ---- products over tiles where some pairs are masked
+// sum + the elements of f (of 16 bits: the rounded ones, two a step)
+template <typename T>
+__device__ __forceinline__ float add_elements(const Frag<T>& f, float sum) {
+  if constexpr (sizeof(T) == 2) {
+    using P2 = typename fast::Pair<T>::v2;
+    P2 x[4], ones;
+    __builtin_memcpy(x, &f, sizeof(f));
+    ones[0] = ones[1] = (T)1.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = fast::Pair<T>::dot(x[i], ones, sum);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += f[i];
+  }
+  return sum;
+}
+
+// ---- tiles where some pairs are masked
 //
 // A masked pair's weight is 0, but 0 times an infinity or a NaN in the tile
-// is NaN: such elements are taken out of the product, and what they add to the
-// pairs that are not masked is added afterwards, one by one.  Whether there are
-// any is looked at first, so ordinary tiles pay for one more read of the tile.
-
-// largest magnitudes so far, as bit patterns (two of 16 bits, or one of 32)
-template <typename T>
-__device__ __forceinline__ uint32_t raise_bits(uint32_t top, const Frag<T>& f) {
-  constexpr int n = (int)sizeof(Frag<T>) / 4;
-  uint32_t u[n];
-  __builtin_memcpy(u, &f, sizeof(f));
-#pragma unroll
-  for (int i = 0; i < n; ++i) {
-    if constexpr (sizeof(T) == 2) {
-      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-      top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
-                                                                   __builtin_bit_cast(u16x2, u[i] & 0x7FFF7FFFu)));
-    } else {
-      const uint32_t m = u[i] & 0x7FFFFFFFu;
-      top = m > top ? m : top;
-    }
-  }
-  return top;
-}
+// is NaN.  So a tile that is not whole for every wave of the workgroup is looked
+// through first (all threads, once: 1/256 of it each); where it holds such an
+// element, what these add to the pairs that are not masked is added to the
+// accumulators one by one, and they become zeros in LDS.
 template <typename T> struct Bits;
 template <> struct Bits<float> { static constexpr uint32_t kExp = 0x7F800000u; };
 template <> struct Bits<__bf16> { static constexpr uint32_t kExp = 0x7F80u; };
 template <> struct Bits<_Float16> { static constexpr uint32_t kExp = 0x7C00u; };
+// the words (two elements of 16 bits, or one) with elements that are not finite made zero
 template <typename T>
-__device__ __forceinline__ bool non_finite(uint32_t top) {
+__device__ __forceinline__ uint32_t finite_word(uint32_t u) {
   constexpr uint32_t e = Bits<T>::kExp;
-  return sizeof(T) == 2 ? (top & 0xFFFFu) >= e || (top >> 16) >= e : top >= e;
+  if constexpr (sizeof(T) == 4) return (u & e) == e ? 0u : u;
+  const uint32_t lo = (u & e) == e ? 0u : u & 0xFFFFu;
+  return (u >> 16 & e) == e ? lo : lo | (u & 0xFFFF0000u);
 }
-template <typename T>
-__device__ __forceinline__ Frag<T> cleaned(const Frag<T>& f) {
-  constexpr int n = (int)sizeof(Frag<T>) / 4;
-  constexpr uint32_t e = Bits<T>::kExp;
-  uint32_t u[n];
-  __builtin_memcpy(u, &f, sizeof(f));
-#pragma unroll
-  for (int i = 0; i < n; ++i) {
-    if constexpr (sizeof(T) == 2) {
-      if ((u[i] & e) == e) u[i] &= 0xFFFF0000u;
-      if ((u[i] >> 16 & e) == e) u[i] &= 0xFFFFu;
-    } else if ((u[i] & e) == e) {
-      u[i] = 0;
-    }
+template <typename TL, typename T>
+__device__ __forceinline__ bool tile_non_finite(const char* tile) {
+  bool bad = false;
+#pragma unroll 2
+  for (int i = 0; i < TL::kBytes / 4096; ++i) {
+    const uint4 u = reinterpret_cast<const uint4*>(tile)[i * 256 + threadIdx.x];
+    bad |= ((u.x ^ finite_word<T>(u.x)) | (u.y ^ finite_word<T>(u.y)) | (u.z ^ finite_word<T>(u.z)) | (u.w ^ finite_word<T>(u.w))) != 0;
   }
-  Frag<T> c;
-  __builtin_memcpy(&c, u, sizeof(c));
-  return c;
+  return bad;
 }
-// acc[t] += X^T W for the tile X (kRows x DP): W's fragments w[m] over the rows 16 m .. 16 m + 15, keep(row) says which
-// rows this lane's column is paired with.  SIGNED: the weights are positive, an infinity stays one; else what is not
-// finite makes NaN.
-template <typename T, int DP, bool SIGNED, int M, typename Keep>
-__device__ __forceinline__ void masked_product(f32x16 (&acc)[DP / 32], const char* tile, int r0, const Frag<T> (&w)[M],
-                                               int lane, Keep keep) {
-  using TL = Tile<T, DP>;
-  constexpr int NDT = DP / 32;
-  uint32_t top = 0;
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int t = 0; t < NDT; ++t) top = raise_bits<T>(top, TL::transposed(tile, r0 + 16 * m, 32 * t, lane));
-  if (!__any(non_finite<T>(top))) {
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-      for (int t = 0; t < NDT; ++t) acc[t] = Att<T>::mma(TL::transposed(tile, r0 + 16 * m, 32 * t, lane), w[m], acc[t]);
-    return;
-  }
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int t = 0; t < NDT; ++t)
-      acc[t] = Att<T>::mma(cleaned<T>(TL::transposed(tile, r0 + 16 * m, 32 * t, lane)), w[m], acc[t]);
-  const int g = lane >> 5;
+// the tile's rows with such elements, as bits (two words of LDS, written by all threads)
+template <typename TL, typename T>
+__device__ __forceinline__ uint64_t rows_non_finite(const char* tile, uint32_t* words) {
+  if (threadIdx.x < 2) words[threadIdx.x] = 0;
+  __syncthreads();
 #pragma unroll 1
-  for (int r = 0; r < 16 * M; ++r) {
-    const bool pair = keep(r0 + r);
+  for (int i = 0; i < TL::kBytes / 4096; ++i) {
+    const uint4 u = reinterpret_cast<const uint4*>(tile)[i * 256 + threadIdx.x];
+    const int row = (i * 256 + (int)threadIdx.x) / TL::kPieces;
+    if (((u.x ^ finite_word<T>(u.x)) | (u.y ^ finite_word<T>(u.y)) | (u.z ^ finite_word<T>(u.z)) | (u.w ^ finite_word<T>(u.w))) != 0)
+      atomicOr(&words[row >> 5], 1u << (row & 31));
+  }
+  __syncthreads();
+  return fast::uniform64((uint64_t)words[1] << 32 | words[0]);
+}
+template <typename TL, typename T>
+__device__ __forceinline__ void clean_tile(char* tile) {
+#pragma unroll 1
+  for (int i = 0; i < TL::kBytes / 4096; ++i) {
+    uint4& u = reinterpret_cast<uint4*>(tile)[i * 256 + threadIdx.x];
+    u = make_uint4(finite_word<T>(u.x), finite_word<T>(u.y), finite_word<T>(u.z), finite_word<T>(u.w));
+  }
+}
+// SIGNED: the weights are positive, an infinity stays one; else what is not finite makes NaN.  keep(row): whether the
+// tile's row is paired with this lane's column.
+template <typename TL, bool SIGNED, int NDT, typename Keep>
+__device__ __forceinline__ void add_non_finite(f32x16 (&acc)[NDT], const char* tile, int g, Keep keep) {
+#pragma unroll 1
+  for (int r = 0; r < TL::kRows; ++r) {
+    const bool pair = keep(r);
 #pragma unroll
-    for (int t = 0; t < NDT; ++t)
+    for (int t = 0; t < NDT; ++t) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const float x = TL::element(tile, r0 + r, 32 * t + kappa(g, j));
+        const float x = TL::element(tile, r, 32 * t + kappa(g, j));
         if (pair && !__builtin_isfinite(x)) acc[t][j] += SIGNED ? x : __builtin_nanf("");
       }
+      asm volatile("" ::: "memory");  // (few of these rare reads in flight: they would take registers from the loop)
+    }
   }
 }
 
