@@ -594,8 +594,10 @@ typedef struct oops_causal_geometry {
   int64_t length;
   int64_t stride[OOPS_CA_OPERANDS][3];
 } oops_causal_geometry;
+size_t oops_causal_attn_forward_workspace_bytes(const oops_causal_geometry* geo); /* 0 without sequences */
 int oops_causal_attn_forward(const oops_causal_geometry* geo, const void* q, const void* k, const void* v,
-                             const void* offsets, void* out, void* out_low, float* lse, void* stream);
+                             const void* offsets, void* out, void* out_low, float* lse, void* workspace, size_t ws_bytes,
+                             void* stream);
 size_t oops_causal_attn_backward_workspace_bytes(const oops_causal_geometry* geo);
 int oops_causal_attn_backward(const oops_causal_geometry* geo, const void* q, const void* k, const void* v,
                               const void* offsets, const void* out, const void* out_low, const float* lse,

@@ -92,6 +92,7 @@ EXPORTED_SYMBOLS = (
     "oops_rms_norm_rotary_forward",
     "oops_rms_norm_rotary_backward_workspace_bytes",
     "oops_rms_norm_rotary_backward",
+    "oops_causal_attn_forward_workspace_bytes",
     "oops_causal_attn_forward",
     "oops_causal_attn_backward_workspace_bytes",
     "oops_causal_attn_backward",
@@ -427,7 +428,7 @@ def load() -> ctypes.CDLL:
         kg, dg = ctypes.POINTER(CacheGeometry), ctypes.POINTER(CacheAttnGeometry)
         lib.oops_rms_norm_rotary_forward.argtypes = [og] + [vp] * 9
         lib.oops_rms_norm_rotary_backward.argtypes = [og] + [vp] * 13 + [sz, vp]
-        lib.oops_causal_attn_forward.argtypes = [cg] + [vp] * 8
+        lib.oops_causal_attn_forward.argtypes = [cg] + [vp] * 8 + [sz, vp]
         lib.oops_causal_attn_backward.argtypes = [cg] + [vp] * 12 + [sz, vp]
         lib.oops_cache_write.argtypes = [kg] + [vp] * 6 + [sz, vp]
         lib.oops_cache_read.argtypes = [kg] + [vp] * 6
@@ -436,6 +437,7 @@ def load() -> ctypes.CDLL:
                      lib.oops_causal_attn_backward, lib.oops_cache_write, lib.oops_cache_read, lib.oops_cache_attn):  # fmt: skip
             call.restype = i32
         for size, geometry in ((lib.oops_rms_norm_rotary_backward_workspace_bytes, og),
+                               (lib.oops_causal_attn_forward_workspace_bytes, cg),
                                (lib.oops_causal_attn_backward_workspace_bytes, cg),
                                (lib.oops_cache_write_workspace_bytes, kg), (lib.oops_cache_attn_workspace_bytes, dg)):  # fmt: skip
             size.argtypes, size.restype = [geometry], sz

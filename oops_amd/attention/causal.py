@@ -137,7 +137,7 @@ def _check(query, key, value, offsets) -> None:
 
 @functools.lru_cache(maxsize=512)
 def _geometry(lib, dtype, shape: tuple, kv_heads: int, e: int, scale: float, sequences: int, i64: bool, strides: tuple) -> tuple:
-    """The launch geometry and the backward's workspace (cached: the library only reads it)."""
+    """The launch geometry and its (forward, backward) workspaces (cached: the library only reads it)."""
 
     b, h, n, d = shape
     g = _lib.CausalGeometry()
@@ -146,7 +146,7 @@ def _geometry(lib, dtype, shape: tuple, kv_heads: int, e: int, scale: float, seq
     for i, s in enumerate(strides):
         g.stride[i][:] = s
     ref = ctypes.pointer(g)
-    return ref, lib.oops_causal_attn_backward_workspace_bytes(ref)
+    return ref, lib.oops_causal_attn_forward_workspace_bytes(ref), lib.oops_causal_attn_backward_workspace_bytes(ref)
 
 
 def _strides(t: Optional[Tensor]) -> tuple:
@@ -192,9 +192,10 @@ def _forward_impl(q: Tensor, k: Tensor, v: Tensor, offsets: Optional[Tensor], sc
     q, k, v = _whole(q), _whole(k), _whole(v)
     low = torch.empty_like(out) if save and out.dtype != torch.float32 else out.new_empty(0)
     lse = torch.empty(q.shape[:3] if save else 0, dtype=torch.float32, device=q.device)
-    geo, _ = _call_geometry(lib, q, k, v, offsets, scale, out)
+    geo, ws_bytes, _ = _call_geometry(lib, q, k, v, offsets, scale, out)
+    ws = _workspace(ws_bytes, q.device)
     rc = call_on(q.device.index, lib.oops_causal_attn_forward, geo, _ptr(q), _ptr(k), _ptr(v), _ptr(offsets), _ptr(out),
-                 _ptr(low), _ptr(lse))  # fmt: skip
+                 _ptr(low), _ptr(lse), _ptr(ws), ws_bytes)  # fmt: skip
     _lib.check(rc, "causal attention forward")
     return out, low, lse
 
@@ -206,7 +207,7 @@ def _backward_impl(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, offsets: Optio
     lib = _lib.load()
     dq, dk, dv = (_result_like(t, t.shape[-1]) if need else t.new_empty(0) for t, need in zip((q, k, v), needs))
     q, k, v, dout = _whole(q), _whole(k), _whole(v), _whole(dout.resolve_neg())
-    geo, ws_bytes = _call_geometry(lib, q, k, v, offsets, scale, out, dout, dq, dk, dv)
+    geo, _, ws_bytes = _call_geometry(lib, q, k, v, offsets, scale, out, dout, dq, dk, dv)
     ws = _workspace(ws_bytes, q.device)
     rc = call_on(q.device.index, lib.oops_causal_attn_backward, geo, _ptr(q), _ptr(k), _ptr(v), _ptr(offsets), _ptr(out),
                  _ptr(low), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), ws_bytes)  # fmt: skip

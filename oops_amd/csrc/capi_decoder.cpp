@@ -102,9 +102,13 @@ oops::CausalArgs causal_args(const oops_causal_geometry& g, const void* q, const
   a.flip = std::signbit(g.scale);
   a.scale = std::fabs(g.scale);
   a.parts = 1;
+  a.blocks = (int32_t)((g.length + 127) / 128);
   return a;
 }
-size_t delta_bytes(const oops_causal_geometry& g) { return align256((size_t)(g.batch * g.heads * g.length) * sizeof(float)); }
+size_t stat_bytes(const oops_causal_geometry& g) { return align256((size_t)(g.batch * g.heads * g.length) * sizeof(float)); }
+size_t order_bytes(const oops_causal_geometry& g) {
+  return g.sequences > 0 && oops::causal_ordered(g) ? align256((size_t)((g.length + 127) / 128) * 2 * sizeof(int32_t)) : 0;
+}
 size_t part_bytes(const oops_causal_geometry& g, int parts, int size) {
   return parts > 1 ? align256((size_t)(g.batch * g.kv_heads * g.length) * size * parts * sizeof(float)) : 0;
 }
@@ -188,25 +192,41 @@ int oops_rms_norm_rotary_backward(const oops_rotary_geometry* geo, const void* q
       "rms_norm_rotary backward");
 }
 
+size_t oops_causal_attn_forward_workspace_bytes(const oops_causal_geometry* geo) {
+  oops::clear_report();
+  if (check_causal(geo, true)) return 0;
+  return order_bytes(*geo);
+}
+
 int oops_causal_attn_forward(const oops_causal_geometry* geo, const void* q, const void* k, const void* v,
-                             const void* offsets, void* out, void* out_low, float* lse, void* stream) {
+                             const void* offsets, void* out, void* out_low, float* lse, void* workspace, size_t ws_bytes,
+                             void* stream) {
   oops::clear_report();
   if (int rc = check_causal(geo, offsets)) return rc;
   if (geo->batch * geo->length == 0) return OOPS_OK;
   if (!q || !k || !v || !out) return report(OOPS_EINVAL, "q, k, v and out must be non-NULL");
   if (!aligned({q, k, v, out, out_low})) return report(OOPS_EINVAL, "operands must lie at multiples of 16 bytes");
+  const size_t order = offsets ? order_bytes(*geo) : 0;
+  if (int rc = oops::report_workspace(workspace, ws_bytes, order)) return rc;
   oops::CausalArgs a = causal_args(*geo, q, k, v, offsets);
   a.out = out;
   a.low = geo->dtype == OOPS_F32 ? nullptr : out_low;
   a.lse = lse;
-  return report_launch(oops::launch_causal_forward(geo->dtype, a, static_cast<hipStream_t>(stream)), "causal attention forward");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e = hipSuccess;
+  if (order) {
+    e = oops::launch_causal_order(a, static_cast<int32_t*>(workspace), st);
+    a.order = static_cast<int32_t*>(workspace);
+  }
+  if (e == hipSuccess) e = oops::launch_causal_forward(geo->dtype, a, st);
+  return report_launch(e, "causal attention forward");
 }
 
 size_t oops_causal_attn_backward_workspace_bytes(const oops_causal_geometry* geo) {
   oops::clear_report();
-  if (check_causal(geo, false)) return 0;
+  if (check_causal(geo, true)) return 0;
   const int parts = oops::causal_grad_parts(*geo);
-  return delta_bytes(*geo) + part_bytes(*geo, parts, geo->key_size) + part_bytes(*geo, parts, geo->value_size);
+  return order_bytes(*geo) + 2 * stat_bytes(*geo) + part_bytes(*geo, parts, geo->key_size) + part_bytes(*geo, parts, geo->value_size);
 }
 
 int oops_causal_attn_backward(const oops_causal_geometry* geo, const void* q, const void* k, const void* v,
@@ -230,10 +250,19 @@ int oops_causal_attn_backward(const oops_causal_geometry* geo, const void* q, co
   a.dv = grad_v;
   a.parts = oops::causal_grad_parts(*geo);
   char* ws = static_cast<char*>(workspace);
-  a.delta = reinterpret_cast<float*>(ws);
-  a.dk_parts = reinterpret_cast<float*>(ws + delta_bytes(*geo));
-  a.dv_parts = reinterpret_cast<float*>(ws + delta_bytes(*geo) + part_bytes(*geo, a.parts, geo->key_size));
-  return report_launch(oops::launch_causal_backward(geo->dtype, a, static_cast<hipStream_t>(stream)), "causal attention backward");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e = hipSuccess;
+  if (offsets && order_bytes(*geo)) {
+    e = oops::launch_causal_order(a, reinterpret_cast<int32_t*>(ws), st);
+    a.order = reinterpret_cast<int32_t*>(ws);
+  }
+  ws += order_bytes(*geo);
+  a.neg_lse = reinterpret_cast<float*>(ws);
+  a.neg_delta = reinterpret_cast<float*>(ws += stat_bytes(*geo));
+  a.dk_parts = reinterpret_cast<float*>(ws += stat_bytes(*geo));
+  a.dv_parts = reinterpret_cast<float*>(ws + part_bytes(*geo, a.parts, geo->key_size));
+  if (e == hipSuccess) e = oops::launch_causal_backward(geo->dtype, a, st);
+  return report_launch(e, "causal attention backward");
 }
 
 size_t oops_cache_write_workspace_bytes(const oops_cache_geometry* geo) {

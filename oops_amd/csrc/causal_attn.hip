@@ -25,10 +25,8 @@ namespace oops {
 namespace causal {
 namespace {
 
-constexpr int kBlock = 128;  // queries of a workgroup
-
 template <typename T, int DP>
-__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void causal_forward_kernel(CausalArgs a, uint32_t blocks) {
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void causal_forward_kernel(CausalArgs a) {
   using TL = Tile<T, DP>;
   using A = Att<T>;
   constexpr int KT = TL::kRows, NS = DP / 16, NDT = DP / 32, SUB = KT / 32;
@@ -37,37 +35,36 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 
   const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
-  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.heads), blocks);
+  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.heads));
   const int b = w.head / a.heads, h = w.head % a.heads;
-  const int block = (int)blocks - 1 - w.block;
+  const int block = a.order ? a.order[w.rank] : a.blocks - 1 - w.rank;
   const int length = (int)a.length;
 
-  const int q0 = block * kBlock + wave * 32, row = q0 + lq;
+  const int block0 = block * kBlock, block1 = std::min(block0 + kBlock, length) - 1;
+  const int q0 = block0 + wave * 32, row = q0 + lq;
+  const bool idle = q0 >= length;  // (a wave behind the last token has no pairs)
+  const int last = std::min(q0 + 31, length - 1);
   const bool valid = row < length;
-  const Span span = span_of(a, valid ? row : length - 1);
+  const Spans spans = spans_of(a, block0, block1, std::min(q0, last), last, std::min(row, last));
   // keys this lane's query is paired with: [start, row]
-  const int start = span.start;
-  const uint32_t reach = valid && start <= row ? (uint32_t)(row - start) : 0u;
+  const int start = spans.own.start;
   const bool empty = !valid || start > row;
-  const int last = q0 + 31 < length ? q0 + 31 : length - 1;
-  // (a wave behind the last token has no pairs)
-  const bool idle = q0 >= length;
+  const uint32_t reach = empty ? 0u : (uint32_t)(row - start);
   const int first_start = __builtin_amdgcn_readlane(start, 0), last_start = __builtin_amdgcn_readlane(start, idle ? 0 : last - q0);
 
-  const Rows qr = rows_of<T>(a.q, a.q_stride, b, h, a.key_size, length);
   const Rows kr = rows_of<T>(a.k, a.k_stride, b, h / a.group, a.key_size, length);
   const Rows vr = rows_of<T>(a.v, a.v_stride, b, h / a.group, a.value_size, length);
+  Frag<T> qf[NS];
+  load_row<T, DP>(qf, rows_of<T>(a.q, a.q_stride, b, h, a.key_size, length), row, valid, g, a.flip);
+
+  const int t0 = std::min(spans.first.start, block0) / KT, t1 = block1 / KT;
   Loader<T, DP> kl, vl;
   kl.init(kr, wave, lane);
   vl.init(vr, wave, lane);
-
-  Frag<T> qf[NS];
-  load_row<T, DP>(qf, qr, row, valid, g, a.flip);
-
-  const int block_start = span_of(a, block * kBlock).start;
-  const int block_last = std::min(block * kBlock + kBlock, length) - 1;
-  const int t0 = std::min(block_start, block * kBlock) / KT, t1 = block_last / KT;
-  const int block_last_start = span_of(a, block_last).start;
+  kl.seek(kr, t0 * KT);
+  vl.seek(vr, t0 * KT);
+  Reads<T, DP> rd;
+  rd.init(lane);
 
   float m_run = kNegInf, neg_m = 0.f, l_run = 0.f;
   f32x16 o[NDT];
@@ -77,18 +74,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
   const float c1 = fmaxf(a.scale * kLog2e, 0x1p-120f);
 
   fast::vmem_wait<0>();  // (the queries, before loads that the compiler does not count)
-  kl.load(kr, (int64_t)t0 * KT, k_lds[0]);
-  vl.load(vr, (int64_t)t0 * KT, v_lds[0]);
-  for (int t = t0; t <= t1; ++t) {
-    const int buf = (t - t0) & 1, k0 = t * KT;
+  kl.next(k_lds[0]);
+  vl.next(v_lds[0]);
+  // (the buffer is a constant, so that its address is part of the instructions)
+  auto step = [&](int t, auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
+    const int k0 = t * KT;
     fast::vmem_wait<0>();
     lds_barrier();
     if (t < t1) {
-      kl.load(kr, (int64_t)(t + 1) * KT, k_lds[buf ^ 1]);
-      vl.load(vr, (int64_t)(t + 1) * KT, v_lds[buf ^ 1]);
+      kl.next(k_lds[buf ^ 1]);
+      vl.next(v_lds[buf ^ 1]);
     }
     auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
-    if (k0 < block_last_start || k0 + KT - 1 > block * kBlock) {
+    if (k0 < spans.last.start || k0 + KT - 1 > block0) {
       // (masked pairs for some wave)
       if (__syncthreads_or(tile_non_finite<TL, T>(v_lds[buf]))) {
         add_non_finite<TL, true>(o, v_lds[buf], g, keep);
@@ -97,19 +96,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
         __syncthreads();
       }
     }
-    if (idle || k0 > last || k0 + KT <= first_start) continue;
-    const bool whole = k0 >= last_start && k0 + KT - 1 <= q0;
-    const char* kt = k_lds[buf];
-    const char* vt = v_lds[buf];
+    if (idle || k0 > last || k0 + KT <= first_start) return;
 
     f32x16 s[SUB];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       s[u] = f32x16{};
 #pragma unroll
-      for (int i = 0; i < NS; ++i) s[u] = A::mma(TL::row(kt, 32 * u + lq, i, g), qf[i], s[u]);
+      for (int i = 0; i < NS; ++i) s[u] = A::mma(rd.row(k_lds[buf], u, i), qf[i], s[u]);
     }
-    if (!whole) {
+    if (k0 < last_start || k0 + KT - 1 > q0) {
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -145,7 +141,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 #pragma unroll
     for (int m = 0; m < KT / 16; ++m)
 #pragma unroll
-      for (int d = 0; d < NDT; ++d) o[d] = A::mma(TL::transposed(vt, 16 * m, 32 * d, lane), p[m], o[d]);
+      for (int d = 0; d < NDT; ++d) o[d] = A::mma(rd.col(v_lds[buf], m, d), p[m], o[d]);
+  };
+  for (int t = t0;;) {
+    step(t, std::integral_constant<int, 0>{});
+    if (++t > t1) break;
+    step(t, std::integral_constant<int, 1>{});
+    if (++t > t1) break;
   }
 
   const float l = fast::sum_halves(l_run);
@@ -167,13 +169,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 
 hipError_t launch_causal_forward(int dtype, const CausalArgs& a, hipStream_t stream) {
   if (a.length == 0 || a.batch == 0) return hipSuccess;
-  const uint32_t blocks = (uint32_t)((a.length + causal::kBlock - 1) / causal::kBlock);
-  const dim3 grid(blocks * (uint32_t)(a.batch * a.heads));
+  const dim3 grid((uint32_t)a.blocks * (uint32_t)(a.batch * a.heads));
   const bool wide = a.key_size > 64 || a.value_size > 64;
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    if (wide) hipLaunchKernelGGL((causal::causal_forward_kernel<T, 128>), grid, dim3(256), 0, stream, a, blocks);
-    else hipLaunchKernelGGL((causal::causal_forward_kernel<T, 64>), grid, dim3(256), 0, stream, a, blocks);
+    if (wide) hipLaunchKernelGGL((causal::causal_forward_kernel<T, 128>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((causal::causal_forward_kernel<T, 64>), grid, dim3(256), 0, stream, a);
     return hipGetLastError();
   };
   if (dtype == OOPS_F32) return go(float{});

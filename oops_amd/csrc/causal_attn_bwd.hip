@@ -22,12 +22,11 @@ namespace oops {
 namespace causal {
 namespace {
 
-constexpr int kBlock = 128;  // queries, or keys, of a workgroup
 template <typename T, int DP>
 constexpr int kOcc = sizeof(T) == 4 && DP == 128 ? 1 : 2;
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(CausalArgs a, uint32_t blocks) {
+__global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(CausalArgs a) {
   using TL = Tile<T, DP>;
   using A = Att<T>;
   constexpr int KT = TL::kRows, NS = DP / 16, NDT = DP / 32, SUB = KT / 32;
@@ -37,40 +36,29 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
 
   const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
-  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.heads), blocks);
+  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.heads));
   const int b = w.head / a.heads, h = w.head % a.heads;
-  const int block = (int)blocks - 1 - w.block;
+  const int block = a.order ? a.order[w.rank] : a.blocks - 1 - w.rank;
   const int length = (int)a.length;
 
-  const int q0 = block * kBlock + wave * 32, row = q0 + lq;
-  const bool valid = row < length;
-  const Span span = span_of(a, valid ? row : length - 1);
-  const int start = span.start;
-  const bool empty = !valid || start > row;
-  const uint32_t reach = empty ? 0u : (uint32_t)(row - start);
-  const int last = q0 + 31 < length ? q0 + 31 : length - 1;
+  const int block0 = block * kBlock, block1 = std::min(block0 + kBlock, length) - 1;
+  const int q0 = block0 + wave * 32, row = q0 + lq;
   const bool idle = q0 >= length;
-  const int first_start = __builtin_amdgcn_readlane(start, 0), last_start = __builtin_amdgcn_readlane(start, idle ? 0 : last - q0);
-
-  const Rows qr = rows_of<T>(a.q, a.q_stride, b, h, a.key_size, length);
-  const Rows kr = rows_of<T>(a.k, a.k_stride, b, h / a.group, a.key_size, length);
-  const Rows vr = rows_of<T>(a.v, a.v_stride, b, h / a.group, a.value_size, length);
-  const Rows dor = rows_of<T>(a.dout, a.do_stride, b, h, a.value_size, length);
-  const Rows outr = rows_of<T>(a.out, a.o_stride, b, h, a.value_size, length);
+  const int last = std::min(q0 + 31, length - 1);
+  const bool valid = row < length;
 
   Frag<T> dof[NS];
-  load_row<T, DP>(dof, dor, row, valid, g);
+  load_row<T, DP>(dof, rows_of<T>(a.dout, a.do_stride, b, h, a.value_size, length), row, valid, g);
   float delta = 0.f;
   {
     Frag<T> of[NS];
-    load_row<T, DP>(of, outr, row, valid, g);
+    load_row<T, DP>(of, rows_of<T>(a.out, a.o_stride, b, h, a.value_size, length), row, valid, g);
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)of[s][i], (float)dof[s][i], delta);
     if (a.low) {
-      const Rows lowr = rows_of<T>(a.low, a.o_stride, b, h, a.value_size, length);
-      load_row<T, DP>(of, lowr, row, valid, g);
+      load_row<T, DP>(of, rows_of<T>(a.low, a.o_stride, b, h, a.value_size, length), row, valid, g);
 #pragma unroll
       for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -78,40 +66,54 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
     }
     delta = fast::sum_halves(delta);
   }
+  const float c1 = fmaxf(a.scale * kLog2e, 0x1p-120f);
   const int64_t stat = ((int64_t)b * a.heads + h) * length + row;
-  if (valid && g == 0) a.delta[stat] = delta;
+  const float lse = valid ? a.lse[stat] : 0.f;
+  if (valid && g == 0) {
+    // (as the second kernel's accumulators start)
+    a.neg_delta[stat] = -delta;
+    a.neg_lse[stat] = -lse / c1;
+  }
   if (!a.dq) return;
-  const float neg_lse = valid ? -a.lse[stat] : 0.f;
-  Frag<T> qf[NS];
-  load_row<T, DP>(qf, qr, row, valid, g, a.flip);
 
+  const Spans spans = spans_of(a, block0, block1, std::min(q0, last), last, std::min(row, last));
+  const int start = spans.own.start;
+  const bool empty = !valid || start > row;
+  const uint32_t reach = empty ? 0u : (uint32_t)(row - start);
+  const int first_start = __builtin_amdgcn_readlane(start, 0), last_start = __builtin_amdgcn_readlane(start, idle ? 0 : last - q0);
+  Frag<T> qf[NS];
+  load_row<T, DP>(qf, rows_of<T>(a.q, a.q_stride, b, h, a.key_size, length), row, valid, g, a.flip);
+
+  const Rows kr = rows_of<T>(a.k, a.k_stride, b, h / a.group, a.key_size, length);
+  const Rows vr = rows_of<T>(a.v, a.v_stride, b, h / a.group, a.value_size, length);
+  const int t0 = std::min(spans.first.start, block0) / KT, t1 = block1 / KT;
   Loader<T, DP> kl, vl;
   kl.init(kr, wave, lane);
   vl.init(vr, wave, lane);
-  const int block_start = span_of(a, block * kBlock).start;
-  const int block_last = std::min(block * kBlock + kBlock, length) - 1;
-  const int t0 = std::min(block_start, block * kBlock) / KT, t1 = block_last / KT;
-  const int block_last_start = span_of(a, block_last).start;
+  kl.seek(kr, t0 * KT);
+  vl.seek(vr, t0 * KT);
+  Reads<T, DP> rd;
+  rd.init(lane);
 
   f32x16 dq[NDT];
 #pragma unroll
   for (int t = 0; t < NDT; ++t) dq[t] = f32x16{};
-  const float c1 = a.scale * kLog2e;
 
   fast::vmem_wait<0>();  // (the rows, before loads that the compiler does not count)
-  kl.load(kr, (int64_t)t0 * KT, k_lds[0]);
-  vl.load(vr, (int64_t)t0 * KT, v_lds[0]);
-  for (int t = t0; t <= t1; ++t) {
-    const int buf = (t - t0) & 1, k0 = t * KT;
+  kl.next(k_lds[0]);
+  vl.next(v_lds[0]);
+  auto step = [&](int t, auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
+    const int k0 = t * KT;
     fast::vmem_wait<0>();
     lds_barrier();
     if (t < t1) {
-      kl.load(kr, (int64_t)(t + 1) * KT, k_lds[buf ^ 1]);
-      vl.load(vr, (int64_t)(t + 1) * KT, v_lds[buf ^ 1]);
+      kl.next(k_lds[buf ^ 1]);
+      vl.next(v_lds[buf ^ 1]);
     }
     auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
     uint64_t lost = 0;
-    if (k0 < block_last_start || k0 + KT - 1 > block * kBlock) {
+    if (k0 < spans.last.start || k0 + KT - 1 > block0) {
       // (masked pairs for some wave)
       if (__syncthreads_or(tile_non_finite<TL, T>(k_lds[buf]))) {
         lost = rows_non_finite<TL, T>(k_lds[buf], lost_lds);
@@ -121,36 +123,39 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
         __syncthreads();
       }
     }
-    if (idle || k0 > last || k0 + KT <= first_start) continue;
+    if (idle || k0 > last || k0 + KT <= first_start) return;
     const bool whole = k0 >= last_start && k0 + KT - 1 <= q0;
-    const char* kt = k_lds[buf];
-    const char* vt = v_lds[buf];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       f32x16 s{}, dp{};
 #pragma unroll
-      for (int i = 0; i < NS; ++i) s = A::mma(TL::row(kt, 32 * u + lq, i, g), qf[i], s);
+      for (int i = 0; i < NS; ++i) s = A::mma(rd.row(k_lds[buf], u, i), qf[i], s);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) dp = A::mma(TL::row(vt, 32 * u + lq, i, g), dof[i], dp);
+      for (int i = 0; i < NS; ++i) dp = A::mma(rd.row(v_lds[buf], u, i), dof[i], dp);
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, neg_lse)) * (dp[j] - delta);
+      for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, -lse)) * (dp[j] - delta);
       if (lost) {
         // (a pair with a lost key: its weight was 0, or made the row's sum NaN)
         const uint32_t rows = (uint32_t)(lost >> (32 * u)) >> (4 * g);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = rows & (1u << kappa(0, j)) ? 0.f * neg_lse : s[j];
+        for (int j = 0; j < 16; ++j) s[j] = rows & (1u << kappa(0, j)) ? 0.f * lse : s[j];
       }
       if (!whole) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[j] = keep(32 * u + kappa(g, j)) ? s[j] : 0.f;
       }
-      Frag<T> ds[2] = {pack<T>(s, 0), pack<T>(s, 1)};
+      const Frag<T> ds[2] = {pack<T>(s, 0), pack<T>(s, 1)};
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int d = 0; d < NDT; ++d) dq[d] = A::mma(TL::transposed(kt, 32 * u + 16 * m, 32 * d, lane), ds[m], dq[d]);
+        for (int d = 0; d < NDT; ++d) dq[d] = A::mma(rd.col(k_lds[buf], 2 * u + m, d), ds[m], dq[d]);
     }
+  };
+  for (int t = t0;;) {
+    step(t, std::integral_constant<int, 0>{});
+    if (++t > t1) break;
+    step(t, std::integral_constant<int, 1>{});
+    if (++t > t1) break;
   }
   if (!valid) return;
   const float scale = a.flip ? -a.scale : a.scale;
@@ -172,10 +177,11 @@ __device__ __forceinline__ void dma4_asm(const fast::u32x4& r, const void* lds, 
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kernel(CausalArgs a, uint32_t blocks) {
+__global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kernel(CausalArgs a) {
   using TL = Tile<T, DP, 32>;
   using A = Att<T>;
   constexpr int QT = 32, NS = DP / 16, NDT = DP / 32;
+  // (registers: with 128 channels dK, dV and K fill them; V is read again from LDS at each step)
   constexpr bool kValuesInLds = DP == 128;
   __shared__ __attribute__((aligned(1024))) char q_lds[2][TL::kBytes];
   __shared__ __attribute__((aligned(1024))) char do_lds[2][TL::kBytes];
@@ -184,51 +190,64 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
 
   const int tid = threadIdx.x, lane = tid & 63, lk = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
-  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.kv_heads * a.parts), blocks);
+  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.kv_heads * a.parts));
   const int part = w.head % a.parts, hk = w.head / a.parts % a.kv_heads, b = w.head / a.parts / a.kv_heads;
-  const int block = w.block;
+  const int block = a.order ? a.order[a.blocks + w.rank] : w.rank;
   const int length = (int)a.length;
 
-  const int k0 = block * kBlock + wave * 32, key = k0 + lk;
-  const bool valid = key < length;
-  const Span span = span_of(a, valid ? key : length - 1);
-  // queries this lane's key is paired with: [key, key + width)
-  const uint32_t width = valid && span.end > key ? (uint32_t)(span.end - key) : 0u;
-  const int last = k0 + 31 < length ? k0 + 31 : length - 1;
+  const int block0 = block * kBlock, block1 = std::min(block0 + kBlock, length) - 1;
+  const int k0 = block0 + wave * 32, key = k0 + lk;
   const bool idle = k0 >= length;
-  const int first_end = __builtin_amdgcn_readlane(span.end, 0);
-  const int last_end = __builtin_amdgcn_readlane(span.end, idle ? 0 : last - k0);
+  const int last = std::min(k0 + 31, length - 1);
+  const bool valid = key < length;
+  const Spans spans = spans_of(a, block0, block1, std::min(k0, last), last, std::min(key, last));
+  // queries this lane's key is paired with: [key, key + width)
+  const int end = spans.own.end;
+  const uint32_t width = valid && end > key ? (uint32_t)(end - key) : 0u;
+  const int first_end = __builtin_amdgcn_readlane(end, 0), last_end = __builtin_amdgcn_readlane(end, idle ? 0 : last - k0);
 
   Frag<T> kf[NS], vf[kValuesInLds ? 1 : NS];
   load_row<T, DP>(kf, rows_of<T>(a.k, a.k_stride, b, hk, a.key_size, length), key, valid, g, a.flip);
   const Rows vr = rows_of<T>(a.v, a.v_stride, b, hk, a.value_size, length);
   if constexpr (!kValuesInLds) load_row<T, DP>(vf, vr, key, valid, g);
 
-  const int block_last = std::min(block * kBlock + kBlock, length) - 1;
-  const int block_end = std::max(span_of(a, block_last).end, block_last + 1);
-  const int block_first_end = span_of(a, block * kBlock).end;
-  const int t0 = block * kBlock / QT, tiles = (block_end - 1) / QT - t0 + 1;
+  const int block_end = std::max(spans.last.end, block1 + 1);
+  const int t0 = block0 / QT, t1 = (block_end - 1) / QT;
   const int h0 = hk * a.group + part * a.group / a.parts, h1 = hk * a.group + (part + 1) * a.group / a.parts;
-  const int steps = (h1 - h0) * tiles;
 
   f32x16 dk[NDT], dv[NDT];
 #pragma unroll
   for (int t = 0; t < NDT; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
-  const float c1 = a.scale * kLog2e;
+  const float c1 = fmaxf(a.scale * kLog2e, 0x1p-120f);
+  Reads<T, DP> rd, rv;
+  rd.init(lane);
+  rv = rd;
+#pragma unroll
+  for (int i = 0; i < TL::kWindows; ++i) rv.row_at[i] += wave * TL::kBytes;
 
+  // the tiles' order: the group's heads, each from the block's first query to the last that is paired with its keys
   Loader<T, DP, 32> ql, dl;
   ql.init(rows_of<T>(a.q, a.q_stride, b, h0, a.key_size, length), wave, lane);
   dl.init(rows_of<T>(a.dout, a.do_stride, b, h0, a.value_size, length), wave, lane);
-  auto load = [&](int step, int buf) {
-    const int h = h0 + step / tiles;
-    const int64_t row0 = (int64_t)(t0 + step % tiles) * QT;
-    ql.load(rows_of<T>(a.q, a.q_stride, b, h, a.key_size, length), row0, q_lds[buf]);
-    dl.load(rows_of<T>(a.dout, a.do_stride, b, h, a.value_size, length), row0, do_lds[buf]);
-    if (wave < 2) {
-      const int64_t left = length - row0;
-      const int n = left < QT ? (int)left : QT;
-      const float* p = (wave == 0 ? a.lse : a.delta) + ((int64_t)b * a.heads + h) * length + row0;
-      dma4_asm(fast::rsrc_words(p, (uint32_t)n * 4), wave == 0 ? lse_lds[buf] : delta_lds[buf], (uint32_t)lane * 4);
+  int load_h = h0, load_t = t0;
+  const float* stats = nullptr;  // of the next tile, for waves 0 and 1
+  auto seek = [&] {
+    ql.seek(rows_of<T>(a.q, a.q_stride, b, load_h, a.key_size, length), load_t * QT);
+    dl.seek(rows_of<T>(a.dout, a.do_stride, b, load_h, a.value_size, length), load_t * QT);
+    stats = (wave == 0 ? a.neg_lse : a.neg_delta) + ((int64_t)b * a.heads + load_h) * length + load_t * QT;
+  };
+  auto load = [&](auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
+    const int n = std::min(ql.left, QT);
+    ql.next(q_lds[buf]);
+    dl.next(do_lds[buf]);
+    if (wave < 2)
+      dma4_asm(fast::rsrc_words(stats, (uint32_t)n * 4), wave == 0 ? lse_lds[buf] : delta_lds[buf], (uint32_t)lane * 4);
+    stats += QT;
+    if (++load_t > t1) {
+      load_t = t0;
+      ++load_h;
+      if (load_h < h1) seek();
     }
   };
 
@@ -236,16 +255,19 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   if constexpr (kValuesInLds) {
     Loader<T, DP, 32> vl;
     vl.init(vr, wave, lane);
-    for (int i = 0; i < 4; ++i) vl.load(vr, block * kBlock + 32 * i, v_lds[i]);
+    vl.seek(vr, block0);
+    for (int i = 0; i < 4; ++i) vl.next(v_lds[i]);
   }
-  load(0, 0);
-  for (int step = 0; step < steps; ++step) {
-    const int buf = step & 1, q0 = (t0 + step % tiles) * QT;
+  seek();
+  load(std::integral_constant<int, 0>{});
+  auto step = [&](int t, auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
+    const int q0 = t * QT;
     fast::vmem_wait<0>();
     lds_barrier();
-    if (step + 1 < steps) load(step + 1, buf ^ 1);
+    if (load_h < h1) load(std::integral_constant<int, buf ^ 1>{});
     auto keep = [&](int r) { return (uint32_t)(q0 + r - key) < width; };
-    if (q0 < block * kBlock + kBlock - 1 || q0 + QT > block_first_end) {
+    if (q0 < block0 + kBlock - 1 || q0 + QT > spans.first.end) {
       // (masked pairs for some wave; a query that is not finite has made its LSE, a dO its delta, NaN or infinite)
       if (__syncthreads_or(tile_non_finite<TL, T>(q_lds[buf]) | tile_non_finite<TL, T>(do_lds[buf]))) {
         add_non_finite<TL, false>(dk, q_lds[buf], g, keep);
@@ -256,31 +278,29 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
         __syncthreads();
       }
     }
-    if (idle || q0 + QT <= k0 || q0 >= last_end) continue;
-    const bool whole = q0 >= k0 + 31 && q0 + QT <= first_end;
-    const char* qt = q_lds[buf];
-    const char* dot = do_lds[buf];
-    f32x16 s{}, dp{};
-#pragma unroll
-    for (int i = 0; i < NS; ++i) s = A::mma(TL::row(qt, lk, i, g), kf[i], s);
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      if constexpr (kValuesInLds) dp = A::mma(TL::row(dot, lk, i, g), TL::row(v_lds[wave], lk, i, g), dp);
-      else dp = A::mma(TL::row(dot, lk, i, g), vf[i], dp);
-    }
+    if (idle || q0 + QT <= k0 || q0 >= last_end) return;
+    // scores and dO.v with -LSE / c1 and -delta in the sums; rows kappa(g, 4 q ..) are consecutive
+    f32x16 s, dp;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      // rows kappa(g, 4 q ..) are consecutive
       const f32x4 lse = *reinterpret_cast<const f32x4*>(&lse_lds[buf][8 * q + 4 * g]);
       const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_lds[buf][8 * q + 4 * g]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 4 * q + i;
-        s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, -lse[i]));
-        dp[j] = s[j] * (dp[j] - delta[i]);
-      }
+      for (int i = 0; i < 4; ++i) s[4 * q + i] = lse[i], dp[4 * q + i] = delta[i];
     }
-    if (!whole) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) s = A::mma(rd.row(q_lds[buf], 0, i), kf[i], s);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      if constexpr (kValuesInLds) dp = A::mma(rd.row(do_lds[buf], 0, i), rv.row(TL::k16 ? v_lds[0] : v_lds[wave], 0, i), dp);
+      else dp = A::mma(rd.row(do_lds[buf], 0, i), vf[i], dp);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      s[j] = __builtin_amdgcn_exp2f(s[j] * c1);
+      dp[j] *= s[j];
+    }
+    if (!(q0 >= k0 + 31 && q0 + QT <= first_end)) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const bool pair = keep(kappa(g, j));
@@ -293,9 +313,19 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int d = 0; d < NDT; ++d) {
-        dv[d] = A::mma(TL::transposed(dot, 16 * m, 32 * d, lane), p[m], dv[d]);
-        dk[d] = A::mma(TL::transposed(qt, 16 * m, 32 * d, lane), ds[m], dk[d]);
+        dv[d] = A::mma(rd.col(do_lds[buf], m, d), p[m], dv[d]);
+        dk[d] = A::mma(rd.col(q_lds[buf], m, d), ds[m], dk[d]);
       }
+  };
+  for (int h = h0, t = t0;;) {
+    auto next = [&] {
+      if (++t > t1) t = t0, ++h;
+      return h < h1;
+    };
+    step(t, std::integral_constant<int, 0>{});
+    if (!next()) break;
+    step(t, std::integral_constant<int, 1>{});
+    if (!next()) break;
   }
   if (!valid) return;
   const float scale = a.flip ? -a.scale : a.scale;
@@ -314,6 +344,48 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   for (int d = 0; d < NDT; ++d) {
     if (a.dk) store_columns<T>(to_k, 32 * d, a.key_size, g, dk[d], scale);
     if (a.dv) store_columns<T>(to_v, 32 * d, a.value_size, g, dv[d], 1.f);
+  }
+}
+
+// Blocks of packed sequences by their work, the heaviest first: [blocks] for blocks of queries (tiles of keys up to the
+// block's last), then [blocks] for blocks of keys (tiles of queries to the end of the last key's sequence).  A
+// counting sort by blocks of 128 tokens; equal ones in any order.
+__global__ __launch_bounds__(1024) void causal_order_kernel(CausalArgs a, int32_t* order) {
+  __shared__ int start[kMaxOrder + 1];
+  for (int side = 0; side < 2; ++side) {
+    for (int i = threadIdx.x; i <= a.blocks; i += 1024) start[i] = 0;
+    __syncthreads();
+    auto weight = [&](int block) {
+      const int block0 = block * kBlock, block1 = std::min(block0 + kBlock, (int)a.length) - 1, token = side ? block1 : block0;
+      int lo = 0, hi = a.sequences + 1;  // the first bound above the token
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (bound(a, mid, a.length) > token) hi = mid;
+        else lo = mid + 1;
+      }
+      const Span s = span_at(a, token, lo);
+      const int tokens = side ? std::max(s.end, block1 + 1) - block0 : block1 + 1 - std::min(s.start, block0);
+      return (tokens + kBlock - 1) / kBlock;  // 1 .. blocks
+    };
+    for (int i = threadIdx.x; i < a.blocks; i += 1024) atomicAdd(&start[a.blocks - weight(i)], 1);
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      // where each weight's blocks begin: a scan, 64 at a time
+      int sum = 0;
+      for (int i = 0; i < a.blocks; i += 64) {
+        const int at = i + (int)threadIdx.x, own = at < a.blocks ? start[at] : 0;
+        int x = own;
+        for (int d = 1; d < 64; d *= 2) {
+          const int y = __shfl_up(x, d);
+          if ((int)threadIdx.x >= d) x += y;
+        }
+        if (at < a.blocks) start[at] = sum + x - own;
+        sum += __shfl(x, 63);
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.blocks; i += 1024) order[side * a.blocks + atomicAdd(&start[a.blocks - weight(i)], 1)] = i;
+    __syncthreads();
   }
 }
 
@@ -336,6 +408,17 @@ __global__ __launch_bounds__(256) void causal_parts_kernel(const float* parts, v
 }  // namespace
 }  // namespace causal
 
+// Whether blocks of packed sequences are put in order first (a launch of some microseconds): where there are more
+// workgroups than places on the chip, so that a heavy block that starts late would be waited for.
+bool causal_ordered(const oops_causal_geometry& g) {
+  const int64_t blocks = (g.length + causal::kBlock - 1) / causal::kBlock;
+  return blocks <= causal::kMaxOrder && blocks * g.batch * g.heads > 512;
+}
+hipError_t launch_causal_order(const CausalArgs& a, int32_t* order, hipStream_t stream) {
+  hipLaunchKernelGGL(causal::causal_order_kernel, dim3(1), dim3(1024), 0, stream, a, order);
+  return hipGetLastError();
+}
+
 // Parts of a group's query heads: workgroups for every CU's two places twice over, so that the heavy blocks (the first
 // keys, paired with every query) find light ones to even them out.
 int causal_grad_parts(const oops_causal_geometry& g) {
@@ -346,17 +429,17 @@ int causal_grad_parts(const oops_causal_geometry& g) {
 
 hipError_t launch_causal_backward(int dtype, const CausalArgs& a, hipStream_t stream) {
   if (a.length == 0 || a.batch == 0) return hipSuccess;
-  const uint32_t blocks = (uint32_t)((a.length + causal::kBlock - 1) / causal::kBlock);
+  const uint32_t blocks = (uint32_t)a.blocks;
   const bool wide = a.key_size > 64 || a.value_size > 64;
   const dim3 grid_q(blocks * (uint32_t)(a.batch * a.heads)), grid_kv(blocks * (uint32_t)(a.batch * a.kv_heads * a.parts));
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    if (wide) hipLaunchKernelGGL((causal::causal_grad_query_kernel<T, 128>), grid_q, dim3(256), 0, stream, a, blocks);
-    else hipLaunchKernelGGL((causal::causal_grad_query_kernel<T, 64>), grid_q, dim3(256), 0, stream, a, blocks);
+    if (wide) hipLaunchKernelGGL((causal::causal_grad_query_kernel<T, 128>), grid_q, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((causal::causal_grad_query_kernel<T, 64>), grid_q, dim3(256), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || (!a.dk && !a.dv)) return e;
-    if (wide) hipLaunchKernelGGL((causal::causal_grad_key_value_kernel<T, 128>), grid_kv, dim3(256), 0, stream, a, blocks);
-    else hipLaunchKernelGGL((causal::causal_grad_key_value_kernel<T, 64>), grid_kv, dim3(256), 0, stream, a, blocks);
+    if (wide) hipLaunchKernelGGL((causal::causal_grad_key_value_kernel<T, 128>), grid_kv, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((causal::causal_grad_key_value_kernel<T, 64>), grid_kv, dim3(256), 0, stream, a);
     e = hipGetLastError();
     auto add = [&](const float* parts, void* out, const int64_t(&s)[3], int size) {
       const int64_t cells = a.batch * a.kv_heads * a.length * size;

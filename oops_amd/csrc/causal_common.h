@@ -7,10 +7,13 @@
 // registers are the other operand of the next product as they stand, if the
 // tile in LDS is read in the same order (tr_frag).
 //
-// Tiles of KT rows (64 of 16 bits, 32 of float32) go from memory straight to
-// LDS in 16-byte pieces.  Piece c of row r is kept in place c ^ swizzle(r): 16
-// lanes that read the same piece of 16 rows, and the 8 lanes groups of a
-// transposed read (32 bytes of each of 8 rows), meet 16 different bank groups.
+// Tiles of 32 or 64 rows go from memory straight to LDS in 16-byte pieces, a
+// kilobyte at a time (4 rows of 128 elements of 16 bits, 8 of 64).  Inside it a
+// row's 64-byte windows change places by the row's lower bits, and kilobytes lie 16
+// or 32 bytes more than their size apart: 16 lanes that read the same piece of 16
+// rows meet 16 different groups of four banks, and so do the 4 rows x 64 bytes of a
+// transposed read.  A lane's addresses are then two or four registers and constants,
+// which the instructions hold themselves.
 #pragma once
 #include "attn_fast_common.h"
 #include "decoder_kernels.h"
@@ -19,6 +22,9 @@ namespace oops {
 namespace causal {
 
 using fast::kOut;
+
+constexpr int kBlock = 128;      // queries, or keys, of a workgroup
+constexpr int kMaxOrder = 8192;  // blocks that are put in order by their work
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
@@ -42,27 +48,56 @@ template <typename T> using Frag = typename Att<T>::Frag;
 template <typename T, int DP, int ROWS = Att<T>::kRows>
 struct Tile {
   static constexpr int kRows = ROWS;
-  static constexpr int kBytes = kRows * DP * (int)sizeof(T);
-  static constexpr int kPieces = DP * (int)sizeof(T) / 16;          // of a row
-  static constexpr int kLoads = kRows * kPieces / 256;              // of a wave, four waves a tile
-  static constexpr int kRowsPerLoad = 64 / kPieces;
   static constexpr bool k16 = sizeof(T) == 2;
+  static constexpr int kRowBytes = DP * (int)sizeof(T);
+  static constexpr int kPieces = kRowBytes / 16;                  // of a row
+  static constexpr int kChunks = kRows * kRowBytes / 1024;        // kilobytes
+  static constexpr int kLoads = kChunks / 4;                      // of a wave, four waves a tile
+  static constexpr int kPitch = 1024 + (!k16 ? 0 : DP == 128 ? 16 : 32);  // between kilobytes
+  static constexpr int kBytes = kChunks * kPitch;
+  static constexpr int kWindows = DP / 32;
 
-  // (the lower bit of the place changes last: 32-byte pairs of 8 rows lie in 8 different pairs of bank groups;
-  // float32 fragments are such pairs)
-  static __device__ __forceinline__ int swizzle(int r) {
-    if constexpr (!k16) return (kPieces == 16 ? r & 7 : r & 15) << 1;
-    else if constexpr (kPieces == 16) return ((r & 7) << 1) | ((r >> 3) & 1);
-    else return (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+  // piece of row r that lies at place p of the row (its own inverse)
+  static __device__ __forceinline__ int placed(int r, int p) {
+    if constexpr (!k16) return p ^ ((kPieces == 16 ? r & 7 : r & 15) << 1);  // (32-byte pairs, which float32 fragments are)
+    else if constexpr (DP == 128) return p ^ ((r & 3) << 2);
+    else return p ^ (((r >> 1) & 1) << 2) ^ ((r >> 2) & 1);
   }
-  static __device__ __forceinline__ int at(int r, int piece) { return r * (DP * (int)sizeof(T)) + ((piece ^ swizzle(r)) << 4); }
+  static __device__ __forceinline__ int at(int r, int piece) {
+    constexpr int n = 1024 / kRowBytes;  // rows of a kilobyte
+    return r / n * kPitch + r % n * kRowBytes + (placed(r, piece) << 4);
+  }
+  // the n-th 16-byte piece in the order of places
+  static __device__ __forceinline__ int nth(int n) { return (n >> 6) * kPitch + (n & 63) * 16; }
+  static __device__ __forceinline__ float element(const char* tile, int r, int c) {
+    constexpr int n = 16 / (int)sizeof(T);
+    return (float)*reinterpret_cast<const T*>(tile + at(r, c / n) + c % n * (int)sizeof(T));
+  }
+};
 
-  // elements 16 s + 8 g .. + 7 of row r
-  static __device__ __forceinline__ Frag<T> row(const char* tile, int r, int s, int g) {
-    if constexpr (k16) {
-      return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const uint4*>(tile + at(r, 2 * s + g)));
+// A lane's fragments of tiles
+template <typename T, int DP>
+struct Reads {
+  using TL = Tile<T, DP, 32>;  // (32 rows are a multiple of every pattern)
+  static constexpr int kStep16 = 16 / (1024 / TL::kRowBytes) * TL::kPitch;  // bytes of 16 rows
+  int row_at[TL::kWindows], col_at[TL::kWindows], lane;
+  __device__ __forceinline__ void init(int lane_) {
+    lane = lane_;
+    if constexpr (TL::k16) {
+      const int lq = lane & 31, g = lane >> 5, j = lane & 15, half = lane >> 4 & 1, r = 4 * g + (j >> 2);
+#pragma unroll
+      for (int w = 0; w < TL::kWindows; ++w) {
+        row_at[w] = TL::at(lq, 4 * w + g);
+        col_at[w] = TL::at(r, 4 * w + 2 * half + ((j & 3) >> 1)) + (j & 1) * 8;
+      }
+    }
+  }
+  // elements 16 s + 8 g .. + 7 of row 32 u + lane % 32
+  __device__ __forceinline__ Frag<T> row(const char* tile, int u, int s) const {
+    if constexpr (TL::k16) {
+      return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const uint4*>(tile + row_at[s >> 1] + (s & 1) * 32 + 2 * u * kStep16));
     } else {
-      const int p = at(r, 4 * s + 2 * g);
+      const int p = TL::at(lane & 31, 4 * s + 2 * (lane >> 5)) + 2 * u * kStep16;
       f32x8 f;
       const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + p), hi = *reinterpret_cast<const f32x4*>(tile + p + 16);
 #pragma unroll
@@ -70,27 +105,21 @@ struct Tile {
       return f;
     }
   }
-  static __device__ __forceinline__ float element(const char* tile, int r, int c) {
-    constexpr int n = 16 / (int)sizeof(T);
-    return (float)*reinterpret_cast<const T*>(tile + at(r, c / n) + c % n * (int)sizeof(T));
-  }
-  // column c0 + lane % 32 of rows r0 + kappa(g, 0..7) (r0 a multiple of 16, c0 of 32)
-  static __device__ __forceinline__ Frag<T> transposed(const char* tile, int r0, int c0, int lane) {
-    if constexpr (k16) {
-      const int j = lane & 15, grp = lane >> 4;
-      const int r = ((grp >> 1) << 2) + (j >> 2), col = c0 + ((grp & 1) << 4) + ((j & 3) << 2);
-      const char* lo_at = tile + r0 * DP * 2 + at(r, col >> 3) + (col & 7) * 2;
-      const char* hi_at = tile + r0 * DP * 2 + at(r + 8, col >> 3) + (col & 7) * 2;
-      const s16x4 lo = lds_read_tr4(lo_at), hi = lds_read_tr4(hi_at);
+  // column 32 t + lane % 32 of rows 16 m + kappa(g, 0..7)
+  __device__ __forceinline__ Frag<T> col(const char* tile, int m, int t) const {
+    if constexpr (TL::k16) {
+      constexpr int n = 1024 / TL::kRowBytes;
+      const char* at = tile + col_at[t] + m * kStep16;
+      const s16x4 lo = lds_read_tr4(at), hi = lds_read_tr4(at + 8 / n * TL::kPitch);
       typedef short s16x8 __attribute__((ext_vector_type(8)));
       const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       return __builtin_bit_cast(Frag<T>, v);
     } else {
-      const int col = c0 + (lane & 31), g = lane >> 5;
+      const int c = 32 * t + (lane & 31), g = lane >> 5;
       f32x8 f;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        f[j] = *reinterpret_cast<const float*>(tile + r0 * DP * 4 + at(kappa(g, j), col >> 2) + (col & 3) * 4);
+        f[j] = *reinterpret_cast<const float*>(tile + m * kStep16 + TL::at(kappa(g, j), c >> 2) + (c & 3) * 4);
       return f;
     }
   }
@@ -108,29 +137,39 @@ __device__ __forceinline__ Rows rows_of(const void* p, const int64_t (&stride)[3
   return Rows{static_cast<const char*>(p) + (b * stride[0] + h * stride[1]) * (int64_t)sizeof(T),
               stride[2] * (int64_t)sizeof(T), size * (int)sizeof(T), count};
 }
-// Rows row0 .. of `r` to the tile at `lds`; rows behind the last and columns behind the size are zeros.  The
-// resource starts at the tile's first row, so that offsets stay small however long the operand is (the host
-// refuses row pitches of 2^24 bytes and more).
+// Rows of an operand to a tile, tile after tile; rows behind the last and columns behind the size are zeros.  The
+// resource starts at the tile's first row, so that offsets stay small however long the operand is (the host refuses row
+// pitches of 2^24 bytes and more).
 template <typename T, int DP, int ROWS = Att<T>::kRows>
 struct Loader {
   using TL = Tile<T, DP, ROWS>;
   uint32_t off[TL::kLoads];
-  int wave;
+  const char* base;  // of the next tile
+  int64_t step;
+  int left, bytes, pitch, wave;  // left: rows from there on
   __device__ __forceinline__ void init(const Rows& r, int wave_, int lane) {
     wave = wave_;
+    bytes = r.bytes;
+    pitch = (int)r.pitch;
+    step = r.pitch * ROWS;
 #pragma unroll
     for (int i = 0; i < TL::kLoads; ++i) {
-      const int row = (wave * TL::kLoads + i) * TL::kRowsPerLoad + lane / TL::kPieces;
-      const int col = ((lane % TL::kPieces) ^ TL::swizzle(row)) * 16;
-      off[i] = col < r.bytes ? (uint32_t)(row * (int)r.pitch + col) : kOut;
+      const int n = (wave * TL::kLoads + i) * 64 + lane, row = n / TL::kPieces;
+      const int col = TL::placed(row, n % TL::kPieces) * 16;
+      off[i] = col < r.bytes ? (uint32_t)(row * pitch + col) : kOut;
     }
   }
-  __device__ __forceinline__ void load(const Rows& r, int64_t row0, const char* lds) const {
-    const int64_t left = r.count - row0;
-    const int n = left < TL::kRows ? (left > 0 ? (int)left : 0) : TL::kRows;
-    const fast::u32x4 rs = fast::rsrc_words(r.base + row0 * r.pitch, n > 0 ? (uint32_t)((n - 1) * (int)r.pitch + r.bytes) : 0u);
+  __device__ __forceinline__ void seek(const Rows& r, int row0) {
+    base = r.base + row0 * r.pitch;
+    left = (int)r.count - row0;
+  }
+  __device__ __forceinline__ void next(const char* lds) {
+    const int n = left < ROWS ? left : ROWS;
+    const fast::u32x4 rs = fast::rsrc_words(base, n > 0 ? (uint32_t)((n - 1) * pitch + bytes) : 0u);
 #pragma unroll
-    for (int i = 0; i < TL::kLoads; ++i) fast::dma16_asm(rs, lds + (wave * TL::kLoads + i) * 1024, off[i], 0);
+    for (int i = 0; i < TL::kLoads; ++i) fast::dma16_asm(rs, lds + (wave * TL::kLoads + i) * TL::kPitch, off[i], 0);
+    base += step;
+    left -= ROWS;
   }
 };
 
@@ -161,24 +200,51 @@ __device__ __forceinline__ int64_t bound(const CausalArgs& a, int i, int64_t len
   const int64_t v = a.offsets_i64 ? static_cast<const int64_t*>(a.offsets)[i] : static_cast<const int32_t*>(a.offsets)[i];
   return v < 0 ? 0 : v > length ? length : v;
 }
+// Numbers of bounds at or before tokens i[0 .. K-1] (the same for all lanes of the wave): 64 bounds at a time, loads that
+// do not wait for each other.
+template <int K>
+__device__ __forceinline__ void bounds_before(const CausalArgs& a, const int (&i)[K], int (&count)[K]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 0; k < K; ++k) count[k] = 0;
+  for (int n = 0; n <= a.sequences; n += 64) {
+    const bool there = n + lane <= a.sequences;
+    const int64_t v = there ? bound(a, n + lane, a.length) : 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) count[k] += __builtin_popcountll(__ballot(there && v <= i[k]));
+  }
+}
 // The sequence that holds token i: [start, end); a token of none has start = i + 1 and end = i.
 struct Span {
   int start, end;
 };
-__device__ __forceinline__ Span span_of(const CausalArgs& a, int i) {
-  const int length = (int)a.length;
-  if (!a.offsets) return Span{0, length};
-  // the first bound above i
-  int lo = 0, hi = a.sequences + 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (bound(a, mid, length) > i) hi = mid;
-    else lo = mid + 1;
-  }
-  if (lo == 0 || lo > a.sequences) return Span{i + 1, i};
-  // (bounds that do not increase: what is read stays inside the operands)
-  const int start = (int)bound(a, lo - 1, length), end = (int)bound(a, lo, length);
+// (bounds that do not increase: what is read stays inside the operands)
+__device__ __forceinline__ Span span_at(const CausalArgs& a, int i, int before) {
+  if (before == 0 || before > a.sequences) return Span{i + 1, i};
+  const int start = (int)bound(a, before - 1, a.length), end = (int)bound(a, before, a.length);
   return Span{start < i ? start : i, end > i ? end : i + 1};
+}
+// For a workgroup's block of tokens [first, last] and this wave's [w0, w1], of which this lane has `token`
+struct Spans {
+  Span first, last, own;
+};
+__device__ __forceinline__ Spans spans_of(const CausalArgs& a, int first, int last, int w0, int w1, int token) {
+  const int length = (int)a.length;
+  if (!a.offsets) return Spans{{0, length}, {0, length}, {0, length}};
+  const int at[3] = {first, last, w0};
+  int n[3];
+  bounds_before<3>(a, at, n);
+  Spans s{span_at(a, first, n[0]), span_at(a, last, n[1]), {token + 1, token}};
+  // the wave's tokens: one sequence after the other
+  int before = n[2], lo = before ? (int)bound(a, before - 1, length) : 0;
+  while (true) {
+    const int hi = before <= a.sequences ? (int)bound(a, before, length) : length;
+    if (before > 0 && before <= a.sequences && token >= lo && token < hi) s.own = Span{lo, hi};
+    if (hi > w1 || before > a.sequences) break;
+    lo = hi;
+    ++before;
+  }
+  return s;
 }
 
 template <typename T>
@@ -229,8 +295,8 @@ template <typename TL, typename T>
 __device__ __forceinline__ bool tile_non_finite(const char* tile) {
   bool bad = false;
 #pragma unroll 2
-  for (int i = 0; i < TL::kBytes / 4096; ++i) {
-    const uint4 u = reinterpret_cast<const uint4*>(tile)[i * 256 + threadIdx.x];
+  for (int i = 0; i < TL::kChunks / 4; ++i) {
+    const uint4 u = *reinterpret_cast<const uint4*>(tile + TL::nth(i * 256 + threadIdx.x));
     bad |= ((u.x ^ finite_word<T>(u.x)) | (u.y ^ finite_word<T>(u.y)) | (u.z ^ finite_word<T>(u.z)) | (u.w ^ finite_word<T>(u.w))) != 0;
   }
   return bad;
@@ -241,8 +307,8 @@ __device__ __forceinline__ uint64_t rows_non_finite(const char* tile, uint32_t* 
   if (threadIdx.x < 2) words[threadIdx.x] = 0;
   __syncthreads();
 #pragma unroll 1
-  for (int i = 0; i < TL::kBytes / 4096; ++i) {
-    const uint4 u = reinterpret_cast<const uint4*>(tile)[i * 256 + threadIdx.x];
+  for (int i = 0; i < TL::kChunks / 4; ++i) {
+    const uint4 u = *reinterpret_cast<const uint4*>(tile + TL::nth(i * 256 + threadIdx.x));
     const int row = (i * 256 + (int)threadIdx.x) / TL::kPieces;
     if (((u.x ^ finite_word<T>(u.x)) | (u.y ^ finite_word<T>(u.y)) | (u.z ^ finite_word<T>(u.z)) | (u.w ^ finite_word<T>(u.w))) != 0)
       atomicOr(&words[row >> 5], 1u << (row & 31));
@@ -253,8 +319,8 @@ __device__ __forceinline__ uint64_t rows_non_finite(const char* tile, uint32_t* 
 template <typename TL, typename T>
 __device__ __forceinline__ void clean_tile(char* tile) {
 #pragma unroll 1
-  for (int i = 0; i < TL::kBytes / 4096; ++i) {
-    uint4& u = reinterpret_cast<uint4*>(tile)[i * 256 + threadIdx.x];
+  for (int i = 0; i < TL::kChunks / 4; ++i) {
+    uint4& u = *reinterpret_cast<uint4*>(tile + TL::nth(i * 256 + threadIdx.x));
     u = make_uint4(finite_word<T>(u.x), finite_word<T>(u.y), finite_word<T>(u.z), finite_word<T>(u.w));
   }
 }
@@ -307,13 +373,13 @@ __device__ __forceinline__ void store_columns(char* row, int d0, int size, int g
   }
 }
 
-// Workgroup `id` of `blocks` blocks of `heads` (batch, head) pairs: the longest blocks first, and, where the heads can
-// be dealt evenly, those of one XCD (workgroups id % 8) next to each other, so that heads that share keys meet in one
-// L2.
+// Workgroup `id` of `heads` (batch, head) pairs: the longest blocks first, and, where the heads can be dealt evenly, those
+// of one XCD (workgroups id % 8) next to each other, so that heads that share keys meet in one L2.  rank counts the
+// blocks from the heaviest.
 struct Work {
-  int head, block;  // block counted from the heaviest
+  int head, rank;
 };
-__device__ __forceinline__ Work work_of(uint32_t id, uint32_t heads, uint32_t /*blocks*/) {
+__device__ __forceinline__ Work work_of(uint32_t id, uint32_t heads) {
   if (heads % kNumXcds == 0) {
     const uint32_t per = heads / kNumXcds, x = id % kNumXcds, r = id / kNumXcds;
     return Work{(int)(x * per + r % per), (int)(r / per)};

@@ -21,7 +21,8 @@ struct CausalArgs {
   const void *q, *k, *v, *offsets, *dout;
   void *out, *low, *dq, *dk, *dv;
   float* lse;          // (batch, heads, length), log2 units
-  float* delta;        // the same shape
+  float *neg_lse, *neg_delta;  // the same shape: -lse over the scores' factor, -delta
+  const int32_t* order;        // blocks of queries, then of keys, the heaviest first (NULL: by their place)
   float *dk_parts, *dv_parts;
   int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], do_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
   int64_t batch, length;
@@ -29,7 +30,10 @@ struct CausalArgs {
   int32_t flip;        // the scale is negative: `scale` is its magnitude, and the scores' sign is changed
   float scale;
   int32_t parts;       // of the query heads of a group in the key/value gradient
+  int32_t blocks;      // of 128 tokens
 };
+bool causal_ordered(const oops_causal_geometry& g);
+hipError_t launch_causal_order(const CausalArgs& a, int32_t* order, hipStream_t stream);
 hipError_t launch_causal_forward(int dtype, const CausalArgs& a, hipStream_t stream);
 int causal_grad_parts(const oops_causal_geometry& g);
 hipError_t launch_causal_backward(int dtype, const CausalArgs& a, hipStream_t stream);
