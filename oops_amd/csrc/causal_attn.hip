@@ -105,6 +105,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 #pragma unroll
       for (int i = 0; i < NS; ++i) s[u] = A::mma(rd.row(k_lds[buf], u, i), qf[i], s[u]);
     }
+    if constexpr (TL::k16) interleave<6, SUB * NS, 1>();
     if (k0 < last_start || k0 + KT - 1 > q0) {
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
@@ -142,6 +143,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
     for (int m = 0; m < KT / 16; ++m)
 #pragma unroll
       for (int d = 0; d < NDT; ++d) o[d] = A::mma(rd.col(v_lds[buf], m, d), p[m], o[d]);
+    if constexpr (TL::k16) {
+      __builtin_amdgcn_sched_group_barrier(0x002, 12, 0);
+      interleave<8, NDT * (KT / 16), 2, 5>();
+    }
   };
   for (int t = t0;;) {
     step(t, std::integral_constant<int, 0>{});

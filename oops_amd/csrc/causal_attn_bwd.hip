@@ -132,6 +132,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
       for (int i = 0; i < NS; ++i) s = A::mma(rd.row(k_lds[buf], u, i), qf[i], s);
 #pragma unroll
       for (int i = 0; i < NS; ++i) dp = A::mma(rd.row(v_lds[buf], u, i), dof[i], dp);
+      if constexpr (TL::k16) interleave<6, 2 * NS, 1>();
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, -lse)) * (dp[j] - delta);
       if (lost) {
@@ -149,6 +150,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
       for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int d = 0; d < NDT; ++d) dq[d] = A::mma(rd.col(k_lds[buf], 2 * u + m, d), ds[m], dq[d]);
+      if constexpr (TL::k16) interleave<8, 2 * NDT, 2>();
     }
   };
   for (int t = t0;;) {
@@ -295,6 +297,11 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
       if constexpr (kValuesInLds) dp = A::mma(rd.row(do_lds[buf], 0, i), rv.row(TL::k16 ? v_lds[0] : v_lds[wave], 0, i), dp);
       else dp = A::mma(rd.row(do_lds[buf], 0, i), vf[i], dp);
     }
+    if constexpr (TL::k16) {
+      // (the statistics' eight reads first)
+      interleave<12, NS, 1>();
+      interleave<kValuesInLds ? 2 : 0, NS, kValuesInLds ? 2 : 1>();
+    }
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       s[j] = __builtin_amdgcn_exp2f(s[j] * c1);
@@ -316,6 +323,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
         dv[d] = A::mma(rd.col(do_lds[buf], m, d), p[m], dv[d]);
         dk[d] = A::mma(rd.col(q_lds[buf], m, d), ds[m], dk[d]);
       }
+    if constexpr (TL::k16) interleave<8, 4 * NDT, 2>();
   };
   for (int h = h0, t = t0;;) {
     auto next = [&] {
@@ -423,7 +431,7 @@ hipError_t launch_causal_order(const CausalArgs& a, int32_t* order, hipStream_t 
 // keys, paired with every query) find light ones to even them out.
 int causal_grad_parts(const oops_causal_geometry& g) {
   const int64_t blocks = (g.length + causal::kBlock - 1) / causal::kBlock * g.batch * g.kv_heads;
-  const int64_t want = blocks > 0 ? (1024 + blocks - 1) / blocks : 1;
+  const int64_t want = blocks > 0 ? (2048 + blocks - 1) / blocks : 1;
   return (int)std::min<int64_t>(want, g.heads / g.kv_heads);
 }
 

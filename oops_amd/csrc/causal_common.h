@@ -195,6 +195,19 @@ __device__ __forceinline__ void load_row(Frag<T> (&f)[DP / 16], const Rows& r, i
   }
 }
 
+// The order of a block's instructions: `ahead` LDS reads first, then after each of `products` matrix instructions `reads`
+// more and `vector` vector ones.  (Left alone, the compiler reads two fragments, waits for both and multiplies.)
+template <int AHEAD, int PRODUCTS, int READS, int VECTOR = 0>
+__device__ __forceinline__ void interleave() {
+  if constexpr (AHEAD > 0) __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < PRODUCTS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    if constexpr (VECTOR > 0) __builtin_amdgcn_sched_group_barrier(0x002, VECTOR, 0);
+  }
+}
+
 // ---- packed sequences: bounds offsets[0 .. n] along the tokens
 __device__ __forceinline__ int64_t bound(const CausalArgs& a, int i, int64_t length) {
   const int64_t v = a.offsets_i64 ? static_cast<const int64_t*>(a.offsets)[i] : static_cast<const int32_t*>(a.offsets)[i];
