@@ -107,10 +107,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
     }
     if constexpr (TL::k16) interleave<6, SUB * NS, 1>();
     if (k0 < last_start || k0 + KT - 1 > q0) {
+      const uint32_t from = here(k0 + 4 * g - start), far = empty ? 0u : reach + 1;
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[u][j] = keep(32 * u + kappa(g, j)) ? s[u][j] : kNegInf;
+        for (int j = 0; j < 16; ++j) s[u][j] = from + 32 * u + kappa(0, j) < far ? s[u][j] : kNegInf;
     }
     float mx = s[0][0];
 #pragma unroll

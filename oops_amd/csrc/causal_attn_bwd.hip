@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   fast::vmem_wait<0>();  // (the rows, before loads that the compiler does not count)
   kl.next(k_lds[0]);
   vl.next(v_lds[0]);
-  auto step = [&](int t, auto buffer) {
+  auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
     constexpr int buf = decltype(buffer)::value;
     const int k0 = t * KT;
     fast::vmem_wait<0>();
@@ -142,8 +142,9 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
         for (int j = 0; j < 16; ++j) s[j] = rows & (1u << kappa(0, j)) ? 0.f * lse : s[j];
       }
       if (!whole) {
+        const uint32_t from = here(k0 + 4 * g - start), far = empty ? 0u : reach + 1;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = keep(32 * u + kappa(g, j)) ? s[j] : 0.f;
+        for (int j = 0; j < 16; ++j) s[j] = from + 32 * u + kappa(0, j) < far ? s[j] : 0.f;
       }
       const Frag<T> ds[2] = {pack<T>(s, 0), pack<T>(s, 1)};
 #pragma unroll
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   }
   seek();
   load(std::integral_constant<int, 0>{});
-  auto step = [&](int t, auto buffer) {
+  auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
     constexpr int buf = decltype(buffer)::value;
     const int q0 = t * QT;
     fast::vmem_wait<0>();
@@ -308,9 +309,10 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
       dp[j] *= s[j];
     }
     if (!(q0 >= k0 + 31 && q0 + QT <= first_end)) {
+      const uint32_t from = here(q0 + 4 * g - key);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const bool pair = keep(kappa(g, j));
+        const bool pair = from + kappa(0, j) < width;
         s[j] = pair ? s[j] : 0.f;
         dp[j] = pair ? dp[j] : 0.f;
       }

@@ -164,7 +164,7 @@ struct Loader {
     left = (int)r.count - row0;
   }
   __device__ __forceinline__ void next(const char* lds) {
-    const int n = left < ROWS ? left : ROWS;
+    const int n = left < ROWS ? left : ROWS;  // (none or fewer behind the last row: the resource is empty)
     const fast::u32x4 rs = fast::rsrc_words(base, n > 0 ? (uint32_t)((n - 1) * pitch + bytes) : 0u);
 #pragma unroll
     for (int i = 0; i < TL::kLoads; ++i) fast::dma16_asm(rs, lds + (wave * TL::kLoads + i) * TL::kPitch, off[i], 0);
@@ -195,8 +195,8 @@ __device__ __forceinline__ void load_row(Frag<T> (&f)[DP / 16], const Rows& r, i
   }
 }
 
-// The order of a block's instructions: `ahead` LDS reads first, then after each of `products` matrix instructions `reads`
-// more and `vector` vector ones.  (Left alone, the compiler reads two fragments, waits for both and multiplies.)
+// The order of a block's instructions: AHEAD LDS reads first, then after each of PRODUCTS matrix instructions READS more,
+// VECTOR vector ones and EXP exponentials.  (Left alone, the compiler reads two fragments, waits for both and multiplies.)
 template <int AHEAD, int PRODUCTS, int READS, int VECTOR = 0>
 __device__ __forceinline__ void interleave() {
   if constexpr (AHEAD > 0) __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
@@ -268,6 +268,12 @@ __device__ __forceinline__ Frag<T> pack(const f32x16& x, int m) {
   return f;
 }
 
+// x, as a value that the compiler does not know more about: what is computed from it stays where it is written (it would
+// else keep sixteen sums in registers, or in scratch, for masked tiles to come)
+__device__ __forceinline__ uint32_t here(int x) {
+  asm volatile("" : "+v"(x));
+  return (uint32_t)x;
+}
 // sum + the elements of f (of 16 bits: the rounded ones, two a step)
 template <typename T>
 __device__ __forceinline__ float add_elements(const Frag<T>& f, float sum) {
