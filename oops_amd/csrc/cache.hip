@@ -192,6 +192,7 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(CacheArgs a) {
 
 constexpr int kTile = 32;      // tokens of a wave's step
 constexpr int kHeadTile = 16;  // query heads of a workgroup
+constexpr int64_t kMaxSplits = 256;
 
 struct DecodeArgs {
   const void *query, *lengths;
@@ -201,6 +202,7 @@ struct DecodeArgs {
   float* parts;  // (batch, heads, splits, size + 2): O, maximum, sum (-1: no token)
   int64_t pages, batch, max_pages, q_batch, q_head;
   int32_t heads, kv_heads, group, tiles, page, lengths_i64, splits;
+  uint32_t page16, per16;  // a page in 16 tokens, and 2^32 over that, rounded down
   float scale;
 };
 
@@ -220,11 +222,13 @@ __device__ __forceinline__ void split(float x, __bf16 (&t)[N]) {
 }
 
 typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
-// a wave's tile as loaded: token lane % 16 of each half, 8 NS channels a lane
+// a wave's tile as loaded: token lane % 16 of each half, 8 NS channels a lane; the halves whose page is there
 template <int NS>
 struct Raw {
+  static constexpr int kScales = NS == 4 ? 1 : NS;
   uint32_t k[2][NS], v[2][NS];
-  uint32_t ks[2][NS == 4 ? 1 : NS], vs[2][NS == 4 ? 1 : NS];
+  uint32_t ks[2][kScales], vs[2][kScales];
+  bool have[2];
 };
 
 // eight codes to bfloat16, times the scale
@@ -248,7 +252,7 @@ __device__ __forceinline__ float sum_rows(float x) {
 }
 
 template <typename T, int NS>
-__global__ __launch_bounds__(kThreads) void cache_attn_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(DecodeArgs a) {
   constexpr int N = Terms<T>::N, D = 32 * NS, ND = D / 16;
   // channels of step s of lane group g: with four steps a lane's sixteen bytes lie together
   auto channel = [](int s, int g) { return NS == 4 ? 32 * g + 8 * s : 32 * s + 8 * g; };
@@ -263,9 +267,9 @@ __global__ __launch_bounds__(kThreads) void cache_attn_kernel(DecodeArgs a) {
   const int h = hk * a.group + tile_at * kHeadTile + c;  // this lane's query head
   const bool head_live = tile_at * kHeadTile + c < a.group;
 
-  int64_t count = a.lengths_i64 ? static_cast<const int64_t*>(a.lengths)[b] : static_cast<const int32_t*>(a.lengths)[b];
-  count = std::min<int64_t>(std::max<int64_t>(count, 0), a.max_pages * a.page);
-  const int steps = (int)((count + kTile - 1) / kTile), per = (steps + a.splits - 1) / a.splits;
+  const int64_t given = a.lengths_i64 ? static_cast<const int64_t*>(a.lengths)[b] : static_cast<const int32_t*>(a.lengths)[b];
+  const int count = (int)std::min<int64_t>(std::max<int64_t>(given, 0), a.max_pages * a.page);
+  const int steps = (count + kTile - 1) / kTile, per = (steps + a.splits - 1) / a.splits;
   const int from = split_at * per, to = std::min(steps, from + per);
 
   bf16x8 q[NS][N];
@@ -282,24 +286,36 @@ __global__ __launch_bounds__(kThreads) void cache_attn_kernel(DecodeArgs a) {
       }
   }
 
-  // page of the 16 tokens from t0, or -1
-  auto page_at = [&](int t0) -> int64_t {
-    if (t0 >= count) return -1;
-    const int64_t id = a.table[b * a.max_pages + t0 / a.page];
-    return id >= 0 && id < a.pages ? id : -1;
+  // 16 tokens: their page in the sequence and their place there, in units of 16 (the quotient is at most one short)
+  auto divided = [&](int t16, uint32_t& place) {
+    uint32_t n = __umulhi((uint32_t)t16, a.per16);
+    place = (uint32_t)t16 - n * a.page16;
+    if (place >= a.page16) ++n, place -= a.page16;
+    return n;
   };
-  auto load = [&](int step, Raw<NS>& r) {
+  // a tile's pages, or -1; read a step before they are used
+  const int32_t* table = a.table + b * a.max_pages;
+  auto pages_of = [&](int step, int32_t (&id)[2]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int t0 = step * kTile + 16 * i;
-      const int64_t id = page_at(t0);
+      uint32_t place;
+      const uint32_t n = divided(2 * step + i, place);
+      id[i] = step < to && step * kTile + 16 * i < count ? table[n] : -1;
+    }
+  };
+  auto load = [&](int step, const int32_t (&id)[2], Raw<NS>& r) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) r.k[i][s] = r.v[i][s] = 0;
 #pragma unroll
-      for (int s = 0; s < (NS == 4 ? 1 : NS); ++s) r.ks[i][s] = r.vs[i][s] = 127;
-      if (id < 0) continue;
+      for (int s = 0; s < Raw<NS>::kScales; ++s) r.ks[i][s] = r.vs[i][s] = 127;
+      r.have[i] = id[i] >= 0 && id[i] < a.pages;
+      if (!r.have[i]) continue;
+      uint32_t place;
+      divided(2 * step + i, place);
       // (places behind the last token lie in the page: what they hold is taken out below)
-      const int64_t row = ((id * a.kv_heads + hk) * 2) * a.page + t0 % a.page + c;
+      const int64_t row = ((int64_t)id[i] * a.kv_heads + hk) * 2 * a.page + place * 16 + c;
       const uint8_t* kc = a.codes + row * (D / 2);
       const uint8_t* vc = kc + (int64_t)a.page * (D / 2);
       const uint8_t* ks = a.scales + row * NS;
@@ -331,24 +347,26 @@ __global__ __launch_bounds__(kThreads) void cache_attn_kernel(DecodeArgs a) {
   char* mine = lds[wave];
 
   Raw<NS> raw;
-  if (from + wave < to) load(from + wave, raw);
+  int32_t id[2];
+  pages_of(from + wave, id);
+  load(from + wave, id, raw);
+  pages_of(from + wave + 4, id);
   for (int step = from + wave; step < to; step += 4) {
     Raw<NS> now = raw;
-    if (step + 4 < to) load(step + 4, raw);
-    const bool have[2] = {page_at(step * kTile) >= 0, page_at(step * kTile + 16) >= 0};
-    if (!have[0] && !have[1]) continue;
+    load(step + 4, id, raw);
+    pages_of(step + 8, id);
+    if (!now.have[0] && !now.have[1]) continue;
     seen = true;
-    const int left = (int)std::min<int64_t>(count - step * kTile, kTile);
-    // tokens of this lane that take part: key and value rows c + 16 i
+    const int left = std::min(count - step * kTile, kTile);
+    // values behind the last token (absent pages have zeros)
+    if (left < kTile)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bool live = have[i] && c + 16 * i < left;
-      if (!live) {
+      const bool live = c + 16 * i < left;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) now.v[i][s] = 0;
+      for (int s = 0; s < NS; ++s) now.v[i][s] = live ? now.v[i][s] : 0;
 #pragma unroll
-        for (int s = 0; s < (NS == 4 ? 1 : NS); ++s) now.vs[i][s] = 127;
-      }
+      for (int s = 0; s < Raw<NS>::kScales; ++s) now.vs[i][s] = live ? now.vs[i][s] : 127;
     }
     // V to LDS in bfloat16
 #pragma unroll
@@ -369,11 +387,11 @@ __global__ __launch_bounds__(kThreads) void cache_attn_kernel(DecodeArgs a) {
         for (int n = 0; n < N; ++n) st[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[s][n], st[i], 0, 0, 0);
       }
     }
-    if (left < kTile || !have[0] || !have[1]) {
+    if (left < kTile || !now.have[0] || !now.have[1]) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) st[i][r] = have[i] && 16 * i + 4 * g + r < left ? st[i][r] * c1 : kNegInf;
+        for (int r = 0; r < 4; ++r) st[i][r] = now.have[i] && 16 * i + 4 * g + r < left ? st[i][r] * c1 : kNegInf;
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i) st[i] *= c1;
@@ -460,35 +478,55 @@ __global__ __launch_bounds__(kThreads) void cache_attn_kernel(DecodeArgs a) {
   }
 }
 
-// The splits of one row, joined in order.
+// The splits of one row, joined: the parts' factors first (a part a lane), then O, four threads a channel, each every
+// fourth part, added in order.
 template <typename T>
-__global__ __launch_bounds__(128) void cache_join_kernel(const float* parts, void* out, int splits, int size) {
-  const int64_t row = blockIdx.x;
-  const float* p = parts + row * splits * (size + 2);
-  const int d = threadIdx.x;
-  float m = kNegInf, l = 0.f, x = 0.f;
-  bool any = false;
-  for (int s = 0; s < splits; ++s)
-    if (p[s * (size + 2) + size + 1] != -1.f) m = fmaxf(m, p[s * (size + 2) + size]), any = true;
-  if (d >= size) return;
-  for (int s = 0; s < splits; ++s) {
-    const float* f = p + s * (size + 2);
-    if (f[size + 1] == -1.f) continue;
-    const float by = m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(f[size] - m);
-    l = __builtin_fmaf(f[size + 1], by, l);
-    x = __builtin_fmaf(f[d], by, x);
+__global__ __launch_bounds__(512) void cache_join_kernel(const float* parts, void* out, int splits, int size) {
+  __shared__ float by[kMaxSplits], sums[4][128], total[2];
+  const float* p = parts + (int64_t)blockIdx.x * splits * (size + 2);
+  const int tid = threadIdx.x;
+  if (tid < 64) {
+    float m = kNegInf, l = 0.f;
+    bool any = false;
+    for (int s = tid; s < splits; s += 64) {
+      const float *f = p + s * (size + 2) + size;
+      if (f[1] != -1.f) m = fmaxf(m, f[0]), any = true;
+    }
+    for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+    for (int s = tid; s < splits; s += 64) {
+      const float *f = p + s * (size + 2) + size;
+      const float w = f[1] == -1.f ? 0.f : m == kNegInf ? 1.f : __builtin_amdgcn_exp2f(f[0] - m);
+      by[s] = w;
+      if (f[1] != -1.f) l = __builtin_fmaf(f[1], w, l);
+    }
+    for (int d = 32; d > 0; d /= 2) l += __shfl_xor(l, d);
+    if (tid == 0) total[0] = l;
+    const bool some = __any(any);
+    if (tid == 0) total[1] = some ? 1.f : 0.f;
   }
-  static_cast<T*>(out)[row * size + d] = (T)(any ? x / l : 0.f);
+  __syncthreads();
+  const int d = tid & 127, quarter = tid >> 7;
+  float x = 0.f;
+  if (d < size) {
+#pragma unroll 4
+    // (a part without tokens has O = 0)
+    for (int s = quarter; s < splits; s += 4) x = __builtin_fmaf(p[s * (size + 2) + d], by[s], x);
+  }
+  sums[quarter][d] = x;
+  __syncthreads();
+  if (tid >= size) return;
+  x = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
+  static_cast<T*>(out)[(int64_t)blockIdx.x * size + tid] = (T)(total[1] > 0.f ? x / total[0] : 0.f);
 }
 
 // Parts of the length: workgroups for eight on every CU, so that sequences of different lengths even out, but no part
-// shorter than one step of each wave.
+// shorter than two steps of each wave.
 int decode_splits(const oops_cache_attn_geometry& g) {
   const int64_t group = g.heads / g.kv_heads;
   const int64_t jobs = g.batch * g.kv_heads * ((group + kHeadTile - 1) / kHeadTile);
   if (jobs == 0) return 1;
-  const int64_t most = (g.max_pages * g.page + 4 * kTile - 1) / (4 * kTile);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + jobs - 1) / jobs, most, 256}));
+  const int64_t most = (g.max_pages * g.page + 8 * kTile - 1) / (8 * kTile);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + jobs - 1) / jobs, most, kMaxSplits}));
 }
 
 }  // namespace
@@ -580,6 +618,8 @@ hipError_t launch_cache_attn(const oops_cache_attn_geometry& g, const void* quer
   a.page = g.page;
   a.lengths_i64 = g.lengths_i64;
   a.splits = decode_splits(g);
+  a.page16 = (uint32_t)g.page / 16;
+  a.per16 = a.page16 == 1 ? 0xFFFFFFFFu : (uint32_t)((uint64_t(1) << 32) / a.page16);
   a.scale = g.scale;
   const dim3 grid((unsigned)(g.batch * g.kv_heads * a.tiles * a.splits));
   return by_type(g.dtype, [&](auto tag) {
@@ -590,7 +630,7 @@ hipError_t launch_cache_attn(const oops_cache_attn_geometry& g, const void* quer
     else hipLaunchKernelGGL((cache_attn_kernel<T, 4>), grid, dim3(kThreads), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    hipLaunchKernelGGL((cache_join_kernel<T>), dim3((unsigned)(g.batch * g.heads)), dim3(128), 0, stream, a.parts, out, a.splits,
+    hipLaunchKernelGGL((cache_join_kernel<T>), dim3((unsigned)(g.batch * g.heads)), dim3(512), 0, stream, a.parts, out, a.splits,
                        g.size);
     return hipGetLastError();
   });
