@@ -150,19 +150,24 @@ def _geometry(lib, dtype, shape: tuple, kv_heads: int, e: int, scale: float, seq
 
 
 def _strides(t: Optional[Tensor]) -> tuple:
-    """Strides of batch, head and token; those of dimensions of one element are not meant."""
+    """Strides of batch, head and token (the library does not read those of dimensions of one element)."""
 
-    if t is None or t.dim() != 4:
-        return (0, 0, 0)
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
+    return (0, 0, 0) if t is None or t.dim() != 4 else t.stride()[:3]
+
+
+@functools.lru_cache(maxsize=1024)
+def _whole_rows(shape: tuple, stride: tuple, el: int) -> bool:
+    """Whether rows are dense and whole 16-byte pieces apart, tokens not too far."""
+
+    if stride[3] != 1 and shape[3] > 1:
+        return False
+    return all(n <= 1 or s * el % 16 == 0 for n, s in zip(shape[:3], stride)) and (shape[2] <= 1 or stride[2] * el < MAX_PITCH)
 
 
 def _whole(t: Tensor) -> Tensor:
     """``t``, or a copy of it whose rows are whole 16-byte pieces at 16-byte addresses."""
 
-    strides = _strides(t)
-    el = t.element_size()
-    if (t.stride(-1) != 1 and t.shape[-1] > 1) or t.data_ptr() % 16 or any(s * el % 16 for s in strides) or strides[2] * el >= MAX_PITCH:
+    if t.data_ptr() % 16 or not _whole_rows(t.shape, t.stride(), t.element_size()):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -178,9 +183,9 @@ def _result_like(t: Tensor, width: int) -> Tensor:
 
 def _call_geometry(lib, q, k, v, offsets, scale, *others) -> tuple:
     sequences = 0 if offsets is None else offsets.shape[0] - 1
-    return _geometry(lib, q.dtype, tuple(q.shape), k.shape[1], v.shape[-1], scale, sequences,
+    return _geometry(lib, q.dtype, q.shape, k.shape[1], v.shape[-1], scale, sequences,
                      offsets is not None and offsets.dtype == torch.int64,
-                     tuple(map(_strides, (q, k, v, *others))))  # fmt: skip
+                     (*(t.stride()[:3] for t in (q, k, v)), *map(_strides, others)))  # fmt: skip
 
 
 def _forward_impl(q: Tensor, k: Tensor, v: Tensor, offsets: Optional[Tensor], scale: float,

@@ -47,38 +47,35 @@ struct CacheArgs {
   int64_t stride[2][3];
   int64_t slots_count, tokens, length;
   int32_t heads, size, page, slots_i64, whole;
+  int32_t lanes, together;  // lanes of a token, and tokens of a workgroup (1: the lanes of one may take several)
 };
 __device__ __forceinline__ int64_t slot_of(const void* slots, int i64, int64_t t) {
   return i64 ? static_cast<const int64_t*>(slots)[t] : static_cast<const int32_t*>(slots)[t];
 }
-// One lane's eight channels of a token's key or value.
-struct Place {
-  int64_t token, slot;
-  int which, head, piece;
+// One lane's eight channels of keys or values: the same for all tokens that it passes.
+struct Lane {
+  int which, head, piece, ahead;  // ahead: of the workgroup's first token
+  bool live;
 };
-__device__ __forceinline__ Place place_of(const CacheArgs& a, int64_t i) {
-  const int pieces = a.size / 8;
-  Place p;
-  p.piece = (int)(i % pieces);
-  i /= pieces;
-  p.head = (int)(i % a.heads);
-  i /= a.heads;
-  p.which = (int)(i & 1);
-  p.token = i >> 1;
-  p.slot = -1;
-  if (p.token < a.tokens) {
-    p.slot = slot_of(a.slots, a.slots_i64, p.token);
-    if (p.slot < 0 || p.slot >= a.slots_count) p.slot = -1;
-  }
-  return p;
+__device__ __forceinline__ Lane lane_of(const CacheArgs& a) {
+  const int i = blockIdx.y * kThreads + threadIdx.x, pieces = a.size / 8;
+  const int ahead = a.together > 1 ? i / a.lanes : 0, n = i - ahead * a.lanes;
+  return Lane{n / (pieces * a.heads), n / pieces % a.heads, n % pieces, ahead < a.together ? ahead : a.together - 1,
+              ahead < a.together && n < a.lanes};
+}
+__device__ __forceinline__ int64_t valid_slot(const CacheArgs& a, int64_t token) {
+  const int64_t s = slot_of(a.slots, a.slots_i64, token);
+  return s >= 0 && s < a.slots_count ? s : -1;
 }
 // row of the codes and scales
-__device__ __forceinline__ int64_t cache_row(const CacheArgs& a, const Place& p) {
-  return ((p.slot / a.page * a.heads + p.head) * 2 + p.which) * a.page + p.slot % a.page;
+__device__ __forceinline__ int64_t cache_row(const CacheArgs& a, const Lane& l, int64_t slot) {
+  const uint32_t page = (uint32_t)slot / (uint32_t)a.page;
+  return (((int64_t)page * a.heads + l.head) * 2 + l.which) * a.page + ((uint32_t)slot - page * (uint32_t)a.page);
 }
-__device__ __forceinline__ int64_t operand_at(const CacheArgs& a, const Place& p) {
-  const int64_t* s = a.stride[p.which];
-  return p.token / a.length * s[0] + p.head * s[1] + p.token % a.length * s[2] + p.piece * 8;
+__device__ __forceinline__ int64_t operand_at(const CacheArgs& a, const Lane& l, int64_t token) {
+  const int64_t* s = a.stride[l.which];
+  const uint32_t b = a.tokens > a.length ? (uint32_t)token / (uint32_t)a.length : 0;
+  return b * s[0] + l.head * s[1] + (token - b * a.length) * s[2] + l.piece * 8;
 }
 
 // ---- of tokens with the same slot the last is kept (long calls: owners are settled first)
@@ -98,62 +95,66 @@ __global__ __launch_bounds__(kThreads) void slot_owner_kernel(const void* slots,
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void cache_write_kernel(CacheArgs a) {
-  const Place p = place_of(a, (int64_t)blockIdx.x * kThreads + threadIdx.x);
-  bool write = p.slot >= 0;
-  if (a.owner) {
-    write = write && a.owner[p.slot] == (int32_t)p.token;
-  } else {
-    // the wave's tokens one after the other, the later slots 64 at a time
-    const int lane = threadIdx.x & 63;
-    const int first = __builtin_amdgcn_readlane((int)p.token, 0), last = __builtin_amdgcn_readlane((int)p.token, 63);
-    for (int t = first; t <= last && t < a.tokens; ++t) {
-      const int64_t mine = slot_of(a.slots, a.slots_i64, t);
-      bool again = false;
-      for (int64_t u = t + 1 + lane; u < a.tokens; u += 64) again |= slot_of(a.slots, a.slots_i64, u) == mine;
-      if (__any(again) && p.token == t) write = false;
-    }
-  }
-  float v[8] = {};
-  if (write) {
-    const T* x = static_cast<const T*>(p.which ? a.value : a.key) + operand_at(a, p);
-    if (a.whole) {
-      uint4 u[sizeof(T) / 2];
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(x)[i];
-      const T* e = reinterpret_cast<const T*>(u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (float)e[i];
+  const Lane l = lane_of(a);
+  const int lane = threadIdx.x & 63;
+  for (int64_t base = (int64_t)blockIdx.x * a.together; base < a.tokens; base += (int64_t)gridDim.x * a.together) {
+    const int64_t token = base + l.ahead;
+    const int64_t slot = l.live && token < a.tokens ? valid_slot(a, token) : -1;
+    bool write = slot >= 0;
+    if (a.owner) {
+      write = write && a.owner[slot] == (int32_t)token;
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+      // the wave's tokens one after the other, the later slots 64 at a time
+      const int first = __builtin_amdgcn_readlane((int)token, 0), last = __builtin_amdgcn_readlane((int)token, 63);
+      for (int t = first; t <= last && t < a.tokens; ++t) {
+        const int64_t mine = slot_of(a.slots, a.slots_i64, t);
+        bool again = false;
+        for (int64_t u = t + 1 + lane; u < a.tokens; u += 64) again |= slot_of(a.slots, a.slots_i64, u) == mine;
+        if (__any(again) && token == t) write = false;
+      }
     }
-  }
-  // the block's largest magnitude as a bit pattern (a NaN's is above infinity's); its lanes are four neighbours
-  uint32_t top = 0;
+    float v[8] = {};
+    if (write) {
+      const T* x = static_cast<const T*>(l.which ? a.value : a.key) + operand_at(a, l, token);
+      if (a.whole) {
+        uint4 u[sizeof(T) / 2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = std::max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
-  top = std::max(top, (uint32_t)__shfl_xor((int)top, 1));
-  top = std::max(top, (uint32_t)__shfl_xor((int)top, 2));
-  if (!write) return;
-  // top = 1.f * 2^(exp - 127) <= 6 * 2^e = 1.5 * 2^(e + 2)
-  const int exp = (int)(top >> 23);
-  const bool lost = exp == 255;
-  int e = exp - ((top & 0x7FFFFFu) > 0x400000u ? 1 : 2);
-  e = lost ? 255 : e < 1 ? 1 : e > 252 ? 252 : e;
-  const float inv = __builtin_bit_cast(float, (uint32_t)(254 - e) << 23);  // 2^(127 - e)
-  uint32_t word = 0;
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(x)[i];
+        const T* e = reinterpret_cast<const T*>(u);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // 2^k units below 2, 2 .. 4 and 4 .. 6: the code is their count from zero
-    const float q = fminf(fabsf(v[i]) * inv, 6.0f);
-    const float c = q < 2.f ? __builtin_rintf(q * 2.f) : q < 4.f ? __builtin_rintf(q) + 2.f : __builtin_rintf(q * 0.5f) + 4.f;
-    const uint32_t sign = __builtin_bit_cast(uint32_t, v[i]) >> 31 << 3;
-    word |= ((uint32_t)c | sign) << (4 * i);
+        for (int i = 0; i < 8; ++i) v[i] = (float)e[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+      }
+    }
+    // the block's largest magnitude as a bit pattern (a NaN's is above infinity's); its lanes are four neighbours
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = std::max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
+    top = std::max(top, (uint32_t)__shfl_xor((int)top, 1));
+    top = std::max(top, (uint32_t)__shfl_xor((int)top, 2));
+    if (!write) continue;
+    // top = 1.f * 2^(exp - 127) <= 6 * 2^e = 1.5 * 2^(e + 2)
+    const int exp = (int)(top >> 23);
+    const bool lost = exp == 255;
+    int e = exp - ((top & 0x7FFFFFu) > 0x400000u ? 1 : 2);
+    e = lost ? 255 : e < 1 ? 1 : e > 252 ? 252 : e;
+    const float inv = __builtin_bit_cast(float, (uint32_t)(254 - e) << 23);  // 2^(127 - e)
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // 2^k units below 2, 2 .. 4 and 4 .. 6: the code is their count from zero
+      const float q = fminf(fabsf(v[i]) * inv, 6.0f);
+      const float c = q < 2.f ? __builtin_rintf(q * 2.f) : q < 4.f ? __builtin_rintf(q) + 2.f : __builtin_rintf(q * 0.5f) + 4.f;
+      const uint32_t sign = __builtin_bit_cast(uint32_t, v[i]) >> 31 << 3;
+      word |= ((uint32_t)c | sign) << (4 * i);
+    }
+    if (lost) word = 0;
+    const int64_t row = cache_row(a, l, slot);
+    *reinterpret_cast<uint32_t*>(a.codes + row * (a.size / 2) + l.piece * 4) = word;
+    if (l.piece % 4 == 0) a.scales[row * (a.size / 32) + l.piece / 4] = (uint8_t)e;
   }
-  if (lost) word = 0;
-  const int64_t row = cache_row(a, p);
-  *reinterpret_cast<uint32_t*>(a.codes + row * (a.size / 2) + p.piece * 4) = word;
-  if (p.piece % 4 == 0) a.scales[row * (a.size / 32) + p.piece / 4] = (uint8_t)e;
 }
 
 __device__ __forceinline__ float scale_value(uint32_t e) {
@@ -167,25 +168,28 @@ __device__ __forceinline__ float code_value(uint32_t c, float scale) {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void cache_read_kernel(CacheArgs a) {
-  const Place p = place_of(a, (int64_t)blockIdx.x * kThreads + threadIdx.x);
-  if (p.token >= a.tokens) return;
-  uint32_t word = 0, e = 1;
-  if (p.slot >= 0) {
-    const int64_t row = cache_row(a, p);
-    word = *reinterpret_cast<const uint32_t*>(a.codes + row * (a.size / 2) + p.piece * 4);
-    e = a.scales[row * (a.size / 32) + p.piece / 4];
+  const Lane l = lane_of(a);
+  if (!l.live) return;
+  for (int64_t token = (int64_t)blockIdx.x * a.together + l.ahead; token < a.tokens; token += (int64_t)gridDim.x * a.together) {
+    const int64_t slot = valid_slot(a, token);
+    uint32_t word = 0, e = 1;
+    if (slot >= 0) {
+      const int64_t row = cache_row(a, l, slot);
+      word = *reinterpret_cast<const uint32_t*>(a.codes + row * (a.size / 2) + l.piece * 4);
+      e = a.scales[row * (a.size / 32) + l.piece / 4];
+    }
+    const float scale = scale_value(e);
+    union {
+      uint4 u[sizeof(T) / 2];
+      T y[8];
+    } r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.y[i] = (T)code_value(word >> (4 * i) & 15, scale);
+    // (results are allocated in whole pieces)
+    uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(l.which ? a.value_out : a.key_out) + operand_at(a, l, token));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) to[i] = r.u[i];
   }
-  const float scale = scale_value(e);
-  union {
-    uint4 u[sizeof(T) / 2];
-    T y[8];
-  } r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r.y[i] = (T)code_value(word >> (4 * i) & 15, scale);
-  // (results are allocated in whole pieces)
-  uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.which ? a.value_out : a.key_out) + operand_at(a, p));
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) to[i] = r.u[i];
 }
 
 // ------------------------------------------------------------------ attention
@@ -549,10 +553,15 @@ CacheArgs cache_args(const oops_cache_geometry& g, const void* codes, const void
   a.size = g.size;
   a.page = g.page;
   a.slots_i64 = g.slots_i64;
+  a.lanes = 2 * g.heads * (g.size / 8);
+  a.together = std::max(1, kThreads / a.lanes);
   return a;
 }
-unsigned cache_grid(const oops_cache_geometry& g) {
-  return (unsigned)((g.batch * g.length * 2 * g.heads * (g.size / 8) + kThreads - 1) / kThreads);
+// lanes of a token along y, tokens along x, sixteen workgroups on every CU at most
+dim3 cache_grid(const CacheArgs& a) {
+  const unsigned y = (unsigned)((a.lanes + kThreads - 1) / kThreads);
+  const int64_t x = (a.tokens + a.together - 1) / a.together;
+  return dim3((unsigned)std::min<int64_t>(x, std::max(1u, 4096 / y)), a.together > 1 ? 1 : y);
 }
 }  // namespace
 
@@ -575,7 +584,7 @@ hipError_t launch_cache_write(const oops_cache_geometry& g, void* codes, void* s
     a.owner = owner;
   }
   return by_type(g.dtype, [&](auto tag) {
-    hipLaunchKernelGGL((cache_write_kernel<decltype(tag)>), dim3(cache_grid(g)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((cache_write_kernel<decltype(tag)>), cache_grid(a), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
   });
 }
@@ -586,7 +595,7 @@ hipError_t launch_cache_read(const oops_cache_geometry& g, const void* codes, co
   a.key_out = key;
   a.value_out = value;
   return by_type(g.dtype, [&](auto tag) {
-    hipLaunchKernelGGL((cache_read_kernel<decltype(tag)>), dim3(cache_grid(g)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((cache_read_kernel<decltype(tag)>), cache_grid(a), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
   });
 }

@@ -43,11 +43,21 @@ int check_rotary(const oops_rotary_geometry* g) {
         if (s < 0) return report(OOPS_EINVAL, "an operand has a negative stride");
   return OOPS_OK;
 }
-size_t rotary_parts_bytes(const oops_rotary_geometry& g, int which) {
-  return align256((size_t)oops::rotary_parts(g, which) * (size_t)g.size * sizeof(float));
+size_t rotary_parts_bytes(const oops_rotary_geometry& g) {
+  return align256((size_t)oops::rotary_parts(g) * (size_t)g.size * sizeof(float));
 }
 
 // ---- causal attention
+// strides of dimensions of one element are nobody's
+oops_causal_geometry with_strides(oops_causal_geometry g) {
+  for (int i = 0; i < OOPS_CA_OPERANDS; ++i) {
+    const bool kv = i == OOPS_CA_K || i == OOPS_CA_V || i == OOPS_CA_DK || i == OOPS_CA_DV;
+    if (g.batch <= 1) g.stride[i][0] = 0;
+    if ((kv ? g.kv_heads : g.heads) <= 1) g.stride[i][1] = 0;
+    if (g.length <= 1) g.stride[i][2] = 0;
+  }
+  return g;
+}
 int check_causal(const oops_causal_geometry* g, bool offsets) {
   if (!g) return report(OOPS_EINVAL, "causal attention geometry is NULL");
   if (!known_dtype(g->dtype)) return report(OOPS_EINVAL, "unknown dtype %lld", g->dtype);
@@ -63,7 +73,8 @@ int check_causal(const oops_causal_geometry* g, bool offsets) {
                   g->length);
   if (offsets && (g->sequences < 0 || g->sequences > kMax31 - 1))
     return report(OOPS_EINVAL, "sequences must not be negative, got %lld", g->sequences);
-  for (const auto& s : g->stride) {
+  const oops_causal_geometry own = with_strides(*g);
+  for (const auto& s : own.stride) {
     if (s[0] < 0 || s[1] < 0 || s[2] < 0) return report(OOPS_EINVAL, "an operand has a negative stride");
     if (s[2] * el >= (1 << 24)) return report(OOPS_EINVAL, "tokens must be less than 2^24 bytes apart, got %lld elements", s[2]);
     if (s[0] * el % 16 || s[1] * el % 16 || s[2] * el % 16) return report(OOPS_EINVAL, "strides must be of whole 16-byte pieces");
@@ -76,7 +87,8 @@ bool aligned(std::initializer_list<const void*> ptrs) {
   return true;
 }
 void set3(int64_t (&to)[3], const int64_t (&from)[3]) { std::copy(from, from + 3, to); }
-oops::CausalArgs causal_args(const oops_causal_geometry& g, const void* q, const void* k, const void* v, const void* offsets) {
+oops::CausalArgs causal_args(const oops_causal_geometry& given, const void* q, const void* k, const void* v, const void* offsets) {
+  const oops_causal_geometry g = with_strides(given);
   oops::CausalArgs a{};
   a.q = q;
   a.k = k;
@@ -125,7 +137,7 @@ int check_cache_shape(int dtype, int heads, int size, int page, int64_t pages) {
 int check_cache(const oops_cache_geometry* g) {
   if (!g) return report(OOPS_EINVAL, "cache geometry is NULL");
   if (int rc = check_cache_shape(g->dtype, g->heads, g->size, g->page, g->pages)) return rc;
-  // (a launch of more than 2^32 lanes is refused by the runtime)
+  if (g->heads > (1 << 16)) return report(OOPS_EINVAL, "heads must be at most 2^16, got %lld", g->heads);
   if (g->batch < 0 || g->length < 0 || !fits(g->batch, g->length, (int64_t)g->heads * (g->size / 4), int64_t(1) << 31))
     return report(OOPS_EINVAL, "batch (%lld) x length (%lld) tokens are too many for one call", g->batch, g->length);
   for (const auto& operand : g->stride)
@@ -165,7 +177,7 @@ int oops_rms_norm_rotary_forward(const oops_rotary_geometry* geo, const void* qu
 size_t oops_rms_norm_rotary_backward_workspace_bytes(const oops_rotary_geometry* geo) {
   oops::clear_report();
   if (check_rotary(geo)) return 0;
-  return rotary_parts_bytes(*geo, 0) + rotary_parts_bytes(*geo, 1);
+  return 2 * rotary_parts_bytes(*geo);
 }
 
 int oops_rms_norm_rotary_backward(const oops_rotary_geometry* geo, const void* query, const void* key,
@@ -183,7 +195,7 @@ int oops_rms_norm_rotary_backward(const oops_rotary_geometry* geo, const void* q
   if (weights)
     if (int rc = oops::report_workspace(workspace, ws_bytes, oops_rms_norm_rotary_backward_workspace_bytes(geo))) return rc;
   float* first = static_cast<float*>(workspace);
-  float* second = weights ? first + rotary_parts_bytes(*geo, 0) / sizeof(float) : nullptr;
+  float* second = weights ? first + rotary_parts_bytes(*geo) / sizeof(float) : nullptr;
   return report_launch(
       oops::launch_rotary_backward(*geo, {query, key}, {query_weight, key_weight}, table, positions,
                                    {grad_query_out, grad_key_out}, {grad_query, grad_key},

@@ -10,7 +10,7 @@ namespace oops {
 // ---- rotary.hip
 hipError_t launch_rotary_forward(const oops_rotary_geometry& g, const void* const (&x)[2], const void* const (&weight)[2],
                                  const float* table, const void* positions, void* const (&y)[2], hipStream_t stream);
-int rotary_parts(const oops_rotary_geometry& g, int which);  // rows of weight-gradient partials
+int rotary_parts(const oops_rotary_geometry& g);  // rows of each side's weight-gradient partials
 hipError_t launch_rotary_backward(const oops_rotary_geometry& g, const void* const (&x)[2], const void* const (&weight)[2],
                                   const float* table, const void* positions, const void* const (&dy)[2],
                                   void* const (&dx)[2], float* const (&parts)[2], void* const (&dweight)[2],
