@@ -85,6 +85,8 @@ def test_values_at_borders(dtype):
     rows += [up, down, near, base * (1 - info.eps), torch.zeros(32, dtype=torch.float64), -torch.zeros(32, dtype=torch.float64)]
     rows += [torch.full((32,), info.smallest_normal, dtype=torch.float64), torch.full((32,), info.smallest_normal * info.eps, dtype=torch.float64)]
     rows += [torch.full((32,), info.max, dtype=torch.float64), torch.linspace(-info.max, info.max, 32, dtype=torch.float64)]
+    if dtype != torch.float16:  # subnormal numbers at the smallest scale, 2^-126
+        rows += [base * 2.0**-126, base * 2.0**-128, near * 2.0**-126]
     x = torch.stack(rows).to(dtype).to(DEV)[None]  # (1, T, 32)
     cache = quantized_cache(4, 1, 32, page_size=16, device=DEV)
     slots = torch.arange(x.shape[1], device=DEV)
