@@ -30,8 +30,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
   using TL = Tile<T, DP>;
   using A = Att<T>;
   constexpr int KT = TL::kRows, NS = DP / 16, NDT = DP / 32, SUB = KT / 32;
-  __shared__ __attribute__((aligned(1024))) char k_lds[2][TL::kBytes];
-  __shared__ __attribute__((aligned(1024))) char v_lds[2][TL::kBytes];
+  // float16's weights as two terms: O, and with it the backward's delta, then has no rounding but its own.  (With one, dQ
+  // of short rows is off by as much again as by the roundings of dS and of dQ.)
+  constexpr bool TWO = __is_same(T, _Float16);
+  using Plane = typename TL::Plane;
+  using PlaneType = typename TL::PlaneType;
+  __shared__ __attribute__((aligned(1024))) char k_lds[A::kBuffers][TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds[A::kBuffers][TL::kBytes];
 
   const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
@@ -78,21 +83,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
   vl.next(v_lds[0]);
   // (the buffer is a constant, so that its address is part of the instructions)
   auto step = [&](int t, auto buffer) {
-    constexpr int buf = decltype(buffer)::value;
+    constexpr int buf = decltype(buffer)::value % A::kBuffers, other = (buf + 1) % A::kBuffers;
     const int k0 = t * KT;
-    fast::vmem_wait<0>();
-    lds_barrier();
+    arrived<T>(kl, k_lds[buf], vl, v_lds[buf]);
     if (t < t1) {
-      kl.next(k_lds[buf ^ 1]);
-      vl.next(v_lds[buf ^ 1]);
+      kl.next(k_lds[other]);
+      vl.next(v_lds[other]);
     }
     auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
     if (k0 < spans.last.start || k0 + KT - 1 > block0) {
       // (masked pairs for some wave)
-      if (__syncthreads_or(tile_non_finite<TL, T>(v_lds[buf]))) {
+      if (__syncthreads_or(tile_non_finite<Plane, PlaneType>(v_lds[buf]))) {
         add_non_finite<TL, true>(o, v_lds[buf], g, keep);
         __syncthreads();
-        clean_tile<TL, T>(v_lds[buf]);
+        clean_tile<Plane, PlaneType>(v_lds[buf]);
         __syncthreads();
       }
     }
@@ -129,7 +133,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 #pragma unroll
       for (int d = 0; d < NDT; ++d) o[d] *= alpha;
     }
-    Frag<T> p[KT / 16];
+    Frag<T> p[KT / 16], rest[TWO ? KT / 16 : 1];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
 #pragma unroll
@@ -137,14 +141,24 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         p[2 * u + m] = pack<T>(s[u], m);
-        l_run = add_elements<T>(p[2 * u + m], l_run);
+        if constexpr (TWO) rest[2 * u + m] = pack_rest<T>(s[u], m, p[2 * u + m]);
+        // (the sum of what is multiplied: a rounding that all weights share leaves no trace)
+        if constexpr (TL::k16 && !TWO) l_run = add_elements<T>(p[2 * u + m], l_run);
+      }
+      if constexpr (!TL::k16 || TWO) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) l_run += s[u][j];
       }
     }
 #pragma unroll
     for (int m = 0; m < KT / 16; ++m)
 #pragma unroll
-      for (int d = 0; d < NDT; ++d) o[d] = A::mma(rd.col(v_lds[buf], m, d), p[m], o[d]);
-    if constexpr (TL::k16) {
+      for (int d = 0; d < NDT; ++d) {
+        const Frag<T> v = rd.col(v_lds[buf], m, d);
+        if constexpr (TWO) o[d] = A::mma(v, rest[m], o[d]);
+        o[d] = A::mma(v, p[m], o[d]);
+      }
+    if constexpr (TL::k16 && !TWO) {
       __builtin_amdgcn_sched_group_barrier(0x002, 12, 0);
       interleave<8, NDT * (KT / 16), 2, 5>();
     }

@@ -30,8 +30,10 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   using TL = Tile<T, DP>;
   using A = Att<T>;
   constexpr int KT = TL::kRows, NS = DP / 16, NDT = DP / 32, SUB = KT / 32;
-  __shared__ __attribute__((aligned(1024))) char k_lds[2][TL::kBytes];
-  __shared__ __attribute__((aligned(1024))) char v_lds[2][TL::kBytes];
+  using Plane = typename TL::Plane;
+  using PlaneType = typename TL::PlaneType;
+  __shared__ __attribute__((aligned(1024))) char k_lds[A::kBuffers][TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds[A::kBuffers][TL::kBytes];
   __shared__ uint32_t lost_lds[2];
 
   const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, g = lane >> 5;
@@ -47,25 +49,10 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   const int last = std::min(q0 + 31, length - 1);
   const bool valid = row < length;
 
-  Frag<T> dof[NS];
-  load_row<T, DP>(dof, rows_of<T>(a.dout, a.do_stride, b, h, a.value_size, length), row, valid, g);
-  float delta = 0.f;
-  {
-    Frag<T> of[NS];
-    load_row<T, DP>(of, rows_of<T>(a.out, a.o_stride, b, h, a.value_size, length), row, valid, g);
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)of[s][i], (float)dof[s][i], delta);
-    if (a.low) {
-      load_row<T, DP>(of, rows_of<T>(a.low, a.o_stride, b, h, a.value_size, length), row, valid, g);
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)of[s][i], (float)dof[s][i], delta);
-    }
-    delta = fast::sum_halves(delta);
-  }
+  const Rows dor = rows_of<T>(a.dout, a.do_stride, b, h, a.value_size, length);
+  float delta = row_dot<T, DP>(rows_of<T>(a.out, a.o_stride, b, h, a.value_size, length), dor, row, valid, g, 0.f);
+  if (a.low) delta = row_dot<T, DP>(rows_of<T>(a.low, a.o_stride, b, h, a.value_size, length), dor, row, valid, g, delta);
+  delta = fast::sum_halves(delta);
   const float c1 = fmaxf(a.scale * kLog2e, 0x1p-120f);
   const int64_t stat = ((int64_t)b * a.heads + h) * length + row;
   const float lse = valid ? a.lse[stat] : 0.f;
@@ -81,7 +68,8 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   const bool empty = !valid || start > row;
   const uint32_t reach = empty ? 0u : (uint32_t)(row - start);
   const int first_start = __builtin_amdgcn_readlane(start, 0), last_start = __builtin_amdgcn_readlane(start, idle ? 0 : last - q0);
-  Frag<T> qf[NS];
+  Frag<T> qf[NS], dof[NS];
+  load_row<T, DP>(dof, dor, row, valid, g);
   load_row<T, DP>(qf, rows_of<T>(a.q, a.q_stride, b, h, a.key_size, length), row, valid, g, a.flip);
 
   const Rows kr = rows_of<T>(a.k, a.k_stride, b, h / a.group, a.key_size, length);
@@ -103,23 +91,22 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   kl.next(k_lds[0]);
   vl.next(v_lds[0]);
   auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
-    constexpr int buf = decltype(buffer)::value;
+    constexpr int buf = decltype(buffer)::value % A::kBuffers, other = (buf + 1) % A::kBuffers;
     const int k0 = t * KT;
-    fast::vmem_wait<0>();
-    lds_barrier();
+    arrived<T>(kl, k_lds[buf], vl, v_lds[buf]);
     if (t < t1) {
-      kl.next(k_lds[buf ^ 1]);
-      vl.next(v_lds[buf ^ 1]);
+      kl.next(k_lds[other]);
+      vl.next(v_lds[other]);
     }
     auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
     uint64_t lost = 0;
     if (k0 < spans.last.start || k0 + KT - 1 > block0) {
       // (masked pairs for some wave)
-      if (__syncthreads_or(tile_non_finite<TL, T>(k_lds[buf]))) {
-        lost = rows_non_finite<TL, T>(k_lds[buf], lost_lds);
+      if (__syncthreads_or(tile_non_finite<Plane, PlaneType>(k_lds[buf]))) {
+        lost = rows_non_finite<Plane, PlaneType>(k_lds[buf], lost_lds);
         add_non_finite<TL, false>(dq, k_lds[buf], g, keep);
         __syncthreads();
-        clean_tile<TL, T>(k_lds[buf]);
+        clean_tile<Plane, PlaneType>(k_lds[buf]);
         __syncthreads();
       }
     }
@@ -186,8 +173,10 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   constexpr int QT = 32, NS = DP / 16, NDT = DP / 32;
   // (registers: with 128 channels dK, dV and K fill them; V is read again from LDS at each step)
   constexpr bool kValuesInLds = DP == 128;
-  __shared__ __attribute__((aligned(1024))) char q_lds[2][TL::kBytes];
-  __shared__ __attribute__((aligned(1024))) char do_lds[2][TL::kBytes];
+  using Plane = typename TL::Plane;
+  using PlaneType = typename TL::PlaneType;
+  __shared__ __attribute__((aligned(1024))) char q_lds[A::kBuffers][TL::kBytes];
+  __shared__ __attribute__((aligned(1024))) char do_lds[A::kBuffers][TL::kBytes];
   __shared__ __attribute__((aligned(1024))) char v_lds[kValuesInLds ? 4 : 1][kValuesInLds ? TL::kBytes : 16];
   __shared__ __attribute__((aligned(1024))) float lse_lds[2][64], delta_lds[2][64];
 
@@ -225,8 +214,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   Reads<T, DP> rd, rv;
   rd.init(lane);
   rv = rd;
-#pragma unroll
-  for (int i = 0; i < TL::kWindows; ++i) rv.row_at[i] += wave * TL::kBytes;
+  rv.shift_rows(wave * TL::kBytes);
 
   // the tiles' order: the group's heads, each from the block's first query to the last that is paired with its keys
   Loader<T, DP, 32> ql, dl;
@@ -240,12 +228,12 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
     stats = (wave == 0 ? a.neg_lse : a.neg_delta) + ((int64_t)b * a.heads + load_h) * length + load_t * QT;
   };
   auto load = [&](auto buffer) {
-    constexpr int buf = decltype(buffer)::value;
+    constexpr int to = decltype(buffer)::value, buf = to % A::kBuffers;
     const int n = std::min(ql.left, QT);
     ql.next(q_lds[buf]);
     dl.next(do_lds[buf]);
     if (wave < 2)
-      dma4_asm(fast::rsrc_words(stats, (uint32_t)n * 4), wave == 0 ? lse_lds[buf] : delta_lds[buf], (uint32_t)lane * 4);
+      dma4_asm(fast::rsrc_words(stats, (uint32_t)n * 4), wave == 0 ? lse_lds[to] : delta_lds[to], (uint32_t)lane * 4);
     stats += QT;
     if (++load_t > t1) {
       load_t = t0;
@@ -259,25 +247,27 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
     Loader<T, DP, 32> vl;
     vl.init(vr, wave, lane);
     vl.seek(vr, block0);
-    for (int i = 0; i < 4; ++i) vl.next(v_lds[i]);
+    for (int i = 0; i < 4; ++i) {
+      vl.next(v_lds[i]);
+      if constexpr (!TL::k16) vl.land(v_lds[i]);
+    }
   }
   seek();
   load(std::integral_constant<int, 0>{});
   auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
-    constexpr int buf = decltype(buffer)::value;
+    constexpr int now = decltype(buffer)::value, buf = now % A::kBuffers;
     const int q0 = t * QT;
-    fast::vmem_wait<0>();
-    lds_barrier();
-    if (load_h < h1) load(std::integral_constant<int, buf ^ 1>{});
+    arrived<T>(ql, q_lds[buf], dl, do_lds[buf]);
+    if (load_h < h1) load(std::integral_constant<int, now ^ 1>{});
     auto keep = [&](int r) { return (uint32_t)(q0 + r - key) < width; };
     if (q0 < block0 + kBlock - 1 || q0 + QT > spans.first.end) {
       // (masked pairs for some wave; a query that is not finite has made its LSE, a dO its delta, NaN or infinite)
-      if (__syncthreads_or(tile_non_finite<TL, T>(q_lds[buf]) | tile_non_finite<TL, T>(do_lds[buf]))) {
+      if (__syncthreads_or(tile_non_finite<Plane, PlaneType>(q_lds[buf]) | tile_non_finite<Plane, PlaneType>(do_lds[buf]))) {
         add_non_finite<TL, false>(dk, q_lds[buf], g, keep);
         add_non_finite<TL, true>(dv, do_lds[buf], g, keep);
         __syncthreads();
-        clean_tile<TL, T>(q_lds[buf]);
-        clean_tile<TL, T>(do_lds[buf]);
+        clean_tile<Plane, PlaneType>(q_lds[buf]);
+        clean_tile<Plane, PlaneType>(do_lds[buf]);
         __syncthreads();
       }
     }
@@ -286,8 +276,8 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
     f32x16 s, dp;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&lse_lds[buf][8 * q + 4 * g]);
-      const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_lds[buf][8 * q + 4 * g]);
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&lse_lds[now][8 * q + 4 * g]);
+      const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_lds[now][8 * q + 4 * g]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * q + i] = lse[i], dp[4 * q + i] = delta[i];
     }
@@ -295,7 +285,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
     for (int i = 0; i < NS; ++i) s = A::mma(rd.row(q_lds[buf], 0, i), kf[i], s);
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      if constexpr (kValuesInLds) dp = A::mma(rd.row(do_lds[buf], 0, i), rv.row(TL::k16 ? v_lds[0] : v_lds[wave], 0, i), dp);
+      if constexpr (kValuesInLds) dp = A::mma(rd.row(do_lds[buf], 0, i), rv.row(v_lds[0], 0, i), dp);
       else dp = A::mma(rd.row(do_lds[buf], 0, i), vf[i], dp);
     }
     if constexpr (TL::k16) {

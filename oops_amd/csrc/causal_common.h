@@ -1,7 +1,10 @@
 // Device code shared by the causal attention kernels (forward and backward).
 //
-// Every product is a 32 x 32 x 16 step on fragments of eight elements a lane
-// (16-bit types: one MFMA; float32: eight exact float32 MFMAs).  Lane (c =
+// Every product is a 32 x 32 x 16 step on fragments of eight elements a lane:
+// one MFMA of a 16-bit type.  float32 operands are three bfloat16 terms, their sum
+// exactly, and a step is six MFMAs, the terms' products down to 2^-16 of the largest
+// (what is left out is below 2^-26): 192 cycles where the float32 matrix unit, exact
+// too, takes 512.  Lane (c =
 // lane % 32, g = lane / 32) holds elements 16 s + 8 g .. + 7 of row c along
 // the contracted axis.  An accumulator's rows are kappa(g, j), so eight of its
 // registers are the other operand of the next product as they stand, if the
@@ -26,41 +29,69 @@ using fast::kOut;
 constexpr int kBlock = 128;      // queries, or keys, of a workgroup
 constexpr int kMaxOrder = 8192;  // blocks that are put in order by their work
 
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-
+// float32 in three bfloat16 terms
+struct Terms3 {
+  bf16x8 t[3];
+};
 template <typename T> struct Att {
   using Frag = typename Elem<T>::Frag;
-  static constexpr int kRows = 64;  // rows of a tile in LDS
-  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return Elem<T>::mma(a, b, c); }
+  static constexpr int kRows = 64;    // rows of a tile in LDS
+  static constexpr int kBuffers = 2;  // tiles filled while others are read
+  static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) { return Elem<T>::mma(a, b, c); }
 };
 template <> struct Att<float> {
-  using Frag = f32x8;
+  using Frag = Terms3;
   static constexpr int kRows = 32;
-  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
-    return c;
+  static constexpr int kBuffers = 1;  // (filled from registers, where the next tile waits)
+  static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
+    using E = Elem<__bf16>;
+    c = E::mma(a.t[1], b.t[1], c);
+    c = E::mma(a.t[0], b.t[2], c);
+    c = E::mma(a.t[2], b.t[0], c);
+    c = E::mma(a.t[0], b.t[1], c);
+    c = E::mma(a.t[1], b.t[0], c);
+    return E::mma(a.t[0], b.t[0], c);
   }
 };
 template <typename T> using Frag = typename Att<T>::Frag;
 
+// eight floats in three terms; an infinity or a NaN is the first term's alone.  CLAMP: finite values above bfloat16's
+// largest stay finite.
+template <bool CLAMP>
+__device__ __forceinline__ Terms3 split3(const float (&x)[8]) {
+  constexpr float kTop = 3.3895313892515355e38f;
+  Terms3 f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v = x[i];
+    if (CLAMP && fabsf(v) > kTop && fabsf(v) < -kNegInf) v = __builtin_copysignf(kTop, v);
+    f.t[0][i] = (__bf16)v;
+    float r = x[i] - (float)f.t[0][i];
+    r = __builtin_isfinite(r) ? r : 0.f;
+    f.t[1][i] = (__bf16)r;
+    f.t[2][i] = (__bf16)(r - (float)f.t[1][i]);
+  }
+  return f;
+}
+
 // ---- tiles in LDS: ROWS rows of DP elements
 template <typename T, int DP, int ROWS = Att<T>::kRows>
 struct Tile {
+  using Plane = Tile;  // what holds the elements' largest terms
+  using PlaneType = T;
   static constexpr int kRows = ROWS;
-  static constexpr bool k16 = sizeof(T) == 2;
-  static constexpr int kRowBytes = DP * (int)sizeof(T);
-  static constexpr int kPieces = kRowBytes / 16;                  // of a row
-  static constexpr int kChunks = kRows * kRowBytes / 1024;        // kilobytes
-  static constexpr int kLoads = kChunks / 4;                      // of a wave, four waves a tile
-  static constexpr int kPitch = 1024 + (!k16 ? 0 : DP == 128 ? 16 : 32);  // between kilobytes
+  static constexpr bool k16 = true;
+  static constexpr int kRowBytes = DP * 2;
+  static constexpr int kPieces = kRowBytes / 16;            // of a row
+  static constexpr int kChunks = kRows * kRowBytes / 1024;  // kilobytes
+  static constexpr int kLoads = kChunks / 4;                // of a wave, four waves a tile
+  static constexpr int kPitch = 1024 + (DP == 128 ? 16 : 32);  // between kilobytes
   static constexpr int kBytes = kChunks * kPitch;
   static constexpr int kWindows = DP / 32;
 
   // piece of row r that lies at place p of the row (its own inverse)
   static __device__ __forceinline__ int placed(int r, int p) {
-    if constexpr (!k16) return p ^ ((kPieces == 16 ? r & 7 : r & 15) << 1);  // (32-byte pairs, which float32 fragments are)
-    else if constexpr (DP == 128) return p ^ ((r & 3) << 2);
+    if constexpr (DP == 128) return p ^ ((r & 3) << 2);
     else return p ^ (((r >> 1) & 1) << 2) ^ ((r >> 2) & 1);
   }
   static __device__ __forceinline__ int at(int r, int piece) {
@@ -70,8 +101,20 @@ struct Tile {
   // the n-th 16-byte piece in the order of places
   static __device__ __forceinline__ int nth(int n) { return (n >> 6) * kPitch + (n & 63) * 16; }
   static __device__ __forceinline__ float element(const char* tile, int r, int c) {
-    constexpr int n = 16 / (int)sizeof(T);
-    return (float)*reinterpret_cast<const T*>(tile + at(r, c / n) + c % n * (int)sizeof(T));
+    return (float)*reinterpret_cast<const T*>(tile + at(r, c >> 3) + (c & 7) * 2);
+  }
+};
+// float32: a tile for each term
+template <int DP, int ROWS>
+struct Tile<float, DP, ROWS> {
+  using Plane = Tile<__bf16, DP, ROWS>;
+  using PlaneType = __bf16;
+  static constexpr int kRows = ROWS;
+  static constexpr bool k16 = false;
+  static constexpr int kBytes = 3 * Plane::kBytes;
+  static constexpr int kWindows = Plane::kWindows;
+  static __device__ __forceinline__ float element(const char* tile, int r, int c) {
+    return Plane::element(tile, r, c) + (Plane::element(tile + Plane::kBytes, r, c) + Plane::element(tile + 2 * Plane::kBytes, r, c));
   }
 };
 
@@ -80,48 +123,45 @@ template <typename T, int DP>
 struct Reads {
   using TL = Tile<T, DP, 32>;  // (32 rows are a multiple of every pattern)
   static constexpr int kStep16 = 16 / (1024 / TL::kRowBytes) * TL::kPitch;  // bytes of 16 rows
-  int row_at[TL::kWindows], col_at[TL::kWindows], lane;
-  __device__ __forceinline__ void init(int lane_) {
-    lane = lane_;
-    if constexpr (TL::k16) {
-      const int lq = lane & 31, g = lane >> 5, j = lane & 15, half = lane >> 4 & 1, r = 4 * g + (j >> 2);
+  int row_at[TL::kWindows], col_at[TL::kWindows];
+  __device__ __forceinline__ void init(int lane) {
+    const int lq = lane & 31, g = lane >> 5, j = lane & 15, half = lane >> 4 & 1, r = 4 * g + (j >> 2);
 #pragma unroll
-      for (int w = 0; w < TL::kWindows; ++w) {
-        row_at[w] = TL::at(lq, 4 * w + g);
-        col_at[w] = TL::at(r, 4 * w + 2 * half + ((j & 3) >> 1)) + (j & 1) * 8;
-      }
+    for (int w = 0; w < TL::kWindows; ++w) {
+      row_at[w] = TL::at(lq, 4 * w + g);
+      col_at[w] = TL::at(r, 4 * w + 2 * half + ((j & 3) >> 1)) + (j & 1) * 8;
     }
+  }
+  // the rows of another tile, `bytes` further on
+  __device__ __forceinline__ void shift_rows(int bytes) {
+#pragma unroll
+    for (int w = 0; w < TL::kWindows; ++w) row_at[w] += bytes;
   }
   // elements 16 s + 8 g .. + 7 of row 32 u + lane % 32
   __device__ __forceinline__ Frag<T> row(const char* tile, int u, int s) const {
-    if constexpr (TL::k16) {
-      return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const uint4*>(tile + row_at[s >> 1] + (s & 1) * 32 + 2 * u * kStep16));
-    } else {
-      const int p = TL::at(lane & 31, 4 * s + 2 * (lane >> 5)) + 2 * u * kStep16;
-      f32x8 f;
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + p), hi = *reinterpret_cast<const f32x4*>(tile + p + 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = lo[i], f[4 + i] = hi[i];
-      return f;
-    }
+    return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const uint4*>(tile + row_at[s >> 1] + (s & 1) * 32 + 2 * u * kStep16));
   }
   // column 32 t + lane % 32 of rows 16 m + kappa(g, 0..7)
   __device__ __forceinline__ Frag<T> col(const char* tile, int m, int t) const {
-    if constexpr (TL::k16) {
-      constexpr int n = 1024 / TL::kRowBytes;
-      const char* at = tile + col_at[t] + m * kStep16;
-      const s16x4 lo = lds_read_tr4(at), hi = lds_read_tr4(at + 8 / n * TL::kPitch);
-      typedef short s16x8 __attribute__((ext_vector_type(8)));
-      const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      return __builtin_bit_cast(Frag<T>, v);
-    } else {
-      const int c = 32 * t + (lane & 31), g = lane >> 5;
-      f32x8 f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        f[j] = *reinterpret_cast<const float*>(tile + m * kStep16 + TL::at(kappa(g, j), c >> 2) + (c & 3) * 4);
-      return f;
-    }
+    constexpr int n = 1024 / TL::kRowBytes;
+    const char* at = tile + col_at[t] + m * kStep16;
+    const s16x4 lo = lds_read_tr4(at), hi = lds_read_tr4(at + 8 / n * TL::kPitch);
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(Frag<T>, v);
+  }
+};
+template <int DP>
+struct Reads<float, DP> {
+  using Plane = typename Tile<float, DP, 32>::Plane;
+  Reads<__bf16, DP> plane;
+  __device__ __forceinline__ void init(int lane) { plane.init(lane); }
+  __device__ __forceinline__ void shift_rows(int bytes) { plane.shift_rows(bytes); }
+  __device__ __forceinline__ Terms3 row(const char* tile, int u, int s) const {
+    return Terms3{plane.row(tile, u, s), plane.row(tile + Plane::kBytes, u, s), plane.row(tile + 2 * Plane::kBytes, u, s)};
+  }
+  __device__ __forceinline__ Terms3 col(const char* tile, int m, int t) const {
+    return Terms3{plane.col(tile, m, t), plane.col(tile + Plane::kBytes, m, t), plane.col(tile + 2 * Plane::kBytes, m, t)};
   }
 };
 
@@ -173,6 +213,66 @@ struct Loader {
   }
 };
 
+// float32: the next tile's elements wait in registers, and become terms when the tile before has been read
+template <int DP>
+struct Loader<float, DP, 32> {
+  using Plane = typename Tile<float, DP, 32>::Plane;
+  static constexpr int kN = DP / 64;  // pieces of eight elements a thread
+  float v[kN][8];
+  const char* base;
+  int64_t pitch;
+  int left, bytes, row[kN], piece[kN];
+  __device__ __forceinline__ void init(const Rows& r, int, int) {
+    pitch = r.pitch;
+    bytes = r.bytes;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int n = (int)threadIdx.x + 256 * i;
+      row[i] = n / (DP / 8);
+      piece[i] = n % (DP / 8);
+    }
+  }
+  __device__ __forceinline__ void seek(const Rows& r, int row0) {
+    base = r.base + row0 * r.pitch;
+    left = (int)r.count - row0;
+  }
+  __device__ __forceinline__ void next(const char*) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const char* p = base + row[i] * pitch;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int col = piece[i] * 32 + 16 * h;
+        f32x4 x{};
+        if (row[i] < left && col < bytes) x = *reinterpret_cast<const f32x4*>(p + col);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i][4 * h + k] = x[k];
+      }
+    }
+    base += pitch * 32;
+    left -= 32;
+  }
+  __device__ __forceinline__ void land(char* tile) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const Terms3 f = split3<true>(v[i]);
+#pragma unroll
+      for (int t = 0; t < 3; ++t) *reinterpret_cast<bf16x8*>(tile + t * Plane::kBytes + Plane::at(row[i], piece[i])) = f.t[t];
+    }
+  }
+};
+// The tile that was asked for last is there, for all waves, in buffer `to` (one tile or two)
+template <typename T, typename L>
+__device__ __forceinline__ void arrived(const L& first, char* to_first, const L& second, char* to_second) {
+  if constexpr (sizeof(T) == 4) {
+    lds_barrier();  // (the tiles before have been read)
+    first.land(to_first);
+    second.land(to_second);
+  }
+  fast::vmem_wait<0>();
+  lds_barrier();
+}
+
 // A row's fragments from memory (zeros behind the size and for absent rows); `flip` changes the sign.
 template <typename T, int DP>
 __device__ __forceinline__ void load_row(Frag<T> (&f)[DP / 16], const Rows& r, int64_t row, bool valid, int g, bool flip = false) {
@@ -191,8 +291,30 @@ __device__ __forceinline__ void load_row(Frag<T> (&f)[DP / 16], const Rows& r, i
         u[i].x ^= m, u[i].y ^= m, u[i].z ^= m, u[i].w ^= m;
       }
     }
-    __builtin_memcpy(&f[s], u, sizeof(f[s]));
+    if constexpr (sizeof(T) == 2) {
+      __builtin_memcpy(&f[s], u, sizeof(f[s]));
+    } else {
+      float x[8];
+      __builtin_memcpy(x, u, sizeof(x));
+      f[s] = split3<true>(x);
+    }
   }
+}
+// sum + the product of two rows (this lane's half of their pieces)
+template <typename T, int DP>
+__device__ __forceinline__ float row_dot(const Rows& a, const Rows& b, int64_t row, bool valid, int g, float sum) {
+  constexpr int n = 16 / (int)sizeof(T);
+  const char *p = a.base + row * a.pitch, *q = b.base + row * b.pitch;
+#pragma unroll
+  for (int s = 0; s < DP / (2 * n); ++s) {
+    const int col = (2 * s + g) * 16;
+    uint4 u = make_uint4(0, 0, 0, 0), v = u;
+    if (valid && col < a.bytes) u = *reinterpret_cast<const uint4*>(p + col), v = *reinterpret_cast<const uint4*>(q + col);
+    const T *x = reinterpret_cast<const T*>(&u), *y = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < n; ++i) sum = __builtin_fmaf((float)x[i], (float)y[i], sum);
+  }
+  return sum;
 }
 
 // The order of a block's instructions: AHEAD LDS reads first, then after each of PRODUCTS matrix instructions READS more,
@@ -260,12 +382,31 @@ __device__ __forceinline__ Spans spans_of(const CausalArgs& a, int first, int la
   return s;
 }
 
+// eight of the accumulator's registers as the other operand
 template <typename T>
 __device__ __forceinline__ Frag<T> pack(const f32x16& x, int m) {
-  Frag<T> f;
+  if constexpr (sizeof(T) == 2) {
+    Frag<T> f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = (T)x[8 * m + i];
-  return f;
+    for (int i = 0; i < 8; ++i) f[i] = (T)x[8 * m + i];
+    return f;
+  } else {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[8 * m + i];
+    return split3<false>(v);
+  }
+}
+// what the rounding of pack took away (16-bit types)
+template <typename T>
+__device__ __forceinline__ Frag<T> pack_rest(const f32x16& x, int m, const Frag<T>& f) {
+  Frag<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float d = x[8 * m + i] - (float)f[i];
+    r[i] = (T)(__builtin_isfinite(d) ? d : 0.f);
+  }
+  return r;
 }
 
 // x, as a value that the compiler does not know more about: what is computed from it stays where it is written (it would
@@ -274,20 +415,15 @@ __device__ __forceinline__ uint32_t here(int x) {
   asm volatile("" : "+v"(x));
   return (uint32_t)x;
 }
-// sum + the elements of f (of 16 bits: the rounded ones, two a step)
+// sum + the elements of f, a fragment of 16 bits (two a step)
 template <typename T>
 __device__ __forceinline__ float add_elements(const Frag<T>& f, float sum) {
-  if constexpr (sizeof(T) == 2) {
-    using P2 = typename fast::Pair<T>::v2;
-    P2 x[4], ones;
-    __builtin_memcpy(x, &f, sizeof(f));
-    ones[0] = ones[1] = (T)1.0f;
+  using P2 = typename fast::Pair<T>::v2;
+  P2 x[4], ones;
+  __builtin_memcpy(x, &f, sizeof(f));
+  ones[0] = ones[1] = (T)1.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum = fast::Pair<T>::dot(x[i], ones, sum);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum += f[i];
-  }
+  for (int i = 0; i < 4; ++i) sum = fast::Pair<T>::dot(x[i], ones, sum);
   return sum;
 }
 
@@ -299,14 +435,12 @@ __device__ __forceinline__ float add_elements(const Frag<T>& f, float sum) {
 // element, what these add to the pairs that are not masked is added to the
 // accumulators one by one, and they become zeros in LDS.
 template <typename T> struct Bits;
-template <> struct Bits<float> { static constexpr uint32_t kExp = 0x7F800000u; };
 template <> struct Bits<__bf16> { static constexpr uint32_t kExp = 0x7F80u; };
 template <> struct Bits<_Float16> { static constexpr uint32_t kExp = 0x7C00u; };
-// the words (two elements of 16 bits, or one) with elements that are not finite made zero
+// two elements of 16 bits, zero where they are not finite
 template <typename T>
 __device__ __forceinline__ uint32_t finite_word(uint32_t u) {
   constexpr uint32_t e = Bits<T>::kExp;
-  if constexpr (sizeof(T) == 4) return (u & e) == e ? 0u : u;
   const uint32_t lo = (u & e) == e ? 0u : u & 0xFFFFu;
   return (u >> 16 & e) == e ? lo : lo | (u & 0xFFFF0000u);
 }
