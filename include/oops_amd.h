@@ -594,7 +594,7 @@ typedef struct oops_causal_geometry {
   int64_t length;
   int64_t stride[OOPS_CA_OPERANDS][3];
 } oops_causal_geometry;
-size_t oops_causal_attn_forward_workspace_bytes(const oops_causal_geometry* geo); /* 0 without sequences */
+size_t oops_causal_attn_forward_workspace_bytes(const oops_causal_geometry* geo);
 int oops_causal_attn_forward(const oops_causal_geometry* geo, const void* q, const void* k, const void* v,
                              const void* offsets, void* out, void* out_low, float* lse, void* workspace, size_t ws_bytes,
                              void* stream);

@@ -113,7 +113,7 @@ oops::CausalArgs causal_args(const oops_causal_geometry& given, const void* q, c
   a.offsets_i64 = g.offsets_i64;
   a.flip = std::signbit(g.scale);
   a.scale = std::fabs(g.scale);
-  a.parts = 1;
+  a.parts = a.key_splits = a.query_splits = 1;
   a.blocks = (int32_t)((g.length + 127) / 128);
   return a;
 }
@@ -121,8 +121,13 @@ size_t stat_bytes(const oops_causal_geometry& g) { return align256((size_t)(g.ba
 size_t order_bytes(const oops_causal_geometry& g) {
   return g.sequences > 0 && oops::causal_ordered(g) ? align256((size_t)((g.length + 127) / 128) * 2 * sizeof(int32_t)) : 0;
 }
-size_t part_bytes(const oops_causal_geometry& g, int parts, int size) {
-  return parts > 1 ? align256((size_t)(g.batch * g.kv_heads * g.length) * size * parts * sizeof(float)) : 0;
+size_t part_bytes(const oops_causal_geometry& g, int heads, int parts, int size) {
+  return parts > 1 ? align256((size_t)(g.batch * heads * g.length) * size * parts * sizeof(float)) : 0;
+}
+// parts of the queries' keys, and of the keys' queries
+int key_splits(const oops_causal_geometry& g) { return oops::causal_splits(g, (g.length + 127) / 128 * g.batch * g.heads); }
+int query_splits(const oops_causal_geometry& g) {
+  return oops::causal_splits(g, (g.length + 127) / 128 * g.batch * g.kv_heads * oops::causal_grad_parts(g));
 }
 
 // ---- cache
@@ -207,7 +212,8 @@ int oops_rms_norm_rotary_backward(const oops_rotary_geometry* geo, const void* q
 size_t oops_causal_attn_forward_workspace_bytes(const oops_causal_geometry* geo) {
   oops::clear_report();
   if (check_causal(geo, true)) return 0;
-  return order_bytes(*geo);
+  const int splits = key_splits(*geo);
+  return order_bytes(*geo) + part_bytes(*geo, geo->heads, splits, geo->value_size) + part_bytes(*geo, geo->heads, splits, 2);
 }
 
 int oops_causal_attn_forward(const oops_causal_geometry* geo, const void* q, const void* k, const void* v,
@@ -219,11 +225,15 @@ int oops_causal_attn_forward(const oops_causal_geometry* geo, const void* q, con
   if (!q || !k || !v || !out) return report(OOPS_EINVAL, "q, k, v and out must be non-NULL");
   if (!aligned({q, k, v, out, out_low})) return report(OOPS_EINVAL, "operands must lie at multiples of 16 bytes");
   const size_t order = offsets ? order_bytes(*geo) : 0;
-  if (int rc = oops::report_workspace(workspace, ws_bytes, order)) return rc;
+  if (int rc = oops::report_workspace(workspace, ws_bytes, oops_causal_attn_forward_workspace_bytes(geo))) return rc;
   oops::CausalArgs a = causal_args(*geo, q, k, v, offsets);
   a.out = out;
   a.low = geo->dtype == OOPS_F32 ? nullptr : out_low;
   a.lse = lse;
+  a.key_splits = key_splits(*geo);
+  char* ws = static_cast<char*>(workspace) + order_bytes(*geo);
+  a.o_parts = reinterpret_cast<float*>(ws);
+  a.stat_parts = reinterpret_cast<float*>(ws + part_bytes(*geo, geo->heads, a.key_splits, geo->value_size));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e = hipSuccess;
   if (order) {
@@ -237,8 +247,9 @@ int oops_causal_attn_forward(const oops_causal_geometry* geo, const void* q, con
 size_t oops_causal_attn_backward_workspace_bytes(const oops_causal_geometry* geo) {
   oops::clear_report();
   if (check_causal(geo, true)) return 0;
-  const int parts = oops::causal_grad_parts(*geo);
-  return order_bytes(*geo) + 2 * stat_bytes(*geo) + part_bytes(*geo, parts, geo->key_size) + part_bytes(*geo, parts, geo->value_size);
+  const int parts = oops::causal_grad_parts(*geo) * query_splits(*geo);
+  return order_bytes(*geo) + 2 * stat_bytes(*geo) + part_bytes(*geo, geo->heads, key_splits(*geo), geo->key_size) +
+         part_bytes(*geo, geo->kv_heads, parts, geo->key_size) + part_bytes(*geo, geo->kv_heads, parts, geo->value_size);
 }
 
 int oops_causal_attn_backward(const oops_causal_geometry* geo, const void* q, const void* k, const void* v,
@@ -261,6 +272,8 @@ int oops_causal_attn_backward(const oops_causal_geometry* geo, const void* q, co
   a.dk = grad_k;
   a.dv = grad_v;
   a.parts = oops::causal_grad_parts(*geo);
+  a.query_splits = query_splits(*geo);
+  a.key_splits = grad_q ? key_splits(*geo) : 1;
   char* ws = static_cast<char*>(workspace);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e = hipSuccess;
@@ -271,8 +284,9 @@ int oops_causal_attn_backward(const oops_causal_geometry* geo, const void* q, co
   ws += order_bytes(*geo);
   a.neg_lse = reinterpret_cast<float*>(ws);
   a.neg_delta = reinterpret_cast<float*>(ws += stat_bytes(*geo));
-  a.dk_parts = reinterpret_cast<float*>(ws += stat_bytes(*geo));
-  a.dv_parts = reinterpret_cast<float*>(ws + part_bytes(*geo, a.parts, geo->key_size));
+  a.dq_parts = reinterpret_cast<float*>(ws += stat_bytes(*geo));
+  a.dk_parts = reinterpret_cast<float*>(ws += part_bytes(*geo, geo->heads, key_splits(*geo), geo->key_size));
+  a.dv_parts = reinterpret_cast<float*>(ws + part_bytes(*geo, geo->kv_heads, a.parts * a.query_splits, geo->key_size));
   if (e == hipSuccess) e = oops::launch_causal_backward(geo->dtype, a, st);
   return report_launch(e, "causal attention backward");
 }

@@ -40,8 +40,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 
   const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
-  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.heads));
-  const int b = w.head / a.heads, h = w.head % a.heads;
+  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.heads * a.key_splits));
+  const int split = w.head % a.key_splits, b = w.head / a.key_splits / a.heads, h = w.head / a.key_splits % a.heads;
   const int block = a.order ? a.order[w.rank] : a.blocks - 1 - w.rank;
   const int length = (int)a.length;
 
@@ -62,7 +62,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
   Frag<T> qf[NS];
   load_row<T, DP>(qf, rows_of<T>(a.q, a.q_stride, b, h, a.key_size, length), row, valid, g, a.flip);
 
-  const int t0 = std::min(spans.first.start, block0) / KT, t1 = block1 / KT;
+  const int tile0 = std::min(spans.first.start, block0) / KT, tiles = block1 / KT + 1 - tile0;
+  const int t0 = tile0 + tiles * split / a.key_splits, t1 = tile0 + tiles * (split + 1) / a.key_splits - 1;
   Loader<T, DP> kl, vl;
   kl.init(kr, wave, lane);
   vl.init(vr, wave, lane);
@@ -79,8 +80,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
   const float c1 = fmaxf(a.scale * kLog2e, 0x1p-120f);
 
   fast::vmem_wait<0>();  // (the queries, before loads that the compiler does not count)
-  kl.next(k_lds[0]);
-  vl.next(v_lds[0]);
+  if (t0 <= t1) {
+    kl.next(k_lds[0]);
+    vl.next(v_lds[0]);
+  }
   // (the buffer is a constant, so that its address is part of the instructions)
   auto step = [&](int t, auto buffer) {
     constexpr int buf = decltype(buffer)::value % A::kBuffers, other = (buf + 1) % A::kBuffers;
@@ -109,7 +112,18 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
 #pragma unroll
       for (int i = 0; i < NS; ++i) s[u] = A::mma(rd.row(k_lds[buf], u, i), qf[i], s[u]);
     }
-    if constexpr (TL::k16) interleave<6, SUB * NS, 1>();
+    if constexpr (TL::k16) {
+      interleave<6, SUB * NS, 1>();
+    } else {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+        mend_scores(s[u], [&] {
+          f32x16 f{};
+#pragma unroll
+          for (int i = 0; i < NS; ++i) f = Elem<__bf16>::mma(rd.row(k_lds[buf], u, i).t[0], qf[i].t[0], f);
+          return f;
+        });
+    }
     if (k0 < last_start || k0 + KT - 1 > q0) {
       const uint32_t from = here(k0 + 4 * g - start), far = empty ? 0u : reach + 1;
 #pragma unroll
@@ -163,7 +177,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
       interleave<8, NDT * (KT / 16), 2, 5>();
     }
   };
-  for (int t = t0;;) {
+  for (int t = t0; t <= t1;) {
     step(t, std::integral_constant<int, 0>{});
     if (++t > t1) break;
     step(t, std::integral_constant<int, 1>{});
@@ -174,6 +188,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
   // (a row without keys: zeros; one whose logits are all -inf: 0 / 0)
   const float inv = empty ? 0.f : 1.0f / l;
   if (!valid) return;
+  if (a.key_splits > 1) {
+    const int64_t at = (((int64_t)split * a.batch + b) * a.heads + h) * length + row;
+    if (g == 0) a.stat_parts[2 * at] = m_run, a.stat_parts[2 * at + 1] = empty ? -1.f : l;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d)
+      store_columns<float>(reinterpret_cast<char*>(a.o_parts + at * a.value_size), 32 * d, a.value_size, g, o[d], 1.f);
+    return;
+  }
   if (a.lse && g == 0) a.lse[((int64_t)b * a.heads + h) * length + row] = empty ? 0.f : m_run + __builtin_amdgcn_logf(l);
   const int64_t at = (b * a.o_stride[0] + h * a.o_stride[1] + row * a.o_stride[2]) * (int64_t)sizeof(T);
 #pragma unroll
@@ -184,17 +206,70 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
   }
 }
 
+// Rows whose keys were split: the parts by their maxima and sums, in order; four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void causal_join_kernel(CausalArgs a, int64_t cells) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= cells) return;
+  const int64_t rows = cells / a.value_size, row = i / a.value_size;
+  const int d = (int)(i - row * a.value_size);
+  float m = kNegInf;
+  for (int s = 0; s < a.key_splits; ++s) m = fmaxf(m, a.stat_parts[2 * (s * rows + row)]);
+  const bool empty = a.stat_parts[2 * row + 1] == -1.f;
+  float l = 0.f;
+  f32x4 x{};
+  for (int s = 0; s < a.key_splits; ++s) {
+    const float part = a.stat_parts[2 * (s * rows + row)], by = part == m ? 1.f : __builtin_amdgcn_exp2f(part - m);
+    l = __builtin_fmaf(a.stat_parts[2 * (s * rows + row) + 1], by, l);
+    const f32x4 o = *reinterpret_cast<const f32x4*>(a.o_parts + s * cells + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = __builtin_fmaf(o[k], by, x[k]);
+  }
+  const float inv = empty ? 0.f : 1.0f / l;
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  v4 y, low;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float v = empty ? 0.f : x[k] * inv;
+    y[k] = (T)v;
+    const float r = v - (float)y[k];
+    low[k] = (T)(__builtin_isfinite(r) ? r : 0.f);
+  }
+  const int64_t token = row % a.length, h = row / a.length % a.heads, b = row / a.length / a.heads;
+  const int64_t at = b * a.o_stride[0] + h * a.o_stride[1] + token * a.o_stride[2] + d;
+  *reinterpret_cast<v4*>(static_cast<T*>(a.out) + at) = y;
+  if (a.low) *reinterpret_cast<v4*>(static_cast<T*>(a.low) + at) = low;
+  if (a.lse && d == 0) a.lse[row] = empty ? 0.f : m + __builtin_amdgcn_logf(l);
+}
+
 }  // namespace
 }  // namespace causal
 
+// Parts of the axis that a workgroup walks along (keys for queries, queries for keys), so that few workgroups fill the
+// chip's 512 places and its longest walk gets shorter; parts of fewer than four tiles cost more in joining than they
+// save.  us of kernels, forward / with the backward, in one part and in parts:
+//   1 head of 16384 tokens, 128 channels, bf16   315 / 1350   119 / 469   (for 1024 places 105 / 428)
+//   2 heads of 4096                               88 /  373    38 / 138   (49 / 185)
+//   8 heads of 2048, float32                     253 /  912   100 / 359   (123 / 460)
+//   2 x 6 heads of 777, 40 channels, float32      60 /  230    37 / 103
+//   the same in bf16: three parts 19 / 61, one 21 / 74, six (of two tiles) 22 / 62
+int causal_splits(const oops_causal_geometry& g, int64_t workgroups) {
+  const int64_t tokens = g.length / std::max(g.sequences, 1), tile = g.dtype == OOPS_F32 ? 32 : 64;
+  return workgroups < 1 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(511 + workgroups) / workgroups, tokens / (4 * tile), 16}));
+}
+
 hipError_t launch_causal_forward(int dtype, const CausalArgs& a, hipStream_t stream) {
   if (a.length == 0 || a.batch == 0) return hipSuccess;
-  const dim3 grid((uint32_t)a.blocks * (uint32_t)(a.batch * a.heads));
+  const dim3 grid((uint32_t)a.blocks * (uint32_t)(a.batch * a.heads * a.key_splits));
+  const int64_t cells = a.batch * a.heads * a.length * a.value_size;
   const bool wide = a.key_size > 64 || a.value_size > 64;
   auto go = [&](auto tag) {
     using T = decltype(tag);
     if (wide) hipLaunchKernelGGL((causal::causal_forward_kernel<T, 128>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((causal::causal_forward_kernel<T, 64>), grid, dim3(256), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.key_splits == 1) return e;
+    hipLaunchKernelGGL((causal::causal_join_kernel<T>), dim3((uint32_t)((cells / 4 + 255) / 256)), dim3(256), 0, stream, a, cells);
     return hipGetLastError();
   };
   if (dtype == OOPS_F32) return go(float{});

@@ -38,8 +38,8 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
 
   const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
-  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.heads));
-  const int b = w.head / a.heads, h = w.head % a.heads;
+  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.heads * a.key_splits));
+  const int split = w.head % a.key_splits, b = w.head / a.key_splits / a.heads, h = w.head / a.key_splits % a.heads;
   const int block = a.order ? a.order[w.rank] : a.blocks - 1 - w.rank;
   const int length = (int)a.length;
 
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   const float c1 = fmaxf(a.scale * kLog2e, 0x1p-120f);
   const int64_t stat = ((int64_t)b * a.heads + h) * length + row;
   const float lse = valid ? a.lse[stat] : 0.f;
-  if (valid && g == 0) {
+  if (valid && g == 0 && split == 0) {
     // (as the second kernel's accumulators start)
     a.neg_delta[stat] = -delta;
     a.neg_lse[stat] = -lse / c1;
@@ -74,7 +74,8 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
 
   const Rows kr = rows_of<T>(a.k, a.k_stride, b, h / a.group, a.key_size, length);
   const Rows vr = rows_of<T>(a.v, a.v_stride, b, h / a.group, a.value_size, length);
-  const int t0 = std::min(spans.first.start, block0) / KT, t1 = block1 / KT;
+  const int tile0 = std::min(spans.first.start, block0) / KT, tiles = block1 / KT + 1 - tile0;
+  const int t0 = tile0 + tiles * split / a.key_splits, t1 = tile0 + tiles * (split + 1) / a.key_splits - 1;
   Loader<T, DP> kl, vl;
   kl.init(kr, wave, lane);
   vl.init(vr, wave, lane);
@@ -88,8 +89,10 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   for (int t = 0; t < NDT; ++t) dq[t] = f32x16{};
 
   fast::vmem_wait<0>();  // (the rows, before loads that the compiler does not count)
-  kl.next(k_lds[0]);
-  vl.next(v_lds[0]);
+  if (t0 <= t1) {
+    kl.next(k_lds[0]);
+    vl.next(v_lds[0]);
+  }
   auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
     constexpr int buf = decltype(buffer)::value % A::kBuffers, other = (buf + 1) % A::kBuffers;
     const int k0 = t * KT;
@@ -119,7 +122,16 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
       for (int i = 0; i < NS; ++i) s = A::mma(rd.row(k_lds[buf], u, i), qf[i], s);
 #pragma unroll
       for (int i = 0; i < NS; ++i) dp = A::mma(rd.row(v_lds[buf], u, i), dof[i], dp);
-      if constexpr (TL::k16) interleave<6, 2 * NS, 1>();
+      if constexpr (TL::k16) {
+        interleave<6, 2 * NS, 1>();
+      } else {
+        mend_scores(s, [&] {
+          f32x16 f{};
+#pragma unroll
+          for (int i = 0; i < NS; ++i) f = Elem<__bf16>::mma(rd.row(k_lds[buf], u, i).t[0], qf[i].t[0], f);
+          return f;
+        });
+      }
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c1, -lse)) * (dp[j] - delta);
       if (lost) {
@@ -141,7 +153,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
       if constexpr (TL::k16) interleave<8, 2 * NDT, 2>();
     }
   };
-  for (int t = t0;;) {
+  for (int t = t0; t <= t1;) {
     step(t, std::integral_constant<int, 0>{});
     if (++t > t1) break;
     step(t, std::integral_constant<int, 1>{});
@@ -149,6 +161,13 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   }
   if (!valid) return;
   const float scale = a.flip ? -a.scale : a.scale;
+  if (a.key_splits > 1) {
+    const int64_t at = (((int64_t)split * a.batch + b) * a.heads + h) * length + row;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d)
+      store_columns<float>(reinterpret_cast<char*>(a.dq_parts + at * a.key_size), 32 * d, a.key_size, g, dq[d], scale);
+    return;
+  }
   char* to = static_cast<char*>(a.dq) + (b * a.dq_stride[0] + h * a.dq_stride[1] + row * a.dq_stride[2]) * (int64_t)sizeof(T);
 #pragma unroll
   for (int d = 0; d < NDT; ++d) store_columns<T>(to, 32 * d, a.key_size, g, dq[d], scale);
@@ -182,8 +201,10 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
 
   const int tid = threadIdx.x, lane = tid & 63, lk = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
-  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.kv_heads * a.parts));
-  const int part = w.head % a.parts, hk = w.head / a.parts % a.kv_heads, b = w.head / a.parts / a.kv_heads;
+  const int parts = a.parts * a.query_splits;
+  const Work w = work_of(blockIdx.x, (uint32_t)(a.batch * a.kv_heads * parts));
+  const int part = w.head % parts, hk = w.head / parts % a.kv_heads, b = w.head / parts / a.kv_heads;
+  const int heads_part = part / a.query_splits, split = part % a.query_splits;
   const int block = a.order ? a.order[a.blocks + w.rank] : w.rank;
   const int length = (int)a.length;
 
@@ -204,8 +225,9 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   if constexpr (!kValuesInLds) load_row<T, DP>(vf, vr, key, valid, g);
 
   const int block_end = std::max(spans.last.end, block1 + 1);
-  const int t0 = block0 / QT, t1 = (block_end - 1) / QT;
-  const int h0 = hk * a.group + part * a.group / a.parts, h1 = hk * a.group + (part + 1) * a.group / a.parts;
+  const int tile0 = block0 / QT, tiles = (block_end - 1) / QT + 1 - tile0;
+  const int t0 = tile0 + tiles * split / a.query_splits, t1 = tile0 + tiles * (split + 1) / a.query_splits - 1;
+  const int h0 = hk * a.group + heads_part * a.group / a.parts, h1 = hk * a.group + (heads_part + 1) * a.group / a.parts;
 
   f32x16 dk[NDT], dv[NDT];
 #pragma unroll
@@ -252,8 +274,12 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
       if constexpr (!TL::k16) vl.land(v_lds[i]);
     }
   }
-  seek();
-  load(std::integral_constant<int, 0>{});
+  if (t0 <= t1) {
+    seek();
+    load(std::integral_constant<int, 0>{});
+  } else {
+    fast::vmem_wait<0>();  // (nothing may land in LDS that is another workgroup's by then)
+  }
   auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
     constexpr int now = decltype(buffer)::value, buf = now % A::kBuffers;
     const int q0 = t * QT;
@@ -292,6 +318,15 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
       // (the statistics' eight reads first)
       interleave<12, NS, 1>();
       interleave<kValuesInLds ? 2 : 0, NS, kValuesInLds ? 2 : 1>();
+    } else {
+      mend_scores(s, [&] {
+        f32x16 f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f[j] = lse_lds[now][kappa(g, j)];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) f = Elem<__bf16>::mma(rd.row(q_lds[buf], 0, i).t[0], kf[i].t[0], f);
+        return f;
+      });
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -317,7 +352,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
       }
     if constexpr (TL::k16) interleave<8, 4 * NDT, 2>();
   };
-  for (int h = h0, t = t0;;) {
+  for (int h = h0, t = t0; t0 <= t1;) {
     auto next = [&] {
       if (++t > t1) t = t0, ++h;
       return h < h1;
@@ -329,7 +364,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   }
   if (!valid) return;
   const float scale = a.flip ? -a.scale : a.scale;
-  if (a.parts > 1) {
+  if (parts > 1) {
     const int64_t at = (((int64_t)part * a.batch + b) * a.kv_heads + hk) * length + key;
 #pragma unroll
     for (int d = 0; d < NDT; ++d) {
@@ -431,24 +466,27 @@ hipError_t launch_causal_backward(int dtype, const CausalArgs& a, hipStream_t st
   if (a.length == 0 || a.batch == 0) return hipSuccess;
   const uint32_t blocks = (uint32_t)a.blocks;
   const bool wide = a.key_size > 64 || a.value_size > 64;
-  const dim3 grid_q(blocks * (uint32_t)(a.batch * a.heads)), grid_kv(blocks * (uint32_t)(a.batch * a.kv_heads * a.parts));
+  const dim3 grid_q(blocks * (uint32_t)(a.batch * a.heads * a.key_splits));
+  const int parts = a.parts * a.query_splits;
+  const dim3 grid_kv(blocks * (uint32_t)(a.batch * a.kv_heads * parts));
   auto go = [&](auto tag) {
     using T = decltype(tag);
     if (wide) hipLaunchKernelGGL((causal::causal_grad_query_kernel<T, 128>), grid_q, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((causal::causal_grad_query_kernel<T, 64>), grid_q, dim3(256), 0, stream, a);
     hipError_t e = hipGetLastError();
+    auto add = [&](const float* from, void* out, const int64_t(&s)[3], int heads, int size, int count) {
+      const int64_t cells = a.batch * heads * a.length * size;
+      hipLaunchKernelGGL((causal::causal_parts_kernel<T>), dim3((uint32_t)((cells / 4 + 255) / 256)), dim3(256), 0, stream, from,
+                         out, s[0], s[1], s[2], (int64_t)heads, a.length, size, count, cells);
+      return hipGetLastError();
+    };
+    if (e == hipSuccess && a.dq && a.key_splits > 1) e = add(a.dq_parts, a.dq, a.dq_stride, a.heads, a.key_size, a.key_splits);
     if (e != hipSuccess || (!a.dk && !a.dv)) return e;
     if (wide) hipLaunchKernelGGL((causal::causal_grad_key_value_kernel<T, 128>), grid_kv, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((causal::causal_grad_key_value_kernel<T, 64>), grid_kv, dim3(256), 0, stream, a);
     e = hipGetLastError();
-    auto add = [&](const float* parts, void* out, const int64_t(&s)[3], int size) {
-      const int64_t cells = a.batch * a.kv_heads * a.length * size;
-      hipLaunchKernelGGL((causal::causal_parts_kernel<T>), dim3((uint32_t)((cells / 4 + 255) / 256)), dim3(256), 0, stream, parts,
-                         out, s[0], s[1], s[2], (int64_t)a.kv_heads, a.length, size, a.parts, cells);
-      return hipGetLastError();
-    };
-    if (e == hipSuccess && a.parts > 1 && a.dk) e = add(a.dk_parts, a.dk, a.dk_stride, a.key_size);
-    if (e == hipSuccess && a.parts > 1 && a.dv) e = add(a.dv_parts, a.dv, a.dv_stride, a.value_size);
+    if (e == hipSuccess && parts > 1 && a.dk) e = add(a.dk_parts, a.dk, a.dk_stride, a.kv_heads, a.key_size, parts);
+    if (e == hipSuccess && parts > 1 && a.dv) e = add(a.dv_parts, a.dv, a.dv_stride, a.kv_heads, a.value_size, parts);
     return e;
   };
   if (dtype == OOPS_F32) return go(float{});

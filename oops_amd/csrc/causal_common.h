@@ -409,6 +409,20 @@ __device__ __forceinline__ Frag<T> pack_rest(const f32x16& x, int m, const Frag<
   return r;
 }
 
+// float32: a score that holds an infinity has met the other operand's lower terms, of either sign, and is NaN; such a
+// score is taken from the largest terms alone, where it is what the formula has.  first(): those products' sum.
+template <typename First>
+__device__ __forceinline__ void mend_scores(f32x16& s, First first) {
+  float t = s[0];
+#pragma unroll
+  for (int j = 1; j < 16; ++j) t += s[j];
+  if (__any(t != t)) {
+    const f32x16 f = first();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[j] = s[j] != s[j] ? f[j] : s[j];
+  }
+}
+
 // x, as a value that the compiler does not know more about: what is computed from it stays where it is written (it would
 // else keep sixteen sums in registers, or in scratch, for masked tiles to come)
 __device__ __forceinline__ uint32_t here(int x) {

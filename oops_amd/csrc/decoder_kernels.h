@@ -23,19 +23,23 @@ struct CausalArgs {
   float* lse;          // (batch, heads, length), log2 units
   float *neg_lse, *neg_delta;  // the same shape: -lse over the scores' factor, -delta
   const int32_t* order;        // blocks of queries, then of keys, the heaviest first (NULL: by their place)
-  float *dk_parts, *dv_parts;
+  float *o_parts, *dq_parts, *dk_parts, *dv_parts;
+  float* stat_parts;           // of o_parts: maximum and sum (-1: a row without keys)
   int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], do_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
   int64_t batch, length;
   int32_t heads, kv_heads, group, key_size, value_size, sequences, offsets_i64;
   int32_t flip;        // the scale is negative: `scale` is its magnitude, and the scores' sign is changed
   float scale;
   int32_t parts;       // of the query heads of a group in the key/value gradient
-  int32_t blocks;      // of 128 tokens
+  int32_t key_splits;   // of a block of queries' keys, in the forward or the queries' gradient
+  int32_t query_splits; // of a block of keys' queries
+  int32_t blocks;       // of 128 tokens
 };
 bool causal_ordered(const oops_causal_geometry& g);
 hipError_t launch_causal_order(const CausalArgs& a, int32_t* order, hipStream_t stream);
 hipError_t launch_causal_forward(int dtype, const CausalArgs& a, hipStream_t stream);
 int causal_grad_parts(const oops_causal_geometry& g);
+int causal_splits(const oops_causal_geometry& g, int64_t workgroups);
 hipError_t launch_causal_backward(int dtype, const CausalArgs& a, hipStream_t stream);
 
 // ---- cache.hip

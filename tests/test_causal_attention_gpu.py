@@ -429,3 +429,43 @@ def test_into_the_gated_output_stage():
     out = gate_attention_output(att, y, wg, wo)
     want = (torch.sigmoid(y.double() @ wg.double().t()) * att.double().transpose(1, 2).flatten(2)) @ wo.double().t()
     assert ((out.double() - want).norm() / want.norm()).item() <= 4 * half(torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offsets", [None, [0, 1100], [0, 3, 1000], [40, 1060], [0, 0, 1100, 1100]])
+def test_few_heads_of_long_rows(dtype, offsets):
+    """Walks that are split into parts and joined, some of which have no tile, or no pair of a row, among them."""
+
+    _run(_case(31, 1, 2, 1, 1100, 48, 64, dtype), offsets)
+    if offsets is None:
+        _run(_case(32, 1, 1, 1, 1100, 128, 128, dtype), scale=-0.05)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_non_finite_values_of_split_rows(dtype):
+    """Tokens before an infinity or a NaN have the values that they have without it; from it on nothing is finite."""
+
+    x = _case(33, 1, 1, 1, 1200, 32, 32, dtype)
+    clean = _run(x)
+    for name, value in (("k", float("nan")), ("v", float("inf")), ("v", float("nan"))):
+        y = {n: t.clone() for n, t in x.items()}
+        y[name][0, 0, 700, 5] = value
+        leaves = [y[n].requires_grad_(True) for n in ("q", "k", "v")]
+        out = causal_attention(*leaves)
+        assert torch.equal(out[:, :, :700], clean[0][:, :, :700])
+        rest = out[:, :, 700:] if name == "k" else out[:, :, 700:, 5]
+        assert not torch.isfinite(rest).any()
+        if name == "v":
+            other = [c for c in range(32) if c != 5]
+            assert torch.equal(out[..., other], clean[0][..., other])
+        dq, _, _ = torch.autograd.grad(out, leaves, x["do"])
+        assert torch.equal(dq[:, :, :700], clean[1][:, :, :700])
+    y = x["k"].clone()
+    y[0, 0, :1150] = 0
+    y[0, 0, :1150, 0] = float("-inf")
+    q = x["q"].abs()
+    # (every logit of a row -inf: 0 / 0; the tokens with others have those alone)
+    out = causal_attention(q, y, x["v"])
+    assert out[:, :, :1150].isnan().all()
+    alone = causal_attention(q[:, :, 1150:].contiguous(), y[:, :, 1150:].contiguous(), x["v"][:, :, 1150:].contiguous())
+    assert ((out[:, :, 1150:].double() - alone.double()).norm() / alone.double().norm()).item() <= 2 * half(dtype) + 2000 * U
