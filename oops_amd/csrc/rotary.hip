@@ -14,6 +14,11 @@
 // tokens and their groups of heads, queries and keys in one launch; dw stays in
 // registers meanwhile, and the workgroups' partial rows are added in a fixed order by
 // a second launch.
+//
+// 8192 tokens of 32 + 8 heads of 128, bfloat16: forward 37 us (4.5 TB/s; one head at a
+// time 50, two 43), backward 61 (4.1 TB/s, two heads at a time; one 66) and 7 for the sums
+// of dw; a large copy reaches 4.9-5.1.  One token of four sequences: 5.4 us, a launch and
+// a chain of loads.
 #include <algorithm>
 
 #include "attn_common.h"
