@@ -66,9 +66,8 @@ def causal_attention(
     accumulators are float32.  As operands of the next product, bfloat16's probabilities are rounded to the type,
     float16's forward ones to two terms of it (22 bits), and in the backward 16-bit types round probabilities and the
     scores' gradients, which in float16 have to stay in its range (scale the loss, as elsewhere).  float32 operands
-    are three bfloat16 terms: a product is off by 2^-23 of itself at most and 2^-26 on average (elements above 3.39e38 lose
-    their last bits).  Infinities and NaN reach the tokens whose sum holds them, and no others: neither earlier tokens
-    nor other sequences.
+    are three bfloat16 terms: a product is off by 2^-23 of itself at most and 2^-26 on average.  Infinities and NaN reach
+    the tokens whose sum holds them, and no others: neither earlier tokens nor other sequences.
     """
 
     _check(query, key, value, offsets)

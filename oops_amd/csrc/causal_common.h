@@ -1,14 +1,14 @@
 // Device code shared by the causal attention kernels (forward and backward).
 //
-// Every product is a 32 x 32 x 16 step on fragments of eight elements a lane:
-// one MFMA of a 16-bit type.  float32 operands are three bfloat16 terms, their sum
+// Every product is a 32 x 32 x 16 step on fragments of eight elements a lane: one
+// MFMA of a 16-bit type.  float32 operands are three bfloat16 terms, their sum
 // exactly, and a step is six MFMAs, the terms' products down to 2^-16 of the largest
-// (what is left out is below 2^-23, and 2^-26 on average): 192 cycles where the float32 matrix unit, exact
-// too, takes 512.  Lane (c =
-// lane % 32, g = lane / 32) holds elements 16 s + 8 g .. + 7 of row c along
-// the contracted axis.  An accumulator's rows are kappa(g, j), so eight of its
-// registers are the other operand of the next product as they stand, if the
-// tile in LDS is read in the same order (tr_frag).
+// (what is left out is below 2^-23, and 2^-26 on average): 192 cycles where the
+// float32 matrix unit takes 512.  Lane (c = lane % 32, g = lane / 32)
+// holds elements 16 s + 8 g .. + 7 of row c along the contracted axis.  An
+// accumulator's rows are kappa(g, j), so eight of its registers are the other
+// operand of the next product as they stand, if the tile in LDS is read in the same
+// order (Reads::col).
 //
 // Tiles of 32 or 64 rows go from memory straight to LDS in 16-byte pieces, a
 // kilobyte at a time (4 rows of 128 elements of 16 bits, 8 of 64).  Inside it a
