@@ -469,3 +469,29 @@ def test_non_finite_values_of_split_rows(dtype):
     assert out[:, :, :1150].isnan().all()
     alone = causal_attention(q[:, :, 1150:].contiguous(), y[:, :, 1150:].contiguous(), x["v"][:, :, 1150:].contiguous())
     assert ((out[:, :, 1150:].double() - alone.double()).norm() / alone.double().norm()).item() <= 2 * half(dtype) + 2000 * U
+
+
+def test_graphs_of_split_rows():
+    """Two captured training steps whose walks are split, replayed in turn beside eager calls: the eager bits each time."""
+
+    cases = [_case(41, 1, 2, 1, 1100, 64, 64, torch.bfloat16), _case(42, 1, 3, 3, 700, 40, 32, torch.float32)]
+    want = []
+    side = torch.cuda.Stream()
+    for x in cases:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want.append(_run_bits(x))
+        torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for x in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = _run_bits(x)
+        graphs.append((graph, got))
+    for _ in range(3):
+        for (graph, got), expected, x in zip(graphs, want, cases):
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(got, expected))
+            assert all(torch.equal(a, b) for a, b in zip(_run_bits(x), expected))
+        torch.cuda.synchronize()

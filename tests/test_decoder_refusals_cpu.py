@@ -159,6 +159,12 @@ def test_causal_entry_points(lib):
     need = lib.oops_causal_attn_forward_workspace_bytes(ctypes.byref(many))
     assert need == (1 << 16) // 128 * 2 * 4 and lib.oops_causal_attn_forward_workspace_bytes(ctypes.byref(geo(sequences=3))) == 0
     _refused(lib, forward(many, offsets=FAKE), 3, "workspace")
+    # few workgroups' walks are split: their parts of the output, and two statistics of each
+    few = geo(length=1024)
+    need = lib.oops_causal_attn_forward_workspace_bytes(ctypes.byref(few))
+    assert need == 4 * (4 * 1024 * 64 * 4 + 4 * 1024 * 2 * 4)
+    _refused(lib, forward(few), 3, "workspace")
+    _refused(lib, forward(few, ws=FAKE, n=need - 1), 3, "workspace")
     need = lib.oops_causal_attn_backward_workspace_bytes(ctypes.byref(geo()))
     stats, parts = 2 * 256, 2 * 8 * 2 * 64 * 4 * 2  # lse and delta; two parts of dk and of dv
     assert need == stats + parts
