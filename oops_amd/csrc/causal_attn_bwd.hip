@@ -166,7 +166,8 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
     if (++t > t1) break;
   }
   if (!valid) return;
-  const float scale = a.flip ? -a.scale : a.scale;
+  // (a row of one key: its weight is 1 whatever the score, and what dS has is the roundings of two sums)
+  const float scale = reach == 0 ? 0.f : a.flip ? -a.scale : a.scale;
   if (a.key_splits > 1) {
     const int64_t at = (((int64_t)split * a.batch + b) * a.heads + h) * length + row;
 #pragma unroll
@@ -191,8 +192,9 @@ __device__ __forceinline__ void dma4_asm(const fast::u32x4& r, const void* lds, 
       : "memory", "m0");
 }
 
+// (float32: one workgroup a CU, whose waves have 512 registers; with two, 42 of 256 spill)
 template <typename T, int DP>
-__global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kernel(CausalArgs a) {
+__global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void causal_grad_key_value_kernel(CausalArgs a) {
   using TL = Tile<T, DP, 32>;
   using A = Att<T>;
   constexpr int QT = 32, NS = DP / 16, NDT = DP / 32;
@@ -223,6 +225,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
   // queries this lane's key is paired with: [key, key + width)
   const int end = spans.own.end;
   const uint32_t width = valid && end > key ? (uint32_t)(end - key) : 0u;
+  const bool alone = valid && spans.own.start == key;  // (the only key of the first row)
   const int first_end = __builtin_amdgcn_readlane(end, 0), last_end = __builtin_amdgcn_readlane(end, idle ? 0 : last - k0);
 
   Frag<T> kf[NS], vf[kValuesInLds ? 1 : NS];
@@ -347,6 +350,12 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_key_value_kern
         s[j] = pair ? s[j] : 0.f;
         dp[j] = pair ? dp[j] : 0.f;
       }
+    }
+    if (__any(alone && key >= q0 && key < q0 + QT)) {
+      // (a row of one key has no dS: what is left is the roundings of two sums, or NaN)
+      const uint32_t from = here(q0 + 4 * g - key);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) dp[j] = alone && from + kappa(0, j) == 0 ? 0.f * dp[j] : dp[j];
     }
     const Frag<T> p[2] = {pack<T>(s, 0), pack<T>(s, 1)}, ds[2] = {pack<T>(dp, 0), pack<T>(dp, 1)};
 #pragma unroll

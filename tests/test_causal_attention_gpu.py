@@ -495,3 +495,12 @@ def test_graphs_of_split_rows():
             assert all(torch.equal(a, b) for a, b in zip(got, expected))
             assert all(torch.equal(a, b) for a, b in zip(_run_bits(x), expected))
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,offsets", [(1, None), (40, list(range(41)))])
+def test_rows_of_one_key(dtype, n, offsets):
+    """A weight that is 1 whatever its score: dQ and dK are zeros, to the last bit."""
+
+    _, dq, dk, _ = _run(_case(51, 2, 4, 2, n, 64, 48, dtype), offsets)
+    assert not dq.any() and not dk.any()
