@@ -17,10 +17,10 @@
 // a lane loads its token's codes as they lie in memory, and the channels' order is
 // the query's fragments'.  S^T leaves the probabilities as the second product's
 // operand; V^T comes from LDS by transposed reads (each wave has a region of its
-// own, so there is no barrier in the loop).  float16 and float32 queries and
-// probabilities are split into two and three bfloat16 terms, whose products are
-// exact and added in float32: a result has its own type's precision whatever the
-// cache's.  Few sequences are split over their length; a second launch joins the
+// own, so there is no barrier in the loop).  float16 and float32 queries are split
+// into two and three bfloat16 terms, probabilities into two (three for float32),
+// whose products are exact and added in float32: a result has its own type's
+// precision whatever the cache's.  Few sequences are split over their length; a second launch joins the
 // parts by their maxima and sums.
 //
 // bfloat16, 8 key heads of 128, 32 query heads: writing 30011 tokens 48 us (157 MB at
@@ -265,18 +265,22 @@ struct DecodeArgs {
   float scale;
 };
 
-template <typename T> struct Terms { static constexpr int N = 2; };
-template <> struct Terms<__bf16> { static constexpr int N = 1; };
-template <> struct Terms<float> { static constexpr int N = 3; };
+// Terms of a query's elements, and of weights: bfloat16's have two like float16's, 16 bits.  (One would round the weights but
+// not their sum, and a rounding that many weights share would stay in the result: up to half a step of bfloat16 beside the
+// result's own, for 178 us in place of 182 of 64 sequences of up to 16384 tokens, 8 key heads of 128.)
+template <typename T> struct Terms { static constexpr int N = 2, kWeight = 2; };
+template <> struct Terms<__bf16> { static constexpr int N = 1, kWeight = 2; };
+template <> struct Terms<float> { static constexpr int N = 3, kWeight = 3; };
 
-// x as bfloat16 terms, whose sum is x for the types above (an infinity or a NaN is the first term's alone)
-template <int N>
+// x as bfloat16 terms, whose sum is x for the types above (an infinity or a NaN is the first term's alone; FINITE: x is no
+// infinity, and a NaN may be every term)
+template <int N, bool FINITE = false>
 __device__ __forceinline__ void split(float x, __bf16 (&t)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     t[i] = (__bf16)x;
     x -= (float)t[i];
-    if (!__builtin_isfinite(x)) x = 0.f;
+    if (!FINITE && !__builtin_isfinite(x)) x = 0.f;
   }
 }
 
@@ -312,7 +316,7 @@ __device__ __forceinline__ float sum_rows(float x) {
 
 template <typename T, int NS>
 __global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(DecodeArgs a) {
-  constexpr int N = Terms<T>::N, D = 32 * NS, ND = D / 16;
+  constexpr int N = Terms<T>::N, W = Terms<T>::kWeight, D = 32 * NS, ND = D / 16;
   // channels of step s of lane group g: with four steps a lane's sixteen bytes lie together
   auto channel = [](int s, int g) { return NS == 4 ? 32 * g + 8 * s : 32 * s + 8 * g; };
   constexpr int kPitch = 2 * D + 32;  // bytes: 8 rows' pieces of 32 bytes lie in different banks
@@ -471,17 +475,17 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(DecodeArgs a) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] *= alpha;
     }
-    bf16x8 p[N];
+    bf16x8 p[W];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float x = __builtin_amdgcn_exp2f(st[i][r] + neg_m);
         l_run += x;
-        __bf16 t[N];
-        split<N>(x, t);
+        __bf16 t[W];
+        split<W, true>(x, t);
 #pragma unroll
-        for (int n = 0; n < N; ++n) p[n][4 * i + r] = t[n];
+        for (int n = 0; n < W; ++n) p[n][4 * i + r] = t[n];
       }
     // O^T += V^T P^T; lane (c, g) gets V[4 g + k][16 d + c] for k = 0..3, then rows + 16
     asm volatile("" ::: "memory");
@@ -492,7 +496,14 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(DecodeArgs a) {
       typedef short s16x8 __attribute__((ext_vector_type(8)));
       const bf16x8 v = __builtin_bit_cast(bf16x8, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
 #pragma unroll
-      for (int n = 0; n < N; ++n) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n], o[d], 0, 0, 0);
+      for (int n = 0; n < W; ++n) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[n], o[d], 0, 0, 0);
+    }
+    // (two of V's fragments ahead of the products: left alone, the compiler waits for each, 8 us of such a batch's)
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      __builtin_amdgcn_sched_group_barrier(0x008, W, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
     asm volatile("" ::: "memory");
   }
