@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from layer_tolerance import U, assert_within, f64, half
+from layer_tolerance import U, assert_within, f64, half, smallest
 from oops_amd import cache_attention, cache_write, quantized_cache
 from oracle import decoder
 
@@ -47,3 +47,19 @@ def test_a_rounding_that_many_weights_share(dtype, n):
         want = decoder.cache_attention(f64(q), kv, table.cpu().numpy(), [n], scale)
         bound = half(dtype) * np.abs(want) * (1 + 2.0**-8) + (2.0**-16 if dtype != torch.float32 else 0) * np.abs(want)
         assert_within(out, want, bound + 2 * (n + 16) * U * np.abs(want), f"part {part:.2f}")
+
+
+def test_queries_above_the_largest_bfloat16():
+    """float32 numbers that bfloat16 would round to infinity: scores that float32 holds, and zeros, are what they are."""
+
+    d, n = 32, 64
+    key, value = torch.zeros(1, n, d, device=DEV), torch.zeros(1, n, d, device=DEV)
+    key[0, :, 0] = torch.tensor([0, 0.5, 1, -1] * (n // 4), device=DEV)
+    value[0] = (torch.arange(n, device=DEV) % 4)[:, None].float()
+    cache, table, kv = _filled(key, value)
+    q = torch.zeros(2, 1, d, device=DEV)
+    q[0, 0, 0], q[1, 0, 0] = 3.4e38, -3.3999e38
+    out = cache_attention(q, *cache, table.expand(2, 1), torch.tensor([n, n], device=DEV), scale=1e-38)
+    want = decoder.cache_attention(f64(q), kv, table.cpu().numpy().repeat(2, 0), [n, n], 1e-38)
+    # a score of up to 3.4: 100 U of it as in the other tests; 64 terms
+    assert_within(out, want, (np.expm1(2 * 104 * U * 3.4) + 200 * U) * 3 + smallest(torch.float32), "out")
