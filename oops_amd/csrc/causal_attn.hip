@@ -104,59 +104,65 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
       vl.next(v_lds[other]);
     }
     auto keep = [&](int r) { return !empty && (uint32_t)(k0 + r - start) <= reach; };
+    const bool mine = !(idle || k0 > last || k0 + KT <= first_start);
+    f32x16 s[SUB];
+    // this tile's scores, and the running maximum with them
+    auto scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        s[u] = f32x16{};
+#pragma unroll
+        for (int i = 0; i < NS; ++i) s[u] = A::mma(rd.row(k_lds[buf], u, i), qf[i], s[u]);
+      }
+      if constexpr (TL::k16) {
+        interleave<6, SUB * NS, 1>();
+      } else {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+          mend_scores(s[u], [&] {
+            f32x16 f{};
+#pragma unroll
+            for (int i = 0; i < NS; ++i) f = Elem<__bf16>::mma(rd.row(k_lds[buf], u, i).t[0], qf[i].t[0], f);
+            return f;
+          });
+      }
+      if (k0 < last_start || k0 + KT - 1 > q0) {
+        const uint32_t from = here(k0 + 4 * g - start), far = empty ? 0u : reach + 1;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[u][j] = from + 32 * u + kappa(0, j) < far ? s[u][j] : kNegInf;
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[u][j]);
+      mx = fast::max_halves(mx) * c1;
+      const bool grow = mx > m_run + fast::kLazyRescale;
+      if (__any(grow)) {
+        const float m_new = grow ? mx : m_run;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+        m_run = m_new;
+        neg_m = m_run == kNegInf ? 0.f : -m_run;
+        l_run *= alpha;
+#pragma unroll
+        for (int d = 0; d < NDT; ++d) o[d] *= alpha;
+      }
+    };
     if (k0 < spans.last.start || k0 + KT - 1 > block0) {
       // (masked pairs for some wave)
       if (__syncthreads_or(tile_non_finite<Plane, PlaneType>(v_lds[buf]))) {
+        // (the maximum first: what is added must not meet the factor that makes room for this tile, which may be 0)
+        if (mine) scores();
         add_non_finite<TL, true>(o, v_lds[buf], g, keep);
         __syncthreads();
         clean_tile<Plane, PlaneType>(v_lds[buf]);
         __syncthreads();
       }
     }
-    if (idle || k0 > last || k0 + KT <= first_start) return;
-
-    f32x16 s[SUB];
-#pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      s[u] = f32x16{};
-#pragma unroll
-      for (int i = 0; i < NS; ++i) s[u] = A::mma(rd.row(k_lds[buf], u, i), qf[i], s[u]);
-    }
-    if constexpr (TL::k16) {
-      interleave<6, SUB * NS, 1>();
-    } else {
-#pragma unroll
-      for (int u = 0; u < SUB; ++u)
-        mend_scores(s[u], [&] {
-          f32x16 f{};
-#pragma unroll
-          for (int i = 0; i < NS; ++i) f = Elem<__bf16>::mma(rd.row(k_lds[buf], u, i).t[0], qf[i].t[0], f);
-          return f;
-        });
-    }
-    if (k0 < last_start || k0 + KT - 1 > q0) {
-      const uint32_t from = here(k0 + 4 * g - start), far = empty ? 0u : reach + 1;
-#pragma unroll
-      for (int u = 0; u < SUB; ++u)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[u][j] = from + 32 * u + kappa(0, j) < far ? s[u][j] : kNegInf;
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[u][j]);
-    mx = fast::max_halves(mx) * c1;
-    const bool grow = mx > m_run + fast::kLazyRescale;
-    if (__any(grow)) {
-      const float m_new = grow ? mx : m_run;
-      const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-      m_run = m_new;
-      neg_m = m_run == kNegInf ? 0.f : -m_run;
-      l_run *= alpha;
-#pragma unroll
-      for (int d = 0; d < NDT; ++d) o[d] *= alpha;
-    }
+    if (!mine) return;
+    scores();
     Frag<T> p[KT / 16], rest[TWO ? KT / 16 : 1];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
