@@ -75,6 +75,9 @@ PLACES = [
     (4, 2, 40, 64, None, 3),  # the first tile that its rows meet
     (4, 2, 40, 128, None, 39),
     (4, 2, 20, 64, [0, 7, 20], 9),  # a sequence inside a tile
+    (4, 2, 300, 128, None, 5),  # rows of later blocks, to whom the tile is whole
+    (4, 2, 300, 128, [0, 130, 300], 140),
+    (1, 1, 1100, 64, None, 70),  # walks in parts
 ]
 
 
@@ -110,3 +113,13 @@ def test_an_infinity_where_the_maximum_rises_far(dtype):
     x["v"][0, 0, 70, 5] = INF
     out = causal_attention(x["q"], x["k"], x["v"], scale=1.0)
     assert (out[0, 0, 70:, 5] == INF).all() and torch.isfinite(out[0, 0, :70]).all() and torch.isfinite(out[0, 0, 70:, 6:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_an_infinity_with_small_weights(dtype):
+    """Weights down to e^-40 or so, positive all the same: the infinity reaches every row that is paired with it."""
+
+    x = _case(2, 1, 1, 400, 64, dtype)
+    y = {name: t.clone() for name, t in x.items()}
+    y["v"][0, 0, 30, 5] = INF
+    assert (_run(y, scale=1.0)[0][0, 0, 30:, 5] == INF).all()
