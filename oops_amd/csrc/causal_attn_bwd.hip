@@ -201,6 +201,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void causal_grad_key
   constexpr int QT = 32, NS = DP / 16, NDT = DP / 32;
   // (registers: with 128 channels dK, dV and K fill them; V is read again from LDS at each step)
   constexpr bool kValuesInLds = DP == 128;
+  constexpr bool kAgain = !__is_same(T, __bf16);
   using Plane = typename TL::Plane;
   using PlaneType = typename TL::PlaneType;
   __shared__ __attribute__((aligned(1024))) char q_lds[A::kBuffers][TL::kBytes];
@@ -284,19 +285,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void causal_grad_key
       if constexpr (!TL::k16) vl.land(v_lds[i]);
     }
   }
-  if (t0 <= t1) {
-    seek();
-    load(std::integral_constant<int, 0>{});
-  } else {
-    fast::vmem_wait<0>();  // (nothing may land in LDS that is another workgroup's by then)
-  }
+  bool careful = false;  // every tile of queries is looked through
   auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
     constexpr int now = decltype(buffer)::value, buf = now % A::kBuffers;
     const int q0 = t * QT;
     arrived<T>(ql, q_lds[buf], dl, do_lds[buf]);
     if (load_h < h1) load(std::integral_constant<int, now ^ 1>{});
     auto keep = [&](int r) { return (uint32_t)(q0 + r - key) < width; };
-    if (q0 < block0 + kBlock - 1 || q0 + QT > spans.first.end) {
+    if (careful || q0 < block0 + kBlock - 1 || q0 + QT > spans.first.end) {
       // (masked pairs for some wave; a query that is not finite has made its LSE, a dO its delta, NaN or infinite)
       if (__syncthreads_or(tile_non_finite<Plane, PlaneType>(q_lds[buf]) | tile_non_finite<Plane, PlaneType>(do_lds[buf]))) {
         add_non_finite<TL, false>(dk, q_lds[buf], g, keep);
@@ -368,15 +364,34 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void causal_grad_key
       }
     if constexpr (TL::k16) interleave<8, 4 * NDT, 2>();
   };
-  for (int h = h0, t = t0; t0 <= t1;) {
-    auto next = [&] {
-      if (++t > t1) t = t0, ++h;
-      return h < h1;
-    };
-    step(t, std::integral_constant<int, 0>{});
-    if (!next()) break;
-    step(t, std::integral_constant<int, 1>{});
-    if (!next()) break;
+  if (t0 > t1) fast::vmem_wait<0>();  // (nothing may land in LDS that is another workgroup's by then)
+#pragma unroll 1
+  while (t0 <= t1) {
+    seek();
+    load(std::integral_constant<int, 0>{});
+    for (int h = h0, t = t0;;) {
+      auto next = [&] {
+        if (++t > t1) t = t0, ++h;
+        return h < h1;
+      };
+      step(t, std::integral_constant<int, 0>{});
+      if (!next()) break;
+      step(t, std::integral_constant<int, 1>{});
+      if (!next()) break;
+    }
+    if constexpr (!kAgain) break;
+    // (as in the forward: an infinity of dO that nothing masks has met lower terms of a weight, or one that underflowed)
+    float any = 0.f;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) any += dv[d][j];
+    if (careful || !a.dv || !__syncthreads_or(any != any && width > 0)) break;
+    careful = true;
+    load_h = h0;
+    load_t = t0;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
   }
   if (!valid) return;
   const float scale = a.flip ? -a.scale : a.scale;

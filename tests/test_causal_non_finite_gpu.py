@@ -76,8 +76,10 @@ PLACES = [
     (4, 2, 40, 128, None, 39),
     (4, 2, 20, 64, [0, 7, 20], 9),  # a sequence inside a tile
     (4, 2, 300, 128, None, 5),  # rows of later blocks, to whom the tile is whole
+    (4, 2, 300, 64, None, 259),  # ... a query behind whole tiles of keys
     (4, 2, 300, 128, [0, 130, 300], 140),
     (1, 1, 1100, 64, None, 70),  # walks in parts
+    (1, 1, 1100, 128, None, 700),
 ]
 
 
@@ -117,9 +119,13 @@ def test_an_infinity_where_the_maximum_rises_far(dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_an_infinity_with_small_weights(dtype):
-    """Weights down to e^-40 or so, positive all the same: the infinity reaches every row that is paired with it."""
+    """Weights down to e^-40 or so, positive all the same: the infinity reaches every row or key that is paired with it."""
 
     x = _case(2, 1, 1, 400, 64, dtype)
     y = {name: t.clone() for name, t in x.items()}
     y["v"][0, 0, 30, 5] = INF
     assert (_run(y, scale=1.0)[0][0, 0, 30:, 5] == INF).all()
+    y = {name: t.clone() for name, t in x.items()}
+    y["do"][0, 0, 390, 5] = -INF
+    dv = _run(y, scale=1.0)[3]
+    assert (dv[0, 0, :391, 5] == -INF).all() and torch.isfinite(dv[0, 0, 391:]).all() and torch.isfinite(dv[..., :5]).all()
