@@ -576,8 +576,8 @@ int oops_rms_norm_rotary_backward(const oops_rotary_geometry* geo, const void* q
  * sequences packed along the tokens, for every batch element; tokens outside them have zero outputs and gradients.
  * Element (b, h, t, i) of an operand is at b * stride[0] + h * stride[1] + t * stride[2] + i; pointers, strides and sizes
  * times the element's size are multiples of 16 bytes, tokens less than 2^24 bytes apart (strides of dimensions of one
- * element are not read).  lse is float32 [batch][heads][length] in log2 units, out_low (16-bit types) the rounding's
- * remainder of out with out's strides; both are NULL where no backward follows. */
+ * element are not read).  lse is float32 [batch][heads][length] in log2 units (NaN where all of a row's scores are -inf),
+ * out_low (16-bit types) the rounding's remainder of out with out's strides; both are NULL where no backward follows. */
 enum oops_causal_operand {
   OOPS_CA_Q, OOPS_CA_K, OOPS_CA_V, OOPS_CA_O, OOPS_CA_DO, OOPS_CA_DQ, OOPS_CA_DK, OOPS_CA_DV, OOPS_CA_OPERANDS
 };

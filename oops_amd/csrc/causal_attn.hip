@@ -35,6 +35,10 @@ namespace oops {
 namespace causal {
 namespace {
 
+// a row's LSE from its maximum and its sum; logits that are all -inf have weights 0 / 0, NaN like the LSE that they get (with
+// -inf, a score that the backward makes of cleaned operands would have a weight of infinity)
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? __builtin_nanf("") : m + __builtin_amdgcn_logf(l); }
+
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void causal_forward_kernel(CausalArgs a) {
   using TL = Tile<T, DP>;
@@ -238,7 +242,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
       store_columns<float>(reinterpret_cast<char*>(a.o_parts + at * a.value_size), 32 * d, a.value_size, g, o[d], 1.f);
     return;
   }
-  if (a.lse && g == 0) a.lse[((int64_t)b * a.heads + h) * length + row] = empty ? 0.f : m_run + __builtin_amdgcn_logf(l);
+  if (a.lse && g == 0) a.lse[((int64_t)b * a.heads + h) * length + row] = empty ? 0.f : log_sum(m_run, l);
   const int64_t at = (b * a.o_stride[0] + h * a.o_stride[1] + row * a.o_stride[2]) * (int64_t)sizeof(T);
 #pragma unroll
   for (int d = 0; d < NDT; ++d) {
@@ -281,7 +285,7 @@ __global__ __launch_bounds__(256) void causal_join_kernel(CausalArgs a, int64_t 
   const int64_t at = b * a.o_stride[0] + h * a.o_stride[1] + token * a.o_stride[2] + d;
   *reinterpret_cast<v4*>(static_cast<T*>(a.out) + at) = y;
   if (a.low) *reinterpret_cast<v4*>(static_cast<T*>(a.low) + at) = low;
-  if (a.lse && d == 0) a.lse[row] = empty ? 0.f : m + __builtin_amdgcn_logf(l);
+  if (a.lse && d == 0) a.lse[row] = empty ? 0.f : log_sum(m, l);
 }
 
 }  // namespace

@@ -129,3 +129,18 @@ def test_an_infinity_with_small_weights(dtype):
     y["do"][0, 0, 390, 5] = -INF
     dv = _run(y, scale=1.0)[3]
     assert (dv[0, 0, :391, 5] == -INF).all() and torch.isfinite(dv[0, 0, 391:]).all() and torch.isfinite(dv[..., :5]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,token", [(1, 0), (40, 39), (40, 0), (300, 299)])
+def test_a_row_whose_scores_are_all_minus_infinity(dtype, n, token):
+    """0 / 0 in its output, and in all gradients that its weights reach."""
+
+    x = _case(3, 1, 1, n, 64, dtype)
+    x["k"][..., 5] = x["k"][..., 5].abs() + 1
+    x["q"][0, 0, token, 5] = -INF
+    out, dq, dk, dv = _run(x)
+    for t in (out[0, 0, token], dq[0, 0, token], dk[0, 0, : token + 1], dv[0, 0, : token + 1]):
+        assert torch.isnan(t).all()
+    others = [i for i in range(n) if i != token]
+    assert torch.isfinite(out[0, 0, others]).all() and torch.isfinite(dv[0, 0, token + 1 :]).all()
