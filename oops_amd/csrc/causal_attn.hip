@@ -91,8 +91,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
   f32x16 o[NDT];
 #pragma unroll
   for (int t = 0; t < NDT; ++t) o[t] = f32x16{};
-  // (a scale of zero: a product too small to count, that leaves the masked pairs' -inf one)
-  const float c1 = fmaxf(a.scale * kLog2e, 0x1p-120f);
+  const float c1 = score_factor(a);
 
   fast::vmem_wait<0>();  // (the queries, before loads that the compiler does not count)
   bool careful = false;  // every tile's values are looked through

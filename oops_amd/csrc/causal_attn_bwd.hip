@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256, (kOcc<T, DP>)) void causal_grad_query_kernel(C
   float delta = row_dot<T, DP>(rows_of<T>(a.out, a.o_stride, b, h, a.value_size, length), dor, row, valid, g, 0.f);
   if (a.low) delta = row_dot<T, DP>(rows_of<T>(a.low, a.o_stride, b, h, a.value_size, length), dor, row, valid, g, delta);
   delta = fast::sum_halves(delta);
-  const float c1 = fmaxf(a.scale * kLog2e, 0x1p-120f);
+  const float c1 = score_factor(a);
   const int64_t stat = ((int64_t)b * a.heads + h) * length + row;
   const float lse = valid ? a.lse[stat] : 0.f;
   if (valid && g == 0 && split == 0) {
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void causal_grad_key
   f32x16 dk[NDT], dv[NDT];
 #pragma unroll
   for (int t = 0; t < NDT; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
-  const float c1 = fmaxf(a.scale * kLog2e, 0x1p-120f);
+  const float c1 = score_factor(a);
   Reads<T, DP> rd, rv;
   rd.init(lane);
   rv = rd;
@@ -394,7 +394,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void causal_grad_key
     for (int t = 0; t < NDT; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
   }
   if (!valid) return;
-  const float scale = a.flip ? -a.scale : a.scale;
+  // (a token of no sequence has zeros, whatever the scale)
+  const float scale = width == 0 ? 0.f : a.flip ? -a.scale : a.scale;
   if (parts > 1) {
     const int64_t at = (((int64_t)part * a.batch + b) * a.kv_heads + hk) * length + key;
 #pragma unroll

@@ -429,6 +429,12 @@ __device__ __forceinline__ uint32_t here(int x) {
   asm volatile("" : "+v"(x));
   return (uint32_t)x;
 }
+// The scores' factor, in log2 units.  A scale of zero is a product too small to count, that leaves the masked pairs' -inf
+// one; one that is NaN stays it.
+__device__ __forceinline__ float score_factor(const CausalArgs& a) {
+  const float c = a.scale * kLog2e;
+  return c < 0x1p-120f ? 0x1p-120f : c;
+}
 // sum + the elements of f, a fragment of 16 bits (two a step)
 template <typename T>
 __device__ __forceinline__ float add_elements(const Frag<T>& f, float sum) {

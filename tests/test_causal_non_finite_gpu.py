@@ -144,3 +144,14 @@ def test_a_row_whose_scores_are_all_minus_infinity(dtype, n, token):
         assert torch.isnan(t).all()
     others = [i for i in range(n) if i != token]
     assert torch.isfinite(out[0, 0, others]).all() and torch.isfinite(dv[0, 0, token + 1 :]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [NAN, INF, -INF])
+@pytest.mark.parametrize("n,offsets", [(40, None), (300, [0, 1, 200, 290])])
+def test_scales_that_are_not_finite(dtype, scale, n, offsets):
+    """Every score is an infinity or a NaN, so every row is 0 / 0 or inf / inf; rows of no sequence are zeros."""
+
+    last = n if offsets is None else offsets[-1]
+    for t in _run(_case(4, 4, 2, n, 64, dtype), offsets, scale):
+        assert torch.isnan(t[:, :, :last]).all() and not t[:, :, last:].any()
