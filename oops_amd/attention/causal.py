@@ -59,8 +59,8 @@ def causal_attention(
             nearer bound.)
         scale: of the scores; default ``D ** -0.5``.
 
-    Returns ``(*prefix, H, L, E)`` in the query's dtype and dimension order.  Gradients reach query, key and value;
-    second derivatives raise.
+    Returns ``(*prefix, H, L, E)`` in the query's dtype and dimension order (head-major where its tokens would be 2^24 bytes
+    or more apart).  Gradients reach query, key and value; second derivatives raise.
 
     Operands whose rows are not whole 16-byte pieces at 16-byte addresses are copied first.  Sums, statistics and
     accumulators are float32.  As operands of the next product, bfloat16's probabilities are rounded to the type,
@@ -174,10 +174,10 @@ def _whole(t: Tensor) -> Tensor:
     return t
 
 
-def _result_like(t: Tensor, width: int) -> Tensor:
+def _result_like(t: Tensor, width: int, empty_like=_empty_like) -> Tensor:
     """A result with ``t``'s order of dimensions, unless its tokens would then lie too far apart."""
 
-    out = _empty_like(t, width)
+    out = empty_like(t, width)
     if out.shape[2] > 1 and out.stride(2) * out.element_size() >= MAX_PITCH:
         return torch.empty(out.shape, dtype=out.dtype, device=out.device)
     return out
@@ -232,7 +232,7 @@ def causal_attention_forward(q: Tensor, k: Tensor, v: Tensor, offsets: Optional[
 
 @causal_attention_forward.register_fake
 def _(q, k, v, offsets, scale, save):
-    out = _fake_like(q, v.shape[-1])
+    out = _result_like(q, v.shape[-1], _fake_like)
     low = torch.empty_like(out) if save and q.dtype != torch.float32 else out.new_empty(0)
     return out, low, q.new_empty(q.shape[:3] if save else (0,), dtype=torch.float32)
 
@@ -246,7 +246,7 @@ def causal_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, off
 
 @causal_attention_backward.register_fake
 def _(dout, q, k, v, offsets, out, low, lse, scale, needs):
-    return tuple(_fake_like(t, t.shape[-1]) if need else t.new_empty(0) for t, need in zip((q, k, v), needs))
+    return tuple(_result_like(t, t.shape[-1], _fake_like) if need else t.new_empty(0) for t, need in zip((q, k, v), needs))
 
 
 # ----------------------------------------------------------------- autograd
