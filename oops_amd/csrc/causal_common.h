@@ -2,9 +2,10 @@
 //
 // Every product is a 32 x 32 x 16 step on fragments of eight elements a lane: one
 // MFMA of a 16-bit type.  float32 operands are three bfloat16 terms, their sum
-// exactly, and a step is six MFMAs, the terms' products down to 2^-16 of the largest
-// (what is left out is below 2^-23, and 2^-26 on average): 192 cycles where the
-// float32 matrix unit takes 512.  Lane (c = lane % 32, g = lane / 32)
+// exactly (above 2^-110 in magnitude: the terms have float32's exponents, and their
+// smallest number is 2^-133), and a step is six MFMAs, the terms' products down to
+// 2^-16 of the largest (what is left out is below 2^-23, and 2^-26 on average): 192
+// cycles where the float32 matrix unit takes 512.  Lane (c = lane % 32, g = lane / 32)
 // holds elements 16 s + 8 g .. + 7 of row c along the contracted axis.  An
 // accumulator's rows are kappa(g, j), so eight of its registers are the other
 // operand of the next product as they stand, if the tile in LDS is read in the same
@@ -497,7 +498,8 @@ __device__ __forceinline__ void clean_tile(char* tile) {
     u = make_uint4(finite_word<T>(u.x), finite_word<T>(u.y), finite_word<T>(u.z), finite_word<T>(u.w));
   }
 }
-// SIGNED: the weights are positive, an infinity stays one; else what is not finite makes NaN.  keep(row): whether the
+// SIGNED: the weights are positive, an infinity stays one (acc must not be rescaled for this tile any more); else what is not
+// finite makes NaN.  keep(row): whether the
 // tile's row is paired with this lane's column.
 template <typename TL, bool SIGNED, int NDT, typename Keep>
 __device__ __forceinline__ void add_non_finite(f32x16 (&acc)[NDT], const char* tile, int g, Keep keep) {
