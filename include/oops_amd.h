@@ -613,7 +613,8 @@ int oops_causal_attn_backward(const oops_causal_geometry* geo, const void* q, co
  * the nearest code, ties to even codes (saturated above 6 * 2^125); one with an infinity or a NaN has e = 255, which
  * stands for NaN.  slots [batch][length]: token's page * page_size + place; others (negative ones, say) are not written
  * and read as zeros; of tokens with the same slot the last is kept.  Element (b, h, t, i) of key and value is at
- * b * stride[0] + h * stride[1] + t * stride[2] + i. */
+ * b * stride[0] + h * stride[1] + t * stride[2] + i.  The workspace of a call of more than 1024 tokens has 4 bytes for each
+ * slot of the cache. */
 typedef struct oops_cache_geometry {
   int32_t dtype;
   int32_t heads;

@@ -5,7 +5,8 @@ quarter of bfloat16's bytes and a little more, and decoding is bound by these by
 that the caller owns,
 
     codes  uint8 (pages, G, 2, page_size, D / 2)     keys ([:, :, 0]) and values; channel 2 i is the low half of byte i
-    scales uint8 (pages, G, 2, page_size, D / 32)    exponents e: a block stands for its codes' values times 2 ** (e - 127)
+    scales uint8 (pages, G, 2, page_size, D / 32)    exponents e, 1..252: a block stands for its codes' values times
+                                                     2 ** (e - 127), with 255 for NaN (0 in an empty cache)
 
 with codes 0..7 for 0, 0.5, 1, 1.5, 2, 3, 4, 6 and 8..15 for their negatives.  Tokens have slots,
 ``page * page_size + place``; which page holds which part of a sequence is the caller's table.  ``cache_write`` puts keys
@@ -69,6 +70,8 @@ def cache_write(codes: Tensor, scales: Tensor, key: Tensor, value: Tensor, slots
     Each block of 32 channels gets the smallest exponent with ``max|block| <= 6 * 2 ** (e - 127)``, ``e`` in 1..252, and
     the nearest codes (ties to the even one), exactly as in real arithmetic; magnitudes above ``6 * 2 ** 125`` become
     that.  A block with an infinity or a NaN gets ``e = 255`` and reads as NaN.
+
+    A call of more than 1024 tokens takes 4 bytes for each slot of the cache as a workspace.
     """
 
     operator = "cache_write"
@@ -134,7 +137,8 @@ def cache_attention(
         scale: of the scores; default ``D ** -0.5``.
 
     Returns ``(*prefix, H, D)`` in the query's dtype; zeros for a sequence without tokens.  What the codes stand for
-    takes part exactly, and sums are float32, so the result has the precision of the query's type.
+    takes part exactly, weights have 16 bits or more, and sums are float32, so the result has the precision of the query's
+    type.  Few sequences take less time with a page table that is not much wider than they are.
     """
 
     operator = "cache_attention"

@@ -25,8 +25,9 @@
 //
 // bfloat16, 8 key heads of 128, 32 query heads: writing 30011 tokens 48 us (157 MB at
 // 3.3 TB/s) and 4 for the slots' owners, reading them 37 (4.3 TB/s); attention of 64
-// sequences of up to 16384 tokens 173 us (4.2 TB/s) and 6 for the join, one sequence
-// of 32768 17 (2.1 TB/s: 256 tokens a workgroup, two steps of each wave) and 6.
+// sequences of up to 16384 tokens 178 us (4.0 TB/s; 222 and 230 with float16 and
+// float32 queries) and 6 for the join, one sequence of 32768 17.6 (2.0 TB/s: 256
+// tokens a workgroup, two steps of each wave) and 6.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -591,8 +592,11 @@ __global__ __launch_bounds__(512) void cache_join_kernel(const float* parts, voi
 }
 
 // Parts of the length: workgroups for eight on every CU, so that sequences of different lengths even out, but no part
-// shorter than two steps of each wave (8 key heads of 128, one sequence of 32768 or of 4096 tokens, us with the join: two
-// steps 28 and 16, one 37 and 15, four 27-30 and 18, eight 30 and 23).
+// shorter than two steps of each wave where a sequence fills its page table (8 key heads of 128, one sequence of 32768 or of
+// 4096 tokens, us with the join: two steps 28 and 16, one 37 and 15, four 27-30 and 18, eight 30 and 23).  The host knows
+// the table's width and not the lengths: few sequences that are short for their table have shorter parts and empty ones.
+// us of a call in a graph with a table that the sequence fills, 4 and 32 times as wide: one sequence of 1024 tokens 11, 10
+// and 18, of 4096 11, 13 and 28, of 32768 23, 32 and 32, four of 2048 12, 16 and 23, 16 of 4096 30 each.
 int decode_splits(const oops_cache_attn_geometry& g) {
   const int64_t group = g.heads / g.kv_heads;
   const int64_t jobs = g.batch * g.kv_heads * ((group + kHeadTile - 1) / kHeadTile);

@@ -16,12 +16,15 @@
 // queries and tiles of keys lie at multiples of their size in the packed row,
 // tiles before a block's first sequence and behind its last query are not read,
 // and a tile is masked pair by pair only where a bound or the diagonal crosses
-// it for this wave.
+// it for this wave.  Such tiles are looked through for infinities and NaN, which 0
+// times them would spread; in float16 and float32 a walk whose sums come out NaN
+// is made again with every tile looked through (a microsecond of a small call's
+// time for the look at the sums).
 //
 // Bound by the matrix units and what stands between their two products.  bfloat16,
-// 16 heads of 16384 tokens and 128 channels: 1040-1060 us, 1040 TFLOP/s of a
+// 16 heads of 16384 tokens and 128 channels: 1040-1065 us, 1040 TFLOP/s of a
 // library's square product's 1380 (matrix units 60% busy, no bank conflicts); five
-// packed sequences of 8192 tokens in all, 32 heads: 235 us, 770 TFLOP/s of the
+// packed sequences of 8192 tokens in all, 32 heads: 231-245 us, 770 TFLOP/s of the
 // pairs that count (9% of the products lie in masked halves of tiles, the rest
 // is four times as many blocks' first tiles and ends).  What it took: the order of
 // LDS reads and products given by hand (1303 -> 1130), padded tiles with constant

@@ -192,8 +192,8 @@ __device__ __forceinline__ void dma4_asm(const fast::u32x4& r, const void* lds, 
       : "memory", "m0");
 }
 
-// (float32: one workgroup a CU, whose waves have 512 registers: 33 us for 2 x 6 heads of 777 tokens and 40 channels; with two,
-// 42 of 256 registers spill and it takes 33-34)
+// (float32: one workgroup a CU, whose waves have 512 registers: 33 us for 2 x 6 heads of 777 tokens and 40 channels before the
+// look at dV's sums, 36 with it; with two workgroups 42 of 256 registers spilled and it took 33-34)
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void causal_grad_key_value_kernel(CausalArgs a) {
   using TL = Tile<T, DP, 32>;
