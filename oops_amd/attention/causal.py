@@ -69,8 +69,8 @@ def causal_attention(
     are three bfloat16 terms: a product is off by 2^-23 of itself at most and 2^-26 on average, where its operands are above
     2^-110 in magnitude; of smaller ones (gradients without a scaled loss, say) up to 2^-134 may be missing.  Infinities
     and NaN reach the tokens whose sum holds them, and no others: neither earlier tokens nor other sequences.  An infinity
-    in a value stays one in its column of the outputs, one in an output's gradient in the value's gradient (NaN where its
-    weight is too small for float32); float16 and float32 calls that hold such values take up to twice the time.
+    in a value stays one in its column of the outputs, one in an output's gradient in the value's gradient (where its
+    weight is zero in float32, one or NaN); float16 and float32 calls that hold such values take up to twice the time.
     """
 
     _check(query, key, value, offsets)

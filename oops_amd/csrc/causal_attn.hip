@@ -38,9 +38,11 @@ namespace oops {
 namespace causal {
 namespace {
 
-// a row's LSE from its maximum and its sum; logits that are all -inf have weights 0 / 0, NaN like the LSE that they get (with
-// -inf, a score that the backward makes of cleaned operands would have a weight of infinity)
+// A row's LSE from its maximum and its sum, and what its O is multiplied with.  Logits that are all -inf have weights 0 / 0, so
+// both are NaN: with -inf, a score that the backward makes of cleaned operands would have a weight of infinity, and with
+// 1 / 0 an infinite value would stay one.
 __device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? __builtin_nanf("") : m + __builtin_amdgcn_logf(l); }
+__device__ __forceinline__ float one_over(float l) { return l == 0.f ? __builtin_nanf("") : 1.0f / l; }
 
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void causal_forward_kernel(CausalArgs a) {
@@ -234,7 +236,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && DP == 128 ? 1 : 2)) void ca
     vl.seek(vr, t0 * KT);
   }
   // (a row without keys: zeros; one whose logits are all -inf: 0 / 0)
-  const float inv = empty ? 0.f : 1.0f / l;
+  const float inv = empty ? 0.f : one_over(l);
   if (!valid) return;
   if (a.key_splits > 1) {
     const int64_t at = (((int64_t)split * a.batch + b) * a.heads + h) * length + row;
@@ -273,7 +275,7 @@ __global__ __launch_bounds__(256) void causal_join_kernel(CausalArgs a, int64_t 
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = __builtin_fmaf(o[k], by, x[k]);
   }
-  const float inv = empty ? 0.f : 1.0f / l;
+  const float inv = empty ? 0.f : one_over(l);
   typedef T v4 __attribute__((ext_vector_type(4)));
   v4 y, low;
 #pragma unroll

@@ -147,6 +147,19 @@ def test_a_row_whose_scores_are_all_minus_infinity(dtype, n, token):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,token", [(1, 0), (40, 0), (1100, 0), (1100, 1000)])
+def test_an_infinity_in_a_row_whose_scores_are_all_minus_infinity(dtype, n, token):
+    """NaN in every column, the infinite value's too; keys of -inf up to the row's own, walks in parts among them."""
+
+    x = _case(5, 1, 1, n, 64, dtype)
+    x["q"][..., 5] = x["q"][..., 5].abs() + 1
+    x["k"][0, 0, : token + 1, 5] = -INF
+    x["v"][0, 0, token // 2, 7] = INF
+    out = causal_attention(x["q"], x["k"], x["v"])
+    assert torch.isnan(out[0, 0, : token + 1]).all() and torch.isfinite(out[0, 0, token + 1 :, 8:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [NAN, INF, -INF])
 @pytest.mark.parametrize("n,offsets", [(40, None), (300, [0, 1, 200, 290])])
 def test_scales_that_are_not_finite(dtype, scale, n, offsets):
