@@ -57,7 +57,8 @@ def causal_attention(
             (of every batch element): sequence n has the tokens ``offsets[n] .. offsets[n + 1] - 1``.  Tokens outside
             all of them are not read; their outputs and gradients are zero.  (Values outside 0..L are taken as the
             nearer bound.)
-        scale: of the scores; default ``D ** -0.5``.
+        scale: of the scores; default ``D ** -0.5``.  (Magnitudes below 2^-120, 0 among them, weigh scores with 2^-120: with
+            nothing, up to scores of 2^90.)
 
     Returns ``(*prefix, H, L, E)`` in the query's dtype and dimension order (head-major where its tokens would be 2^24 bytes
     or more apart).  Gradients reach query, key and value; second derivatives raise.
